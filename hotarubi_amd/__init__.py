@@ -13,6 +13,9 @@ include/hotarubi_gpu.h (libhotarubi_gpu.so, built by hotarubi_amd.build):
   linear(...)                a linear layer as LinearEmitter::Emit emits it
                              (tools/compiler/kernels.cpp:343-395) + epilogue
   encode_mxint8(x)           EncodeMxint8 + PackAbuf (formats.cpp:114-162)
+  kv_plan, norm_rope, kv_append, kv_read, kv_attention
+                             a serving step's attention over a paged MXFP4
+                             cache (torch tensors; no counterpart)
 
 Errors raise HbError; a command the reference rejects with Fail raises
 HbBadCommand carrying the reference's message.  The library is loaded from
@@ -60,6 +63,9 @@ EXPORTS = (
     "hb_image_alloc", "hb_image_set_reuse", "hb_image_define", "hb_image_put", "hb_image_get",
     "hb_image_region", "hb_image_region_count", "hb_image_region_at", "hb_image_end",
     "hb_image_base", "hb_linear_group_async",
+    "hb_kv_plan", "hb_kv_plan_async", "hb_norm_rope", "hb_norm_rope_async", "hb_kv_append",
+    "hb_kv_append_async", "hb_kv_read", "hb_kv_read_async", "hb_kv_attention",
+    "hb_kv_attention_async",
 )
 
 
@@ -115,6 +121,46 @@ class _LinearDesc(C.Structure):
                 ("pieces", _Piece * MAX_PIECES), ("onto", C.c_uint32), ("c", C.c_void_p),
                 ("n_ops", C.c_uint32), ("ops", _EpOp * MAX_OPS), ("tbuf", C.c_void_p),
                 ("q_out", C.c_void_p), ("flags", C.c_uint32), ("a_stride", C.c_uint32)]
+
+
+class _KvPlanDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in
+                ("lens", "new_tokens", "free_pages", "free_count", "table", "cu", "kv_lens",
+                 "slots", "positions", "status")] + \
+               [(n, C.c_uint32) for n in
+                ("batch", "columns", "table_stride", "page_size", "size", "free_size")]
+
+
+class _NormRopeDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out")] + \
+               [(n, C.c_uint64) for n in
+                ("q_token", "q_head", "k_token", "k_head", "q_out_token", "q_out_head",
+                 "k_out_token", "k_out_head")] + \
+               [("gamma_q", C.c_void_p), ("gamma_k", C.c_void_p), ("positions", C.c_void_p),
+                ("position_stride", C.c_uint64), ("inv_freq", C.c_void_p), ("eps", C.c_float)] + \
+               [(n, C.c_uint32) for n in
+                ("type", "tokens", "q_heads", "k_heads", "dim", "rot", "interleaved", "axes")] + \
+               [("sections", C.c_uint32 * 3)]
+
+
+class _KvCache(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("pages", C.c_uint32), ("heads", C.c_uint32),
+                ("page_size", C.c_uint32), ("dim", C.c_uint32)]
+
+
+class _KvRowsDesc(C.Structure):
+    _fields_ = [("cache", _KvCache), ("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_uint64) for n in ("k_token", "k_head", "v_token", "v_head")] + \
+               [("slots", C.c_void_p), ("type", C.c_uint32), ("tokens", C.c_uint32)]
+
+
+class _KvAttentionDesc(C.Structure):
+    _fields_ = [("cache", _KvCache), ("q", C.c_void_p), ("out", C.c_void_p)] + \
+               [(n, C.c_uint64) for n in ("q_token", "q_head", "out_token", "out_head")] + \
+               [(n, C.c_void_p) for n in ("table", "cu", "kv_lens", "prefix")] + \
+               [(n, C.c_uint32) for n in
+                ("type", "tokens", "q_heads", "batch", "columns", "table_stride", "max_new",
+                 "max_kv", "window")] + [("scale", C.c_float), ("softcap", C.c_float)]
 
 
 @dataclass
@@ -228,6 +274,16 @@ def lib():
                                        C.POINTER(C.c_uint64)]),
             "hb_image_end": (C.c_uint64, [vp]),
             "hb_image_base": (vp, [vp]),
+            "hb_kv_plan": (i, [vp, C.POINTER(_KvPlanDesc)]),
+            "hb_kv_plan_async": (i, [vp, C.POINTER(_KvPlanDesc)]),
+            "hb_norm_rope": (i, [vp, C.POINTER(_NormRopeDesc)]),
+            "hb_norm_rope_async": (i, [vp, C.POINTER(_NormRopeDesc)]),
+            "hb_kv_append": (i, [vp, C.POINTER(_KvRowsDesc)]),
+            "hb_kv_append_async": (i, [vp, C.POINTER(_KvRowsDesc)]),
+            "hb_kv_read": (i, [vp, C.POINTER(_KvRowsDesc)]),
+            "hb_kv_read_async": (i, [vp, C.POINTER(_KvRowsDesc)]),
+            "hb_kv_attention": (i, [vp, C.POINTER(_KvAttentionDesc)]),
+            "hb_kv_attention_async": (i, [vp, C.POINTER(_KvAttentionDesc)]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -259,6 +315,7 @@ class Context:
         h = C.c_void_p()
         _check(lib().hb_ctx_create(device, C.byref(h)))
         self.handle = h
+        self.device = device
 
     def close(self):
         if self.handle:
@@ -690,3 +747,202 @@ def encode_mxfp8(x, rows: int, cols: int, out, ctx: Context | None = None) -> No
     """hb_encode_mxfp8: a device fp32 [rows][cols] as MXFP8 E4M3 DDR words."""
     ctx = ctx or default_context()
     _check(lib().hb_encode_mxfp8(ctx.handle, _ptr(x), rows, cols, _ptr(out)))
+
+
+# ---------------------------------------------------- serving operators --
+# These take torch tensors: sizes, types and strides come from them.
+
+HB_TYPE_F32, HB_TYPE_BF16, HB_TYPE_F16 = range(3)
+_types = None  # torch.dtype -> hb_type, and the other types the checks name
+
+
+def _torch_types():
+    global _types
+    if _types is None:
+        import torch
+        _types = ({torch.float32: HB_TYPE_F32, torch.bfloat16: HB_TYPE_BF16,
+                   torch.float16: HB_TYPE_F16}, torch.int32, torch.uint8, torch.float64,
+                  torch.float32)
+    return _types
+
+
+def _invalid(message: str):
+    return HbError(HB_EINVAL, message)
+
+
+def _on(t, device: int, name: str) -> int:
+    """Address of a tensor on the context's device."""
+    if t.get_device() != device:
+        raise _invalid(f"{name} is on {t.device}, the context on cuda:{device}")
+    return t.data_ptr()
+
+
+def _vector(t, dtype, name: str, count: int | None, device: int) -> int:
+    """Address of a contiguous vector (of `count` elements)."""
+    if t.dtype != dtype or t.dim() != 1 or (count is not None and t.shape[0] != count) or \
+            not t.is_contiguous():
+        raise _invalid(f"{name} must be {'n' if count is None else count} contiguous {dtype} "
+                       f"elements, not {tuple(t.shape)} of {t.dtype}")
+    return _on(t, device, name)
+
+
+def _heads(t, dtype, name: str, shape, device: int):
+    """(address, token stride, head stride) of [tokens][heads][dim] rows."""
+    if t.dtype != dtype or t.dim() != 3 or (shape is not None and t.shape != shape):
+        raise _invalid(f"{name} is {tuple(t.shape)} of {t.dtype}, not "
+                       f"{'[tokens][heads][dim]' if shape is None else tuple(shape)} of {dtype}")
+    stride = t.stride()
+    if stride[2] != 1 and t.shape[2] > 1:
+        raise _invalid(f"{name}: a head's elements must be neighbours")
+    return _on(t, device, name), stride[0], stride[1]
+
+
+def _table(t, device: int):
+    if t.dtype != _torch_types()[1] or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise _invalid(f"table must be int32 rows, not {tuple(t.shape)} of {t.dtype}")
+    return _on(t, device, "table"), t.shape[0], t.shape[1], t.stride(0)
+
+
+def _cache(t, device: int) -> _KvCache:
+    size = t.shape
+    if t.dtype != _torch_types()[2] or len(size) != 4 or size[3] % 34 or not t.is_contiguous():
+        raise _invalid("the cache must be contiguous uint8 [pages][heads][page / 32][34 dim], not "
+                       f"{tuple(size)} of {t.dtype}")
+    return _KvCache(_on(t, device, "cache"), size[0], size[1], 32 * size[2], size[3] // 34)
+
+
+def _kind(t, name: str) -> int:
+    kind = _torch_types()[0].get(t.dtype)
+    if kind is None:
+        raise _invalid(f"{name} is {t.dtype} (float32, bfloat16 or float16)")
+    return kind
+
+
+def _count(value, name: str) -> int:
+    if not 0 <= value < 1 << 32:  # ctypes would wrap it
+        raise _invalid(f"{name} = {value}")
+    return value
+
+
+def kv_plan(lens, new_tokens, free_pages, free_count, table, page_size: int, cu, kv_lens, slots,
+            positions, status, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_plan: a serving step's plan on the device.  lens, new_tokens int32
+    [batch]; free_pages int32 (a stack of free_count [1] pages); table int32
+    [batch][columns] gets the new pages; cu [batch + 1], kv_lens [batch], slots
+    and positions [size], status [2] (pages taken, requests refused) are
+    written."""
+    ctx = ctx or default_context()
+    i32, dev = _torch_types()[1], ctx.device
+    at, batch, columns, stride = _table(table, dev)
+    slots_at = _vector(slots, i32, "slots", None, dev)
+    size = slots.shape[0]
+    d = _KvPlanDesc(_vector(lens, i32, "lens", batch, dev),
+                    _vector(new_tokens, i32, "new_tokens", batch, dev),
+                    _vector(free_pages, i32, "free_pages", None, dev),
+                    _vector(free_count, i32, "free_count", 1, dev), at,
+                    _vector(cu, i32, "cu", batch + 1, dev),
+                    _vector(kv_lens, i32, "kv_lens", batch, dev), slots_at,
+                    _vector(positions, i32, "positions", size, dev),
+                    _vector(status, i32, "status", 2, dev), batch, columns, stride,
+                    _count(page_size, "page_size"), size, free_pages.shape[0])
+    fn = lib().hb_kv_plan if sync else lib().hb_kv_plan_async
+    _check(fn(ctx.handle, C.byref(d)))
+
+
+def norm_rope(q, positions, inv_freq, q_out, k=None, k_out=None, gamma_q=None, gamma_k=None,
+              eps: float = 1e-6, sections=None, interleaved: bool = False,
+              ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_norm_rope: RMS norm of every head of q (and k) with gamma (None: not
+    normalised) and the rotation of its first 2 * len(inv_freq) elements.  q
+    [tokens][heads][dim]; positions int32 [axes][tokens] (or [tokens]);
+    inv_freq float64; sections: the pairs of each axis."""
+    ctx = ctx or default_context()
+    _, i32, _, f64, f32 = _torch_types()
+    kind, dev, dtype = _kind(q, "q"), ctx.device, q.dtype
+    qa, qt, qh = _heads(q, dtype, "q", None, dev)
+    tokens, heads, dim = q.shape
+    oa, ot, oh = _heads(q_out, dtype, "q_out", q.shape, dev)
+    ka = kt = kh = pa = pt = ph = k_heads = 0
+    if k is not None:
+        if k_out is None:
+            raise _invalid("k without k_out")
+        ka, kt, kh = _heads(k, dtype, "k", None, dev)
+        if k.shape[0] != tokens or k.shape[2] != dim:
+            raise _invalid(f"k is {tuple(k.shape)}, q {tuple(q.shape)}")
+        pa, pt, ph = _heads(k_out, dtype, "k_out", k.shape, dev)
+        k_heads = k.shape[1]
+    if positions.dim() == 1:
+        positions = positions[None]
+    axes = positions.shape[0]
+    if positions.dtype != i32 or positions.dim() != 2 or positions.shape[1] != tokens or \
+            (tokens > 1 and positions.stride(1) != 1):
+        raise _invalid(f"positions must be int32 [axes][{tokens}], not "
+                       f"{tuple(positions.shape)} of {positions.dtype}")
+    freq = _vector(inv_freq, f64, "inv_freq", None, dev)
+    half = inv_freq.shape[0]
+    sections = sections if sections is not None else (half,)
+    if len(sections) != axes or not 1 <= axes <= 3 or min(sections) < 0:
+        raise _invalid(f"sections {tuple(sections)} for {axes} position axes")
+    d = _NormRopeDesc(qa, ka, oa, pa, qt, qh, kt, kh, ot, oh, pt, ph,
+                      None if gamma_q is None else _vector(gamma_q, f32, "gamma_q", dim, dev),
+                      None if gamma_k is None else _vector(gamma_k, f32, "gamma_k", dim, dev),
+                      _on(positions, dev, "positions"), positions.stride(0), freq, eps, kind, tokens, heads, k_heads,
+                      dim, 2 * half, 1 if interleaved else 0, axes,
+                      (C.c_uint32 * 3)(*sections))
+    fn = lib().hb_norm_rope if sync else lib().hb_norm_rope_async
+    _check(fn(ctx.handle, C.byref(d)))
+
+
+def _kv_rows(fn, k, v, slots, cache, ctx) -> None:
+    ctx = ctx or default_context()
+    kind, dev = _kind(k, "k"), ctx.device
+    c = _cache(cache, dev)
+    tokens = k.shape[0]
+    shape = (tokens, c.heads, c.dim)
+    ka, kt, kh = _heads(k, k.dtype, "k", shape, dev)
+    va, vt, vh = _heads(v, k.dtype, "v", shape, dev)
+    d = _KvRowsDesc(c, ka, va, kt, kh, vt, vh,
+                    _vector(slots, _torch_types()[1], "slots", tokens, dev), kind, tokens)
+    _check(fn(ctx.handle, C.byref(d)))
+
+
+def kv_cache_shape(pages: int, heads: int, page_size: int, dim: int) -> tuple[int, int, int, int]:
+    """Shape of a paged MXFP4 cache (uint8)."""
+    return pages, heads, page_size // 32, 34 * dim
+
+
+def kv_append(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_append: rows k, v [tokens][heads][dim] into the cache (uint8
+    [pages][heads][page / 32][34 dim]) at int32 slots."""
+    _kv_rows(lib().hb_kv_append if sync else lib().hb_kv_append_async, k, v, slots, cache, ctx)
+
+
+def kv_read(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_read: the stored values of slots into k, v [tokens][heads][dim]."""
+    _kv_rows(lib().hb_kv_read if sync else lib().hb_kv_read_async, k, v, slots, cache, ctx)
+
+
+def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
+                 prefix=None, window: int = 0, softcap: float = 0.0,
+                 ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_attention: q [tokens][heads][dim] of ragged requests (rows
+    [cu[b], cu[b + 1]) are the last tokens of request b's kv_lens[b]) against
+    the paged cache, into out.  Causal; prefix int32 [batch]: leading keys that
+    every row sees; window: keys a row sees, itself among them (0: all);
+    softcap: scores as softcap * tanh(score / softcap)."""
+    ctx = ctx or default_context()
+    i32, dev = _torch_types()[1], ctx.device
+    kind, c = _kind(q, "q"), _cache(cache, dev)
+    qa, qt, qh = _heads(q, q.dtype, "q", None, dev)
+    tokens, heads, dim = q.shape
+    if dim != c.dim:
+        raise _invalid(f"q has heads of {dim} elements, the cache of {c.dim}")
+    oa, ot, oh = _heads(out, q.dtype, "out", q.shape, dev)
+    at, batch, columns, stride = _table(table, dev)
+    d = _KvAttentionDesc(c, qa, oa, qt, qh, ot, oh, at, _vector(cu, i32, "cu", batch + 1, dev),
+                         _vector(kv_lens, i32, "kv_lens", batch, dev),
+                         None if prefix is None else _vector(prefix, i32, "prefix", batch, dev),
+                         kind, tokens, heads, batch, columns, stride, _count(max_new, "max_new"),
+                         _count(max_kv, "max_kv"), _count(window, "window"), scale, softcap)
+    fn = lib().hb_kv_attention if sync else lib().hb_kv_attention_async
+    _check(fn(ctx.handle, C.byref(d)))

@@ -20,7 +20,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhotarubi_gpu.so")
 SOURCES = ["hb_api.hip", "hb_gemm.hip", "hb_fast.hip", "hb_fast4.hip", "hb_skinny.hip", "hb_vec.hip",
-           "hb_dma.hip", "hb_wave.hip", "hb_panel.hip", "hb_stream.hip", "hb_w8.hip", "hb_prep.hip"]
+           "hb_dma.hip", "hb_wave.hip", "hb_panel.hip", "hb_stream.hip", "hb_w8.hip", "hb_prep.hip",
+           "hb_kv.hip", "hb_attn.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 DEVICE_FLAGS = [
@@ -35,7 +36,10 @@ DEVICE_FLAGS = [
 # Per-source flags.  hb_skinny.hip: the single-layer split kernel's leading
 # arguments (pointers and sizes, 13 dwords) are preloaded into SGPRs by the
 # hardware, so its first operand loads need no argument round trip.
-SOURCE_FLAGS = {"hb_skinny.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=11"]}
+# hb_kv.hip: cache rows keep FP32 subnormals, which MXFP4's smallest scales
+# reach, and its tensors are ordinary floats rather than the NPU's.
+SOURCE_FLAGS = {"hb_skinny.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=11"],
+                "hb_kv.hip": ["-fno-gpu-flush-denormals-to-zero"]}
 
 
 def build(asm: bool = False, verbose: bool = False) -> str:

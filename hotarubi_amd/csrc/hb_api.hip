@@ -1370,6 +1370,237 @@ int hb_t32_split8_async(hb_ctx* ctx, const void* src, uint64_t src_stride, uint3
 
 }  // extern "C"
 
+// ---------------------------------------------------- serving operators --
+// The descriptors are checked before the context, with no device call, and a
+// call over no rows is no launch.
+namespace {
+
+int CheckType(uint32_t type) {
+  if (type > HB_TYPE_F16) return Fail(HB_EINVAL, "tensor type %u (0 fp32, 1 bf16, 2 fp16)", type);
+  return HB_OK;
+}
+
+bool Misaligned(const void* p, uint64_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes != 0;
+}
+
+int CheckCache(const hb_kv_cache& c) {
+  if (!c.base) return Fail(HB_EINVAL, "null cache");
+  if (Misaligned(c.base, 16)) return Fail(HB_EINVAL, "the cache must be 16-byte aligned");
+  if (c.dim != 64 && c.dim != 128 && c.dim != 256)
+    return Fail(HB_EUNSUPPORTED, "cache of head size %u (64, 128, 256)", c.dim);
+  if (c.page_size < 32 || c.page_size % 32 != 0)
+    return Fail(HB_EINVAL, "page size %u is not a multiple of 32", c.page_size);
+  if (c.pages < 1 || c.heads < 1) return Fail(HB_EINVAL, "cache of %u pages, %u heads", c.pages, c.heads);
+  // record and slot numbers are 32 bits wide
+  if ((unsigned __int128)c.pages * c.heads * (c.page_size / 32) >= 0xFFFFFFFFu)
+    return Fail(HB_EINVAL, "cache of %u pages x %u heads x %u tokens has 2^32 records or more",
+                c.pages, c.heads, c.page_size);
+  return HB_OK;
+}
+
+int Launched(hb_ctx* ctx, hipError_t err, const char* what, bool sync) {
+  if (err != hipSuccess) return HipFail(err, what);
+  if (sync) HB_HIP(hipStreamSynchronize(ctx->stream));
+  return HB_OK;
+}
+
+int KvPlan(hb_ctx* ctx, const hb_kv_plan_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  const void* ints[] = {d->lens, d->new_tokens, d->free_pages, d->free_count, d->table,
+                        d->cu,   d->kv_lens,    d->slots,      d->positions,  d->status};
+  // tensors of no elements may have no address
+  const uint64_t count[] = {d->batch,     d->batch, d->free_size, 1,       (uint64_t)d->batch * d->columns,
+                            d->batch + 1ull, d->batch, d->size,   d->size, 2};
+  for (int i = 0; i < 10; ++i) {
+    if (!ints[i] && count[i] > 0) return Fail(HB_EINVAL, "null step plan argument");
+    if (Misaligned(ints[i], 4)) return Fail(HB_EINVAL, "step plan arrays must be 4-byte aligned");
+  }
+  if (d->page_size < 32 || d->page_size % 32 != 0)
+    return Fail(HB_EINVAL, "page size %u is not a multiple of 32", d->page_size);
+  if (d->size > 0x7FFFFFFFu || d->free_size > 0x7FFFFFFFu || d->batch > 0x7FFFFFFFu)
+    return Fail(HB_EINVAL, "step plan of %u requests, %u tokens, %u free pages", d->batch, d->size,
+                d->free_size);
+  if (d->batch > 0 && d->columns > d->table_stride && d->batch > 1)
+    return Fail(HB_EINVAL, "table rows of %u entries are %u apart", d->columns, d->table_stride);
+  if (d->batch > 0 && (d->lens == d->kv_lens || d->new_tokens == d->kv_lens))
+    return Fail(HB_EINVAL, "kv_lens must not be an input");
+  if (int rc = Enter(ctx)) return rc;
+  hb::PlanArgs a{d->lens,   d->new_tokens, d->free_pages, d->free_count, d->table,
+                 d->cu,     d->kv_lens,    d->slots,      d->positions,  d->status,
+                 d->batch,  d->columns,    d->table_stride, d->page_size, d->size, d->free_size};
+  return Launched(ctx, hb::LaunchPlan(a, ctx->stream), "step plan launch", sync);
+}
+
+int NormRope(hb_ctx* ctx, const hb_norm_rope_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (int rc = CheckType(d->type)) return rc;
+  if (d->dim < 2 || d->dim % 2 != 0 || d->dim > 512)
+    return Fail(HB_EUNSUPPORTED, "heads of %u elements (an even count up to 512)", d->dim);
+  if (d->rot % 2 != 0 || d->rot > d->dim)
+    return Fail(HB_EINVAL, "%u turned elements of a head of %u", d->rot, d->dim);
+  if (d->axes < 1 || d->axes > 3) return Fail(HB_EINVAL, "%u position axes (1 to 3)", d->axes);
+  uint64_t pairs = 0;
+  for (uint32_t i = 0; i < d->axes; ++i) pairs += d->sections[i];
+  if (pairs != d->rot / 2)
+    return Fail(HB_EINVAL, "sections of %llu pairs for %u", (unsigned long long)pairs, d->rot / 2);
+  if (!(d->eps >= 0.f)) return Fail(HB_EINVAL, "negative eps");
+  if (d->q_heads < 1 || (d->k != nullptr && d->k_heads < 1) || d->q_heads > 0xFFFFFF ||
+      d->k_heads > 0xFFFFFF)
+    return Fail(HB_EINVAL, "%u query and %u key heads", d->q_heads, d->k_heads);
+  if (d->tokens == 0) return ctx ? HB_OK : Enter(ctx);
+  if (d->tokens > 0x3FFFFFFu) return Fail(HB_EINVAL, "%u tokens", d->tokens);
+  if (!d->q || !d->q_out || (d->k == nullptr) != (d->k_out == nullptr) ||
+      (d->rot > 0 && (!d->positions || !d->inv_freq)))
+    return Fail(HB_EINVAL, "null norm and rotation argument");
+  const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;
+  if (Misaligned(d->q, size) || Misaligned(d->k, size) || Misaligned(d->q_out, size) ||
+      Misaligned(d->k_out, size) || Misaligned(d->gamma_q, 4) || Misaligned(d->gamma_k, 4) ||
+      Misaligned(d->positions, 4) || Misaligned(d->inv_freq, 8))
+    return Fail(HB_EINVAL, "norm and rotation buffers must be aligned to their elements");
+  if (int rc = Enter(ctx)) return rc;
+  hb::RopeArgs a{};
+  a.q = d->q;
+  a.k = d->k;
+  a.q_out = d->q_out;
+  a.k_out = d->k_out;
+  a.q_token = d->q_token;
+  a.q_head = d->q_head;
+  a.q_out_token = d->q_out_token;
+  a.q_out_head = d->q_out_head;
+  if (d->k) {
+    a.k_token = d->k_token;
+    a.k_head = d->k_head;
+    a.k_out_token = d->k_out_token;
+    a.k_out_head = d->k_out_head;
+    a.k_heads = d->k_heads;
+  }
+  a.gamma_q = d->gamma_q;
+  a.gamma_k = d->gamma_k;
+  a.positions = d->positions;
+  a.position_stride = d->position_stride;
+  a.inv_freq = d->inv_freq;
+  a.eps = d->eps;
+  a.type = d->type;
+  a.tokens = d->tokens;
+  a.q_heads = d->q_heads;
+  a.dim = d->dim;
+  a.rot = d->rot;
+  a.neighbours = d->interleaved ? 1u : 0u;
+  a.sections[0] = d->axes > 1 ? d->sections[0] : 0xFFFFFFFFu;
+  a.sections[1] = d->axes > 2 ? d->sections[0] + d->sections[1] : 0xFFFFFFFFu;
+  return Launched(ctx, hb::LaunchRope(a, ctx->stream), "norm and rotation launch", sync);
+}
+
+int KvRows(hb_ctx* ctx, const hb_kv_rows_desc* d, bool read, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (int rc = CheckType(d->type)) return rc;
+  if (int rc = CheckCache(d->cache)) return rc;
+  if (d->tokens == 0) return ctx ? HB_OK : Enter(ctx);
+  if ((uint64_t)d->tokens * d->cache.heads > 0x7FFFFFFFu)
+    return Fail(HB_EINVAL, "%u tokens of %u heads in one call", d->tokens, d->cache.heads);
+  if (!d->k || !d->v || !d->slots) return Fail(HB_EINVAL, "null cache row argument");
+  const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;
+  if (Misaligned(d->k, size) || Misaligned(d->v, size) || Misaligned(d->slots, 4))
+    return Fail(HB_EINVAL, "cache rows must be aligned to their elements");
+  if (int rc = Enter(ctx)) return rc;
+  hb::KvRowsArgs a{};
+  if (read) {
+    a.k_out = d->k;
+    a.v_out = d->v;
+  } else {
+    a.k = d->k;
+    a.v = d->v;
+  }
+  a.k_token = d->k_token;
+  a.k_head = d->k_head;
+  a.v_token = d->v_token;
+  a.v_head = d->v_head;
+  a.slots = d->slots;
+  a.cache = static_cast<uint8_t*>(d->cache.base);
+  a.type = d->type;
+  a.tokens = d->tokens;
+  a.pages = d->cache.pages;
+  a.heads = d->cache.heads;
+  a.groups = d->cache.page_size / 32;
+  a.dim = d->cache.dim;
+  return Launched(ctx, hb::LaunchKvRows(a, read, ctx->stream), "cache row launch", sync);
+}
+
+int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (int rc = CheckType(d->type)) return rc;
+  if (int rc = CheckCache(d->cache)) return rc;
+  if (d->q_heads < 1 || d->q_heads % d->cache.heads != 0)
+    return Fail(HB_EINVAL, "%u query heads over %u K/V heads", d->q_heads, d->cache.heads);
+  if (!(d->scale == d->scale) || !(d->softcap >= 0.f))
+    return Fail(HB_EINVAL, "scale %g, softcap %g", (double)d->scale, (double)d->softcap);
+  if (d->tokens == 0 || d->batch == 0 || d->max_new == 0) return ctx ? HB_OK : Enter(ctx);
+  if (!d->q || !d->out || !d->cu || !d->kv_lens || (d->columns > 0 && !d->table))
+    return Fail(HB_EINVAL, "null attention argument");
+  const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;
+  if (Misaligned(d->q, size) || Misaligned(d->out, size) || Misaligned(d->table, 4) ||
+      Misaligned(d->cu, 4) || Misaligned(d->kv_lens, 4) || Misaligned(d->prefix, 4))
+    return Fail(HB_EINVAL, "attention buffers must be aligned to their elements");
+  if (d->batch > 1 && d->columns > d->table_stride)
+    return Fail(HB_EINVAL, "table rows of %u entries are %u apart", d->columns, d->table_stride);
+  const uint32_t max_new = std::min(d->max_new, d->tokens);
+  // positions, and rows of a request, are 31 bits wide
+  if ((uint64_t)d->columns * d->cache.page_size > 0x7FFFFF00u ||
+      (uint64_t)max_new * d->q_heads > 0x7FFFFF00u || d->tokens > 0x7FFFFFFFu ||
+      (uint64_t)d->batch * d->cache.heads > 0x7FFFFFFFu)
+    return Fail(HB_EINVAL, "attention of %u requests, %u new tokens, %u keys", d->batch, max_new,
+                d->max_kv);
+  if (int rc = Enter(ctx)) return rc;
+  hb::AttnArgs a{};
+  a.q = d->q;
+  a.out = d->out;
+  a.q_token = d->q_token;
+  a.q_head = d->q_head;
+  a.out_token = d->out_token;
+  a.out_head = d->out_head;
+  a.cache = static_cast<const uint8_t*>(d->cache.base);
+  a.table = d->table;
+  a.cu = d->cu;
+  a.kv_lens = d->kv_lens;
+  a.prefix = d->prefix;
+  a.type = d->type;
+  a.tokens = d->tokens;
+  a.batch = d->batch;
+  a.q_heads = d->q_heads;
+  a.heads = d->cache.heads;
+  a.dim = d->cache.dim;
+  a.pages = d->cache.pages;
+  a.groups = d->cache.page_size / 32;
+  a.columns = d->columns;
+  a.table_stride = d->table_stride;
+  a.max_new = max_new;
+  a.max_kv = (uint32_t)std::min<uint64_t>(d->max_kv, (uint64_t)d->columns * d->cache.page_size);
+  a.window = d->window;
+  a.scale = d->scale;
+  a.cap = d->softcap;
+  return Launched(ctx, hb::LaunchAttention(a, ctx->ws, ctx->stream), "attention launch", sync);
+}
+
+}  // namespace
+
+extern "C" {
+
+int hb_kv_plan(hb_ctx* ctx, const hb_kv_plan_desc* d) { return KvPlan(ctx, d, true); }
+int hb_kv_plan_async(hb_ctx* ctx, const hb_kv_plan_desc* d) { return KvPlan(ctx, d, false); }
+int hb_norm_rope(hb_ctx* ctx, const hb_norm_rope_desc* d) { return NormRope(ctx, d, true); }
+int hb_norm_rope_async(hb_ctx* ctx, const hb_norm_rope_desc* d) { return NormRope(ctx, d, false); }
+int hb_kv_append(hb_ctx* ctx, const hb_kv_rows_desc* d) { return KvRows(ctx, d, false, true); }
+int hb_kv_append_async(hb_ctx* ctx, const hb_kv_rows_desc* d) { return KvRows(ctx, d, false, false); }
+int hb_kv_read(hb_ctx* ctx, const hb_kv_rows_desc* d) { return KvRows(ctx, d, true, true); }
+int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* d) { return KvRows(ctx, d, true, false); }
+int hb_kv_attention(hb_ctx* ctx, const hb_kv_attention_desc* d) { return KvAttention(ctx, d, true); }
+int hb_kv_attention_async(hb_ctx* ctx, const hb_kv_attention_desc* d) {
+  return KvAttention(ctx, d, false);
+}
+
+}  // extern "C"
+
 // ---------------------------------------------------------- DDR images --
 
 extern "C" {

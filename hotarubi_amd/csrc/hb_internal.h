@@ -413,4 +413,53 @@ hipError_t LaunchVecRows(const VecRowArgs& a, uint8_t* abuf, uint32_t* fbuf, con
 hipError_t LaunchRowsDdr(const VecRowArgs& a, const VecRowDdr& d, const uint64_t* tbuf,
                          hipStream_t stream);
 
+// Serving operators (hb_kv.hip, hb_attn.hip) over the paged MXFP4 cache.
+struct PlanArgs {
+  const int32_t *lens, *new_tokens, *free_pages, *free_count;
+  int32_t *table, *cu, *kv_lens, *slots, *positions, *status;
+  uint32_t batch, columns, table_stride, page, size, free_size;
+};
+hipError_t LaunchPlan(const PlanArgs& a, hipStream_t stream);
+// Strides are elements, of a token's row and of a head.
+struct RopeArgs {
+  const void *q, *k;
+  void *q_out, *k_out;
+  uint64_t q_token, q_head, k_token, k_head, q_out_token, q_out_head, k_out_token, k_out_head;
+  const float *gamma_q, *gamma_k;  // null: not normalised
+  const int32_t* positions;        // [axes][position_stride]
+  uint64_t position_stride;
+  const double* inv_freq;          // [rot / 2]
+  float eps;
+  uint32_t type, tokens, q_heads, k_heads, dim, rot, neighbours;
+  uint32_t sections[2];            // where the second and third axis' pairs start
+  uint32_t lanes, parts;           // set by the launcher
+};
+hipError_t LaunchRope(const RopeArgs& a, hipStream_t stream);
+struct KvRowsArgs {
+  const void *k, *v;               // append
+  void *k_out, *v_out;             // read
+  uint64_t k_token, k_head, v_token, v_head;
+  const int32_t* slots;
+  uint8_t* cache;
+  uint32_t type, tokens, pages, heads, groups, dim;
+  uint32_t vec;                    // set by the launcher
+};
+// tokens * heads < 2^31
+hipError_t LaunchKvRows(const KvRowsArgs& a, bool read, hipStream_t stream);
+struct AttnArgs {
+  const void* q;
+  void* out;
+  uint64_t q_token, q_head, out_token, out_head;  // elements
+  const uint8_t* cache;
+  const int32_t *table, *cu, *kv_lens, *prefix;   // prefix may be null
+  uint32_t type, tokens, batch, q_heads, heads, dim, pages, groups, columns, table_stride;
+  uint32_t max_new, max_kv, window;
+  float scale, cap;                               // cap 0: scores as they are
+  // set by the launcher: tiles of rows of one (request, K/V head), splits of
+  // a tile's records, records of a split, and the partial results
+  uint32_t tiles, splits, split_records;
+  float* ws;
+};
+hipError_t LaunchAttention(const AttnArgs& a, Workspace& ws, hipStream_t stream);
+
 }  // namespace hb

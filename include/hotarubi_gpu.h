@@ -539,6 +539,166 @@ typedef struct hb_rows_desc {
 int hb_rows(hb_ctx* ctx, const hb_rows_desc* desc);
 int hb_rows_async(hb_ctx* ctx, const hb_rows_desc* desc);
 
+/* ------------------------------------------------ serving operators -- */
+
+/* Attention of a serving step over a paged cache held in MXFP4, and what
+ * feeds it (no counterpart in the reference, whose attention instructions run
+ * over one request's activations).  A step is
+ *   hb_kv_plan       block tables, slots and positions from request lengths
+ *   hb_norm_rope     norm of every query and key head and the rotation
+ *   hb_kv_append     the new tokens' K and V into the cache
+ *   hb_kv_attention  the new tokens' queries against their requests' keys
+ * on the context's stream; hb_kv_read gives stored values back.  Requests are
+ * ragged: the new tokens of request b are rows [cu[b], cu[b + 1]) of the
+ * step's token tensors, its last kv_lens[b] - (cu[b + 1] - cu[b]) keys and
+ * those behind them.
+ *
+ * The cache is uint8 [pages][heads][page_size / 32][34 dim], 16-byte aligned:
+ * a record per 32 tokens of one head holding K codes (16 dim bytes), V codes
+ * (16 dim), K scales (dim) and V scales (dim), elements E2M1 with an E8M0
+ * scale per token and 32 columns (255: NaN).  With g = 0..3, n, c = 0..15 and
+ * `chunk` counting 16-byte pieces:
+ *   K codes  [chunk dim/64][g][n][16 B]: (g, n) holds, in chunk order, columns
+ *            [g dim/4, (g + 1) dim/4) of token n and then of token 16 + n
+ *   V codes  [chunk dim/64][g][c][16 B]: (g, c) holds columns
+ *            [c dim/16, (c + 1) dim/16) of tokens 4g..4g+3, then 16+4g..16+4g+3
+ *   K scales [dim/32][n][2]: tokens n, 16 + n
+ *   V scales [dim/32][g][8]: tokens 4g..4g+3, 16+4g..16+4g+3
+ * Even columns are low nibbles.  A slot is page * page_size + the token's
+ * place in its page.  page_size is a multiple of 32, dim 64, 128 or 256.
+ *
+ * Tensor types of these operators. */
+typedef enum hb_type { HB_TYPE_F32 = 0, HB_TYPE_BF16 = 1, HB_TYPE_F16 = 2 } hb_type;
+
+/* The step plan.  lens[b] tokens of request b are cached (its table row holds
+ * their ceil(lens[b] / page_size) pages), new_tokens[b] are to come.  Pages
+ * for them are taken from the top of the stack free_pages[0 .. *free_count)
+ * in the order of the requests, and entered into the table.  A request is
+ * refused (its tokens get slot -1, its pages are not taken) if its pages pass
+ * the table's columns, its tokens `size`, or the pages wanted by it and the
+ * requests before it, whether they got them or not, the free ones.
+ *   table      int32 [batch][columns], rows table_stride elements apart;
+ *              entries of new pages are written, no others
+ *   cu         int32 [batch + 1]: 0 and the running sum of new_tokens
+ *   kv_lens    int32 [batch]: lens + new_tokens (lens where refused)
+ *   slots, positions  int32 [size]: of each new token; past the last -1
+ *   status     int32 [2]: pages taken, requests refused.  *free_count is left
+ *              as it is: the caller takes status[0] from it.
+ * Negative lengths count as 0.  Outputs share no memory with inputs, the
+ * table apart.  The sum of the new tokens is below 2^31; a slot of 2^31 or
+ * more is -1. */
+typedef struct hb_kv_plan_desc {
+  const int32_t* lens;
+  const int32_t* new_tokens;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* table;
+  int32_t* cu;
+  int32_t* kv_lens;
+  int32_t* slots;
+  int32_t* positions;
+  int32_t* status;
+  uint32_t batch, columns, table_stride, page_size, size, free_size;
+} hb_kv_plan_desc;
+int hb_kv_plan(hb_ctx* ctx, const hb_kv_plan_desc* desc);
+int hb_kv_plan_async(hb_ctx* ctx, const hb_kv_plan_desc* desc);
+
+/* Norm and rotation of every query and key head, one pass:
+ *   y = x * gamma / sqrt(mean(x^2) + eps) over the head's dim elements (as x
+ *   where gamma is null), then elements (a, b) of pair i < rot / 2 become
+ *   (a cos t - b sin t, b cos t + a sin t), t = position * inv_freq[i],
+ *   in 32 bits (t in 64), rounded once.  Pairs are (i, i + rot / 2), or
+ *   (2 i, 2 i + 1) with interleaved; elements from rot on are not turned.
+ *   axes       1 to 3 position axes: pairs [0, sections[0]) turn by the first
+ *              axis' position, the next sections[1] by the second's, ...; the
+ *              sections' sum is rot / 2
+ *   positions  int32 [axes][tokens], rows position_stride elements apart
+ *   inv_freq   float64 [rot / 2]
+ *   q, k       [tokens][heads][dim] of `type`, dim even up to 512; strides
+ *              of tokens and heads in elements, a head's elements are
+ *              neighbours.  q_out = q with q's strides (and k's) is allowed.
+ * k null: the query heads only. */
+typedef struct hb_norm_rope_desc {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  uint64_t q_token, q_head, k_token, k_head;
+  uint64_t q_out_token, q_out_head, k_out_token, k_out_head;
+  const float* gamma_q;
+  const float* gamma_k;
+  const int32_t* positions;
+  uint64_t position_stride;
+  const double* inv_freq;
+  float eps;
+  uint32_t type, tokens, q_heads, k_heads, dim, rot, interleaved, axes;
+  uint32_t sections[3];
+} hb_norm_rope_desc;
+int hb_norm_rope(hb_ctx* ctx, const hb_norm_rope_desc* desc);
+int hb_norm_rope_async(hb_ctx* ctx, const hb_norm_rope_desc* desc);
+
+/* The paged cache as the calls take it. */
+typedef struct hb_kv_cache {
+  void* base;
+  uint32_t pages, heads, page_size, dim;
+} hb_kv_cache;
+
+/* K and V rows [tokens][heads][dim] of `type` into the cache at int32
+ * slots[token], and the stored values of slots back out.  Encoding: per 32
+ * columns the exponent floor(log2 max|x|) - 2 within [-126, 125] (0 for
+ * zeros), elements rounded to nearest even on the E2M1 grid and saturated at
+ * 6.  A token's head with an infinity or NaN in K or V is stored as NaN keys
+ * (scale bytes 255) and zero values.  A slot below 0 or past the cache's
+ * pages is not written, and reads as zeros.  Slots written by one call differ
+ * from each other.  tokens * heads is below 2^31.  Strides in elements. */
+typedef struct hb_kv_rows_desc {
+  hb_kv_cache cache;
+  void* k;  /* hb_kv_append reads k and v, hb_kv_read writes them */
+  void* v;
+  uint64_t k_token, k_head, v_token, v_head;
+  const int32_t* slots;
+  uint32_t type, tokens;
+} hb_kv_rows_desc;
+int hb_kv_append(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+int hb_kv_append_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+int hb_kv_read(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+
+/* Attention of ragged requests over the cache.  Row i of request b, of
+ * n = cu[b + 1] - cu[b], is at position p = kv_lens[b] - n + i and sees key j
+ * (j < kv_lens[b]) if
+ *   j <= p and (window == 0 or p - j < window), or j < prefix[b];
+ * query head h reads K/V head h / (q_heads / heads).  Scores are
+ * scale * q.k, softcap * tanh(scale * q.k / softcap) where softcap > 0;
+ *   out = sum_j softmax(scores)_j v_j, 0 for a row that sees no key.
+ * q and out are [tokens][q_heads][dim] of `type`, strides in elements.  Scores,
+ * maxima and sums are in 32 bits.  bf16 q enters the products as it is and the
+ * softmax's weights rounded to bf16; fp16 and fp32 enter as two and three
+ * bf16 parts (fp32 weights to 2^-24, fp16 ones to 2^-16 of their value).
+ * Rows outside every request are not written.  max_new and max_kv bound the
+ * requests' new tokens and keys; they choose the split of the work, and rows
+ * of a request past max_new are not computed.  A block table entry that names
+ * no page of the cache hides its keys.  A stored NaN (a scale of 255) makes
+ * the rows that see its token NaN, no others.
+ * Long caches are split over workgroups that meet in the context's workspace,
+ * in a fixed order: results do not change from call to call.  A larger split
+ * than before grows the workspace, so a first call belongs before a capture. */
+typedef struct hb_kv_attention_desc {
+  hb_kv_cache cache;
+  const void* q;
+  void* out;
+  uint64_t q_token, q_head, out_token, out_head;
+  const int32_t* table;
+  const int32_t* cu;
+  const int32_t* kv_lens;
+  const int32_t* prefix; /* null: none */
+  uint32_t type, tokens, q_heads, batch, columns, table_stride;
+  uint32_t max_new, max_kv, window;
+  float scale, softcap; /* softcap 0: none */
+} hb_kv_attention_desc;
+int hb_kv_attention(hb_ctx* ctx, const hb_kv_attention_desc* desc);
+int hb_kv_attention_async(hb_ctx* ctx, const hb_kv_attention_desc* desc);
+
 /* --------------------------------------------------------- formats -- */
 
 /* EncodeMxint8 + PackAbuf on device: x fp32 row-major [rows][cols] ->
