@@ -8,19 +8,24 @@
 // the same registers, with no trip through LDS; the record's layout gives the
 // lane its K and V codes for both products as they lie.
 #include <algorithm>
+#include <cmath>
 
 #include "hb_internal.h"
 #include "hb_kv.h"
+#include "hb_ring.h"
 
 namespace hb {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 template <uint32_t parts>
 struct TypeOf;  // the tensors' type by the bf16 parts that hold its values exactly
@@ -44,7 +49,7 @@ constexpr uint32_t kWaves = 4, kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 // A row's maximum moves once a score passes it by this much (in powers of
 // two): between moves P is at most 2^8, and nothing is rescaled.
-constexpr float kSlack = 8.f;
+constexpr float kSlack = 8.f, kLift = 7.f;
 
 // ---------------------------------------------------------------- records --
 
@@ -55,20 +60,43 @@ struct Record {
   uint32_t vs[2];                 // scale bytes of the lane's 8 tokens
 };
 
+// Records go from memory into LDS by direct loads, kDepth of them under way or
+// waiting per wave (a ring of its own, no barrier): what a CU needs in flight
+// to draw its share of HBM is 40 KB or more, which registers do not hold.
 template <uint32_t D>
-__device__ __forceinline__ void LoadRecord(const uint8_t* base, Record<D>& r) {
+struct Ring {
+  static constexpr uint32_t kSlot = D == 64 ? 2304 : 34 * D;  // whole loads
+  static constexpr uint32_t kOps = D / 32 + (D == 256 ? 2 : 1);
+  static constexpr uint32_t kDepth = D == 64 ? 7 : D == 128 ? 4 : 2;
+};
+template <uint32_t D>
+__device__ __forceinline__ void FetchRecord(const uint8_t* base, uint32_t lds) {
+  const uint32_t lane = threadIdx.x % 64;
+#pragma unroll
+  for (uint32_t c = 0; c < D / 32; ++c) ring::Dma16(base + c * 1024, lane * 16, lds + c * 1024);
+  // 2 D bytes of scales; the upper lanes repeat the lower ones' where that is
+  // half a load
+  ring::Dma4(base + 32 * D, (D == 64 ? lane % 32 : lane) * 4, lds + 32 * D);
+  if (D == 256) ring::Dma4(base + 32 * D + 256, lane * 4, lds + 32 * D + 256);
+}
+template <uint32_t D>
+__device__ __forceinline__ void ReadKeys(const uint8_t* slot, Record<D>& r) {
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
 #pragma unroll
-  for (uint32_t c = 0; c < D / 64; ++c) {
-    r.k[c] = *reinterpret_cast<const u32x4*>(base + c * 1024 + lane * 16);
-    r.v[c] = *reinterpret_cast<const u32x4*>(base + 16 * D + c * 1024 + lane * 16);
-  }
+  for (uint32_t c = 0; c < D / 64; ++c)
+    r.k[c] = *reinterpret_cast<const u32x4*>(slot + c * 1024 + lane * 16);
   const uint32_t block = D == 256 ? 2 * g : g * D / 128;
-  r.ks[0] = *reinterpret_cast<const uint16_t*>(base + 32 * D + block * 32 + n * 2);
+  r.ks[0] = *reinterpret_cast<const uint16_t*>(slot + 32 * D + block * 32 + n * 2);
   if (D == 256)
-    r.ks[D == 256] = *reinterpret_cast<const uint16_t*>(base + 32 * D + block * 32 + 32 + n * 2);
-  const uint2 vs =
-      *reinterpret_cast<const uint2*>(base + 33 * D + n * D / 512 * 32 + g * 8);
+    r.ks[D == 256] = *reinterpret_cast<const uint16_t*>(slot + 32 * D + block * 32 + 32 + n * 2);
+}
+template <uint32_t D>
+__device__ __forceinline__ void ReadValues(const uint8_t* slot, Record<D>& r) {
+  const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
+#pragma unroll
+  for (uint32_t c = 0; c < D / 64; ++c)
+    r.v[c] = *reinterpret_cast<const u32x4*>(slot + 16 * D + c * 1024 + lane * 16);
+  const uint2 vs = *reinterpret_cast<const uint2*>(slot + 33 * D + n * D / 512 * 32 + g * 8);
   r.vs[0] = vs.x;
   r.vs[1] = vs.y;
 }
@@ -83,15 +111,6 @@ __device__ __forceinline__ uint32_t Two(uint32_t word, float scale) {
   return __builtin_bit_cast(uint32_t,
                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, sel));
 }
-__device__ __forceinline__ uint32_t TwoOf(uint32_t word, float scale, uint32_t sel) {
-  switch (sel) {  // the instruction's byte is an immediate: folded where sel is known
-    case 0: return Two<0>(word, scale);
-    case 1: return Two<1>(word, scale);
-    case 2: return Two<2>(word, scale);
-    default: return Two<3>(word, scale);
-  }
-}
-
 // Operand of K: tokens 16 tile + n, the lane's columns 8 s .. 8 s + 7.
 template <uint32_t D>
 __device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, uint32_t s) {
@@ -106,17 +125,57 @@ __device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, 
   return __builtin_bit_cast(bf16x8, x);
 }
 
+// P V in f16 for the 16-bit types: P's error is then below the output's
+// rounding (2^-12 of each weight against bf16's 2^-9), and V is exact in f16
+// wherever its scale bytes lie in [104, 140] (0.5 x 2^-23 .. 6 x 2^13).  Other
+// records take V in bf16 and each f16 weight as two bf16 parts.  fp32 takes three bf16 parts of P.
+template <bool half>
+struct Value;
+template <>
+struct Value<true> {
+  typedef f16x8 type;
+};
+template <>
+struct Value<false> {
+  typedef bf16x8 type;
+};
+// Nonzero where one of the 4 bytes lies outside [104, 140].
+__device__ __forceinline__ uint32_t OutsideHalf(uint32_t x) {
+  const uint32_t low = x & 0x7F7F7F7Fu;
+  return (((low + 0x73737373u) & x) | ~((low + 0x18181818u) | x)) & 0x80808080u;
+}
+
+template <int sel, bool half>
+__device__ __forceinline__ uint32_t TwoAs(uint32_t word, float scale) {
+  if constexpr (half)
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, sel));
+  else
+    return Two<sel>(word, scale);
+}
+template <bool half>
+__device__ __forceinline__ uint32_t TwoOf(uint32_t word, float scale, uint32_t sel) {
+  switch (sel) {  // the instruction's byte is an immediate: folded where sel is known
+    case 0: return TwoAs<0, half>(word, scale);
+    case 1: return TwoAs<1, half>(word, scale);
+    case 2: return TwoAs<2, half>(word, scale);
+    default: return TwoAs<3, half>(word, scale);
+  }
+}
+
 // Operands of V^T for the lane's columns 2 i and 2 i + 1 (rows c of column
 // tiles 2 i and 2 i + 1) over the record's 32 tokens.  A byte holds two columns
 // of one token, so two conversions meet in two byte permutes.
-template <uint32_t D>
-__device__ __forceinline__ void ValueOperands(const Record<D>& r, uint32_t i, bf16x8* even,
-                                              bf16x8* odd) {
+template <uint32_t D, bool half>
+__device__ __forceinline__ void ValueOperands(const Record<D>& r, uint32_t i,
+                                              typename Value<half>::type* even,
+                                              typename Value<half>::type* odd) {
+  typedef typename Value<half>::type V;
   uint32_t x[8];
 #pragma unroll
   for (uint32_t j = 0; j < 8; ++j) {
     const uint32_t byte = j * (D / 32) + i;
-    x[j] = TwoOf(r.v[byte / 16][byte / 4 % 4], ScaleOf(r.vs[j / 4], j % 4), byte % 4);
+    x[j] = TwoOf<half>(r.v[byte / 16][byte / 4 % 4], ScaleOf(r.vs[j / 4], j % 4), byte % 4);
   }
   u32x4 lo, hi;
 #pragma unroll
@@ -124,8 +183,14 @@ __device__ __forceinline__ void ValueOperands(const Record<D>& r, uint32_t i, bf
     lo[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
     hi[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
   }
-  *even = __builtin_bit_cast(bf16x8, lo);
-  *odd = __builtin_bit_cast(bf16x8, hi);
+  *even = __builtin_bit_cast(V, lo);
+  *odd = __builtin_bit_cast(V, hi);
+}
+__device__ __forceinline__ f32x4 Product(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 Product(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // fp32 values as bf16 parts: one part rounds to nearest; two or three cut 8
@@ -200,6 +265,8 @@ __device__ __forceinline__ void LoadQuery(const AttnArgs& a, uint64_t at, bool v
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = (float)x[j];
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] *= a.sign;
   ToParts<parts>(y, out);
 }
 
@@ -229,12 +296,10 @@ struct Rows {
   int32_t see_all, see_from, see_pre;  // every row sees keys see_from .. see_all, and < see_pre
 };
 
-// One record: scores, their running maximum and sum, and P V.
+// One record: the products of its keys ...
 template <uint32_t parts, uint32_t D, uint32_t R>
-__device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<D>& r,
-                                     int32_t key0, Rows<parts, D, R>& w) {
-  const uint32_t g = threadIdx.x % 64 / 16;
-  f32x4 s[R][2];
+__device__ __forceinline__ void Scores(const Record<D>& r, const Rows<parts, D, R>& w,
+                                       f32x4 (&s)[R][2]) {
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -246,51 +311,57 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
       for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
         for (uint32_t p = parts; p-- > 0;)
-          s[t][tile] =
-              __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, w.q[t][p][i], s[t][tile], 0, 0, 0);
+          s[t][tile] = Product(k, w.q[t][p][i], s[t][tile]);
     }
   }
-  float y[R][8];
+}
+
+// ... and the scores' running maximum and sum, and P V.
+template <uint32_t parts, uint32_t D, uint32_t R>
+__device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<D>& r,
+                                     int32_t key0, f32x4 (&s)[R][2], Rows<parts, D, R>& w) {
+  const uint32_t g = threadIdx.x % 64 / 16;
+  float c = a.scale * kLog2e;  // scores in powers of two: s c
+  if (a.cap > 0.f) {           // cap tanh(s scale / cap)
 #pragma unroll
-  for (uint32_t t = 0; t < R; ++t)
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      float x = s[t][j / 4][j % 4] * a.scale;
-      if (a.cap > 0.f) {
-        // cap tanh(x / cap)
-        if constexpr (parts == 3) {
-          x = a.cap * tanhf(x / a.cap);
-        } else {
-          const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e / a.cap));
-          x = a.cap * fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
-        }
-      }
-      y[t][j] = x * kLog2e;
-    }
-  // Scale bytes of 252 and above: a token whose V has a scale of NaN gives NaN
-  // scores to the rows that see it and nothing to others (0 x NaN would reach
-  // every row of the tile); past the request's end any byte may lie.
-  {
-    const uint32_t t0 = ~r.vs[0] & 0xFCFCFCFCu, t1 = ~r.vs[1] & 0xFCFCFCFCu;
-    const uint32_t odd = (((t0 - 0x01010101u) & ~t0) | ((t1 - 0x01010101u) & ~t1)) & 0x80808080u;
-    if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
-      uint32_t nan = 0;
+    for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) {
-        const uint32_t byte = (r.vs[j / 4] >> (8 * (j % 4))) & 255u;
-        const int32_t key = key0 + (int32_t)(j / 4 * 16 + 4 * g + j % 4);
-        nan |= (uint32_t)(byte == 255u) << j;
-        if (byte == 255u || key >= span.total)
-          r.vs[j / 4] = (r.vs[j / 4] & ~(255u << (8 * (j % 4)))) | 127u << (8 * (j % 4));
+        float x = s[t][j / 4][j % 4];
+        if constexpr (parts == 3) {
+          x = a.cap * kLog2e * tanhf(x * a.scale / a.cap);
+        } else {
+          const float e = __builtin_amdgcn_exp2f(x * (2.f * c / a.cap));
+          x = a.cap * kLog2e * fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+        }
+        s[t][j / 4][j % 4] = x;
       }
+    c = 1.f;
+  }
+  // Unusual scale bytes of V: a token whose V has a scale of NaN gives NaN
+  // scores to the rows that see it and nothing to others (0 x NaN would reach
+  // every row of the tile); past the request's end any byte may lie.
+  constexpr bool half = parts < 3;
+  bool wide = false;
+  if (__builtin_amdgcn_ballot_w64((OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1])) != 0) != 0) {
+    uint32_t nan = 0;
 #pragma unroll
-      for (uint32_t d = 1; d < 16; d *= 2) nan |= __shfl_xor(nan, d);
-#pragma unroll
-      for (uint32_t t = 0; t < R; ++t)
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-          if (nan >> j & 1) y[t][j] = __builtin_nanf("");
+    for (uint32_t j = 0; j < 8; ++j) {
+      const uint32_t byte = (r.vs[j / 4] >> (8 * (j % 4))) & 255u;
+      const int32_t key = key0 + (int32_t)(j / 4 * 16 + 4 * g + j % 4);
+      nan |= (uint32_t)(byte == 255u) << j;
+      if (byte == 255u || key >= span.total)
+        r.vs[j / 4] = (r.vs[j / 4] & ~(255u << (8 * (j % 4)))) | 127u << (8 * (j % 4));
     }
+#pragma unroll
+    for (uint32_t d = 1; d < 16; d *= 2) nan |= __shfl_xor(nan, d);
+#pragma unroll
+    for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j)
+        if (nan >> j & 1) s[t][j / 4][j % 4] = __builtin_nanf("");
+    wide = half && __builtin_amdgcn_ballot_w64(
+                       (OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1])) != 0) != 0;
   }
   const bool full = (key0 >= w.see_from && key0 + 31 <= w.see_all) || key0 + 32 <= w.see_pre;
   if (!full) {
@@ -301,14 +372,16 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
         const int32_t key = key0 + (int32_t)(j / 4 * 16 + 4 * g + j % 4);
         const Sight& v = w.see[t];
         const bool sees = (key >= v.lo && key <= v.hi) || key < v.pre;
-        y[t][j] = sees ? y[t][j] : -__builtin_inff();
+        s[t][j / 4][j % 4] = sees ? s[t][j / 4][j % 4] : -__builtin_inff();
       }
   }
-  bf16x8 pt[R][parts];
+  typename Value<half>::type pt[R][half ? 1 : parts];
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
-    float top = fmaxf(fmaxf(fmaxf(y[t][0], y[t][1]), fmaxf(y[t][2], y[t][3])),
-                      fmaxf(fmaxf(y[t][4], y[t][5]), fmaxf(y[t][6], y[t][7])));
+    const f32x4 x = s[t][0], y = s[t][1];
+    const float top = c * fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
     if (__builtin_amdgcn_ballot_w64(top > w.m[t] + kSlack) != 0) {
       const float m = fmaxf(w.m[t], RowMax(top));
       // rows that have seen nothing yet stay at -inf, with o and l zero
@@ -316,41 +389,71 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
       w.m[t] = m;
       w.l[t] *= shrink;
 #pragma unroll
-      for (uint32_t c = 0; c < D / 16; ++c) w.o[t][c] *= shrink;
+      for (uint32_t i = 0; i < D / 16; ++i) w.o[t][i] *= shrink;
     }
-    const float m = w.m[t] == -__builtin_inff() ? 0.f : w.m[t];
+    // weights carry 2^kLift: at most 2^15, and as small as 2^-31 of the
+    // maximum before f16 goes subnormal
+    const float ref = (w.m[t] == -__builtin_inff() ? 0.f : w.m[t]) - kLift;
     float p[8], sum = 0.f;
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(y[t][j] - m);
+      p[j] = __builtin_amdgcn_exp2f(fmaf(j < 4 ? x[j % 4] : y[j % 4], c, -ref));
       sum += p[j];
     }
     w.l[t] += sum;
-    ToParts<parts>(p, pt[t]);
+    if constexpr (half) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const f16x2 two = __builtin_convertvector(f32x2{p[j], p[j + 1]}, f16x2);
+        pt[t][0][j] = two[0];
+        pt[t][0][j + 1] = two[1];
+      }
+    } else {
+      ToParts<parts>(p, pt[t]);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (half) {
+    if (wide) {  // V in bf16, on the two bf16 parts of an f16 weight
+#pragma unroll
+      for (uint32_t t = 0; t < R; ++t) {
+        float p[8];
+        bf16x8 part[2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = (float)pt[t][0][j];
+        ToParts<2>(p, part);
+#pragma unroll
+        for (uint32_t i = 0; i < D / 32; ++i) {
+          bf16x8 v[2];
+          ValueOperands<D, false>(r, i, &v[0], &v[1]);
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) {
+            w.o[t][2 * i + h] = Product(v[h], part[1], w.o[t][2 * i + h]);
+            w.o[t][2 * i + h] = Product(v[h], part[0], w.o[t][2 * i + h]);
+          }
+        }
+      }
+      return;
+    }
   }
 #pragma unroll
   for (uint32_t i = 0; i < D / 32; ++i) {
-    bf16x8 v[2];
-    ValueOperands<D>(r, i, &v[0], &v[1]);
+    typename Value<half>::type v[2];
+    ValueOperands<D, half>(r, i, &v[0], &v[1]);
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
-        for (uint32_t p = parts; p-- > 0;)
-          w.o[t][2 * i + h] =
-              __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[h], pt[t][p], w.o[t][2 * i + h], 0, 0, 0);
+        for (uint32_t p = half ? 1 : parts; p-- > 0;)
+          w.o[t][2 * i + h] = Product(v[h], pt[t][p], w.o[t][2 * i + h]);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 constexpr uint32_t kNoRecord = 0xFFFFFFFFu;
 
-// The records of a wave, `step` apart: 64 block table entries at a time, one a
-// lane.
-struct Pages {
-  const int32_t* row;
-  uint32_t mine;  // this lane's record of the present 64
-};
+// The record a wave's lane takes in its turn i.
 __device__ __forceinline__ uint32_t PageRecord(const AttnArgs& a, const KvWalk& walk,
                                                const int32_t* row, uint32_t head, uint32_t i,
                                                uint32_t end) {
@@ -366,11 +469,19 @@ __device__ __forceinline__ uint32_t PageRecord(const AttnArgs& a, const KvWalk& 
 template <uint32_t D>
 constexpr uint32_t kPartial = D + 4;
 
+// The waves' results of a workgroup, in LDS.
+template <uint32_t D, uint32_t R>
+struct Merge {
+  float o[kWaves][R * 16][D + 4], m[kWaves][R * 16], l[kWaves][R * 16];
+};
+
 // split: the workgroup's waves share R tiles of 16 rows and take its records
 // in turn; else each wave has R tiles of its own and takes every record.
 template <uint32_t parts, uint32_t D, uint32_t R, bool split>
-__global__ __launch_bounds__(kThreads) void AttnKernel(const AttnArgs a) {
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = lane % 16, g = lane / 16;
+// two workgroups a CU (their rings fill its LDS), so 256 registers a wave
+__global__ __launch_bounds__(kThreads, 2) void AttnKernel(const AttnArgs a) {
+  const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t unit = blockIdx.x / a.splits, part = blockIdx.x % a.splits;
   const uint32_t head = unit % a.heads, rest = unit / a.heads;
   const uint32_t b = rest / a.tiles, tile = a.tiles - 1 - rest % a.tiles;
@@ -418,26 +529,58 @@ __global__ __launch_bounds__(kThreads) void AttnKernel(const AttnArgs a) {
   const int32_t* const row = a.table + (uint64_t)b * a.table_stride;
   const uint32_t step = split ? kWaves : 1, first = begin + (split ? wave : 0);
   const uint32_t count = first < end ? (end - first + step - 1) / step : 0;
-  for (uint32_t i0 = 0; i0 < count; i0 += 64) {
-    const uint32_t mine = PageRecord(a, walk, row, head, first + (i0 + lane) * step, end);
-    const uint32_t chunk = min(64u, count - i0);
-    Record<D> r[2];
-    uint32_t at[2];
-    auto load = [&](uint32_t i, uint32_t slot) {
-      at[slot] = i < chunk ? (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)i) : kNoRecord;
-      if (at[slot] != kNoRecord)
-        LoadRecord<D>(a.cache + (uint64_t)at[slot] * KvRecordBytes(D), r[slot]);
-    };
-    load(0, 0);
-    load(1, 1);
-    for (uint32_t i = 0; i < chunk; i += 2) {
+  typedef Ring<D> Ring;
+  constexpr uint32_t kRing = kWaves * Ring::kDepth * Ring::kSlot;
+  constexpr uint32_t kMerge = split ? sizeof(Merge<D, R>) : 0;
+  __shared__ __align__(16) uint8_t lds[kRing > kMerge ? kRing : kMerge];
+  uint8_t* const slots = lds + wave * (Ring::kDepth * Ring::kSlot);
+  const uint32_t slots_at =
+      (uint32_t) reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)slots);
+  // block table entries of 64 records at a time, one a lane; the ring reaches
+  // into the next 64
+  auto pages = [&](uint32_t i) {
+    return PageRecord(a, walk, row, head, first + (i + lane) * step, end);
+  };
+  uint32_t now = pages(0), after = count > 64 ? pages(64) : kNoRecord;
+  uint32_t read_at[Ring::kDepth];
+  auto fetch = [&](uint32_t i, uint32_t base, uint32_t slot) {  // base <= i < base + 128
+    const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(
+        (int)(i - base < 64 ? now : after), (int)((i - base) % 64));
+    read_at[slot] = from;
+    FetchRecord<D>(a.cache + (from == kNoRecord ? 0 : (uint64_t)from * KvRecordBytes(D)),
+                   slots_at + slot * Ring::kSlot);
+  };
+  asm volatile("" ::: "memory");
 #pragma unroll
-      for (uint32_t u = 0; u < 2; ++u) {
-        if (at[u] != kNoRecord) {
-          const int32_t key0 = (int32_t)(32 * KvWalkRecord(walk, first + (i0 + i + u) * step));
-          Step<parts, D, R>(a, span, r[u], key0, w);
+  for (uint32_t u = 0; u < Ring::kDepth; ++u)
+    if (u < count) fetch(u, 0, u);
+  for (uint32_t i0 = 0, base = 0; i0 < count; i0 += Ring::kDepth) {
+#pragma unroll
+    for (uint32_t u = 0; u < Ring::kDepth; ++u) {
+      const uint32_t i = i0 + u;
+      if (i >= count) break;
+      if (i + Ring::kDepth <= count) ring::WaitVm<(Ring::kDepth - 1) * Ring::kOps>();
+      else ring::WaitVm<0>();
+      asm volatile("" ::: "memory");
+      const bool present = read_at[u] != kNoRecord;
+      Record<D> r;
+      f32x4 s[R][2];
+      ReadKeys<D>(slots + u * Ring::kSlot, r);
+      ReadValues<D>(slots + u * Ring::kSlot, r);
+      ring::WaitLds();  // the slot has been read
+      asm volatile("" ::: "memory");
+      if (i + Ring::kDepth < count) {
+        if (i + Ring::kDepth - base >= 128) {
+          base += 64;
+          now = after;
+          after = pages(base + 64);
         }
-        load(i + u + 2, u);
+        fetch(i + Ring::kDepth, base, u);
+      }
+      if (present) {
+        Scores<parts, D, R>(r, w, s);
+        const int32_t key0 = (int32_t)(32 * KvWalkRecord(walk, first + i * step));
+        Step<parts, D, R>(a, span, r, key0, s, w);
       }
     }
   }
@@ -465,9 +608,11 @@ __global__ __launch_bounds__(kThreads) void AttnKernel(const AttnArgs a) {
     }
   } else {
     // the waves' sums meet in LDS, in the waves' order
-    constexpr uint32_t kPad = D + 4;
-    __shared__ float so[kWaves][R * 16][kPad];
-    __shared__ float sm[kWaves][R * 16], sl[kWaves][R * 16];
+    Merge<D, R>& sum = *reinterpret_cast<Merge<D, R>*>(lds);
+    auto& so = sum.o;
+    auto& sm = sum.m;
+    auto& sl = sum.l;
+    __syncthreads();  // every ring has been read
 #pragma unroll
     for (uint32_t t = 0; t < R; ++t) {
 #pragma unroll
@@ -600,7 +745,7 @@ hipError_t LaunchOf(AttnArgs& a, Workspace& ws, hipStream_t stream) {
   if (a.window > 0 && a.prefix == nullptr)
     records = std::min<uint64_t>(records, ((uint64_t)a.window + 16 * R + 62) / 32);
   records = std::max<uint64_t>(records, 1);
-  const uint64_t want = std::max<uint64_t>(1, 8 * cus / units);
+  const uint64_t want = std::max<uint64_t>(1, 2 * cus / units);
   const uint64_t most = std::max<uint64_t>(1, records / (2 * kWaves));
   uint64_t splits = std::min(want, most);
   a.split_records = (uint32_t)((records + splits - 1) / splits);
@@ -635,6 +780,10 @@ hipError_t LaunchDim(AttnArgs& a, Workspace& ws, hipStream_t stream) {
 
 hipError_t LaunchAttention(const AttnArgs& in, Workspace& ws, hipStream_t stream) {
   AttnArgs a = in;
+  // scores as |scale| (q sign): the maximum of the products is then that of
+  // the scores
+  a.sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;
+  a.scale = a.scale == 0.f ? 1.f : std::abs(a.scale);
   switch (a.type) {
     case HB_TYPE_BF16: return LaunchDim<1>(a, ws, stream);
     case HB_TYPE_F16: return LaunchDim<2>(a, ws, stream);

@@ -458,6 +458,7 @@ struct AttnArgs {
   // set by the launcher: tiles of rows of one (request, K/V head), splits of
   // a tile's records, records of a split, and the partial results
   uint32_t tiles, splits, split_records;
+  float sign;  // of scale, which is positive then
   float* ws;
 };
 hipError_t LaunchAttention(const AttnArgs& a, Workspace& ws, hipStream_t stream);

@@ -44,6 +44,12 @@ __device__ __forceinline__ void Dma16(const uint8_t* base, uint32_t voff, uint32
                :: "v"(voff), "s"(UniformAddress(base)), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "memory");
 }
+// The same with 4 bytes a lane.
+__device__ __forceinline__ void Dma4(const uint8_t* base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+               :: "v"(voff), "s"(UniformAddress(base)), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
 
 // Wait until at most kN of this wave's vector memory operations are
 // outstanding (s_waitcnt vmcnt(kN), the other counters left alone).
