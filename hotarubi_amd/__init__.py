@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass, fields
 
 import numpy as np
@@ -121,46 +122,6 @@ class _LinearDesc(C.Structure):
                 ("pieces", _Piece * MAX_PIECES), ("onto", C.c_uint32), ("c", C.c_void_p),
                 ("n_ops", C.c_uint32), ("ops", _EpOp * MAX_OPS), ("tbuf", C.c_void_p),
                 ("q_out", C.c_void_p), ("flags", C.c_uint32), ("a_stride", C.c_uint32)]
-
-
-class _KvPlanDesc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in
-                ("lens", "new_tokens", "free_pages", "free_count", "table", "cu", "kv_lens",
-                 "slots", "positions", "status")] + \
-               [(n, C.c_uint32) for n in
-                ("batch", "columns", "table_stride", "page_size", "size", "free_size")]
-
-
-class _NormRopeDesc(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out")] + \
-               [(n, C.c_uint64) for n in
-                ("q_token", "q_head", "k_token", "k_head", "q_out_token", "q_out_head",
-                 "k_out_token", "k_out_head")] + \
-               [("gamma_q", C.c_void_p), ("gamma_k", C.c_void_p), ("positions", C.c_void_p),
-                ("position_stride", C.c_uint64), ("inv_freq", C.c_void_p), ("eps", C.c_float)] + \
-               [(n, C.c_uint32) for n in
-                ("type", "tokens", "q_heads", "k_heads", "dim", "rot", "interleaved", "axes")] + \
-               [("sections", C.c_uint32 * 3)]
-
-
-class _KvCache(C.Structure):
-    _fields_ = [("base", C.c_void_p), ("pages", C.c_uint32), ("heads", C.c_uint32),
-                ("page_size", C.c_uint32), ("dim", C.c_uint32)]
-
-
-class _KvRowsDesc(C.Structure):
-    _fields_ = [("cache", _KvCache), ("k", C.c_void_p), ("v", C.c_void_p)] + \
-               [(n, C.c_uint64) for n in ("k_token", "k_head", "v_token", "v_head")] + \
-               [("slots", C.c_void_p), ("type", C.c_uint32), ("tokens", C.c_uint32)]
-
-
-class _KvAttentionDesc(C.Structure):
-    _fields_ = [("cache", _KvCache), ("q", C.c_void_p), ("out", C.c_void_p)] + \
-               [(n, C.c_uint64) for n in ("q_token", "q_head", "out_token", "out_head")] + \
-               [(n, C.c_void_p) for n in ("table", "cu", "kv_lens", "prefix")] + \
-               [(n, C.c_uint32) for n in
-                ("type", "tokens", "q_heads", "batch", "columns", "table_stride", "max_new",
-                 "max_kv", "window")] + [("scale", C.c_float), ("softcap", C.c_float)]
 
 
 @dataclass
@@ -274,16 +235,16 @@ def lib():
                                        C.POINTER(C.c_uint64)]),
             "hb_image_end": (C.c_uint64, [vp]),
             "hb_image_base": (vp, [vp]),
-            "hb_kv_plan": (i, [vp, C.POINTER(_KvPlanDesc)]),
-            "hb_kv_plan_async": (i, [vp, C.POINTER(_KvPlanDesc)]),
-            "hb_norm_rope": (i, [vp, C.POINTER(_NormRopeDesc)]),
-            "hb_norm_rope_async": (i, [vp, C.POINTER(_NormRopeDesc)]),
-            "hb_kv_append": (i, [vp, C.POINTER(_KvRowsDesc)]),
-            "hb_kv_append_async": (i, [vp, C.POINTER(_KvRowsDesc)]),
-            "hb_kv_read": (i, [vp, C.POINTER(_KvRowsDesc)]),
-            "hb_kv_read_async": (i, [vp, C.POINTER(_KvRowsDesc)]),
-            "hb_kv_attention": (i, [vp, C.POINTER(_KvAttentionDesc)]),
-            "hb_kv_attention_async": (i, [vp, C.POINTER(_KvAttentionDesc)]),
+            "hb_kv_plan": (i, [vp, vp]),
+            "hb_kv_plan_async": (i, [vp, vp]),
+            "hb_norm_rope": (i, [vp, vp]),
+            "hb_norm_rope_async": (i, [vp, vp]),
+            "hb_kv_append": (i, [vp, vp]),
+            "hb_kv_append_async": (i, [vp, vp]),
+            "hb_kv_read": (i, [vp, vp]),
+            "hb_kv_read_async": (i, [vp, vp]),
+            "hb_kv_attention": (i, [vp, vp]),
+            "hb_kv_attention_async": (i, [vp, vp]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -750,19 +711,25 @@ def encode_mxfp8(x, rows: int, cols: int, out, ctx: Context | None = None) -> No
 
 
 # ---------------------------------------------------- serving operators --
-# These take torch tensors: sizes, types and strides come from them.
+# These take torch tensors: sizes, types and strides come from them.  Steps of
+# few tokens wait for the host, so the descriptors are packed in one go, and
+# the checks read each property of a tensor once.
 
 HB_TYPE_F32, HB_TYPE_BF16, HB_TYPE_F16 = range(3)
-_types = None  # torch.dtype -> hb_type, and the other types the checks name
+#: the descriptors of include/hotarubi_gpu.h, field for field
+KV_PLAN_DESC = struct.Struct("@10P6I")
+NORM_ROPE_DESC = struct.Struct("@4P8Q3PQPf8I3I")
+KV_ROWS_DESC = struct.Struct("@P4I2P4QP2I")
+KV_ATTENTION_DESC = struct.Struct("@P4I2P4Q4P9I2f")
+_types = None  # (torch.dtype -> hb_type, int32, uint8, float64, float32)
 
 
 def _torch_types():
     global _types
-    if _types is None:
-        import torch
-        _types = ({torch.float32: HB_TYPE_F32, torch.bfloat16: HB_TYPE_BF16,
-                   torch.float16: HB_TYPE_F16}, torch.int32, torch.uint8, torch.float64,
-                  torch.float32)
+    import torch
+    _types = ({torch.float32: HB_TYPE_F32, torch.bfloat16: HB_TYPE_BF16,
+               torch.float16: HB_TYPE_F16}, torch.int32, torch.uint8, torch.float64,
+              torch.float32)
     return _types
 
 
@@ -770,58 +737,70 @@ def _invalid(message: str):
     return HbError(HB_EINVAL, message)
 
 
-def _on(t, device: int, name: str) -> int:
-    """Address of a tensor on the context's device."""
-    if t.get_device() != device:
-        raise _invalid(f"{name} is on {t.device}, the context on cuda:{device}")
+def _vector(t, dtype, name: str, count: int, device: int) -> int:
+    """Address of a contiguous vector of `count` elements (-1: any)."""
+    if t.dtype is not dtype or t.stride() != (1,) or t.get_device() != device or \
+            (t.shape[0] != count and count >= 0):
+        if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous() or \
+                (t.shape[0] != count and count >= 0):
+            raise _invalid(f"{name} must be {'n' if count < 0 else count} contiguous {dtype} "
+                           f"elements, not {tuple(t.shape)} of {t.dtype}")
+        _place(t, name, device)
     return t.data_ptr()
 
 
-def _vector(t, dtype, name: str, count: int | None, device: int) -> int:
-    """Address of a contiguous vector (of `count` elements)."""
-    if t.dtype != dtype or t.dim() != 1 or (count is not None and t.shape[0] != count) or \
-            not t.is_contiguous():
-        raise _invalid(f"{name} must be {'n' if count is None else count} contiguous {dtype} "
-                       f"elements, not {tuple(t.shape)} of {t.dtype}")
-    return _on(t, device, name)
+def _place(t, name: str, device: int) -> None:
+    if t.get_device() != device:
+        raise _invalid(f"{name} is on {t.device}, the context on cuda:{device}")
 
 
 def _heads(t, dtype, name: str, shape, device: int):
     """(address, token stride, head stride) of [tokens][heads][dim] rows."""
-    if t.dtype != dtype or t.dim() != 3 or (shape is not None and t.shape != shape):
+    stride = t.stride()
+    if t.dtype is not dtype or len(stride) != 3 or (shape is not None and t.shape != shape):
         raise _invalid(f"{name} is {tuple(t.shape)} of {t.dtype}, not "
                        f"{'[tokens][heads][dim]' if shape is None else tuple(shape)} of {dtype}")
-    stride = t.stride()
     if stride[2] != 1 and t.shape[2] > 1:
         raise _invalid(f"{name}: a head's elements must be neighbours")
-    return _on(t, device, name), stride[0], stride[1]
+    if t.get_device() != device:
+        _place(t, name, device)
+    return t.data_ptr(), stride[0], stride[1]
 
 
-def _table(t, device: int):
-    if t.dtype != _torch_types()[1] or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+def _table(t, i32, device: int):
+    """(address, rows, entries of a row, row stride) of a block table."""
+    stride = t.stride()
+    if t.dtype is not i32 or len(stride) != 2 or (stride[1] != 1 and t.shape[1] > 1):
         raise _invalid(f"table must be int32 rows, not {tuple(t.shape)} of {t.dtype}")
-    return _on(t, device, "table"), t.shape[0], t.shape[1], t.stride(0)
+    if t.get_device() != device:
+        _place(t, "table", device)
+    batch, columns = t.shape
+    return t.data_ptr(), batch, columns, stride[0]
 
 
-def _cache(t, device: int) -> _KvCache:
+def _cache(t, u8, device: int):
+    """(address, pages, heads, page size, head size) of a cache."""
     size = t.shape
-    if t.dtype != _torch_types()[2] or len(size) != 4 or size[3] % 34 or not t.is_contiguous():
+    if t.dtype is not u8 or len(size) != 4 or size[3] % 34 or not t.is_contiguous():
         raise _invalid("the cache must be contiguous uint8 [pages][heads][page / 32][34 dim], not "
                        f"{tuple(size)} of {t.dtype}")
-    return _KvCache(_on(t, device, "cache"), size[0], size[1], 32 * size[2], size[3] // 34)
+    if t.get_device() != device:
+        _place(t, "cache", device)
+    return t.data_ptr(), size[0], size[1], 32 * size[2], size[3] // 34
 
 
-def _kind(t, name: str) -> int:
-    kind = _torch_types()[0].get(t.dtype)
+def _kind(kinds, t, name: str) -> int:
+    kind = kinds.get(t.dtype)
     if kind is None:
         raise _invalid(f"{name} is {t.dtype} (float32, bfloat16 or float16)")
     return kind
 
 
-def _count(value, name: str) -> int:
-    if not 0 <= value < 1 << 32:  # ctypes would wrap it
-        raise _invalid(f"{name} = {value}")
-    return value
+def _desc(layout: struct.Struct, *values) -> bytes:
+    try:
+        return layout.pack(*values)
+    except struct.error as e:  # a size that its field does not hold
+        raise _invalid(f"argument out of range: {e}") from None
 
 
 def kv_plan(lens, new_tokens, free_pages, free_count, table, page_size: int, cu, kv_lens, slots,
@@ -832,21 +811,20 @@ def kv_plan(lens, new_tokens, free_pages, free_count, table, page_size: int, cu,
     and positions [size], status [2] (pages taken, requests refused) are
     written."""
     ctx = ctx or default_context()
-    i32, dev = _torch_types()[1], ctx.device
-    at, batch, columns, stride = _table(table, dev)
-    slots_at = _vector(slots, i32, "slots", None, dev)
+    i32, dev = (_types or _torch_types())[1], ctx.device
+    at, batch, columns, stride = _table(table, i32, dev)
+    slots_at = _vector(slots, i32, "slots", -1, dev)
+    free_at = _vector(free_pages, i32, "free_pages", -1, dev)
     size = slots.shape[0]
-    d = _KvPlanDesc(_vector(lens, i32, "lens", batch, dev),
-                    _vector(new_tokens, i32, "new_tokens", batch, dev),
-                    _vector(free_pages, i32, "free_pages", None, dev),
-                    _vector(free_count, i32, "free_count", 1, dev), at,
-                    _vector(cu, i32, "cu", batch + 1, dev),
-                    _vector(kv_lens, i32, "kv_lens", batch, dev), slots_at,
-                    _vector(positions, i32, "positions", size, dev),
-                    _vector(status, i32, "status", 2, dev), batch, columns, stride,
-                    _count(page_size, "page_size"), size, free_pages.shape[0])
-    fn = lib().hb_kv_plan if sync else lib().hb_kv_plan_async
-    _check(fn(ctx.handle, C.byref(d)))
+    d = _desc(KV_PLAN_DESC, _vector(lens, i32, "lens", batch, dev),
+              _vector(new_tokens, i32, "new_tokens", batch, dev), free_at,
+              _vector(free_count, i32, "free_count", 1, dev), at,
+              _vector(cu, i32, "cu", batch + 1, dev),
+              _vector(kv_lens, i32, "kv_lens", batch, dev), slots_at,
+              _vector(positions, i32, "positions", size, dev),
+              _vector(status, i32, "status", 2, dev), batch, columns, stride, page_size, size,
+              free_pages.shape[0])
+    _check((lib().hb_kv_plan if sync else lib().hb_kv_plan_async)(ctx.handle, d))
 
 
 def norm_rope(q, positions, inv_freq, q_out, k=None, k_out=None, gamma_q=None, gamma_k=None,
@@ -857,8 +835,8 @@ def norm_rope(q, positions, inv_freq, q_out, k=None, k_out=None, gamma_q=None, g
     [tokens][heads][dim]; positions int32 [axes][tokens] (or [tokens]);
     inv_freq float64; sections: the pairs of each axis."""
     ctx = ctx or default_context()
-    _, i32, _, f64, f32 = _torch_types()
-    kind, dev, dtype = _kind(q, "q"), ctx.device, q.dtype
+    kinds, i32, _, f64, f32 = _types or _torch_types()
+    kind, dev, dtype = _kind(kinds, q, "q"), ctx.device, q.dtype
     qa, qt, qh = _heads(q, dtype, "q", None, dev)
     tokens, heads, dim = q.shape
     oa, ot, oh = _heads(q_out, dtype, "q_out", q.shape, dev)
@@ -867,43 +845,46 @@ def norm_rope(q, positions, inv_freq, q_out, k=None, k_out=None, gamma_q=None, g
         if k_out is None:
             raise _invalid("k without k_out")
         ka, kt, kh = _heads(k, dtype, "k", None, dev)
-        if k.shape[0] != tokens or k.shape[2] != dim:
+        k_tokens, k_heads, k_dim = k.shape
+        if k_tokens != tokens or k_dim != dim:
             raise _invalid(f"k is {tuple(k.shape)}, q {tuple(q.shape)}")
         pa, pt, ph = _heads(k_out, dtype, "k_out", k.shape, dev)
-        k_heads = k.shape[1]
     if positions.dim() == 1:
         positions = positions[None]
-    axes = positions.shape[0]
-    if positions.dtype != i32 or positions.dim() != 2 or positions.shape[1] != tokens or \
-            (tokens > 1 and positions.stride(1) != 1):
+    stride = positions.stride()
+    if positions.dtype is not i32 or len(stride) != 2 or positions.shape[1] != tokens or \
+            (tokens > 1 and stride[1] != 1):
         raise _invalid(f"positions must be int32 [axes][{tokens}], not "
                        f"{tuple(positions.shape)} of {positions.dtype}")
-    freq = _vector(inv_freq, f64, "inv_freq", None, dev)
+    if positions.get_device() != dev:
+        _place(positions, "positions", dev)
+    axes = positions.shape[0]
+    freq = _vector(inv_freq, f64, "inv_freq", -1, dev)
     half = inv_freq.shape[0]
-    sections = sections if sections is not None else (half,)
-    if len(sections) != axes or not 1 <= axes <= 3 or min(sections) < 0:
+    if sections is None:
+        sections = (half,)
+    if len(sections) != axes or not 1 <= axes <= 3:
         raise _invalid(f"sections {tuple(sections)} for {axes} position axes")
-    d = _NormRopeDesc(qa, ka, oa, pa, qt, qh, kt, kh, ot, oh, pt, ph,
-                      None if gamma_q is None else _vector(gamma_q, f32, "gamma_q", dim, dev),
-                      None if gamma_k is None else _vector(gamma_k, f32, "gamma_k", dim, dev),
-                      _on(positions, dev, "positions"), positions.stride(0), freq, eps, kind, tokens, heads, k_heads,
-                      dim, 2 * half, 1 if interleaved else 0, axes,
-                      (C.c_uint32 * 3)(*sections))
-    fn = lib().hb_norm_rope if sync else lib().hb_norm_rope_async
-    _check(fn(ctx.handle, C.byref(d)))
+    d = _desc(NORM_ROPE_DESC, qa, ka, oa, pa, qt, qh, kt, kh, ot, oh, pt, ph,
+              0 if gamma_q is None else _vector(gamma_q, f32, "gamma_q", dim, dev),
+              0 if gamma_k is None else _vector(gamma_k, f32, "gamma_k", dim, dev),
+              positions.data_ptr(), stride[0], freq, eps, kind, tokens, heads, k_heads, dim,
+              2 * half, 1 if interleaved else 0, axes, *sections, *(0,) * (3 - axes))
+    _check((lib().hb_norm_rope if sync else lib().hb_norm_rope_async)(ctx.handle, d))
 
 
 def _kv_rows(fn, k, v, slots, cache, ctx) -> None:
-    ctx = ctx or default_context()
-    kind, dev = _kind(k, "k"), ctx.device
-    c = _cache(cache, dev)
-    tokens = k.shape[0]
-    shape = (tokens, c.heads, c.dim)
-    ka, kt, kh = _heads(k, k.dtype, "k", shape, dev)
-    va, vt, vh = _heads(v, k.dtype, "v", shape, dev)
-    d = _KvRowsDesc(c, ka, va, kt, kh, vt, vh,
-                    _vector(slots, _torch_types()[1], "slots", tokens, dev), kind, tokens)
-    _check(fn(ctx.handle, C.byref(d)))
+    kinds, i32, u8, _, _ = _types or _torch_types()
+    dev, dtype = ctx.device, k.dtype
+    c = _cache(cache, u8, dev)
+    kind = _kind(kinds, k, "k")
+    ka, kt, kh = _heads(k, dtype, "k", None, dev)
+    tokens, heads, dim = k.shape
+    if heads != c[2] or dim != c[4]:
+        raise _invalid(f"k is {tuple(k.shape)}, the cache has {c[2]} heads of {c[4]}")
+    va, vt, vh = _heads(v, dtype, "v", k.shape, dev)
+    _check(fn(ctx.handle, _desc(KV_ROWS_DESC, *c, ka, va, kt, kh, vt, vh,
+                                _vector(slots, i32, "slots", tokens, dev), kind, tokens)))
 
 
 def kv_cache_shape(pages: int, heads: int, page_size: int, dim: int) -> tuple[int, int, int, int]:
@@ -914,12 +895,14 @@ def kv_cache_shape(pages: int, heads: int, page_size: int, dim: int) -> tuple[in
 def kv_append(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -> None:
     """hb_kv_append: rows k, v [tokens][heads][dim] into the cache (uint8
     [pages][heads][page / 32][34 dim]) at int32 slots."""
-    _kv_rows(lib().hb_kv_append if sync else lib().hb_kv_append_async, k, v, slots, cache, ctx)
+    _kv_rows(lib().hb_kv_append if sync else lib().hb_kv_append_async, k, v, slots, cache,
+             ctx or default_context())
 
 
 def kv_read(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -> None:
     """hb_kv_read: the stored values of slots into k, v [tokens][heads][dim]."""
-    _kv_rows(lib().hb_kv_read if sync else lib().hb_kv_read_async, k, v, slots, cache, ctx)
+    _kv_rows(lib().hb_kv_read if sync else lib().hb_kv_read_async, k, v, slots, cache,
+             ctx or default_context())
 
 
 def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
@@ -931,18 +914,19 @@ def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, s
     every row sees; window: keys a row sees, itself among them (0: all);
     softcap: scores as softcap * tanh(score / softcap)."""
     ctx = ctx or default_context()
-    i32, dev = _torch_types()[1], ctx.device
-    kind, c = _kind(q, "q"), _cache(cache, dev)
-    qa, qt, qh = _heads(q, q.dtype, "q", None, dev)
+    kinds, i32, u8, _, _ = _types or _torch_types()
+    dev, dtype = ctx.device, q.dtype
+    c = _cache(cache, u8, dev)
+    kind = _kind(kinds, q, "q")
+    qa, qt, qh = _heads(q, dtype, "q", None, dev)
     tokens, heads, dim = q.shape
-    if dim != c.dim:
-        raise _invalid(f"q has heads of {dim} elements, the cache of {c.dim}")
-    oa, ot, oh = _heads(out, q.dtype, "out", q.shape, dev)
-    at, batch, columns, stride = _table(table, dev)
-    d = _KvAttentionDesc(c, qa, oa, qt, qh, ot, oh, at, _vector(cu, i32, "cu", batch + 1, dev),
-                         _vector(kv_lens, i32, "kv_lens", batch, dev),
-                         None if prefix is None else _vector(prefix, i32, "prefix", batch, dev),
-                         kind, tokens, heads, batch, columns, stride, _count(max_new, "max_new"),
-                         _count(max_kv, "max_kv"), _count(window, "window"), scale, softcap)
-    fn = lib().hb_kv_attention if sync else lib().hb_kv_attention_async
-    _check(fn(ctx.handle, C.byref(d)))
+    if dim != c[4]:
+        raise _invalid(f"q has heads of {dim} elements, the cache of {c[4]}")
+    oa, ot, oh = _heads(out, dtype, "out", q.shape, dev)
+    at, batch, columns, stride = _table(table, i32, dev)
+    d = _desc(KV_ATTENTION_DESC, *c, qa, oa, qt, qh, ot, oh, at,
+              _vector(cu, i32, "cu", batch + 1, dev),
+              _vector(kv_lens, i32, "kv_lens", batch, dev),
+              0 if prefix is None else _vector(prefix, i32, "prefix", batch, dev), kind, tokens,
+              heads, batch, columns, stride, max_new, max_kv, window, scale, softcap)
+    _check((lib().hb_kv_attention if sync else lib().hb_kv_attention_async)(ctx.handle, d))

@@ -276,47 +276,26 @@ __device__ __forceinline__ void StorePairs(T* x, uint32_t p, const RopeArgs& g, 
 // y = x gamma / sqrt(mean(x^2) + eps) of every query and key head, then each
 // pair of its first rot elements turned by position x frequency: one read and
 // one write of the rows.  A lane holds four pairs, so 8 to 64 lanes hold a
-// head and a wave several; the pairs, and with them the cosines and sines
-// (64-bit angles), are the same for every head, so a wave takes a token's
-// heads one after another on the angles of one computation.  `parts` waves
-// share a token where tokens are few.
+// head and a wave several; the pairs, and with them the cosines and sines, are
+// the same for every head, so a wave computes a token's angles once, a lane
+// each (64 bits), while its first heads load, passes them through LDS and
+// takes the token's heads one after another.  `parts` waves share a token
+// where tokens are few.
 template <class T, bool vec, bool neighbours>
 __global__ __launch_bounds__(kThreads) void RopeKernel(const RopeArgs g) {
-  const uint32_t lane = threadIdx.x % 64, wave = blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
+  constexpr uint32_t kBatch = 2;  // heads of a lane in flight
+  __shared__ float turns[kThreads / 64][256][2];
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t in = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t wave = blockIdx.x * (kThreads / 64) + in;
   const uint32_t token = wave / g.parts, part = wave % g.parts;
   if (token >= g.tokens) return;
   const uint32_t per = 64 / g.lanes, p = lane % g.lanes * 4, half = g.rot / 2;
   const uint32_t heads = g.q_heads + g.k_heads;
   const bool holds = p < g.dim / 2;
-  float c[4], s[4], gq[8], gk[8];
-#pragma unroll
-  for (uint32_t j = 0; j < 4; ++j) {
-    c[j] = 1.f;
-    s[j] = 0.f;
-    gq[j] = gq[4 + j] = gk[j] = gk[4 + j] = 1.f;
-    if (p + j < half) {
-      const uint32_t i = p + j;
-      const uint32_t axis = (i >= g.sections[0] ? 1u : 0u) + (i >= g.sections[1] ? 1u : 0u);
-      const double turns = g.inv_freq[i] * 0.15915494309189533577;
-      Turn((double)g.positions[axis * g.position_stride + token] * turns, &c[j], &s[j]);
-    }
-    if (p + j < g.dim / 2) {
-      const Pairs at = PairsOf<neighbours>(p + j, g.dim, g.rot);
-      if (g.gamma_q) {
-        gq[j] = g.gamma_q[at.a];
-        gq[4 + j] = g.gamma_q[at.b];
-      }
-      if (g.gamma_k) {
-        gk[j] = g.gamma_k[at.a];
-        gk[4 + j] = g.gamma_k[at.b];
-      }
-    }
-  }
-  const float inv_dim = 1.f / (float)g.dim;
-  constexpr uint32_t kBatch = 4;  // heads of a lane in flight
   const uint32_t step = per * g.parts;
-  for (uint32_t h0 = part * per + lane / g.lanes; h0 < heads; h0 += step * kBatch) {
-    float a[kBatch][4], b[kBatch][4];
+  float a[kBatch][4], b[kBatch][4];
+  auto load = [&](uint32_t h0) {
 #pragma unroll
     for (uint32_t u = 0; u < kBatch; ++u) {
       const uint32_t h = h0 + u * step;
@@ -330,6 +309,43 @@ __global__ __launch_bounds__(kThreads) void RopeKernel(const RopeArgs g) {
         LoadPairs<T, vec, neighbours>(x, p, g, a[u], b[u]);
       }
     }
+  };
+  uint32_t h0 = part * per + lane / g.lanes;
+  load(h0);
+  for (uint32_t i = lane; i < half; i += 64) {
+    const uint32_t axis = (i >= g.sections[0] ? 1u : 0u) + (i >= g.sections[1] ? 1u : 0u);
+    const double turn = g.inv_freq[i] * 0.15915494309189533577;
+    Turn((double)g.positions[axis * g.position_stride + token] * turn, &turns[in][i][0],
+         &turns[in][i][1]);
+  }
+  float gq[8], gk[8];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    gq[j] = gq[4 + j] = gk[j] = gk[4 + j] = 1.f;
+    if (p + j < g.dim / 2) {
+      const Pairs at = PairsOf<neighbours>(p + j, g.dim, g.rot);
+      if (g.gamma_q) {
+        gq[j] = g.gamma_q[at.a];
+        gq[4 + j] = g.gamma_q[at.b];
+      }
+      if (g.gamma_k) {
+        gk[j] = g.gamma_k[at.a];
+        gk[4 + j] = g.gamma_k[at.b];
+      }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  float c[4], s[4];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    const bool turned = p + j < half;
+    c[j] = turned ? turns[in][p + j][0] : 1.f;
+    s[j] = turned ? turns[in][p + j][1] : 0.f;
+  }
+  const float inv_dim = 1.f / (float)g.dim;
+  while (h0 < heads) {
 #pragma unroll
     for (uint32_t u = 0; u < kBatch; ++u) {
       const uint32_t h = h0 + u * step;
@@ -360,6 +376,8 @@ __global__ __launch_bounds__(kThreads) void RopeKernel(const RopeArgs g) {
         StorePairs<T, vec, neighbours>(y, p, g, a[u], b[u]);
       }
     }
+    h0 += step * kBatch;
+    load(h0);
   }
 }
 
@@ -425,29 +443,40 @@ __device__ __forceinline__ uint32_t LoadV(const uint8_t* record, uint32_t dim, u
 }
 
 // K and V rows of one token and head into the cache: 8 columns of both a
-// lane, so 8, 16 or 32 lanes hold a head and four a block.  A row with an
-// infinity or NaN in K or V is stored as NaN keys and zero values.
+// lane, so 8, 16 or 32 lanes hold a head and four a block.  A workgroup takes
+// neighbouring tokens of one head: where their slots are neighbours too, as
+// in a prompt, a record's bytes of several tokens leave in one store (a token's
+// own lie 2 to 16 bytes long all over the record).  A row with an infinity or
+// NaN in K or V is stored as NaN keys and zero values.
+template <uint32_t dim>
+struct RowLanes {
+  static constexpr uint32_t kLanes = dim / 8, kTokens = kThreads / kLanes;
+  uint32_t token, head, col;
+  __device__ __forceinline__ explicit RowLanes(uint32_t heads) {
+    head = blockIdx.x % heads;
+    token = blockIdx.x / heads * kTokens + threadIdx.x / kLanes;
+    col = threadIdx.x % kLanes * 8;
+  }
+};
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
-  constexpr uint32_t kLanes = dim / 8;
-  const uint32_t lane = threadIdx.x % 64;
-  const uint32_t item = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const uint32_t token = item / g.heads, head = item % g.heads, col = lane % kLanes * 8;
-  uint64_t record = 0;
-  uint32_t t = 0;
-  const bool has = token < g.tokens &&
-                   KvSlot(g.slots[token], g.pages, g.heads, g.groups, &record, &t);
+  const RowLanes<dim> at(g.heads);
+  constexpr uint32_t kLanes = RowLanes<dim>::kLanes;
   float k[8] = {}, v[8] = {};
-  if (has) {
-    Load8(static_cast<const T*>(g.k) + token * g.k_token + head * g.k_head + col, g.vec, k);
-    Load8(static_cast<const T*>(g.v) + token * g.v_token + head * g.v_head + col, g.vec, v);
+  int32_t slot = -1;
+  if (at.token < g.tokens) {
+    slot = g.slots[at.token];
+    Load8(static_cast<const T*>(g.k) + at.token * g.k_token + at.head * g.k_head + at.col, g.vec,
+          k);
+    Load8(static_cast<const T*>(g.v) + at.token * g.v_token + at.head * g.v_head + at.col, g.vec,
+          v);
   }
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     top = max(top, max(__float_as_uint(k[j]) & 0x7FFFFFFFu, __float_as_uint(v[j]) & 0x7FFFFFFFu));
   const uint64_t odd = __builtin_amdgcn_ballot_w64(top >= 0x7F800000u);
-  const uint64_t mine = (~0ull >> (64 - kLanes)) << (lane / kLanes * kLanes);
+  const uint64_t mine = (~0ull >> (64 - kLanes)) << (threadIdx.x % 64 / kLanes * kLanes);
   const bool bad = (odd & mine) != 0;
   if (bad) {
 #pragma unroll
@@ -455,13 +484,15 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
   }
   uint32_t ks, vs;
   const uint32_t kc = Encode8(k, &ks), vc = Encode8(v, &vs);
-  if (!has) return;
-  uint8_t* const to = g.cache + (record + (uint64_t)head * g.groups) * KvRecordBytes(dim);
-  *reinterpret_cast<uint32_t*>(to + KvKCode(dim, t, col)) = kc;
-  StoreV(to, dim, t, col, vc);
-  if (col % 32 == 0) {
-    to[KvKScale(dim, t, col)] = bad ? 255 : (uint8_t)ks;
-    to[KvVScale(dim, t, col)] = (uint8_t)vs;
+  uint64_t record;
+  uint32_t t;
+  if (!KvSlot(slot, g.pages, g.heads, g.groups, &record, &t)) return;
+  uint8_t* const to = g.cache + (record + (uint64_t)at.head * g.groups) * KvRecordBytes(dim);
+  *reinterpret_cast<uint32_t*>(to + KvKCode(dim, t, at.col)) = kc;
+  StoreV(to, dim, t, at.col, vc);
+  if (at.col % 32 == 0) {
+    to[KvKScale(dim, t, at.col)] = bad ? 255 : (uint8_t)ks;
+    to[KvVScale(dim, t, at.col)] = (uint8_t)vs;
   }
 }
 
@@ -511,25 +542,23 @@ __device__ __forceinline__ void Store8(T* to, bool vec, const T* y) {
 // The stored values of slots, on AppendKernel's lanes.
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void ReadKernel(const KvRowsArgs g) {
-  constexpr uint32_t kLanes = dim / 8;
-  const uint32_t item = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const uint32_t token = item / g.heads, head = item % g.heads, col = threadIdx.x % kLanes * 8;
-  if (token >= g.tokens) return;
+  const RowLanes<dim> at(g.heads);
+  if (at.token >= g.tokens) return;
   uint64_t record;
   uint32_t t;
   uint32_t kc = 0, vc = 0, ks = 127, vs = 127;
-  if (KvSlot(g.slots[token], g.pages, g.heads, g.groups, &record, &t)) {
-    const uint8_t* from = g.cache + (record + (uint64_t)head * g.groups) * KvRecordBytes(dim);
-    kc = *reinterpret_cast<const uint32_t*>(from + KvKCode(dim, t, col));
-    vc = LoadV(from, dim, t, col);
-    ks = from[KvKScale(dim, t, col)];
-    vs = from[KvVScale(dim, t, col)];
+  if (KvSlot(g.slots[at.token], g.pages, g.heads, g.groups, &record, &t)) {
+    const uint8_t* from = g.cache + (record + (uint64_t)at.head * g.groups) * KvRecordBytes(dim);
+    kc = *reinterpret_cast<const uint32_t*>(from + KvKCode(dim, t, at.col));
+    vc = LoadV(from, dim, t, at.col);
+    ks = from[KvKScale(dim, t, at.col)];
+    vs = from[KvVScale(dim, t, at.col)];
   }
   T y[8];
   Decode8(kc, ks, y);
-  Store8(static_cast<T*>(g.k_out) + token * g.k_token + head * g.k_head + col, g.vec, y);
+  Store8(static_cast<T*>(g.k_out) + at.token * g.k_token + at.head * g.k_head + at.col, g.vec, y);
   Decode8(vc, vs, y);
-  Store8(static_cast<T*>(g.v_out) + token * g.v_token + head * g.v_head + col, g.vec, y);
+  Store8(static_cast<T*>(g.v_out) + at.token * g.v_token + at.head * g.v_head + at.col, g.vec, y);
 }
 
 template <class T>
@@ -599,8 +628,8 @@ hipError_t LaunchKvRows(const KvRowsArgs& in, bool read, hipStream_t stream) {
       read ? reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)
            : reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
   a.vec = strides % 4 == 0 && bases % (4 * size) == 0;
-  const uint64_t threads = (uint64_t)a.tokens * a.heads * (a.dim / 8);
-  const uint32_t grid = (uint32_t)((threads + kThreads - 1) / kThreads);
+  const uint32_t tokens = kThreads / (a.dim / 8);  // of a workgroup
+  const uint32_t grid = (a.tokens + tokens - 1) / tokens * a.heads;
   switch (a.type) {
     case HB_TYPE_F32: return LaunchKvRowsOf<float>(a, read, grid, stream);
     case HB_TYPE_BF16: return LaunchKvRowsOf<__bf16>(a, read, grid, stream);
