@@ -462,5 +462,8 @@ struct AttnArgs {
   float* ws;
 };
 hipError_t LaunchAttention(const AttnArgs& a, Workspace& ws, hipStream_t stream);
+// Many rows of 16-bit types (hb_prompt.hip).
+bool PromptEligible(const AttnArgs& a);
+hipError_t LaunchPrompt(const AttnArgs& a, hipStream_t stream);
 
 }  // namespace hb
