@@ -252,34 +252,41 @@ __device__ __forceinline__ bool OutAligned(const AttnArgs& a) {
          reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(typename TypeOf<parts>::type)) == 0;
 }
 
-// 8 elements of a query row as fp32, with the scale's sign; zeros past the
-// rows.
-template <uint32_t parts>
-__device__ __forceinline__ void LoadEight(const AttnArgs& a, uint64_t at, bool valid, float* y) {
+// The lane's D / 4 elements of a query row, as they lie; zeros past the rows.
+// The loads of a row are under way together.
+template <uint32_t parts, uint32_t D>
+struct Query {
   typedef typename TypeOf<parts>::type T;
   typedef typename TypeOf<parts>::four V;
-  const bool vec = QueryAligned<parts>(a);
-  const T* x = static_cast<const T*>(a.q) + at;
+  V x[D / 16];
+  __device__ __forceinline__ void Load(const AttnArgs& a, uint64_t at, bool valid) {
+    const T* from = static_cast<const T*>(a.q) + at;
+    const V zero = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = 0.f;
-  if (valid && vec) {
-    const V lo = reinterpret_cast<const V*>(x)[0], hi = reinterpret_cast<const V*>(x)[1];
+    for (uint32_t i = 0; i < D / 16; ++i) x[i] = zero;
+    if (QueryAligned<parts>(a)) {
+      if (valid) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = (float)(j < 4 ? lo[j % 4] : hi[j % 4]);
-  } else if (valid) {
+        for (uint32_t i = 0; i < D / 16; ++i) x[i] = reinterpret_cast<const V*>(from)[i];
+      }
+    } else if (valid) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = (float)x[j];
+      for (uint32_t i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) x[i][j] = from[4 * i + j];
+    }
   }
+  // elements 8 i .. 8 i + 7 as fp32, with the scale's sign
+  __device__ __forceinline__ void Eight(const AttnArgs& a, uint32_t i, float* y) const {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] *= a.sign;
-}
-template <uint32_t parts>
-__device__ __forceinline__ void LoadQuery(const AttnArgs& a, uint64_t at, bool valid,
-                                          bf16x8* out) {
-  float y[8];
-  LoadEight<parts>(a, at, valid, y);
-  ToParts<parts>(y, out);
-}
+    for (uint32_t j = 0; j < 8; ++j) y[j] = a.sign * (float)x[2 * i + j / 4][j % 4];
+  }
+  __device__ __forceinline__ void Parts(const AttnArgs& a, uint32_t i, bf16x8* out) const {
+    float y[8];
+    Eight(a, i, y);
+    ToParts<parts>(y, out);
+  }
+};
 
 template <uint32_t parts>
 __device__ __forceinline__ void StoreFour(const AttnArgs& a, uint64_t at, bool vec, f32x4 y) {
@@ -389,26 +396,37 @@ __device__ __forceinline__ void Scores(const Record<D>& r, const Rows<parts, D, 
   }
 }
 
+// tanh(x).  `fine`: to 2^-23 or so of 1, by the odd series to x^13 where 1 - 2 /
+// (1 + e^2x) cancels, and a reciprocal with one Newton step elsewhere.
+template <bool fine>
+__device__ __forceinline__ float Tanh(float x) {
+  const float d = 1.f + __builtin_amdgcn_exp2f(x * (2.f * kLog2e));
+  float r = __builtin_amdgcn_rcpf(d);
+  if constexpr (!fine) return fmaf(-2.f, r, 1.f);
+  const float near_one = fmaf(fmaf(-d, r, 1.f), r, r);
+  r = d < 1e30f ? near_one : 0.f;  // (inf * 0 in the step)
+  const float y = x * x;
+  float p = fmaf(y, 21844.f / 6081075.f, -1382.f / 155925.f);
+  p = fmaf(y, p, 62.f / 2835.f);
+  p = fmaf(y, p, -17.f / 315.f);
+  p = fmaf(y, p, 2.f / 15.f);
+  p = fmaf(y, p, -1.f / 3.f);
+  const float small = fmaf(x * y, p, x), large = fmaf(-2.f, r, 1.f);
+  return y < 0.2f ? small : x != x ? x : large;
+}
+
 // Scores to powers of two: they are s c with the c returned.  Capped ones
-// (softcap tanh(s scale / softcap)) are done here; fp32 takes the library's
-// tanh, the 16-bit types 1 - 2 / (1 + e^2x), off by 2^-23 of the cap.
+// (softcap tanh(s scale / softcap)) are done here; the 16-bit types take the
+// plain 1 - 2 / (1 + e^2x), off by 2^-22 of the cap.
 template <uint32_t parts, uint32_t R>
 __device__ __forceinline__ float Capped(const AttnArgs& a, f32x4 (&s)[R][2]) {
-  const float c = a.scale * kLog2e;
-  if (!(a.cap > 0.f)) return c;
+  if (!(a.cap > 0.f)) return a.scale * kLog2e;
+  const float in = a.scale / a.cap, out = a.cap * kLog2e;
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      float x = s[t][j / 4][j % 4];
-      if constexpr (parts == 3) {
-        x = a.cap * kLog2e * tanhf(x * a.scale / a.cap);
-      } else {
-        const float e = __builtin_amdgcn_exp2f(x * (2.f * c / a.cap));
-        x = a.cap * kLog2e * fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
-      }
-      s[t][j / 4][j % 4] = x;
-    }
+    for (uint32_t j = 0; j < 8; ++j)
+      s[t][j / 4][j % 4] = out * Tanh<parts == 3>(in * s[t][j / 4][j % 4]);
   return 1.f;
 }
 
@@ -439,29 +457,38 @@ __device__ __forceinline__ float Max3(float a, float b, float c) {
   return y;
 }
 
-// The running maximum and sum of tile t, and the record's weights.  They
-// carry 2^kLift: at most 2^15, and as small as 2^-31 of the maximum before f16
-// goes subnormal.
+// The running maximum of tile t moves where a score passes it by kSlack, and
+// what it had so far shrinks; true where it did, by *shrink.
 template <uint32_t D, uint32_t R>
-__device__ __forceinline__ void Weights(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
-                                        float* p) {
+__device__ __forceinline__ bool Raise(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
+                                      float* shrink) {
   const f32x4 x = s[0], y = s[1];
   const float top =
       c * Max3(Max3(x[0], x[1], x[2]), Max3(x[3], y[0], y[1]), fmaxf(y[2], y[3]));
-  if (__builtin_amdgcn_ballot_w64(top > w.m[t] + kSlack) != 0) {
-    const float m = fmaxf(w.m[t], RowMax(top));
-    // rows that have seen nothing yet stay at -inf, with o and l zero
-    const float shrink = m == w.m[t] ? 1.f : __builtin_amdgcn_exp2f(w.m[t] - m);
-    w.m[t] = m;
-    w.l[t] *= shrink;
+  if (__builtin_amdgcn_ballot_w64(top > w.m[t] + kSlack) == 0) return false;
+  const float m = fmaxf(w.m[t], RowMax(top));
+  // rows that have seen nothing yet stay at -inf, with o and l zero
+  *shrink = m == w.m[t] ? 1.f : __builtin_amdgcn_exp2f(w.m[t] - m);
+  w.m[t] = m;
+  w.l[t] *= *shrink;
 #pragma unroll
-    for (uint32_t i = 0; i < D / 16; ++i) w.o[t][i] *= shrink;
-  }
-  const float ref = kLift - (w.m[t] == -__builtin_inff() ? 0.f : w.m[t]);
+  for (uint32_t i = 0; i < D / 16; ++i) w.o[t][i] *= *shrink;
+  return true;
+}
+// What a row's weights are relative to.
+__device__ __forceinline__ float Reference(float m) {
+  return kLift - (m == -__builtin_inff() ? 0.f : m);
+}
+// The record's weights and their sum.  They carry 2^kLift: at most 2^15, and
+// as small as 2^-31 of the maximum before f16 goes subnormal.
+template <uint32_t D, uint32_t R>
+__device__ __forceinline__ void Weights(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
+                                        float* p) {
+  const float ref = Reference(w.m[t]);
   float sum = 0.f;
 #pragma unroll
   for (uint32_t j = 0; j < 8; ++j) {
-    p[j] = __builtin_amdgcn_exp2f(fmaf(j < 4 ? x[j % 4] : y[j % 4], c, ref));
+    p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], c, ref));
     sum += p[j];
   }
   w.l[t] += sum;
@@ -511,7 +538,8 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
-    float p[8];
+    float p[8], shrink;
+    Raise<D, R>(w, t, s[t], c, &shrink);
     Weights<D, R>(w, t, s[t], c, p);
     if constexpr (half) pt[t][0] = HalfWeights(p);
     else ToParts<parts>(p, pt[t]);

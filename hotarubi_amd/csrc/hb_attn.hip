@@ -34,7 +34,8 @@ struct Merge {
 // in turn; else each wave has R tiles of its own and takes every record.
 template <uint32_t parts, uint32_t D, uint32_t R, bool split>
 // two workgroups a CU (their rings fill its LDS), so 256 registers a wave
-__global__ __launch_bounds__(kThreads, 2) void AttnKernel(const AttnArgs a) {
+// where those do
+__global__ __launch_bounds__(kThreads, D == 256 && parts > 1 ? 1 : 2) void AttnKernel(const AttnArgs a) {
   const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t unit = blockIdx.x / a.splits, part = blockIdx.x % a.splits;
@@ -58,17 +59,12 @@ __global__ __launch_bounds__(kThreads, 2) void AttnKernel(const AttnArgs a) {
   Rows<parts, D, R> w;
   const RowSet set{span, group, head, row0, rows, last};
   Begin<D, R>(a, set, w);
+  Query<parts, D> query[R];
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
     uint64_t at;
     const bool valid = QueryAt<parts, D>(a, set, t, &at);
-#pragma unroll
-    for (uint32_t i = 0; i < D / 32; ++i) {
-      bf16x8 x[parts];
-      LoadQuery<parts>(a, at + 8 * i, valid, x);
-#pragma unroll
-      for (uint32_t p = 0; p < parts; ++p) w.q[t][p][i] = x[p];
-    }
+    query[t].Load(a, at, valid);
   }
 
   const int32_t* const row = a.table + (uint64_t)b * a.table_stride;
@@ -87,46 +83,53 @@ __global__ __launch_bounds__(kThreads, 2) void AttnKernel(const AttnArgs a) {
     return PageRecord(a, walk, row, head, first + (i + lane) * step, end);
   };
   uint32_t now = pages(0), after = count > 64 ? pages(64) : kNoRecord;
-  uint32_t read_at[Ring::kDepth];
+  uint32_t hidden = 0;  // a bit per slot: no page, the slot holds record 0
   auto fetch = [&](uint32_t i, uint32_t base, uint32_t slot) {  // base <= i < base + 128
     const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(
         (int)(i - base < 64 ? now : after), (int)((i - base) % 64));
-    read_at[slot] = from;
+    hidden = (hidden & ~(1u << slot)) | (uint32_t)(from == kNoRecord) << slot;
     FetchRecord<D>(a.cache + (from == kNoRecord ? 0 : (uint64_t)from * KvRecordBytes(D)),
                    slots_at + slot * Ring::kSlot);
   };
   asm volatile("" ::: "memory");
+#pragma unroll 1
+  for (uint32_t u = 0; u < min(count, Ring::kDepth); ++u) fetch(u, 0, u);
+  // the queries' loads are under way with the first records'
 #pragma unroll
-  for (uint32_t u = 0; u < Ring::kDepth; ++u)
-    if (u < count) fetch(u, 0, u);
-  for (uint32_t i0 = 0, base = 0; i0 < count; i0 += Ring::kDepth) {
+  for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
-    for (uint32_t u = 0; u < Ring::kDepth; ++u) {
-      const uint32_t i = i0 + u;
-      if (i >= count) break;
-      if (i + Ring::kDepth <= count) ring::WaitVm<(Ring::kDepth - 1) * Ring::kOps>();
-      else ring::WaitVm<0>();
-      asm volatile("" ::: "memory");
-      const bool present = read_at[u] != kNoRecord;
-      Record<D> r;
+    for (uint32_t i = 0; i < D / 32; ++i) {
+      bf16x8 x[parts];
+      query[t].Parts(a, i, x);
+#pragma unroll
+      for (uint32_t p = 0; p < parts; ++p) w.q[t][p][i] = x[p];
+    }
+  // one copy of the step: what a launch of few records waits for most is its
+  // code
+#pragma unroll 1
+  for (uint32_t i = 0, base = 0, u = 0; i < count; ++i, u = u + 1 == Ring::kDepth ? 0 : u + 1) {
+    if (i + Ring::kDepth <= count) ring::WaitVm<(Ring::kDepth - 1) * Ring::kOps>();
+    else ring::WaitVm<0>();
+    asm volatile("" ::: "memory");
+    const bool present = (hidden >> u & 1) == 0;
+    Record<D> r;
+    ReadKeys<D>(slots + u * Ring::kSlot, r);
+    ReadValues<D>(slots + u * Ring::kSlot, r);
+    ring::WaitLds();  // the slot has been read
+    asm volatile("" ::: "memory");
+    if (i + Ring::kDepth < count) {
+      if (i + Ring::kDepth - base >= 128) {
+        base += 64;
+        now = after;
+        after = pages(base + 64);
+      }
+      fetch(i + Ring::kDepth, base, u);
+    }
+    if (present) {
       f32x4 s[R][2];
-      ReadKeys<D>(slots + u * Ring::kSlot, r);
-      ReadValues<D>(slots + u * Ring::kSlot, r);
-      ring::WaitLds();  // the slot has been read
-      asm volatile("" ::: "memory");
-      if (i + Ring::kDepth < count) {
-        if (i + Ring::kDepth - base >= 128) {
-          base += 64;
-          now = after;
-          after = pages(base + 64);
-        }
-        fetch(i + Ring::kDepth, base, u);
-      }
-      if (present) {
-        Scores<parts, D, R>(r, w, s);
-        const int32_t key0 = (int32_t)(32 * KvWalkRecord(walk, first + i * step));
-        Step<parts, D, R>(a, span, r, key0, s, w);
-      }
+      Scores<parts, D, R>(r, w, s);
+      const int32_t key0 = (int32_t)(32 * KvWalkRecord(walk, first + i * step));
+      Step<parts, D, R>(a, span, r, key0, s, w);
     }
   }
 #pragma unroll
@@ -297,7 +300,8 @@ hipError_t LaunchDim(AttnArgs& a, Workspace& ws, hipStream_t stream) {
   switch (a.dim) {
     case 64: return two ? LaunchOf<parts, 64, 2>(a, ws, stream) : LaunchOf<parts, 64, 1>(a, ws, stream);
     case 128:
-      return two ? LaunchOf<parts, 128, 2>(a, ws, stream) : LaunchOf<parts, 128, 1>(a, ws, stream);
+      // (two tiles of three parts take more than 256 registers)
+      return two && parts < 3 ? LaunchOf<parts, 128, 2>(a, ws, stream) : LaunchOf<parts, 128, 1>(a, ws, stream);
     case 256: return LaunchOf<parts, 256, 1>(a, ws, stream);
   }
   return hipErrorInvalidValue;

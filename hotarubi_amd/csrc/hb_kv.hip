@@ -57,6 +57,11 @@ __device__ __forceinline__ int64_t BlockSum(int64_t x, int64_t* part, int64_t* t
   return x;
 }
 
+// Pages of `tokens` tokens.
+__device__ __forceinline__ uint32_t Pages(uint32_t tokens, uint32_t page) {
+  return tokens / page + (tokens % page != 0 ? 1u : 0u);
+}
+
 // Two sums over the requests (tokens, then the pages of those that fit), then
 // a thread per token: its request by bisection, its position, its slot, and
 // the table entry where it is the first token of a new page.  Every workgroup
@@ -71,16 +76,17 @@ __global__ __launch_bounds__(kThreads) void PlanKernel(const PlanArgs a) {
   __shared__ int32_t have_len[kPlanChunk];
   __shared__ uint8_t fine[kPlanChunk];
   const uint32_t tid = threadIdx.x;
-  const int64_t page = a.page;
+  const uint32_t page = a.page;
   const int64_t free_count = max(0, min(*a.free_count, (int32_t)a.free_size));
   int64_t tokens = 0, pages = 0, taken = 0, refused = 0;
   for (uint32_t base = 0; base < a.batch; base += kPlanChunk) {
     const uint32_t chunk = min(kPlanChunk, a.batch - base);
-    int64_t len[kPlanEach], more[kPlanEach], need[kPlanEach], sum = 0, total;
+    uint32_t len[kPlanEach], more[kPlanEach], need[kPlanEach];
+    int64_t sum = 0, total;
     for (uint32_t j = 0; j < kPlanEach; ++j) {
       const uint32_t i = tid * kPlanEach + j;
-      len[j] = i < chunk ? max(0, a.lens[base + i]) : 0;
-      more[j] = i < chunk ? max(0, a.new_tokens[base + i]) : 0;
+      len[j] = i < chunk ? (uint32_t)max(0, a.lens[base + i]) : 0u;
+      more[j] = i < chunk ? (uint32_t)max(0, a.new_tokens[base + i]) : 0u;
       sum += more[j];
     }
     int64_t at = tokens + BlockSum(sum, part, &total) - sum;
@@ -90,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void PlanKernel(const PlanArgs a) {
     for (uint32_t j = 0; j < kPlanEach; ++j) {
       const uint32_t i = tid * kPlanEach + j;
       at += more[j];
-      const int64_t used = (len[j] + page - 1) / page, want = (len[j] + more[j] + page - 1) / page;
+      const uint32_t used = Pages(len[j], page), want = Pages(len[j] + more[j], page);
       const bool f = want <= a.columns && at <= a.size;
       need[j] = f ? want - used : 0;
       fits |= (uint32_t)f << j;
@@ -133,10 +139,12 @@ __global__ __launch_bounds__(kThreads) void PlanKernel(const PlanArgs a) {
         else lo = mid + 1;
       }
       const int64_t begin = lo > 0 ? ends[lo - 1] : tokens;
-      const int64_t pos = have_len[lo] + (t - begin);
+      // below 2^32: the request's tokens are within `size`, or its slot is not
+      // looked up
+      const uint32_t pos = (uint32_t)have_len[lo] + (uint32_t)(t - begin);
       int64_t slot = -1;
       if (fine[lo]) {
-        const int64_t col = pos / page, used = (have_len[lo] + page - 1) / page;
+        const uint32_t col = pos / page, used = Pages((uint32_t)have_len[lo], page);
         int32_t* const row = a.table + (uint64_t)(base + lo) * a.table_stride;
         int32_t p;
         if (col >= used) {
@@ -146,7 +154,7 @@ __global__ __launch_bounds__(kThreads) void PlanKernel(const PlanArgs a) {
         } else {
           p = row[col];
         }
-        if (p >= 0) slot = p * page + pos % page;
+        if (p >= 0) slot = (int64_t)p * page + pos % page;
         if (slot > 0x7FFFFFFF) slot = -1;
       }
       a.slots[t] = (int32_t)slot;

@@ -25,19 +25,12 @@ struct Operand<2> {
   typedef f16x8 type;
 };
 
+// Waves of a workgroup and 16-row tiles of a wave: two waves a SIMD, so 256
+// registers each, of which sums and queries take 6 D / 16 a tile.
 template <uint32_t D>
-struct Shape;
-template <>
-struct Shape<64> {
-  static constexpr uint32_t kWaves = 4, kTiles = 4, kBlocks = 2;
-};
-template <>
-struct Shape<128> {
-  static constexpr uint32_t kWaves = 8, kTiles = 2, kBlocks = 2;
-};
-template <>
-struct Shape<256> {
-  static constexpr uint32_t kWaves = 4, kTiles = 2, kBlocks = 1;
+struct Shape {
+  static constexpr uint32_t kWaves = D == 64 ? 4 : 8, kTiles = D == 64 ? 4 : D == 128 ? 2 : 1;
+  static constexpr uint32_t kRows = 16 * kWaves * kTiles;
 };
 
 // A wave's share of a stage (two records), as loaded: kKeys operand blocks of K
@@ -46,15 +39,47 @@ template <uint32_t D>
 struct Share {
   static constexpr uint32_t kKeys = D / 8 / Shape<D>::kWaves;
   static constexpr uint32_t kPairs = D / 16 / Shape<D>::kWaves;
-  static_assert(kKeys == (D == 256 ? 8 : 2) && kPairs == (D == 256 ? 4 : 1), "shares");
   alignas(16) uint32_t k[kKeys];
   uint32_t ks[D == 256 ? 2 : 1];
   u32x4 v[D / 64];
   uint32_t vs[2];
 };
 
+// Rows of q and out pass through LDS, a wave's own part of it: a lane wants the
+// D / 4 columns that are its of one row, memory whole rows (64 lines a load
+// otherwise, at a line a cycle: 8 us of a workgroup's life).  A row's 16-byte
+// pieces are permuted by the row, so that rows do not meet in a bank.
+template <uint32_t D>
+__device__ __forceinline__ uint32_t PieceAt(uint32_t row, uint32_t piece) {
+  return row * (D * 2) + (piece ^ (row % (D / 8))) * 16;
+}
+template <uint32_t D>
+struct RowPiece {  // the lane's piece of its `i`-th row of a tile, in memory's order
+  uint32_t row, piece;
+  __device__ __forceinline__ explicit RowPiece(uint32_t i) {
+    const uint32_t lane = threadIdx.x % 64;
+    row = i * (512 / D) + lane / (D / 8);
+    piece = lane % (D / 8);
+  }
+};
+template <uint32_t D>
+__device__ __forceinline__ uint64_t RowStart(const RowSet& set, uint32_t row, uint64_t token,
+                                             uint64_t head) {
+  return (uint64_t)(set.span.first + row / set.group) * token +
+         (uint64_t)(set.head * set.group + row % set.group) * head;
+}
+__device__ __forceinline__ bool Whole(const void* base, uint64_t token, uint64_t head) {
+  return (token | head) % 8 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0;
+}
+// Ends what the wave's LDS accesses before may still do.
+__device__ __forceinline__ void WaveFence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <uint32_t parts, uint32_t D>
-__global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void PromptKernel(
+__global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
     const AttnArgs a) {
   constexpr uint32_t kWaves = Shape<D>::kWaves, R = Shape<D>::kTiles, kSteps = D / 32;
   constexpr uint32_t kKeys = Share<D>::kKeys, kPairs = Share<D>::kPairs;
@@ -90,16 +115,28 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
   State<D, R> w;
   Q q[R][kSteps];
   Begin<D, R>(a, set, w);
+  uint8_t* const rows_lds = reinterpret_cast<uint8_t*>(stages) + wave * (R * 16 * D * 2);
+  static_assert(kWaves * R * 16 * D * 2 <= sizeof stages, "the rows fit the stages");
+  const bool whole = Whole(a.q, a.q_token, a.q_head);
+  Query<parts, D> query[R];
+  u32x4 piece[R][D / 32];
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
-    uint64_t at;
-    const bool valid = QueryAt<parts, D>(a, set, t, &at);
+    if (whole) {
 #pragma unroll
-    for (uint32_t i = 0; i < kSteps; ++i) {
-      float y[8];
-      LoadEight<parts>(a, at + 8 * i, valid, y);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[t][i][j] = (typename TypeOf<parts>::type)y[j];
+      for (uint32_t i = 0; i < D / 32; ++i) {
+        const RowPiece<D> mine(i);
+        const uint32_t row = row0 + t * 16 + mine.row;
+        piece[t][i] = u32x4{0, 0, 0, 0};
+        if (row < rows)
+          piece[t][i] = *reinterpret_cast<const u32x4*>(
+              static_cast<const typename TypeOf<parts>::type*>(a.q) +
+              RowStart<D>(set, row, a.q_token, a.q_head) + mine.piece * 8);
+      }
+    } else {
+      uint64_t at;
+      const bool valid = QueryAt<parts, D>(a, set, t, &at);
+      query[t].Load(a, at, valid);
     }
   }
   // the keys that any row of the wave sees
@@ -132,10 +169,10 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
       const uint8_t* from = a.cache + (uint64_t)k_at * KvRecordBytes(D);
       const uint32_t word = k_tile * kSteps + k_step;
       const uint8_t* x = from + word / 4 * 1024 + lane * 16 + word % 4 * 4;
-      if constexpr (kKeys == 8) {
+      // within one 16-byte piece
+      if constexpr (kKeys == 4) {
         *reinterpret_cast<u32x4*>(share.k) = *reinterpret_cast<const u32x4*>(x);
-        *reinterpret_cast<u32x4*>(share.k + 4) = *reinterpret_cast<const u32x4*>(x + 1024);
-      } else {  // within one 16-byte piece
+      } else {
         const uint2 two = *reinterpret_cast<const uint2*>(x);
         share.k[0] = two.x;
         share.k[1] = two.y;
@@ -158,6 +195,32 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
 
   bool slow = false;
   load(0);
+  if (whole) {
+#pragma unroll
+    for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+      for (uint32_t i = 0; i < D / 32; ++i) {
+        const RowPiece<D> mine(i);
+        *reinterpret_cast<u32x4*>(rows_lds + t * (32 * D) +
+                                  PieceAt<D>(mine.row, mine.piece)) = piece[t][i];
+      }
+    WaveFence();
+#pragma unroll
+    for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+      for (uint32_t i = 0; i < kSteps; ++i)
+        *reinterpret_cast<u32x4*>(&query[t].x[2 * i]) = *reinterpret_cast<const u32x4*>(
+            rows_lds + t * (32 * D) + PieceAt<D>(n, g * (D / 32) + i));
+  }
+#pragma unroll
+  for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+    for (uint32_t i = 0; i < kSteps; ++i) {
+      float y[8];
+      query[t].Eight(a, i, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[t][i][j] = (typename TypeOf<parts>::type)y[j];
+    }
   __syncthreads();  // odd
   for (uint32_t i = 0; i < count; i += 2) {
     Stage& stage = stages[i / 2 % 2];
@@ -199,7 +262,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
           uint32_t word;
           if constexpr (D == 64) word = share.v[0][e / 2] >> ((e % 2 * 2 + v_pair) * 8);
           else if constexpr (D == 128) word = share.v[e / 4][e % 4] >> (v_pair * 8);
-          else word = share.v[e / 2][e % 2 * 2 + (v_pair ? 1 : 0)] >> (j * 8);
+          else word = (v_pair < 4 ? share.v[e / 2][e % 2 * 2] : share.v[e / 2][e % 2 * 2 + 1]) >> ((v_pair % 4 + j) * 8);
           x[e] = TwoAs<0, true>(word, ScaleOf(share.vs[e / 4], e % 4));
         }
         u32x4 lo, hi;
@@ -247,7 +310,8 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
       f16x8 pt[R];
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t) {
-        float p[8];
+        float p[8], shrink;
+        Raise<D, R>(w, t, s[t], c, &shrink);
         Weights<D, R>(w, t, s[t], c, p);
         pt[t] = HalfWeights(p);
       }
@@ -260,10 +324,42 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
     }
   }
   if (!slow) {
-    if (!has_rows) return;
 #pragma unroll
     for (uint32_t t = 0; t < R; ++t) w.l[t] = RowSum(w.l[t]);
-    Finish<parts, D, R>(a, set, w);
+    if (!Whole(a.out, a.out_token, a.out_head)) {
+      if (has_rows) Finish<parts, D, R>(a, set, w);
+      return;
+    }
+    __syncthreads();  // the stages have been read
+    typedef typename TypeOf<parts>::four V;
+#pragma unroll
+    for (uint32_t t = 0; t < R; ++t) {
+      const float inv = w.l[t] == 0.f ? 0.f : 1.f / w.l[t];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+        for (uint32_t c = 0; c < D / 16; c += 4) {
+          V y;
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j)
+            y[j] = (typename TypeOf<parts>::type)(w.o[t][c + j][i] * inv);
+          const uint32_t col = (4 * g + i) * (D / 16) + c;
+          *reinterpret_cast<V*>(rows_lds + t * (32 * D) + PieceAt<D>(n, col / 8) + col % 8 * 2) = y;
+        }
+    }
+    WaveFence();
+#pragma unroll
+    for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+      for (uint32_t i = 0; i < D / 32; ++i) {
+        const RowPiece<D> mine(i);
+        const uint32_t row = row0 + t * 16 + mine.row;
+        if (row < rows)
+          *reinterpret_cast<u32x4*>(static_cast<typename TypeOf<parts>::type*>(a.out) +
+                                    RowStart<D>(set, row, a.out_token, a.out_head) +
+                                    mine.piece * 8) = *reinterpret_cast<const u32x4*>(
+              rows_lds + t * (32 * D) + PieceAt<D>(mine.row, mine.piece));
+      }
     return;
   }
   // scale bytes that f16 does not hold: the rows again, a tile at a time, on
@@ -277,10 +373,12 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
     Begin<D, 1>(a, one, v);
     uint64_t from;
     const bool valid = QueryAt<parts, D>(a, one, 0, &from);
+    Query<parts, D> again;
+    again.Load(a, from, valid);
 #pragma unroll
     for (uint32_t i = 0; i < kSteps; ++i) {
       bf16x8 x[parts];
-      LoadQuery<parts>(a, from + 8 * i, valid, x);
+      again.Parts(a, i, x);
 #pragma unroll
       for (uint32_t p = 0; p < parts; ++p) v.q[0][p][i] = x[p];
     }
@@ -302,34 +400,36 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, D == 256 ? 1 : 2) void Promp
   }
 }
 
-template <uint32_t parts, uint32_t D>
-hipError_t LaunchOf(const AttnArgs& a, uint32_t grid, hipStream_t stream) {
-  PromptKernel<parts, D><<<grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
-  return hipGetLastError();
-}
-
 }  // namespace
 
 bool PromptEligible(const AttnArgs& a) {
   if (a.type == HB_TYPE_F32) return false;
   const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
-  const uint64_t tile = a.dim == 256 ? 128 : 256;
+  const uint64_t tile = a.dim == 256 ? Shape<256>::kRows : Shape<128>::kRows;
   return rows >= tile / 2 &&
          (rows + tile - 1) / tile * a.batch * a.heads >= (uint64_t)DeviceCus() / 2;
 }
 
+template <uint32_t D>
+static hipError_t LaunchDim(AttnArgs& a, hipStream_t stream) {
+  const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
+  const uint64_t tiles = (rows + Shape<D>::kRows - 1) / Shape<D>::kRows;
+  const uint64_t grid = tiles * a.batch * a.heads;
+  if (grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  a.tiles = (uint32_t)tiles;
+  if (a.type == HB_TYPE_F16)
+    PromptKernel<2, D><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
+  else
+    PromptKernel<1, D><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
 hipError_t LaunchPrompt(const AttnArgs& in, hipStream_t stream) {
   AttnArgs a = in;
-  const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
-  const uint64_t tile = a.dim == 256 ? 128 : 256;
-  a.tiles = (uint32_t)((rows + tile - 1) / tile);
-  const uint64_t grid = (uint64_t)a.tiles * a.batch * a.heads;
-  if (grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  const bool half = a.type == HB_TYPE_F16;
   switch (a.dim) {
-    case 64: return half ? LaunchOf<2, 64>(a, grid, stream) : LaunchOf<1, 64>(a, grid, stream);
-    case 128: return half ? LaunchOf<2, 128>(a, grid, stream) : LaunchOf<1, 128>(a, grid, stream);
-    default: return half ? LaunchOf<2, 256>(a, grid, stream) : LaunchOf<1, 256>(a, grid, stream);
+    case 64: return LaunchDim<64>(a, stream);
+    case 128: return LaunchDim<128>(a, stream);
+    default: return LaunchDim<256>(a, stream);
   }
 }
 
