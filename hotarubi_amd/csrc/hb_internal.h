@@ -462,8 +462,8 @@ struct AttnArgs {
   float* ws;
 };
 hipError_t LaunchAttention(const AttnArgs& a, Workspace& ws, hipStream_t stream);
-// Many rows of 16-bit types (hb_prompt.hip).
-bool PromptEligible(const AttnArgs& a);
+// Many rows of 16-bit types (hb_prompt.hip); the rows of a workgroup.
+uint32_t PromptRows(uint32_t dim);
 hipError_t LaunchPrompt(const AttnArgs& a, hipStream_t stream);
 
 }  // namespace hb

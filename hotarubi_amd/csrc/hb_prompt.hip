@@ -402,12 +402,8 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
 
 }  // namespace
 
-bool PromptEligible(const AttnArgs& a) {
-  if (a.type == HB_TYPE_F32) return false;
-  const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
-  const uint64_t tile = a.dim == 256 ? Shape<256>::kRows : Shape<128>::kRows;
-  return rows >= tile / 2 &&
-         (rows + tile - 1) / tile * a.batch * a.heads >= (uint64_t)DeviceCus() / 2;
+uint32_t PromptRows(uint32_t dim) {
+  return dim == 64 ? Shape<64>::kRows : dim == 128 ? Shape<128>::kRows : Shape<256>::kRows;
 }
 
 template <uint32_t D>
