@@ -760,7 +760,7 @@ def _heads(t, dtype, name: str, shape, device: int):
     if t.dtype is not dtype or len(stride) != 3 or (shape is not None and t.shape != shape):
         raise _invalid(f"{name} is {tuple(t.shape)} of {t.dtype}, not "
                        f"{'[tokens][heads][dim]' if shape is None else tuple(shape)} of {dtype}")
-    if stride[2] != 1 and t.shape[2] > 1:
+    if stride[2] != 1 and t.shape[2] > 1 and t.numel() > 0:
         raise _invalid(f"{name}: a head's elements must be neighbours")
     if t.get_device() != device:
         _place(t, name, device)
@@ -770,7 +770,8 @@ def _heads(t, dtype, name: str, shape, device: int):
 def _table(t, i32, device: int):
     """(address, rows, entries of a row, row stride) of a block table."""
     stride = t.stride()
-    if t.dtype is not i32 or len(stride) != 2 or (stride[1] != 1 and t.shape[1] > 1):
+    if t.dtype is not i32 or len(stride) != 2 or \
+            (stride[1] != 1 and t.shape[1] > 1 and t.numel() > 0):
         raise _invalid(f"table must be int32 rows, not {tuple(t.shape)} of {t.dtype}")
     if t.get_device() != device:
         _place(t, "table", device)
