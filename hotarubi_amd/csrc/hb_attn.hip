@@ -370,6 +370,9 @@ __global__ __launch_bounds__(kThreads) void JoinKernel(const AttnArgs a) {
   StoreFour<parts>(a, at, OutAligned<parts>(a), y * (l == 0.f ? 0.f : 1.f / l));
 }
 
+// What the workspace may hold of opened records (hb_prompt.hip).
+constexpr uint64_t kMostOpened = 1ull << 30;
+
 // How a call's work may be divided, and about how long that takes: workgroups
 // of a fixed cost and a cost a record, two to a CU, in rounds.  The constants
 // are measured ones; what was compared is at Divide.
@@ -395,12 +398,17 @@ double Rounds(const Sizes& z, double groups, double slots, double fixed, double 
   return rounds <= 1 ? longest : std::max(longest, (rounds + 0.3) * usual);
 }
 
-Division ByPrompt(const Sizes& z, uint64_t tile) {
-  const double record = z.dim == 64 ? 1.05 : z.dim == 128 ? 1.17 : 1.9;
+Division ByPrompt(const Sizes& z, uint64_t tile, uint64_t opened) {
+  // us a record of a workgroup with a CU to itself, and how much more beside
+  // another
+  const double alone = z.dim == 64 ? 0.75 : z.dim == 128 ? 0.62 : 1.25;
+  const double more = z.dim == 64 ? 0.6 : z.dim == 128 ? 0.72 : 0;
+  const double cus = (double)z.cus, slots = z.dim == 256 ? cus : 2 * cus;
   const double groups = (double)(z.pairs * ((z.rows + tile - 1) / tile));
+  const double beside = std::min(1.0, std::max(0.0, groups / cus - 1));
   return {Division::kByPrompt, 0, 1,
-          Rounds(z, groups, (double)(z.dim == 64 ? 2 * z.cus : z.cus), 8, record, 1) +
-              z.bytes / 20e6};
+          Rounds(z, groups, slots, 7, alone * (1 + beside * more), 1) + z.bytes / 20e6 + 3 +
+              (double)opened / 4e6};
 }
 
 Division ByWaves(const Sizes& z, Division::Way way, uint32_t tiles_of_16) {
@@ -426,15 +434,17 @@ Division ByWaves(const Sizes& z, Division::Way way, uint32_t tiles_of_16) {
                         (1 + beside * (d == 2 ? 0.5 : 0.35));
   const double share = way == Division::kByRows ? 1 : 1.0 / (double)(kWaves * splits);
   return {way, tiles_of_16, splits,
-          Rounds(z, groups, slots, way == Division::kByRows ? 5 : 6, record, share) +
+          Rounds(z, groups, slots, (way == Division::kByRows ? 2 : 3) + 3 * tiles_of_16, record,
+                 share) +
               (splits > 1 ? 6 : 0) + z.bytes / 8e6};
 }
 
 // The shortest.  Measured, us (bf16; prompt / rows / splits; one or two tiles a
-// wave): 32 x 50 new tokens behind 150, D 64, 15 on 5 heads: 17 / 12, 15 / 19, 16;
-// the same, D 128, 32 on 8: 20 / 29, 23 / 43, 39; 1 x 500 behind 2,000: 97 /
-// 74, 92 / 53, 40; 2 x 1,500 behind 1,000: 140 / 202, 153 / 215, 154; 1 x 8
-// behind 16,000: 439 / 411, 527 / 20, 23.
+// wave): 32 x 50 new tokens behind 150, D 64, 15 on 5 heads: 19 / 12, 15 / 19, 16;
+// the same, D 128, 32 on 8: 33 / 28, 23 / 42, 38; 1 x 500 behind 2,000: 65 /
+// 71, 90 / 53, 40; 2 x 1,500 behind 1,000: 122 / 200, 152 / 216, 153; 1 x 8
+// behind 16,000: 285 / 413, 527 / 17, 22.  Over 60 such calls the choice is
+// within 5% of the best for 50, and 1.25 times it at worst.
 Division Divide(const AttnArgs& a) {
   Sizes z;
   z.pairs = (uint64_t)a.batch * a.heads;
@@ -462,7 +472,8 @@ Division Divide(const AttnArgs& a) {
     take(ByWaves(z, Division::kBySplits, 2));
     if (z.rows > 32 * (kWaves - 1)) take(ByWaves(z, Division::kByRows, 2));
   }
-  if (z.parts < 3 && z.rows > 32) take(ByPrompt(z, PromptRows(z.dim)));
+  if (z.parts < 3 && z.rows > 32 && PromptBytes(a) <= kMostOpened)
+    take(ByPrompt(z, PromptRows(z.dim), PromptBytes(a)));
   return best;
 }
 
@@ -539,7 +550,7 @@ hipError_t LaunchAttention(const AttnArgs& in, Workspace& ws, hipStream_t stream
   a.sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;
   a.scale = a.scale == 0.f ? 1.f : std::abs(a.scale);
   const Division how = Divide(a);
-  if (how.way == Division::kByPrompt) return LaunchPrompt(a, stream);
+  if (how.way == Division::kByPrompt) return LaunchPrompt(a, ws, stream);
   switch (a.type) {
     case HB_TYPE_BF16: return LaunchDim<1>(a, how, ws, stream);
     case HB_TYPE_F16: return LaunchDim<2>(a, how, ws, stream);

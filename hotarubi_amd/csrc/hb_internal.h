@@ -460,10 +460,15 @@ struct AttnArgs {
   uint32_t tiles, splits, split_records;
   float sign;  // of scale, which is positive then
   float* ws;
+  // prompts: records of a request that are opened, and where
+  uint32_t opened;
+  uint8_t* opened_at;
 };
 hipError_t LaunchAttention(const AttnArgs& a, Workspace& ws, hipStream_t stream);
-// Many rows of 16-bit types (hb_prompt.hip); the rows of a workgroup.
+// Many rows of 16-bit types (hb_prompt.hip); the rows of a workgroup, and the
+// workspace of a launch.
 uint32_t PromptRows(uint32_t dim);
-hipError_t LaunchPrompt(const AttnArgs& a, hipStream_t stream);
+uint64_t PromptBytes(const AttnArgs& a);
+hipError_t LaunchPrompt(const AttnArgs& a, Workspace& ws, hipStream_t stream);
 
 }  // namespace hb

@@ -2,9 +2,10 @@
 //
 // Where a record serves many rows the conversion of its codes, not their
 // bytes, is what counts (per record and wave 64 conversions and 32 permutes
-// beside 32 products): here a workgroup's waves convert two records together, a
-// share each, into LDS in the order of the operands, and every wave reads them
-// for its own R tiles of 16 rows.
+// beside 32 products): here a launch of its own converts every record that a
+// request looks at, once, into the workspace in the order of the matrix cores'
+// operands, and the workgroups of all its rows draw them from there straight
+// into LDS, for every wave's R tiles of 16 rows.
 #include <algorithm>
 
 #include "hb_attn.h"
@@ -25,25 +26,94 @@ struct Operand<2> {
   typedef f16x8 type;
 };
 
-// Waves of a workgroup and 16-row tiles of a wave: two waves a SIMD, so 256
-// registers each, of which sums and queries take 6 D / 16 a tile.
+// Waves of a workgroup, 16-row tiles of a wave, workgroups of a CU and stages
+// (of two records) in LDS.  Four waves a SIMD hide each other's waits: at D 128
+// two workgroups of 8 waves with a tile each took prompts of up to 4,096 tokens
+// in 369 us, one of 8 waves with two tiles in 406, one of 16 with one in 379.
 template <uint32_t D>
 struct Shape {
-  static constexpr uint32_t kWaves = D == 64 ? 4 : 8, kTiles = D == 64 ? 4 : D == 128 ? 2 : 1;
+  static constexpr uint32_t kWaves = 8, kTiles = D == 64 ? 2 : 1, kGroups = D == 256 ? 1 : 2;
   static constexpr uint32_t kRows = 16 * kWaves * kTiles;
+  static constexpr uint32_t kStages = 2;
 };
 
-// A wave's share of a stage (two records), as loaded: kKeys operand blocks of K
-// (8 columns a lane of 16 tokens) and kPairs pairs of column tiles of V.
+// A record as operands: K [token tile][step][lane][16 B], then V^T [column
+// tile][lane][16 B].
 template <uint32_t D>
-struct Share {
-  static constexpr uint32_t kKeys = D / 8 / Shape<D>::kWaves;
-  static constexpr uint32_t kPairs = D / 16 / Shape<D>::kWaves;
-  alignas(16) uint32_t k[kKeys];
-  uint32_t ks[D == 256 ? 2 : 1];
-  u32x4 v[D / 64];
-  uint32_t vs[2];
-};
+constexpr uint32_t kOpened = 128 * D;
+
+// The place of record r of a request's walk among its opened records.
+__device__ __forceinline__ uint32_t OpenedAt(const KvWalk& walk, uint32_t r) {
+  return r < walk.head ? r : walk.head + r - walk.from;
+}
+
+// A wave a record.  `odd` says where f16 does not hold a scale (K's count for
+// f16 queries): the rows that look at it take the general steps.  Tokens past
+// the request's end, where any byte may lie, are given a scale of 1.
+template <uint32_t parts, uint32_t D>
+__global__ __launch_bounds__(256) void OpenKernel(const AttnArgs a) {
+  const uint32_t lane = threadIdx.x % 64, n = lane % 16;
+  const uint32_t at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t pair = at / a.opened, i = at % a.opened, b = pair / a.heads;
+  if (b >= a.batch) return;
+  const KvSpan span =
+      KvRequest(a.cu[b], a.cu[b + 1], a.kv_lens[b], a.prefix ? a.prefix[b] : 0, a.tokens,
+                a.max_new, (uint64_t)a.columns * a.groups * 32);
+  if (span.rows == 0) return;
+  const int32_t pos0 = span.total - span.count;
+  const KvWalk walk =
+      KvRecords(pos0, pos0 + (int32_t)span.rows - 1, span.total, span.prefix, a.window);
+  if (i >= walk.count) return;
+  uint32_t* const odd = reinterpret_cast<uint32_t*>(a.ws) + at;
+  const uint32_t record = __builtin_amdgcn_readfirstlane(PageRecord(
+      a, walk, a.table + (uint64_t)b * a.table_stride, pair % a.heads, i, walk.count));
+  if (record == kNoRecord) {
+    if (lane == 0) *odd = 0;
+    return;
+  }
+  const uint8_t* from = a.cache + (uint64_t)record * KvRecordBytes(D);
+  Record<D> r;
+  ReadKeys<D>(from, r);
+  ReadValues<D>(from, r);
+  const int32_t key0 = (int32_t)(32 * KvWalkRecord(walk, i));
+  if (key0 + 32 > span.total) {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (KeyOf(key0, j) >= span.total)
+        r.vs[j / 4] = (r.vs[j / 4] & ~(255u << (8 * (j % 4)))) | 127u << (8 * (j % 4));
+#pragma unroll
+    for (uint32_t k = 0; k < (D == 256 ? 2 : 1); ++k) {
+      if (key0 + (int32_t)n >= span.total) r.ks[k] = (r.ks[k] & 0xFF00u) | 127u;
+      if (key0 + 16 + (int32_t)n >= span.total) r.ks[k] = (r.ks[k] & 0xFFu) | 127u << 8;
+    }
+  }
+  uint32_t outside = OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1]);
+  if constexpr (parts == 2)
+    outside |= OutsideHalf(r.ks[0] | (D == 256 ? r.ks[D == 256] : 0x7F7Fu) << 16);
+  const uint64_t any = __builtin_amdgcn_ballot_w64(outside != 0);
+  if (lane == 0) *odd = any != 0;
+  u32x4* const to = reinterpret_cast<u32x4*>(a.opened_at + (uint64_t)at * kOpened<D>) + lane;
+#pragma unroll
+  for (uint32_t tile = 0; tile < 2; ++tile)
+#pragma unroll
+    for (uint32_t e = 0; e < D / 32; ++e) {
+      const uint32_t word = tile * (D / 32) + e, w = r.k[word / 4][word % 4];
+      const float scale = ScaleOf(r.ks[D == 256 ? e / 4 : 0], tile);
+      u32x4 x;
+      x[0] = TwoAs<0, parts == 2>(w, scale);
+      x[1] = TwoAs<1, parts == 2>(w, scale);
+      x[2] = TwoAs<2, parts == 2>(w, scale);
+      x[3] = TwoAs<3, parts == 2>(w, scale);
+      to[word * 64] = x;
+    }
+#pragma unroll
+  for (uint32_t e = 0; e < D / 32; ++e) {
+    f16x8 v[2];
+    ValueOperands<D, true>(r, e, &v[0], &v[1]);
+    to[(D / 16 + 2 * e) * 64] = __builtin_bit_cast(u32x4, v[0]);
+    to[(D / 16 + 2 * e + 1) * 64] = __builtin_bit_cast(u32x4, v[1]);
+  }
+}
 
 // Rows of q and out pass through LDS, a wave's own part of it: a lane wants the
 // D / 4 columns that are its of one row, memory whole rows (64 lines a load
@@ -79,17 +149,18 @@ __device__ __forceinline__ void WaveFence() {
 }
 
 template <uint32_t parts, uint32_t D>
-__global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
+__global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void PromptKernel(
     const AttnArgs a) {
   constexpr uint32_t kWaves = Shape<D>::kWaves, R = Shape<D>::kTiles, kSteps = D / 32;
-  constexpr uint32_t kKeys = Share<D>::kKeys, kPairs = Share<D>::kPairs;
-  constexpr bool half_keys = parts == 2;
+  constexpr uint32_t kStages = Shape<D>::kStages;
   typedef typename Operand<parts>::type Q;
   struct Stage {
-    u32x4 k[2][2][kSteps][64], v[2][D / 16][64];
+    struct {
+      u32x4 k[2][kSteps][64], v[D / 16][64];
+    } record[2];
   };
-  __shared__ Stage stages[2];
-  __shared__ uint32_t odd[2];
+  static_assert(sizeof(Stage) == 2 * kOpened<D>, "records lie as they are opened");
+  __shared__ __align__(16) Stage stages[kStages];
 
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -143,58 +214,27 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
   const int32_t wave_hi = base_pos + (int32_t)(set.last / group);
   const int32_t wave_lo = SightOf(span, row0 / group, true, a.window).lo;
 
-  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   const int32_t* const row = a.table + (uint64_t)b * a.table_stride;
   const uint32_t count = walk.count;
+  // the request's opened records; those of pages that are not there, which
+  // nothing was written for, are passed over below
+  const KvWalk all = KvRecords(base_pos, base_pos + (int32_t)span.rows - 1, span.total,
+                               span.prefix, a.window);
+  const uint64_t first_opened = ((uint64_t)b * a.heads + head) * a.opened;
+  bool slow = all.count > a.opened;
+  for (uint32_t i = lane; i < count && !slow; i += 64) {
+    const uint32_t r = OpenedAt(all, KvWalkRecord(walk, i));
+    slow = reinterpret_cast<const uint32_t*>(a.ws)[first_opened + r] != 0;
+  }
+  slow = __builtin_amdgcn_ballot_w64(slow) != 0;
+  auto key_of = [&](uint32_t i) { return (int32_t)(32 * KvWalkRecord(walk, i)); };
   auto pages = [&](uint32_t i) { return PageRecord(a, walk, row, head, i + lane, count); };
   uint32_t base = 0, now = pages(0), after = count > 64 ? pages(64) : kNoRecord;
-  auto place = [&](uint32_t i) {  // base <= i < base + 128
-    return i < count ? (uint32_t)__builtin_amdgcn_readlane(
-                           (int)(i - base < 64 ? now : after), (int)((i - base) % 64))
-                     : kNoRecord;
+  auto hidden = [&](uint32_t i) {  // base <= i < base + 128
+    return i >= count || __builtin_amdgcn_readlane((int)(i - base < 64 ? now : after),
+                                                   (int)((i - base) % 64)) == (int)kNoRecord;
   };
 
-  // the wave's share: K blocks wave * kKeys .. of [record][token tile][step],
-  // V pairs wave * kPairs .. of [record][pair]
-  const uint32_t k_record = wave * kKeys / (2 * kSteps), k_tile = wave * kKeys / kSteps % 2,
-                 k_step = wave * kKeys % kSteps;
-  const uint32_t v_record = wave * kPairs / kSteps, v_pair = wave * kPairs % kSteps;
-  Share<D> share;
-  uint32_t at[2];
-  auto load = [&](uint32_t i) {
-    at[0] = place(i);
-    at[1] = place(i + 1);
-    const uint32_t k_at = k_record ? at[1] : at[0], v_at = v_record ? at[1] : at[0];
-    if (k_at != kNoRecord) {
-      const uint8_t* from = a.cache + (uint64_t)k_at * KvRecordBytes(D);
-      const uint32_t word = k_tile * kSteps + k_step;
-      const uint8_t* x = from + word / 4 * 1024 + lane * 16 + word % 4 * 4;
-      // within one 16-byte piece
-      if constexpr (kKeys == 4) {
-        *reinterpret_cast<u32x4*>(share.k) = *reinterpret_cast<const u32x4*>(x);
-      } else {
-        const uint2 two = *reinterpret_cast<const uint2*>(x);
-        share.k[0] = two.x;
-        share.k[1] = two.y;
-      }
-      const uint32_t block = D == 256 ? 2 * g : g * D / 128;
-      share.ks[0] = from[32 * D + block * 32 + n * 2 + k_tile];
-      if (D == 256) share.ks[D == 256] = from[32 * D + block * 32 + 32 + n * 2 + k_tile];
-    }
-    if (v_at != kNoRecord) {
-      const uint8_t* from = a.cache + (uint64_t)v_at * KvRecordBytes(D);
-#pragma unroll
-      for (uint32_t c = 0; c < D / 64; ++c)
-        share.v[c] = *reinterpret_cast<const u32x4*>(from + 16 * D + c * 1024 + lane * 16);
-      const uint2 vs = *reinterpret_cast<const uint2*>(from + 33 * D + n * D / 512 * 32 + g * 8);
-      share.vs[0] = vs.x;
-      share.vs[1] = vs.y;
-    }
-  };
-  auto key_of = [&](uint32_t i) { return (int32_t)(32 * KvWalkRecord(walk, i)); };
-
-  bool slow = false;
-  load(0);
   if (whole) {
 #pragma unroll
     for (uint32_t t = 0; t < R; ++t)
@@ -221,77 +261,48 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[t][i][j] = (typename TypeOf<parts>::type)y[j];
     }
-  __syncthreads();  // odd
-  for (uint32_t i = 0; i < count; i += 2) {
-    Stage& stage = stages[i / 2 % 2];
-    const uint32_t here[2] = {at[0], at[1]};
-    uint32_t bad = 0;
-    if (here[k_record] != kNoRecord) {
+  __syncthreads();  // the rows have left the stages
+
+  // a stage's loads, kOps pieces of 1 KB a wave
+  constexpr uint32_t kOps = 2 * kOpened<D> / 1024 / kWaves;
+  static_assert(kOps * kWaves * 512 == kOpened<D>, "whole loads");
+  const uint32_t stages_at = (uint32_t) reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) uint8_t*)reinterpret_cast<uint8_t*>(stages));
+  auto fetch = [&](uint32_t i, uint32_t stage) {
 #pragma unroll
-      for (uint32_t j = 0; j < kKeys; ++j) {
-        const float scale = __uint_as_float(share.ks[D == 256 ? (k_step + j) / 4 : 0] << 23);
-        u32x4 x;
-        x[0] = TwoAs<0, half_keys>(share.k[j], scale);
-        x[1] = TwoAs<1, half_keys>(share.k[j], scale);
-        x[2] = TwoAs<2, half_keys>(share.k[j], scale);
-        x[3] = TwoAs<3, half_keys>(share.k[j], scale);
-        stage.k[k_record][k_tile][k_step + j][lane] = x;
-      }
-      if constexpr (half_keys) {
-        const bool outside = share.ks[0] - 104 > 36 ||
-                             (D == 256 && share.ks[D == 256] - 104 > 36);
-        bad |= outside && key_of(i + k_record) + (int32_t)(16 * k_tile + n) < span.total;
-      }
+    for (uint32_t e = 0; e < kOps; ++e) {
+      const uint32_t piece = wave * kOps + e, u = piece / (kOpened<D> / 1024);
+      // past the last record the stage holds it twice
+      const uint32_t r = OpenedAt(all, KvWalkRecord(walk, min(i + u, count - 1)));
+      ring::Dma16(a.opened_at + (first_opened + r) * kOpened<D> +
+                      piece % (kOpened<D> / 1024) * 1024,
+                  lane * 16, stages_at + stage * (uint32_t)sizeof(Stage) + piece * 1024);
     }
-    if (here[v_record] != kNoRecord) {
-      const int32_t key0 = key_of(i + v_record);
-      if (key0 + 32 > span.total) {  // past the request's end any byte may lie
+  };
+  if (!slow) {
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-          if (KeyOf(key0, j) >= span.total)
-            share.vs[j / 4] =
-                (share.vs[j / 4] & ~(255u << (8 * (j % 4)))) | 127u << (8 * (j % 4));
-      }
-      bad |= OutsideHalf(share.vs[0]) | OutsideHalf(share.vs[1]);
-#pragma unroll
-      for (uint32_t j = 0; j < kPairs; ++j) {
-        uint32_t x[8];
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-          // byte e * kSteps + v_pair + j of the lane's, at byte 0 of a word
-          uint32_t word;
-          if constexpr (D == 64) word = share.v[0][e / 2] >> ((e % 2 * 2 + v_pair) * 8);
-          else if constexpr (D == 128) word = share.v[e / 4][e % 4] >> (v_pair * 8);
-          else word = (v_pair < 4 ? share.v[e / 2][e % 2 * 2] : share.v[e / 2][e % 2 * 2 + 1]) >> ((v_pair % 4 + j) * 8);
-          x[e] = TwoAs<0, true>(word, ScaleOf(share.vs[e / 4], e % 4));
-        }
-        u32x4 lo, hi;
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-          lo[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);
-          hi[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
-        }
-        stage.v[v_record][2 * (v_pair + j)][lane] = lo;
-        stage.v[v_record][2 * (v_pair + j) + 1][lane] = hi;
-      }
-    }
-    if (__builtin_amdgcn_ballot_w64(bad != 0) != 0 && lane == 0) odd[i / 2 % 2] = 1;
-    if (i + 2 < count) {
-      if (i + 4 - base > 128) {
-        base += 64;
-        now = after;
-        after = pages(base + 64);
-      }
-      load(i + 2);
-    }
-    __syncthreads();
-    if (odd[i / 2 % 2] != 0) {  // the same for every wave: the next stage has a flag of its own
-      slow = true;
-      break;
+    for (uint32_t e = 0; e < kStages - 1; ++e)
+      if (2 * e < count) fetch(2 * e, e);
+  }
+#pragma unroll 1
+  for (uint32_t i = 0, now_in = 0; i < count && !slow; i += 2) {
+    Stage& stage = stages[now_in];
+    if (i + 2 * (kStages - 1) <= count) ring::WaitVm<(kStages - 2) * kOps>();
+    else ring::WaitVm<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // every wave's loads of the stage; the stage before is read
+    asm volatile("" ::: "memory");
+    const uint32_t before = now_in == 0 ? kStages - 1 : now_in - 1;
+    if (i + 2 * (kStages - 1) < count) fetch(i + 2 * (kStages - 1), before);
+    now_in = now_in + 1 == kStages ? 0 : now_in + 1;
+    if (i + 1 - base >= 128) {
+      base += 64;
+      now = after;
+      after = pages(base + 64);
     }
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
-      if (here[u] == kNoRecord || !has_rows) continue;
+      if (!has_rows || hidden(i + u)) continue;
       const int32_t key0 = key_of(i + u);
       if (!((key0 <= wave_hi && key0 + 31 >= wave_lo) || key0 < span.prefix)) continue;
       f32x4 s[R][2];
@@ -301,7 +312,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
       for (uint32_t e = 0; e < kSteps; ++e)
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
-          const Q x = __builtin_bit_cast(Q, stage.k[u][k][e][lane]);
+          const Q x = __builtin_bit_cast(Q, stage.record[u].k[k][e][lane]);
 #pragma unroll
           for (uint32_t t = 0; t < R; ++t) s[t][k] = Product(x, q[t][e], s[t][k]);
         }
@@ -317,7 +328,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
       }
 #pragma unroll
       for (uint32_t e = 0; e < D / 16; ++e) {
-        const f16x8 x = __builtin_bit_cast(f16x8, stage.v[u][e][lane]);
+        const f16x8 x = __builtin_bit_cast(f16x8, stage.record[u].v[e][lane]);
 #pragma unroll
         for (uint32_t t = 0; t < R; ++t) w.o[t][e] = Product(x, pt[t], w.o[t][e]);
       }
@@ -326,6 +337,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2) void PromptKernel(
   if (!slow) {
 #pragma unroll
     for (uint32_t t = 0; t < R; ++t) w.l[t] = RowSum(w.l[t]);
+    ring::WaitVm<0>();  // no load into LDS outlives its stage
     if (!Whole(a.out, a.out_token, a.out_head)) {
       if (has_rows) Finish<parts, D, R>(a, set, w);
       return;
@@ -406,26 +418,45 @@ uint32_t PromptRows(uint32_t dim) {
   return dim == 64 ? Shape<64>::kRows : dim == 128 ? Shape<128>::kRows : Shape<256>::kRows;
 }
 
-template <uint32_t D>
-static hipError_t LaunchDim(AttnArgs& a, hipStream_t stream) {
+// Records of a request that may be looked at, and the bytes of a launch's
+// opened ones.
+static uint64_t OpenedRecords(const AttnArgs& a) {
+  uint64_t records = ((uint64_t)a.max_kv + 31) / 32;
+  if (a.window > 0 && a.prefix == nullptr)
+    records = std::min<uint64_t>(records, ((uint64_t)a.window + a.max_new + 62) / 32);
+  return std::max<uint64_t>(records, 1);
+}
+uint64_t PromptBytes(const AttnArgs& a) {
+  const uint64_t records = OpenedRecords(a) * a.batch * a.heads;
+  return records * 128 * a.dim + (records * 4 + 15) / 16 * 16;
+}
+
+template <uint32_t parts, uint32_t D>
+static hipError_t LaunchOf(AttnArgs& a, hipStream_t stream) {
   const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
   const uint64_t tiles = (rows + Shape<D>::kRows - 1) / Shape<D>::kRows;
-  const uint64_t grid = tiles * a.batch * a.heads;
-  if (grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  const uint64_t pairs = (uint64_t)a.batch * a.heads, records = pairs * a.opened;
+  const uint64_t grid = tiles * pairs;
+  if (grid > 0x7FFFFFFFu || records > 0x7FFFFFFFu) return hipErrorInvalidValue;
   a.tiles = (uint32_t)tiles;
-  if (a.type == HB_TYPE_F16)
-    PromptKernel<2, D><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
-  else
-    PromptKernel<1, D><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
+  OpenKernel<parts, D><<<(uint32_t)((records + 3) / 4), 256, 0, stream>>>(a);
+  PromptKernel<parts, D><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
   return hipGetLastError();
 }
 
-hipError_t LaunchPrompt(const AttnArgs& in, hipStream_t stream) {
+hipError_t LaunchPrompt(const AttnArgs& in, Workspace& ws, hipStream_t stream) {
   AttnArgs a = in;
+  const hipError_t err = GrowWorkspace(ws, PromptBytes(a), stream);
+  if (err != hipSuccess) return err;
+  a.opened = (uint32_t)OpenedRecords(a);
+  a.ws = ws.ptr + kSplitCounters;  // a word a record, then the records
+  a.opened_at = reinterpret_cast<uint8_t*>(a.ws) +
+                ((uint64_t)a.opened * a.batch * a.heads * 4 + 15) / 16 * 16;
+  const bool half = a.type == HB_TYPE_F16;
   switch (a.dim) {
-    case 64: return LaunchDim<64>(a, stream);
-    case 128: return LaunchDim<128>(a, stream);
-    default: return LaunchDim<256>(a, stream);
+    case 64: return half ? LaunchOf<2, 64>(a, stream) : LaunchOf<1, 64>(a, stream);
+    case 128: return half ? LaunchOf<2, 128>(a, stream) : LaunchOf<1, 128>(a, stream);
+    default: return half ? LaunchOf<2, 256>(a, stream) : LaunchOf<1, 256>(a, stream);
   }
 }
 
