@@ -501,8 +501,10 @@ hipError_t LaunchOf(AttnArgs& a, const Division& how, Workspace& ws, hipStream_t
   // Requests of different lengths, with enough records that the sums over the
   // requests (about 5 us a workgroup) are less than what uneven workgroups
   // leave idle: 64 requests of 1,000 to 8,191 keys 84 us in splits, 72 in shares.
+  // (Every record that the tables have room for is counted in 32 bits, whatever
+  // kv_lens says.)
   if (tiles == 1 && a.batch > 1 && a.batch <= kMaxShared && units * records >= kLeastShared * cus &&
-      units * records < 0x7FFFFFFFu) {
+      units * std::max<uint64_t>((uint64_t)a.columns * a.groups, 1) < 0x7FFFFFFFu) {
     a.splits = (uint32_t)(2 * cus);
     const hipError_t err =
         GrowWorkspace(ws, (units + a.splits) * stored * kPartial<D> * 4, stream);

@@ -26,15 +26,14 @@ struct Operand<2> {
   typedef f16x8 type;
 };
 
-// Waves of a workgroup, 16-row tiles of a wave, workgroups of a CU and stages
-// (of two records) in LDS.  Four waves a SIMD hide each other's waits: at D 128
+// Waves of a workgroup, 16-row tiles of a wave, workgroups of a CU (each holds
+// two stages of two records in LDS).  Four waves a SIMD hide each other's waits: at D 128
 // two workgroups of 8 waves with a tile each took prompts of up to 4,096 tokens
 // in 369 us, one of 8 waves with two tiles in 406, one of 16 with one in 379.
 template <uint32_t D>
 struct Shape {
   static constexpr uint32_t kWaves = 8, kTiles = D == 64 ? 2 : 1, kGroups = D == 256 ? 1 : 2;
   static constexpr uint32_t kRows = 16 * kWaves * kTiles;
-  static constexpr uint32_t kStages = 2;
 };
 
 // A record as operands: K [token tile][step][lane][16 B], then V^T [column
@@ -152,7 +151,6 @@ template <uint32_t parts, uint32_t D>
 __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void PromptKernel(
     const AttnArgs a) {
   constexpr uint32_t kWaves = Shape<D>::kWaves, R = Shape<D>::kTiles, kSteps = D / 32;
-  constexpr uint32_t kStages = Shape<D>::kStages;
   typedef typename Operand<parts>::type Q;
   struct Stage {
     struct {
@@ -160,7 +158,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
     } record[2];
   };
   static_assert(sizeof(Stage) == 2 * kOpened<D>, "records lie as they are opened");
-  __shared__ __align__(16) Stage stages[kStages];
+  __shared__ __align__(16) Stage stages[2];
 
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -179,7 +177,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
       KvRecords(base_pos + (int32_t)(first_row / group), base_pos + (int32_t)(last_row / group),
                 span.total, span.prefix, a.window);
 
-  // a wave past the rows converts its share and computes nothing
+  // a wave past the rows loads its share and computes nothing
   const uint32_t row0 = first_row + wave * R * 16;
   const RowSet set{span, group, head, row0, rows, max(row0, min(row0 + R * 16, rows) - 1)};
   const bool has_rows = row0 < rows;
@@ -279,22 +277,19 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
                   lane * 16, stages_at + stage * (uint32_t)sizeof(Stage) + piece * 1024);
     }
   };
-  if (!slow) {
-#pragma unroll
-    for (uint32_t e = 0; e < kStages - 1; ++e)
-      if (2 * e < count) fetch(2 * e, e);
-  }
+  if (!slow && count > 0) fetch(0, 0);
 #pragma unroll 1
-  for (uint32_t i = 0, now_in = 0; i < count && !slow; i += 2) {
-    Stage& stage = stages[now_in];
-    if (i + 2 * (kStages - 1) <= count) ring::WaitVm<(kStages - 2) * kOps>();
-    else ring::WaitVm<0>();
+  for (uint32_t i = 0; i < count && !slow; i += 2) {
+    const uint32_t in = i / 2 % 2;
+    const Stage& stage = stages[in];
+    ring::WaitVm<0>();
+    ring::WaitLds();
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // every wave's loads of the stage; the stage before is read
+    // every wave's loads of the stage are there, and its reads of the other
+    // are done
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const uint32_t before = now_in == 0 ? kStages - 1 : now_in - 1;
-    if (i + 2 * (kStages - 1) < count) fetch(i + 2 * (kStages - 1), before);
-    now_in = now_in + 1 == kStages ? 0 : now_in + 1;
+    if (i + 2 < count) fetch(i + 2, 1 - in);
     if (i + 1 - base >= 128) {
       base += 64;
       now = after;
