@@ -7,6 +7,17 @@
 // O^T = V^T P^T wants them, so P goes from the softmax to the next product in
 // the same registers, with no trip through LDS; the record's layout gives the
 // lane its K and V codes for both products as they lie.
+//
+// With o, m and l of a row over the keys so far, a record of scores s (in
+// powers of two) makes m' = max(m, max s), o' = o 2^(m - m') + sum 2^(s - m') v
+// and l' = l 2^(m - m') + sum 2^(s - m'); parts of a row's keys join by the same
+// rule, and out = o / l, or 0 where l = 0.  The cache is read once, 34 D bytes a
+// record and head.  Few rows are bound by that: 8 query heads on each of 8 over
+// 262,147 keys, D 128, 285 MB, take 51 us and 5 for the join (5.6 TB/s before
+// it; the card copies at 4.9, reads and writes together), and 64 requests of
+// 1,000 to 8,191 keys, 321 MB, 70 us and 6.  Rows of 32 bits want three products
+// where others want one: 32 requests of 50 rows behind 150 keys, 15 heads on 5,
+// D 64, take 14.0 us in fp32 and 11.7 in bf16.
 #include <algorithm>
 #include <cmath>
 
@@ -234,9 +245,13 @@ __device__ __forceinline__ uint32_t Stored(const AttnArgs& a) {
   return min(R * 16, a.max_new * (a.q_heads / a.heads));
 }
 
+// What a wave waits for is memory or its own chain of products, softmax and
+// products (0.7 to 1.8 us a record by itself), so its records come ahead of it
+// through a ring of direct loads (the long cache above took 98 us with records
+// loaded into registers) and few rows are split over as many workgroups as the
+// card holds.  Two of them a CU (their rings fill its LDS), so 256 registers a
+// wave where those do.
 template <uint32_t parts, uint32_t D, uint32_t R, Mode mode>
-// two workgroups a CU (their rings fill its LDS), so 256 registers a wave
-// where those do
 __global__ __launch_bounds__(kThreads, D == 256 && parts > 1 ? 1 : 2) void AttnKernel(
     const AttnArgs a) {
   typedef Ring<D> Ring;
@@ -311,7 +326,8 @@ __global__ __launch_bounds__(kThreads, D == 256 && parts > 1 ? 1 : 2) void AttnK
 }
 
 // The parts of a row in their order: lane groups take every kGroups-th, then
-// meet in LDS.
+// meet in LDS.  A launch of its own, so that no workgroup waits for another; 4.8
+// us for 64 rows of 512 parts in all, 6.4 for 2,048 rows: latency.
 template <uint32_t parts, uint32_t D, uint32_t R, Mode mode>
 __global__ __launch_bounds__(kThreads) void JoinKernel(const AttnArgs a) {
   constexpr uint32_t kLanes = D / 4, kGroups = kThreads / kLanes;
@@ -420,16 +436,17 @@ Division ByWaves(const Sizes& z, Division::Way way, uint32_t tiles_of_16) {
   const double slots = z.dim == 256 && z.parts > 1 ? (double)z.cus : 2.0 * (double)z.cus;
   const uint32_t d = z.dim == 64 ? 0 : z.dim == 128 ? 1 : 2;
   const uint64_t tiles = (z.rows + 16 * tiles_of_16 - 1) / (16 * tiles_of_16);
-  const uint64_t units = z.pairs * (way == Division::kByRows ? (tiles + kWaves - 1) / kWaves : tiles);
+  const uint64_t units =
+      z.pairs * (way == Division::kByRows ? (tiles + kWaves - 1) / kWaves : tiles);
   uint64_t splits = 1;
   if (way == Division::kBySplits) {
-    splits = std::max<uint64_t>(
-        1, std::min(2 * z.cus / units, z.most / (2 * kWaves)));
+    splits = std::max<uint64_t>(1, std::min(2 * z.cus / units, z.most / (2 * kWaves)));
     const uint64_t each = (z.most + splits - 1) / splits;
     splits = (z.most + each - 1) / each;
   }
   const double groups = (double)(units * splits);
-  const double beside = std::min(slots / (double)z.cus - 1, std::max(0.0, groups / (double)z.cus - 1));
+  const double beside =
+      std::min(slots / (double)z.cus - 1, std::max(0.0, groups / (double)z.cus - 1));
   const double record = alone[z.parts - 1][tiles_of_16 - 1][d] *
                         (1 + beside * (d == 2 ? 0.5 : 0.35));
   const double share = way == Division::kByRows ? 1 : 1.0 / (double)(kWaves * splits);

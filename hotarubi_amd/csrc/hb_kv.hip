@@ -35,7 +35,6 @@ constexpr uint32_t kThreads = 256;
 
 // ------------------------------------------------------------------- plan --
 
-
 // Inclusive sum over the workgroup's threads; *total the sum of all.  `part`
 // holds a value per wave.
 __device__ __forceinline__ int64_t BlockSum(int64_t x, int64_t* part, int64_t* total) {
@@ -292,8 +291,10 @@ __device__ __forceinline__ void StorePairs(T* x, uint32_t p, const RopeArgs& g, 
 // head and a wave several; the pairs, and with them the cosines and sines, are
 // the same for every head, so a wave computes a token's angles once, a lane
 // each (64 bits), while its first heads load, passes them through LDS and
-// takes the token's heads one after another.  `parts` waves share a token
-// where tokens are few.
+// takes the token's heads one after another (angles made by every lane for
+// itself took 37 us where this takes 32).  `parts` waves share a token where
+// tokens are few.  Memory bounds it: 8,192 tokens of 32 + 8 heads of 128 in
+// bf16, 168 MB, 32 us = 5.2 TB/s; 16 tokens of 20 heads of 64 3.9 us, latency.
 template <class T, bool vec, bool neighbours>
 __global__ __launch_bounds__(kThreads) void RopeKernel(const RopeArgs g) {
   constexpr uint32_t kBatch = 2;  // heads of a lane in flight
@@ -460,7 +461,9 @@ __device__ __forceinline__ uint32_t LoadV(const uint8_t* record, uint32_t dim, u
 // neighbouring tokens of one head: where their slots are neighbours too, as
 // in a prompt, a record's bytes of several tokens leave in one store (a token's
 // own lie 2 to 16 bytes long all over the record).  A row with an infinity or
-// NaN in K or V is stored as NaN keys and zero values.
+// NaN in K or V is stored as NaN keys and zero values.  Memory bounds it:
+// 16,001 tokens of 5 heads of 64 in fp32, 41 MB read and 6 MB written, 9.3 us =
+// 5.0 TB/s (13.2 with a token's heads side by side); 64 tokens of 8 heads 3 us.
 template <uint32_t dim>
 struct RowLanes {
   static constexpr uint32_t kLanes = dim / 8, kTokens = kThreads / kLanes;
@@ -552,7 +555,9 @@ __device__ __forceinline__ void Store8(T* to, bool vec, const T* y) {
   }
 }
 
-// The stored values of slots, on AppendKernel's lanes.
+// The stored values of slots, on AppendKernel's lanes: codes times scales are
+// exact in all three types wherever the type's range holds them.  Memory
+// bounds it: the rows above back to fp32 in 11.9 us, 4.0 TB/s.
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void ReadKernel(const KvRowsArgs g) {
   const RowLanes<dim> at(g.heads);

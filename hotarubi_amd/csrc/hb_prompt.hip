@@ -5,7 +5,16 @@
 // beside 32 products): here a launch of its own converts every record that a
 // request looks at, once, into the workspace in the order of the matrix cores'
 // operands, and the workgroups of all its rows draw them from there straight
-// into LDS, for every wave's R tiles of 16 rows.
+// into LDS, for every wave's R tiles of 16 rows.  No one unit bounds
+// it: at D 128 a wave's record is 256 cycles of products, about 260 of the
+// softmax's 33 vector instructions and 8 exponentials, and 16 KB read from LDS
+// (at D 64 the softmax is twice the products).  Three prompts of up to 4,096
+// tokens, 32 heads on 8, D 128, bf16, 346 GFLOP, take 375 us, 13 of them for
+// opening (924 TFLOP/s; a large library product reaches 1,231), and 400 with
+// the calls back to back; with the conversion in each workgroup they took 454.
+// At D 256 one workgroup fills a CU's LDS, so a wave waits on its own chain, 1.3
+// us a record: eight chunks of 100 to 256 tokens, fp16, a window of 1,024 and
+// capped scores, take 63 us, 13 of them for opening and 7 for the cap.
 #include <algorithm>
 
 #include "hb_attn.h"

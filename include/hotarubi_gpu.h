@@ -672,17 +672,20 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * scale * q.k, softcap * tanh(scale * q.k / softcap) where softcap > 0;
  *   out = sum_j softmax(scores)_j v_j, 0 for a row that sees no key.
  * q and out are [tokens][q_heads][dim] of `type`, strides in elements.  Scores,
- * maxima and sums are in 32 bits.  bf16 q enters the products as it is and the
- * softmax's weights rounded to bf16; fp16 and fp32 enter as two and three
- * bf16 parts (fp32 weights to 2^-24, fp16 ones to 2^-16 of their value).
+ * maxima and sums are in 32 bits, and q and the cache's values enter the
+ * products exactly.  The softmax's weights enter theirs in f16 for bf16 and
+ * fp16 tensors (each off by 2^-12 of its value at most, their sum is of the
+ * unrounded ones) and as three bf16 parts for fp32 ones (2^-24).
  * Rows outside every request are not written.  max_new and max_kv bound the
  * requests' new tokens and keys; they choose the split of the work, and rows
  * of a request past max_new are not computed.  A block table entry that names
  * no page of the cache hides its keys.  A stored NaN (a scale of 255) makes
  * the rows that see its token NaN, no others.
  * Long caches are split over workgroups that meet in the context's workspace,
- * in a fixed order: results do not change from call to call.  A larger split
- * than before grows the workspace, so a first call belongs before a capture. */
+ * in a fixed order: results do not change from call to call.  Prompts keep
+ * the records they look at in the workspace as operands while the call runs,
+ * 128 dim bytes a record and 1 GiB at most.  A larger call than before grows
+ * the workspace, so a first call belongs before a capture. */
 typedef struct hb_kv_attention_desc {
   hb_kv_cache cache;
   const void* q;
