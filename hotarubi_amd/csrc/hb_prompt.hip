@@ -38,7 +38,10 @@ struct Operand<2> {
 // Waves of a workgroup, 16-row tiles of a wave, workgroups of a CU (each holds
 // two stages of two records in LDS).  Four waves a SIMD hide each other's waits: at D 128
 // two workgroups of 8 waves with a tile each took prompts of up to 4,096 tokens
-// in 369 us, one of 8 waves with two tiles in 406, one of 16 with one in 379.
+// in 369 us, one of 8 waves with two tiles in 406, one of 16 with one in 379.  At
+// D 64 two tiles stay: three workgroups with one took prompts of 4,096 tokens in
+// 137 us for 146 (15 heads on 5), but 182 for 171 (32 on 8) and short ones in 47
+// for 44.
 template <uint32_t D>
 struct Shape {
   static constexpr uint32_t kWaves = 8, kTiles = D == 64 ? 2 : 1, kGroups = D == 256 ? 1 : 2;
