@@ -677,8 +677,9 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * fp16 tensors (each off by 2^-12 of its value at most, their sum is of the
  * unrounded ones) and as three bf16 parts for fp32 ones (2^-24).
  * Rows outside every request are not written.  max_new and max_kv bound the
- * requests' new tokens and keys; they choose the split of the work, and rows
- * of a request past max_new are not computed.  A block table entry that names
+ * requests' new tokens and keys; they choose the split of the work (a max_kv
+ * that is too small costs time, no keys), and rows of a request past max_new
+ * are not computed.  A block table entry that names
  * no page of the cache hides its keys.  A stored NaN (a scale of 255) makes
  * the rows that see its token NaN, no others.
  * Long caches are split over workgroups that meet in the context's workspace,

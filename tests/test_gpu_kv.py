@@ -599,6 +599,47 @@ def test_rows_and_requests_past_the_bounds_are_not_computed(gpu):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_keys_past_max_kv_are_seen_by_prompts(gpu, dtype, dim):
+    """max_kv is too small: what it lays out does not hold every record."""
+    say("prompt past max_kv", dtype, dim)
+    gen = torch.Generator(device=DEV).manual_seed(dim + 1)
+    s = build(gen, [(700, 128, 0), (190, 128, 20)] * 4, 64, 4, dim, dtype, 16)
+    for most in (1, 200, 699):
+        check(gpu, dict(s, max_kv=most))
+        check(gpu, dict(s, max_kv=most), window=100)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_keys_past_max_kv_are_seen_by_ragged_requests(gpu, dtype):
+    say("ragged past max_kv", dtype)
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    heads, dim, page = 8, 64, 64
+    cache = make_cache(gen, 64, heads, page, dim)
+    lens = [3000 + 701 * (b % 7) for b in range(64)]
+    table = torch.randint(0, 64, (64, max(lens) // page + 1), generator=gen, device=DEV,
+                          dtype=torch.int32)
+    q = torch.randn((64, 16, dim), generator=gen, device=DEV).to(dtype)
+    for most in (1, 2000):
+        check(gpu, dict(q=q, cache=cache, table=table, cu=ints(list(range(65))),
+                        kv_lens=ints(lens), prefix=None, max_new=1, max_kv=most))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompts_with_window_prefix_and_missing_pages(gpu, dtype, dim):
+    """The records a prompt looks at are two ranges, with pages missing in both."""
+    say("prompt, two ranges", dtype, dim)
+    gen = torch.Generator(device=DEV).manual_seed(dim + 2)
+    s = build(gen, [(1100, 260, 200), (900, 200, 40), (300, 300, 0)] * 3, 32, 4, dim, dtype, 16)
+    check(gpu, s, window=100)
+    s["table"][0, 1], s["table"][0, 30], s["table"][1, 0] = -1, s["cache"].shape[0], -7
+    s["table"][2, 8:] = -1
+    check(gpu, s, window=100)
+    check(gpu, s, window=500, cap=2.0)
+
+
 # ------------------------------------------------------------ as a step --
 
 def step(ctx, st, sync=False):
