@@ -379,9 +379,12 @@ __global__ __launch_bounds__(kThreads) void RopeKernel(const RopeArgs g) {
       }
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
+        // past rot each element is left alone: a turn by 0 would carry an
+        // infinity or NaN to the other one of its pair
+        const bool turned = p + j < half;
         const float x = a[u][j], y = b[u][j];
-        a[u][j] = fmaf(x, c[j], -(y * s[j]));
-        b[u][j] = fmaf(y, c[j], x * s[j]);
+        a[u][j] = turned ? fmaf(x, c[j], -(y * s[j])) : x;
+        b[u][j] = turned ? fmaf(y, c[j], x * s[j]) : y;
       }
       if (h < heads && holds) {
         T* y = is_q ? static_cast<T*>(g.q_out) + token * g.q_out_token + h * g.q_out_head
