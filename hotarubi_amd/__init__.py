@@ -27,6 +27,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import struct
+import threading
 from dataclasses import dataclass, fields
 
 import numpy as np
@@ -711,7 +712,10 @@ def encode_mxfp8(x, rows: int, cols: int, out, ctx: Context | None = None) -> No
 
 
 # ---------------------------------------------------- serving operators --
-# These take torch tensors: sizes, types and strides come from them.  Steps of
+# These take torch tensors: sizes, types and strides come from them.  Without
+# `ctx` a call is ordered on torch's current stream, like torch's own; with one
+# it is ordered on that context's stream (Context.set_stream), and with sync
+# False the caller orders torch's work on the same tensors with it.  Steps of
 # few tokens wait for the host, so the descriptors are packed in one go, and
 # the checks read each property of a tensor once.
 
@@ -735,6 +739,28 @@ def _torch_types():
 
 def _invalid(message: str):
     return HbError(HB_EINVAL, message)
+
+
+_own = threading.local()  # a host thread's contexts, by device and stream
+
+
+def _torch_context(t, name: str) -> Context:
+    """The context of a call that names none: one of its own for torch's
+    current stream on t's device, so that the call comes after the torch work
+    issued before it and before what is issued next, and calls on two streams
+    do not share a workspace."""
+    import torch
+    device = t.get_device()
+    if device < 0:
+        raise _invalid(f"{name} is on {t.device}, not on a GPU")
+    stream = torch.cuda.current_stream(device).cuda_stream
+    contexts = _own.__dict__
+    ctx = contexts.get((device, stream))
+    if ctx is None:
+        ctx = Context(device)
+        ctx.set_stream(stream)
+        contexts[device, stream] = ctx
+    return ctx
 
 
 def _vector(t, dtype, name: str, count: int, device: int) -> int:
@@ -811,7 +837,7 @@ def kv_plan(lens, new_tokens, free_pages, free_count, table, page_size: int, cu,
     [batch][columns] gets the new pages; cu [batch + 1], kv_lens [batch], slots
     and positions [size], status [2] (pages taken, requests refused) are
     written."""
-    ctx = ctx or default_context()
+    ctx = ctx or _torch_context(lens, "lens")
     i32, dev = (_types or _torch_types())[1], ctx.device
     at, batch, columns, stride = _table(table, i32, dev)
     slots_at = _vector(slots, i32, "slots", -1, dev)
@@ -835,7 +861,7 @@ def norm_rope(q, positions, inv_freq, q_out, k=None, k_out=None, gamma_q=None, g
     normalised) and the rotation of its first 2 * len(inv_freq) elements.  q
     [tokens][heads][dim]; positions int32 [axes][tokens] (or [tokens]);
     inv_freq float64; sections: the pairs of each axis."""
-    ctx = ctx or default_context()
+    ctx = ctx or _torch_context(q, "q")
     kinds, i32, _, f64, f32 = _types or _torch_types()
     kind, dev, dtype = _kind(kinds, q, "q"), ctx.device, q.dtype
     qa, qt, qh = _heads(q, dtype, "q", None, dev)
@@ -897,13 +923,13 @@ def kv_append(k, v, slots, cache, ctx: Context | None = None, sync: bool = True)
     """hb_kv_append: rows k, v [tokens][heads][dim] into the cache (uint8
     [pages][heads][page / 32][34 dim]) at int32 slots."""
     _kv_rows(lib().hb_kv_append if sync else lib().hb_kv_append_async, k, v, slots, cache,
-             ctx or default_context())
+             ctx or _torch_context(k, "k"))
 
 
 def kv_read(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -> None:
     """hb_kv_read: the stored values of slots into k, v [tokens][heads][dim]."""
     _kv_rows(lib().hb_kv_read if sync else lib().hb_kv_read_async, k, v, slots, cache,
-             ctx or default_context())
+             ctx or _torch_context(k, "k"))
 
 
 def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
@@ -914,7 +940,7 @@ def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, s
     the paged cache, into out.  Causal; prefix int32 [batch]: leading keys that
     every row sees; window: keys a row sees, itself among them (0: all);
     softcap: scores as softcap * tanh(score / softcap)."""
-    ctx = ctx or default_context()
+    ctx = ctx or _torch_context(q, "q")
     kinds, i32, u8, _, _ = _types or _torch_types()
     dev, dtype = ctx.device, q.dtype
     c = _cache(cache, u8, dev)

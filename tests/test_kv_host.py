@@ -270,3 +270,21 @@ def test_c_entry_points_refuse_null_and_misaligned_descriptors():
         assert text in hb.last_error() or "records" in hb.last_error(), (kw, hb.last_error())
     # no rows, no launch: only the context is looked at
     assert attend(batch=0, cu=0) == hb.HB_EINVAL and hb.last_error() == "null context"
+
+
+def test_without_a_context_tensors_must_be_on_a_gpu():
+    """A call without `ctx` is ordered on torch's current stream of its
+    tensors' device: there is none for host memory."""
+    rows = torch.zeros(5, 2, 64)
+    for call, name in [
+            (lambda: hb.kv_plan(lens=ints(3), new_tokens=ints(3), free_pages=ints(8),
+                                free_count=ints(1), table=ints(3, 5), page_size=32, cu=ints(4),
+                                kv_lens=ints(3), slots=ints(9), positions=ints(9),
+                                status=ints(2)), "lens"),
+            (lambda: hb.norm_rope(q=rows, positions=ints(5), q_out=rows,
+                                  inv_freq=torch.zeros(8, dtype=torch.float64)), "q"),
+            (lambda: hb.kv_append(k=rows, v=rows, slots=ints(5), cache=cache()), "k"),
+            (lambda: hb.kv_read(k=rows, v=rows, slots=ints(5), cache=cache()), "k"),
+            (lambda: hb.kv_attention(q=rows, out=rows, cache=cache(), table=ints(1, 1), cu=ints(2),
+                                     kv_lens=ints(1), max_new=5, max_kv=64, scale=1.0), "q")]:
+        refused(call, f"{name} is on cpu, not on a GPU")
