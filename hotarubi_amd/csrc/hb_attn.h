@@ -95,8 +95,14 @@ __device__ __forceinline__ void ReadValues(const uint8_t* slot, Record<D>& r) {
 __device__ __forceinline__ float ScaleOf(uint32_t bytes, uint32_t i) {
   return __uint_as_float(((bytes >> (8 * i)) & 255u) << 23);
 }
+// The same of K.  Scales of 253 and 254, whose products pass the types' range,
+// count as 255: NaN.
+__device__ __forceinline__ float KeyScale(uint32_t bytes, uint32_t i) {
+  const uint32_t e = (bytes >> (8 * i)) & 255u;
+  return __uint_as_float(e >= 253u ? 255u << 23 : e << 23);
+}
 
-// Two codes, byte `sel` of a word, as bf16 values (exact: E2M1 on any E8M0).
+// Two codes, byte `sel` of a word, as bf16 values (exact: E2M1 on E8M0 up to 252).
 template <int sel>
 __device__ __forceinline__ uint32_t Two(uint32_t word, float scale) {
   return __builtin_bit_cast(uint32_t,
@@ -107,7 +113,7 @@ template <uint32_t D>
 __device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, uint32_t s) {
   const uint32_t word = tile * (D / 32) + s;
   const uint32_t w = r.k[word / 4][word % 4];
-  const float scale = ScaleOf(r.ks[D == 256 ? s / 4 : 0], tile);
+  const float scale = KeyScale(r.ks[D == 256 ? s / 4 : 0], tile);
   u32x4 x;
   x[0] = Two<0>(w, scale);
   x[1] = Two<1>(w, scale);
@@ -509,9 +515,10 @@ template <uint32_t parts, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<D>& r,
                                      int32_t key0, f32x4 (&s)[R][2], Rows<parts, D, R>& w) {
   const float c = Capped<parts, R>(a, s);
-  // Unusual scale bytes of V: a token whose V has a scale of NaN gives NaN
-  // scores to the rows that see it and nothing to others (0 x NaN would reach
-  // every row of the tile); past the request's end any byte may lie.
+  // Unusual scale bytes of V: a token whose V has a scale of NaN, or one whose
+  // products pass the types' range (253, 254), gives NaN scores to the rows
+  // that see it and nothing to others (0 x NaN would reach every row of the
+  // tile); past the request's end any byte may lie.
   constexpr bool half = parts < 3;
   bool wide = false;
   if (__builtin_amdgcn_ballot_w64((OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1])) != 0) != 0) {
@@ -519,8 +526,8 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
       const uint32_t byte = (r.vs[j / 4] >> (8 * (j % 4))) & 255u;
-      nan |= (uint32_t)(byte == 255u) << j;
-      if (byte == 255u || KeyOf(key0, j) >= span.total)
+      nan |= (uint32_t)(byte >= 253u) << j;
+      if (byte >= 253u || KeyOf(key0, j) >= span.total)
         r.vs[j / 4] = (r.vs[j / 4] & ~(255u << (8 * (j % 4)))) | 127u << (8 * (j % 4));
     }
 #pragma unroll

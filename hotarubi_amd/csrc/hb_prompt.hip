@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void OpenKernel(const AttnArgs a) {
 #pragma unroll
     for (uint32_t e = 0; e < D / 32; ++e) {
       const uint32_t word = tile * (D / 32) + e, w = r.k[word / 4][word % 4];
-      const float scale = ScaleOf(r.ks[D == 256 ? e / 4 : 0], tile);
+      const float scale = KeyScale(r.ks[D == 256 ? e / 4 : 0], tile);
       u32x4 x;
       x[0] = TwoAs<0, parts == 2>(w, scale);
       x[1] = TwoAs<1, parts == 2>(w, scale);

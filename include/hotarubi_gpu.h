@@ -556,8 +556,9 @@ int hb_rows_async(hb_ctx* ctx, const hb_rows_desc* desc);
  * The cache is uint8 [pages][heads][page_size / 32][34 dim], 16-byte aligned:
  * a record per 32 tokens of one head holding K codes (16 dim bytes), V codes
  * (16 dim), K scales (dim) and V scales (dim), elements E2M1 with an E8M0
- * scale per token and 32 columns (255: NaN).  With g = 0..3, n, c = 0..15 and
- * `chunk` counting 16-byte pieces:
+ * scale per token and 32 columns (255: NaN; hb_kv_append writes up to 252, and
+ * hb_kv_attention takes 253 and 254, whose products pass the tensors' types, as
+ * 255).  With g = 0..3, n, c = 0..15 and `chunk` counting 16-byte pieces:
  *   K codes  [chunk dim/64][g][n][16 B]: (g, n) holds, in chunk order, columns
  *            [g dim/4, (g + 1) dim/4) of token n and then of token 16 + n
  *   V codes  [chunk dim/64][g][c][16 B]: (g, c) holds columns
@@ -680,8 +681,8 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * requests' new tokens and keys; they choose the split of the work (a max_kv
  * that is too small costs time, no keys), and rows of a request past max_new
  * are not computed.  A block table entry that names
- * no page of the cache hides its keys.  A stored NaN (a scale of 255) makes
- * the rows that see its token NaN, no others.
+ * no page of the cache hides its keys.  A stored NaN (a scale of 253 or more)
+ * makes the rows that see its token NaN, no others.
  * Long caches are split over workgroups that meet in the context's workspace,
  * in a fixed order: results do not change from call to call.  Prompts keep
  * the records they look at in the workspace as operands while the call runs,

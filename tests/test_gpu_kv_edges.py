@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import hotarubi_amd as hb
-from test_gpu_kv import DEV, HALF, TINY, TYPES, build, rope_reference, say
+from test_gpu_kv import DEV, HALF, TINY, TYPES, build, record_map, rope_reference, say
 
 pytestmark = pytest.mark.gpu
 
@@ -56,6 +56,113 @@ def test_rotation_of_infinities_and_nans(gpu, dtype, dim, rot, interleaved):
             tail, there = x[..., rot:], ~x[..., rot:].isnan()
             assert same(out[..., rot:][there], tail[there])
             assert same(torch.signbit(out[..., rot:][there]), torch.signbit(tail[there]))
+
+
+# ------------------------------------------------------------- attention --
+
+def reference(s, scale, window, cap):
+    """fp64 rows and their tolerance, as test_gpu_kv's, but with what weights
+    too small for f16 lose (2^-32 of the largest weight each) by the columns'
+    own values, scale bytes of 253 and more as NaN, and caps above 64 off by
+    the score's own roundings instead of the cap's."""
+    q, cache, table = s["q"], s["cache"], s["table"]
+    tokens, hq, d = q.shape
+    group, half = hq // cache.shape[1], q.dtype is not torch.float32
+    at, col = record_map(d), torch.arange(d, device=DEV) % 2 * 4
+    grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device=DEV)
+    grid = torch.cat([grid, -grid])
+
+    def rows(rec, codes, scales):
+        e = rec[:, scales].double()
+        x = grid[(rec[:, codes].int() >> col) & 15] * torch.exp2(e - 127)
+        return torch.where(e >= 253, math.nan, x).reshape(-1, d)
+
+    out = torch.zeros((tokens, hq, d), dtype=torch.float64, device=DEV)
+    tol = torch.zeros_like(out)
+    cu, lens = s["cu"].tolist(), s["kv_lens"].tolist()
+    for b, total in enumerate(lens):
+        n = cu[b + 1] - cu[b]
+        if n == 0 or total == 0:
+            continue
+        mine = slice(cu[b], cu[b + 1])
+        key = torch.arange(total, device=DEV)
+        pos = total - n + torch.arange(n, device=DEV)[:, None]
+        see = (key <= pos) & (pos - key < window if window else key >= 0)
+        if s["prefix"] is not None:
+            see = see | (key < s["prefix"][b])
+        pages = table[b, :-(-total // (32 * cache.shape[2]))].long()
+        for h in range(cache.shape[1]):
+            rec = cache[pages, h].reshape(-1, 34 * d)
+            k, v = rows(rec, at[0], at[2])[:total], rows(rec, at[1], at[3])[:total]
+            dead = k.isnan().any(-1) | v.isnan().any(-1)
+            k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+            for g in range(h * group, (h + 1) * group):
+                x = q[mine, g].double()
+                y = x @ k.T * scale
+                ds = (d + 8) * 2.0**-24 * (x.abs() @ k.abs().T * abs(scale))
+                if cap:
+                    y = cap * torch.tanh(y / cap)
+                    ds = ds + (cap * 2.0**-21 if cap <= 64 else 2.0**-21 * y.abs())
+                y = torch.where(dead, math.nan, y).masked_fill(~see, -math.inf)
+                top = torch.nan_to_num(y, nan=-math.inf).amax(-1, keepdim=True)
+                p = torch.exp(y - torch.where(top.isinf(), 0, top))
+                p = p / torch.where(see.any(-1, keepdim=True), p.sum(-1, keepdim=True), 1)
+                out[mine, g] = p @ v
+                ds = torch.where(see, ds, 0).amax(-1, keepdim=True)
+                tol[mine, g] = p @ v.abs() * (2 * ds + (2.0**-11 if half else 0) +
+                                              total * 2.0**-23 + 2.0**-21)
+                tol[mine, g] += 2.0**-32 * (see.double() @ v.abs())
+    return out, tol
+
+
+def compare(gpu, s, scale=None, window=0, cap=0.0):
+    q, d = s["q"], s["q"].shape[-1]
+    scale = d ** -0.5 if scale is None else scale
+    out = torch.full_like(q, 7.0)
+    hb.kv_attention(q=q, out=out, cache=s["cache"], table=s["table"], cu=s["cu"],
+                    kv_lens=s["kv_lens"], max_new=s["max_new"], max_kv=s["max_kv"], scale=scale,
+                    prefix=s["prefix"], window=window, softcap=cap, ctx=gpu)
+    want, tol = reference(s, scale, window, cap)
+    got = out.double()
+    assert same(got.isnan(), want.isnan())
+    tol = tol + HALF[q.dtype] * want.abs() + TINY[q.dtype]
+    most = torch.finfo(q.dtype).max  # what rounds past it is an infinity
+    over = want.abs() - tol > most * (1 + HALF[q.dtype])
+    assert (got[over] == torch.sign(want[over]) * math.inf).all()
+    there = ~want.isnan() & (want.abs() + tol < most)
+    worst = ((got - want).abs() / tol)[there].max().item() if there.any() else 0.0
+    assert worst <= 1, f"{worst} of the tolerance"
+
+
+# few rows; waves with rows of their own; prompts: (requests, K/V heads), a query head each
+ROWS = {"one": ([(300, 1, 0), (270, 1, 10)], 2), "rows": ([(300, 90, 0), (270, 70, 10)], 16),
+        "prompt": ([(300, 200, 0), (270, 200, 10)] * 4, 40)}
+
+
+def set_scale(s, b, token, which, value, block=None):
+    """Scale bytes of K (2) or V (3) of a request's token, of all heads."""
+    at = record_map(s["q"].shape[-1])[which, token % 32]
+    at = at.unique() if block is None else at[32 * block:32 * block + 1]
+    page, group = token // 32 // s["cache"].shape[2], token // 32 % s["cache"].shape[2]
+    s["cache"][int(s["table"][b, page]), :, group, at] = value
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", list(ROWS))
+def test_scales_past_the_types_range(gpu, dtype, dim, rows):
+    """Scale bytes of 253 and 254, whose products pass bf16 and fp32, make the
+    rows that see their token NaN and no others."""
+    say("scales past the range", dtype, dim, rows)
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    requests, hk = ROWS[rows]
+    s = build(gen, requests, 32, hk, dim, dtype, hk)
+    for which in (2, 3):
+        for b, token, value in ((0, 299 if rows == "one" else 230, 253), (1, 20, 254)):
+            t = dict(s, cache=s["cache"].clone())
+            set_scale(t, b, token, which, value, block=dim // 32 - 1)
+            compare(gpu, t)
+            compare(gpu, t, window=64)
 
 
 # --------------------------------------------------------------- streams --
