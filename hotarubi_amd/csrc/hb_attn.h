@@ -41,6 +41,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // A row's maximum moves once a score passes it by this much (in powers of
 // two): between moves P is at most 2^8, and nothing is rescaled.
 constexpr float kSlack = 8.f, kLift = 7.f;
+// What the maximum is set too high by once a wave has met values that sums of
+// such weights could carry past fp32: P is below 2^-48 then, 2^31 keys' sum
+// below 2^-17, and no value is too large.
+constexpr float kRoom = 64.f;
 
 // ---------------------------------------------------------------- records --
 
@@ -125,7 +129,8 @@ __device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, 
 // P V in f16 for the 16-bit types: P's error is then below the output's
 // rounding (2^-12 of each weight against bf16's 2^-9), and V is exact in f16
 // wherever its scale bytes lie in [104, 140] (0.5 x 2^-23 .. 6 x 2^13).  Other
-// records take V in bf16 and each f16 weight as two bf16 parts.  fp32 takes three bf16 parts of P.
+// records take V in bf16 and each weight as two bf16 parts (2^-16 of it).  fp32
+// takes three bf16 parts of P.
 template <bool half>
 struct Value;
 template <>
@@ -140,6 +145,11 @@ struct Value<false> {
 __device__ __forceinline__ uint32_t OutsideHalf(uint32_t x) {
   const uint32_t low = x & 0x7F7F7F7Fu;
   return (((low + 0x73737373u) & x) | ~((low + 0x18181818u) | x)) & 0x80808080u;
+}
+// Nonzero where one of the 4 bytes is 206 or more: values of up to 2^81 do not
+// pass fp32 in sums of 2^31 weights of 2^15.
+__device__ __forceinline__ uint32_t Large(uint32_t x) {
+  return ((x & 0x7F7F7F7Fu) + 0x32323232u) & x & 0x80808080u;
 }
 
 template <int sel, bool half>
@@ -315,6 +325,7 @@ template <uint32_t D, uint32_t R>
 struct State {
   f32x4 o[R][D / 16];
   float m[R], l[R];
+  float slack;  // kSlack, less kRoom once large values were met
   Sight see[R];
   int32_t see_all, see_from, see_pre;  // every row sees keys see_from .. see_all, and < see_pre
 };
@@ -343,6 +354,7 @@ __device__ __forceinline__ void Begin(const AttnArgs& a, const RowSet& set, Stat
 #pragma unroll
     for (uint32_t c = 0; c < D / 16; ++c) w.o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  w.slack = kSlack;
   w.see_all = min(span.total - span.count + (int32_t)(set.row0 / set.group), span.total - 1);
   w.see_from = SightOf(span, set.last / set.group, true, a.window).lo;
   w.see_pre = span.prefix;
@@ -464,22 +476,24 @@ __device__ __forceinline__ float Max3(float a, float b, float c) {
 }
 
 // The running maximum of tile t moves where a score passes it by kSlack, and
-// what it had so far shrinks; true where it did, by *shrink.
+// what it had so far shrinks.  With `slack` kSlack - kRoom it moves to kRoom
+// above the largest score.
 template <uint32_t D, uint32_t R>
-__device__ __forceinline__ bool Raise(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
-                                      float* shrink) {
+__device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
+                                      float slack) {
   const f32x4 x = s[0], y = s[1];
   const float top =
       c * Max3(Max3(x[0], x[1], x[2]), Max3(x[3], y[0], y[1]), fmaxf(y[2], y[3]));
-  if (__builtin_amdgcn_ballot_w64(top > w.m[t] + kSlack) == 0) return false;
-  const float m = fmaxf(w.m[t], RowMax(top));
+  if (__builtin_amdgcn_ballot_w64(top > w.m[t] + slack) == 0) return;
+  float m = RowMax(top);
+  if (slack != kSlack) m += kSlack - slack;
+  m = fmaxf(w.m[t], m);
   // rows that have seen nothing yet stay at -inf, with o and l zero
-  *shrink = m == w.m[t] ? 1.f : __builtin_amdgcn_exp2f(w.m[t] - m);
+  const float shrink = m == w.m[t] ? 1.f : __builtin_amdgcn_exp2f(w.m[t] - m);
   w.m[t] = m;
-  w.l[t] *= *shrink;
+  w.l[t] *= shrink;
 #pragma unroll
-  for (uint32_t i = 0; i < D / 16; ++i) w.o[t][i] *= *shrink;
-  return true;
+  for (uint32_t i = 0; i < D / 16; ++i) w.o[t][i] *= shrink;
 }
 // What a row's weights are relative to.
 __device__ __forceinline__ float Reference(float m) {
@@ -537,29 +551,24 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j)
         if (nan >> j & 1) s[t][j / 4][j % 4] = __builtin_nanf("");
+    if (__builtin_amdgcn_ballot_w64((Large(r.vs[0]) | Large(r.vs[1])) != 0) != 0)
+      w.slack = kSlack - kRoom;
     wide = half && __builtin_amdgcn_ballot_w64(
                        (OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1])) != 0) != 0;
   }
+  // weights below 2^-48 are none in f16
+  if (half && w.slack != kSlack) wide = true;
   Hide<D, R>(w, key0, s);
   typename Value<half>::type pt[R][half ? 1 : parts];
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
-    float p[8], shrink;
-    Raise<D, R>(w, t, s[t], c, &shrink);
+    float p[8];
+    Raise<D, R>(w, t, s[t], c, w.slack);
     Weights<D, R>(w, t, s[t], c, p);
-    if constexpr (half) pt[t][0] = HalfWeights(p);
-    else ToParts<parts>(p, pt[t]);
-  }
-  __builtin_amdgcn_sched_barrier(0);
-  if constexpr (half) {
-    if (wide) {  // V in bf16, on the two bf16 parts of an f16 weight
-#pragma unroll
-      for (uint32_t t = 0; t < R; ++t) {
-        float p[8];
+    if constexpr (half) {
+      if (wide) {  // V in bf16, on two bf16 parts of a weight
         bf16x8 part[2];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = (float)pt[t][0][j];
         ToParts<2>(p, part);
 #pragma unroll
         for (uint32_t i = 0; i < D / 32; ++i) {
@@ -571,10 +580,15 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
             w.o[t][2 * i + h] = Product(v[h], part[0], w.o[t][2 * i + h]);
           }
         }
+      } else {
+        pt[t][0] = HalfWeights(p);
       }
-      return;
+    } else {
+      ToParts<parts>(p, pt[t]);
     }
   }
+  __builtin_amdgcn_sched_barrier(0);
+  if (half && wide) return;
 #pragma unroll
   for (uint32_t i = 0; i < D / 32; ++i) {
     typename Value<half>::type v[2];

@@ -238,6 +238,46 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
   }
   slow = __builtin_amdgcn_ballot_w64(slow) != 0;
   auto key_of = [&](uint32_t i) { return (int32_t)(32 * KvWalkRecord(walk, i)); };
+  // Scale bytes that f16 does not hold, or more records than were opened: the
+  // rows a tile at a time on the general steps.  (Here, before the loop, so that
+  // nothing of this stays in registers through it.)
+  if (slow) {
+#pragma unroll 1
+    for (uint32_t t = 0; t < R; ++t) {
+      const uint32_t r0 = row0 + t * 16;
+      if (r0 >= rows) return;
+      const RowSet one{span, group, head, r0, rows, min(r0 + 16, rows) - 1};
+      Rows<parts, D, 1> v;
+      Begin<D, 1>(a, one, v);
+      uint64_t from;
+      const bool valid = QueryAt<parts, D>(a, one, 0, &from);
+      Query<parts, D> again;
+      again.Load(a, from, valid);
+#pragma unroll
+      for (uint32_t i = 0; i < kSteps; ++i) {
+        bf16x8 x[parts];
+        again.Parts(a, i, x);
+#pragma unroll
+        for (uint32_t p = 0; p < parts; ++p) v.q[0][p][i] = x[p];
+      }
+#pragma unroll 1
+      for (uint32_t i = 0; i < count; ++i) {
+        const uint32_t record =
+            __builtin_amdgcn_readfirstlane(PageRecord(a, walk, row, head, i, count));
+        if (record == kNoRecord) continue;
+        const uint8_t* at_record = a.cache + (uint64_t)record * KvRecordBytes(D);
+        Record<D> r;
+        ReadKeys<D>(at_record, r);
+        ReadValues<D>(at_record, r);
+        f32x4 s[1][2];
+        Scores<parts, D, 1>(r, v, s);
+        Step<parts, D, 1>(a, span, r, key_of(i), s, v);
+      }
+      v.l[0] = RowSum(v.l[0]);
+      Finish<parts, D, 1>(a, one, v);
+    }
+    return;
+  }
   auto pages = [&](uint32_t i) { return PageRecord(a, walk, row, head, i + lane, count); };
   uint32_t base = 0, now = pages(0), after = count > 64 ? pages(64) : kNoRecord;
   auto hidden = [&](uint32_t i) {  // base <= i < base + 128
@@ -289,9 +329,9 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
                   lane * 16, stages_at + stage * (uint32_t)sizeof(Stage) + piece * 1024);
     }
   };
-  if (!slow && count > 0) fetch(0, 0);
+  if (count > 0) fetch(0, 0);
 #pragma unroll 1
-  for (uint32_t i = 0; i < count && !slow; i += 2) {
+  for (uint32_t i = 0; i < count; i += 2) {
     const uint32_t in = i / 2 % 2;
     const Stage& stage = stages[in];
     ring::WaitVm<0>();
@@ -328,8 +368,8 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
       f16x8 pt[R];
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t) {
-        float p[8], shrink;
-        Raise<D, R>(w, t, s[t], c, &shrink);
+        float p[8];
+        Raise<D, R>(w, t, s[t], c, kSlack);  // (V is within f16 here)
         Weights<D, R>(w, t, s[t], c, p);
         pt[t] = HalfWeights(p);
       }
@@ -341,82 +381,43 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
       }
     }
   }
-  if (!slow) {
 #pragma unroll
-    for (uint32_t t = 0; t < R; ++t) w.l[t] = RowSum(w.l[t]);
-    ring::WaitVm<0>();  // no load into LDS outlives its stage
-    if (!Whole(a.out, a.out_token, a.out_head)) {
-      if (has_rows) Finish<parts, D, R>(a, set, w);
-      return;
-    }
-    __syncthreads();  // the stages have been read
-    typedef typename TypeOf<parts>::four V;
-#pragma unroll
-    for (uint32_t t = 0; t < R; ++t) {
-      const float inv = w.l[t] == 0.f ? 0.f : 1.f / w.l[t];
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-        for (uint32_t c = 0; c < D / 16; c += 4) {
-          V y;
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j)
-            y[j] = (typename TypeOf<parts>::type)(w.o[t][c + j][i] * inv);
-          const uint32_t col = (4 * g + i) * (D / 16) + c;
-          *reinterpret_cast<V*>(rows_lds + t * (32 * D) + PieceAt<D>(n, col / 8) + col % 8 * 2) = y;
-        }
-    }
-    WaveFence();
-#pragma unroll
-    for (uint32_t t = 0; t < R; ++t)
-#pragma unroll
-      for (uint32_t i = 0; i < D / 32; ++i) {
-        const RowPiece<D> mine(i);
-        const uint32_t row = row0 + t * 16 + mine.row;
-        if (row < rows)
-          *reinterpret_cast<u32x4*>(static_cast<typename TypeOf<parts>::type*>(a.out) +
-                                    RowStart<D>(set, row, a.out_token, a.out_head) +
-                                    mine.piece * 8) = *reinterpret_cast<const u32x4*>(
-              rows_lds + t * (32 * D) + PieceAt<D>(mine.row, mine.piece));
-      }
+  for (uint32_t t = 0; t < R; ++t) w.l[t] = RowSum(w.l[t]);
+  ring::WaitVm<0>();  // no load into LDS outlives its stage
+  if (!Whole(a.out, a.out_token, a.out_head)) {
+    if (has_rows) Finish<parts, D, R>(a, set, w);
     return;
   }
-  // scale bytes that f16 does not hold: the rows again, a tile at a time, on
-  // the general steps
-#pragma unroll 1
+  __syncthreads();  // the stages have been read
+  typedef typename TypeOf<parts>::four V;
+#pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
-    const uint32_t r0 = row0 + t * 16;
-    if (r0 >= rows) return;
-    const RowSet one{span, group, head, r0, rows, min(r0 + 16, rows) - 1};
-    Rows<parts, D, 1> v;
-    Begin<D, 1>(a, one, v);
-    uint64_t from;
-    const bool valid = QueryAt<parts, D>(a, one, 0, &from);
-    Query<parts, D> again;
-    again.Load(a, from, valid);
+    const float inv = w.l[t] == 0.f ? 0.f : 1.f / w.l[t];
 #pragma unroll
-    for (uint32_t i = 0; i < kSteps; ++i) {
-      bf16x8 x[parts];
-      again.Parts(a, i, x);
+    for (uint32_t i = 0; i < 4; ++i)
 #pragma unroll
-      for (uint32_t p = 0; p < parts; ++p) v.q[0][p][i] = x[p];
-    }
-#pragma unroll 1
-    for (uint32_t i = 0; i < count; ++i) {
-      const uint32_t record =
-          __builtin_amdgcn_readfirstlane(PageRecord(a, walk, row, head, i, count));
-      if (record == kNoRecord) continue;
-      const uint8_t* at_record = a.cache + (uint64_t)record * KvRecordBytes(D);
-      Record<D> r;
-      ReadKeys<D>(at_record, r);
-      ReadValues<D>(at_record, r);
-      f32x4 s[1][2];
-      Scores<parts, D, 1>(r, v, s);
-      Step<parts, D, 1>(a, span, r, key_of(i), s, v);
-    }
-    v.l[0] = RowSum(v.l[0]);
-    Finish<parts, D, 1>(a, one, v);
+      for (uint32_t c = 0; c < D / 16; c += 4) {
+        V y;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+          y[j] = (typename TypeOf<parts>::type)(w.o[t][c + j][i] * inv);
+        const uint32_t col = (4 * g + i) * (D / 16) + c;
+        *reinterpret_cast<V*>(rows_lds + t * (32 * D) + PieceAt<D>(n, col / 8) + col % 8 * 2) = y;
+      }
   }
+  WaveFence();
+#pragma unroll
+  for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+    for (uint32_t i = 0; i < D / 32; ++i) {
+      const RowPiece<D> mine(i);
+      const uint32_t row = row0 + t * 16 + mine.row;
+      if (row < rows)
+        *reinterpret_cast<u32x4*>(static_cast<typename TypeOf<parts>::type*>(a.out) +
+                                  RowStart<D>(set, row, a.out_token, a.out_head) +
+                                  mine.piece * 8) = *reinterpret_cast<const u32x4*>(
+            rows_lds + t * (32 * D) + PieceAt<D>(mine.row, mine.piece));
+    }
 }
 
 }  // namespace

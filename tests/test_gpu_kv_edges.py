@@ -3,6 +3,7 @@ that are not finite, sizes at the ends of their range, against plain 64-bit
 implementations."""
 from __future__ import annotations
 
+import functools
 import math
 import threading
 
@@ -10,9 +11,11 @@ import pytest
 import torch
 
 import hotarubi_amd as hb
-from test_gpu_kv import DEV, HALF, TINY, TYPES, build, record_map, rope_reference, say
+from test_gpu_kv import DEV, HALF, TINY, TYPES, build, rope_reference, say
+from test_gpu_kv import record_map as make_record_map
 
 pytestmark = pytest.mark.gpu
+record_map = functools.lru_cache(make_record_map)
 
 
 def same(a, b):
@@ -141,10 +144,10 @@ ROWS = {"one": ([(300, 1, 0), (270, 1, 10)], 2), "rows": ([(300, 90, 0), (270, 7
 
 def set_scale(s, b, token, which, value, block=None):
     """Scale bytes of K (2) or V (3) of a request's token, of all heads."""
-    at = record_map(s["q"].shape[-1])[which, token % 32]
-    at = at.unique() if block is None else at[32 * block:32 * block + 1]
+    at = record_map(s["q"].shape[-1])[which, token % 32, ::32]
+    at = at if block is None else at[block:block + 1]
     page, group = token // 32 // s["cache"].shape[2], token // 32 % s["cache"].shape[2]
-    s["cache"][int(s["table"][b, page]), :, group, at] = value
+    s["cache"][s["table"][b, page].long(), :, group, at] = value
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -163,6 +166,34 @@ def test_scales_past_the_types_range(gpu, dtype, dim, rows):
             set_scale(t, b, token, which, value, block=dim // 32 - 1)
             compare(gpu, t)
             compare(gpu, t, window=64)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", list(ROWS))
+def test_values_of_any_size(gpu, dtype, dim, rows):
+    """V from the smallest scale to the largest that is stored (252), alone and
+    among ordinary tokens, in whole rows and in one block of 32 columns."""
+    say("values of any size", dtype, dim, rows)
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    requests, hk = ROWS[rows]
+    s = build(gen, requests, 32, hk, dim, dtype, hk)
+    for changes in ([(0, 3, 252)], [(0, 3, 206), (0, 4, 200)], [(0, 40, 230), (1, 250, 252)],
+                    [(0, 3, 180), (0, 70, 240), (0, 71, 252)], [(1, 33, 30)]):
+        for block in (None, 1):
+            t = dict(s, cache=s["cache"].clone())
+            for b, token, value in changes:
+                set_scale(t, b, token, 3, value, block)
+            compare(gpu, t)
+    for b, (keys, _, _) in enumerate(requests):  # every token alike, and rising
+        for t in range(keys):
+            set_scale(s, b, t, 3, 252)
+    compare(gpu, s)
+    compare(gpu, s, scale=3.0)
+    for b, (keys, _, _) in enumerate(requests):
+        for t in range(keys):
+            set_scale(s, b, t, 3, 100 + 152 * t // keys)
+    compare(gpu, s)
 
 
 # --------------------------------------------------------------- streams --
