@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -1533,7 +1534,7 @@ int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
   if (int rc = CheckCache(d->cache)) return rc;
   if (d->q_heads < 1 || d->q_heads % d->cache.heads != 0)
     return Fail(HB_EINVAL, "%u query heads over %u K/V heads", d->q_heads, d->cache.heads);
-  if (!(d->scale == d->scale) || !(d->softcap >= 0.f))
+  if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.f)
     return Fail(HB_EINVAL, "scale %g, softcap %g", (double)d->scale, (double)d->softcap);
   if (d->tokens == 0 || d->batch == 0 || d->max_new == 0) return ctx ? HB_OK : Enter(ctx);
   if (!d->q || !d->out || !d->cu || !d->kv_lens || (d->columns > 0 && !d->table))

@@ -435,8 +435,10 @@ __device__ __forceinline__ float Tanh(float x) {
 
 // Scores to powers of two: they are s c with the c returned.  Capped ones
 // (softcap tanh(s scale / softcap)) are done here; the 16-bit types take the
-// plain 1 - 2 / (1 + e^2x), off by 2^-22 of the cap.
-template <uint32_t parts, uint32_t R>
+// plain 1 - 2 / (1 + e^2x), off by 2^-22 of the cap, while that is at most
+// kPlainCap and the scores so off by 2^-16.
+constexpr float kPlainCap = 64.f;
+template <bool fine, uint32_t R>
 __device__ __forceinline__ float Capped(const AttnArgs& a, f32x4 (&s)[R][2]) {
   if (!(a.cap > 0.f)) return a.scale * kLog2e;
   const float in = a.scale / a.cap, out = a.cap * kLog2e;
@@ -444,7 +446,7 @@ __device__ __forceinline__ float Capped(const AttnArgs& a, f32x4 (&s)[R][2]) {
   for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j)
-      s[t][j / 4][j % 4] = out * Tanh<parts == 3>(in * s[t][j / 4][j % 4]);
+      s[t][j / 4][j % 4] = out * Tanh<fine>(in * s[t][j / 4][j % 4]);
   return 1.f;
 }
 
@@ -528,7 +530,8 @@ __device__ __forceinline__ f16x8 HalfWeights(const float* p) {
 template <uint32_t parts, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<D>& r,
                                      int32_t key0, f32x4 (&s)[R][2], Rows<parts, D, R>& w) {
-  const float c = Capped<parts, R>(a, s);
+  const float c =
+      parts == 3 || a.cap > kPlainCap ? Capped<true, R>(a, s) : Capped<false, R>(a, s);
   // Unusual scale bytes of V: a token whose V has a scale of NaN, or one whose
   // products pass the types' range (253, 254), gives NaN scores to the rows
   // that see it and nothing to others (0 x NaN would reach every row of the

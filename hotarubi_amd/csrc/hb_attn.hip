@@ -568,6 +568,14 @@ hipError_t LaunchAttention(const AttnArgs& in, Workspace& ws, hipStream_t stream
   // the scores
   a.sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;
   a.scale = a.scale == 0.f ? 1.f : std::abs(a.scale);
+  // A cap past 2^60 changes no score below 2^48 in 32 bits, and larger scores
+  // that differ are 2^24 apart; one below 2^-60 leaves all weights alike.
+  if (a.cap > 0x1p60f) {
+    a.cap = 0.f;
+  } else if (a.cap > 0.f && a.cap < 0x1p-60f) {
+    a.cap = a.sign = 0.f;
+    a.scale = 1.f;
+  }
   const Division how = Divide(a);
   if (how.way == Division::kByPrompt) return LaunchPrompt(a, ws, stream);
   switch (a.type) {

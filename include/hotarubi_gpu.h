@@ -670,7 +670,8 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * (j < kv_lens[b]) if
  *   j <= p and (window == 0 or p - j < window), or j < prefix[b];
  * query head h reads K/V head h / (q_heads / heads).  Scores are
- * scale * q.k, softcap * tanh(scale * q.k / softcap) where softcap > 0;
+ * scale * q.k, softcap * tanh(scale * q.k / softcap) where softcap > 0 (both
+ * finite);
  *   out = sum_j softmax(scores)_j v_j, 0 for a row that sees no key.
  * q and out are [tokens][q_heads][dim] of `type`, strides in elements.  Scores,
  * maxima and sums are in 32 bits, and q and the cache's values enter the

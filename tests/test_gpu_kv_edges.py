@@ -196,6 +196,21 @@ def test_values_of_any_size(gpu, dtype, dim, rows):
     compare(gpu, s)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", list(ROWS))
+def test_caps_of_any_size(gpu, dtype, dim, rows):
+    """A cap far above the scores leaves them as they are, one far below makes
+    them alike; scores of ordinary size throughout."""
+    say("caps", dtype, dim, rows)
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    requests, hk = ROWS[rows]
+    s = build(gen, requests, 32, hk, dim, dtype, hk)
+    for cap in (1e-38, 1e-20, 1e-3, 5.0, 64.0, 65.0, 1000.0, 1e5, 1e7, 1e15, 1e19, 1e30, 3e38):
+        compare(gpu, s, cap=cap)
+    compare(gpu, s, cap=1e5, scale=-1.0)
+
+
 # --------------------------------------------------------------- streams --
 
 def attend(s, out, **kw):

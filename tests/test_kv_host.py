@@ -288,3 +288,9 @@ def test_without_a_context_tensors_must_be_on_a_gpu():
             (lambda: hb.kv_attention(q=rows, out=rows, cache=cache(), table=ints(1, 1), cu=ints(2),
                                      kv_lens=ints(1), max_new=5, max_kv=64, scale=1.0), "q")]:
         refused(call, f"{name} is on cpu, not on a GPU")
+
+
+def test_scales_and_caps_that_are_not_finite_are_refused():
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        refused(lambda: attention(scale=bad), "scale")
+        refused(lambda: attention(softcap=bad), "softcap")
