@@ -37,9 +37,11 @@ DEVICE_FLAGS = [
 # arguments (pointers and sizes, 13 dwords) are preloaded into SGPRs by the
 # hardware, so its first operand loads need no argument round trip.
 # hb_kv.hip: cache rows keep FP32 subnormals, which MXFP4's smallest scales
-# reach, and its tensors are ordinary floats rather than the NPU's.
+# reach, and its tensors are ordinary floats rather than the NPU's; so do the
+# attention kernels that read them.
 SOURCE_FLAGS = {"hb_skinny.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=11"],
-                "hb_kv.hip": ["-fno-gpu-flush-denormals-to-zero"]}
+                **dict.fromkeys(["hb_kv.hip", "hb_attn.hip", "hb_prompt.hip"],
+                                ["-fno-gpu-flush-denormals-to-zero"])}
 
 
 def build(asm: bool = False, verbose: bool = False) -> str:

@@ -675,7 +675,7 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  *   out = sum_j softmax(scores)_j v_j, 0 for a row that sees no key.
  * q and out are [tokens][q_heads][dim] of `type`, strides in elements.  Scores,
  * maxima and sums are in 32 bits, and q and the cache's values enter the
- * products exactly.  The softmax's weights enter theirs in f16 for bf16 and
+ * products exactly, subnormal ones too (fp32 q to 2^-133).  The softmax's weights enter theirs in f16 for bf16 and
  * fp16 tensors (each off by 2^-12 of its value at most, their sum is of the
  * unrounded ones) and as three bf16 parts for fp32 ones (2^-24).
  * Rows outside every request are not written.  max_new and max_kv bound the

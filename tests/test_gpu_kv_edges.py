@@ -197,6 +197,40 @@ def test_values_of_any_size(gpu, dtype, dim, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_one_key_gives_its_value(gpu, dtype):
+    """One key, scale byte by scale byte: the row is the stored value, rounded."""
+    say("one key", dtype)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    requests = [(1, 1, 0)] * 253
+    s = build(gen, requests, 32, 2, 64, dtype, 4)
+    for b in range(253):
+        set_scale(s, b, 0, 3, b)
+    compare(gpu, s)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", list(ROWS))
+def test_subnormal_queries(gpu, dtype, dim, rows):
+    """Queries that are subnormal in a 16-bit type, and those of 2^-110 in fp32
+    (below that the third bf16 part is subnormal and loses bits), on keys as
+    large as they are small, give the scores of their products."""
+    say("subnormal queries", dtype, dim, rows)
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    requests, hk = ROWS[rows]
+    s = build(gen, requests, 32, hk, dim, dtype, hk)
+    small, scale = {torch.float16: (2.0**-17, 138), torch.bfloat16: (2.0**-128, 250),
+                    torch.float32: (2.0**-108, 230)}[dtype]
+    s["q"] = (s["q"].float() * small).to(dtype)
+    if dtype is torch.float32:
+        s["q"] += torch.copysign(torch.full_like(s["q"], 2.0**-110), s["q"])
+    else:
+        assert (s["q"].abs() < torch.finfo(dtype).smallest_normal).any()
+    s["cache"][..., 32 * dim:33 * dim] = scale
+    compare(gpu, s)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("rows", list(ROWS))
 def test_caps_of_any_size(gpu, dtype, dim, rows):
