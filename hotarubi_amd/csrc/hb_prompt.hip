@@ -242,8 +242,9 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
   auto key_of = [&](uint32_t i) { return (int32_t)(32 * KvWalkRecord(walk, i)); };
   // Scale bytes that f16 does not hold, or more records than were opened: the
   // rows a tile at a time on the general steps.  (Here, before the loop, so that
-  // nothing of this stays in registers through it.)
-  if (slow) {
+  // nothing of this stays in registers through it; and told to be unlikely, so
+  // that its code lies behind: short prompts at D 64 36.9 us for 38.2.)
+  if (__builtin_expect(slow, 0)) {
 #pragma unroll 1
     for (uint32_t t = 0; t < R; ++t) {
       const uint32_t r0 = row0 + t * 16;
