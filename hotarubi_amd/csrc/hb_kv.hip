@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kThreads) void PlanKernel(const PlanArgs a) {
       const uint32_t i = tid * kPlanEach + j;
       at += more[j];
       const uint32_t used = Pages(len[j], page), want = Pages(len[j] + more[j], page);
-      const bool f = want <= a.columns && at <= a.size;
+      const bool f = want <= a.columns && at <= a.size && len[j] + more[j] <= 0x7FFFFFFFu;
       need[j] = f ? want - used : 0;
       fits |= (uint32_t)f << j;
       sum += need[j];

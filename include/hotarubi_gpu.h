@@ -576,8 +576,9 @@ typedef enum hb_type { HB_TYPE_F32 = 0, HB_TYPE_BF16 = 1, HB_TYPE_F16 = 2 } hb_t
  * for them are taken from the top of the stack free_pages[0 .. *free_count)
  * in the order of the requests, and entered into the table.  A request is
  * refused (its tokens get slot -1, its pages are not taken) if its pages pass
- * the table's columns, its tokens `size`, or the pages wanted by it and the
- * requests before it, whether they got them or not, the free ones.
+ * the table's columns, its keys 2^31 - 1, its tokens `size`, or the pages
+ * wanted by it and the requests before it, whether they got them or not, the
+ * free ones.
  *   table      int32 [batch][columns], rows table_stride elements apart;
  *              entries of new pages are written, no others
  *   cu         int32 [batch + 1]: 0 and the running sum of new_tokens

@@ -7,11 +7,12 @@ import functools
 import math
 import threading
 
+import numpy as np
 import pytest
 import torch
 
 import hotarubi_amd as hb
-from test_gpu_kv import DEV, HALF, TINY, TYPES, build, rope_reference, say
+from test_gpu_kv import DEV, HALF, TINY, TYPES, build, rope_reference, run_plan, say
 from test_gpu_kv import record_map as make_record_map
 
 pytestmark = pytest.mark.gpu
@@ -59,6 +60,26 @@ def test_rotation_of_infinities_and_nans(gpu, dtype, dim, rot, interleaved):
             tail, there = x[..., rot:], ~x[..., rot:].isnan()
             assert same(out[..., rot:][there], tail[there])
             assert same(torch.signbit(out[..., rot:][there]), torch.signbit(tail[there]))
+
+
+# ------------------------------------------------------------------ plan --
+
+def test_lengths_past_31_bits_are_refused(gpu):
+    """A request whose keys would pass 2^31 - 1 is refused like one whose pages
+    pass the table; the one beside it goes on."""
+    say("plan, lengths past 31 bits")
+    most, page, columns = 2**31 - 1, 1 << 20, 2060
+    for lens, new, fine in (([most - 3, 5], [3, 2], 1), ([most - 3, 5], [4, 2], 0),
+                            ([most, 5], [1, 2], 0), ([most, 5], [0, 2], 1)):
+        table = np.full((2, columns), -1)
+        table[0, :2048], table[1, 0] = 1, 3
+        got = run_plan(gpu, lens, new, [8, 9], 2, table, page, 6)
+        _, cu, kv, slots, positions, status = [g.tolist() for g in got]
+        assert cu == [0, new[0], new[0] + 2] and status == [0, 1 - fine]
+        assert kv == [lens[0] + (new[0] if fine else 0), 7]
+        assert slots[new[0]:new[0] + 2] == [3 * page + 5, 3 * page + 6]
+        assert (slots[0] >= 0) == (fine == 1) or new[0] == 0
+        assert positions[new[0] + 2:] == [-1] * (4 - new[0])
 
 
 # ------------------------------------------------------------- attention --
