@@ -67,7 +67,7 @@ EXPORTS = (
     "hb_image_base", "hb_linear_group_async",
     "hb_kv_plan", "hb_kv_plan_async", "hb_norm_rope", "hb_norm_rope_async", "hb_kv_append",
     "hb_kv_append_async", "hb_kv_read", "hb_kv_read_async", "hb_kv_attention",
-    "hb_kv_attention_async",
+    "hb_kv_attention_async", "hb_kv_attention_way",
 )
 
 
@@ -246,6 +246,7 @@ def lib():
             "hb_kv_read_async": (i, [vp, vp]),
             "hb_kv_attention": (i, [vp, vp]),
             "hb_kv_attention_async": (i, [vp, vp]),
+            "hb_kv_attention_way": (i, [vp, vp]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -932,6 +933,25 @@ def kv_read(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -
              ctx or _torch_context(k, "k"))
 
 
+def _attention_desc(dev: int, q, out, cache, table, cu, kv_lens, max_new, max_kv, scale, prefix,
+                    window, softcap) -> bytes:
+    kinds, i32, u8, _, _ = _types or _torch_types()
+    dtype = q.dtype
+    c = _cache(cache, u8, dev)
+    kind = _kind(kinds, q, "q")
+    qa, qt, qh = _heads(q, dtype, "q", None, dev)
+    tokens, heads, dim = q.shape
+    if dim != c[4]:
+        raise _invalid(f"q has heads of {dim} elements, the cache of {c[4]}")
+    oa, ot, oh = _heads(out, dtype, "out", q.shape, dev)
+    at, batch, columns, stride = _table(table, i32, dev)
+    return _desc(KV_ATTENTION_DESC, *c, qa, oa, qt, qh, ot, oh, at,
+                 _vector(cu, i32, "cu", batch + 1, dev),
+                 _vector(kv_lens, i32, "kv_lens", batch, dev),
+                 0 if prefix is None else _vector(prefix, i32, "prefix", batch, dev), kind, tokens,
+                 heads, batch, columns, stride, max_new, max_kv, window, scale, softcap)
+
+
 def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
                  prefix=None, window: int = 0, softcap: float = 0.0,
                  ctx: Context | None = None, sync: bool = True) -> None:
@@ -941,19 +961,24 @@ def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, s
     every row sees; window: keys a row sees, itself among them (0: all);
     softcap: scores as softcap * tanh(score / softcap)."""
     ctx = ctx or _torch_context(q, "q")
-    kinds, i32, u8, _, _ = _types or _torch_types()
-    dev, dtype = ctx.device, q.dtype
-    c = _cache(cache, u8, dev)
-    kind = _kind(kinds, q, "q")
-    qa, qt, qh = _heads(q, dtype, "q", None, dev)
-    tokens, heads, dim = q.shape
-    if dim != c[4]:
-        raise _invalid(f"q has heads of {dim} elements, the cache of {c[4]}")
-    oa, ot, oh = _heads(out, dtype, "out", q.shape, dev)
-    at, batch, columns, stride = _table(table, i32, dev)
-    d = _desc(KV_ATTENTION_DESC, *c, qa, oa, qt, qh, ot, oh, at,
-              _vector(cu, i32, "cu", batch + 1, dev),
-              _vector(kv_lens, i32, "kv_lens", batch, dev),
-              0 if prefix is None else _vector(prefix, i32, "prefix", batch, dev), kind, tokens,
-              heads, batch, columns, stride, max_new, max_kv, window, scale, softcap)
+    d = _attention_desc(ctx.device, q, out, cache, table, cu, kv_lens, max_new, max_kv, scale,
+                        prefix, window, softcap)
     _check((lib().hb_kv_attention if sync else lib().hb_kv_attention_async)(ctx.handle, d))
+
+
+#: hb_kv_way's `way`
+KV_WAYS = ("none", "rows", "splits", "shares", "prompt")
+KV_WAY = struct.Struct("@4IQ")
+
+
+def kv_attention_way(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
+                     prefix=None, window: int = 0, softcap: float = 0.0):
+    """hb_kv_attention_way: how kv_attention would divide this call's work on
+    the current device: (one of KV_WAYS, 16-row tiles of a wave, splits of the
+    keys, bytes of workspace).  Nothing is run."""
+    way = C.create_string_buffer(KV_WAY.size)
+    _check(lib().hb_kv_attention_way(
+        _attention_desc(q.get_device(), q, out, cache, table, cu, kv_lens, max_new, max_kv, scale,
+                        prefix, window, softcap), way))
+    kind, tiles, splits, _, workspace = KV_WAY.unpack(way.raw)
+    return KV_WAYS[kind], tiles, splits, workspace

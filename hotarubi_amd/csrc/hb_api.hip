@@ -1528,7 +1528,8 @@ int KvRows(hb_ctx* ctx, const hb_kv_rows_desc* d, bool read, bool sync) {
   return Launched(ctx, hb::LaunchKvRows(a, read, ctx->stream), "cache row launch", sync);
 }
 
-int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
+// The checks, and the launch's arguments; *empty where there are no rows.
+int AttentionArgs(const hb_kv_attention_desc* d, hb::AttnArgs* to, bool* empty) {
   if (!d) return Fail(HB_EINVAL, "null descriptor");
   if (int rc = CheckType(d->type)) return rc;
   if (int rc = CheckCache(d->cache)) return rc;
@@ -1536,7 +1537,8 @@ int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
     return Fail(HB_EINVAL, "%u query heads over %u K/V heads", d->q_heads, d->cache.heads);
   if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.f)
     return Fail(HB_EINVAL, "scale %g, softcap %g", (double)d->scale, (double)d->softcap);
-  if (d->tokens == 0 || d->batch == 0 || d->max_new == 0) return ctx ? HB_OK : Enter(ctx);
+  *empty = d->tokens == 0 || d->batch == 0 || d->max_new == 0;
+  if (*empty) return HB_OK;
   if (!d->q || !d->out || !d->cu || !d->kv_lens || (d->columns > 0 && !d->table))
     return Fail(HB_EINVAL, "null attention argument");
   const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;
@@ -1552,8 +1554,7 @@ int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
       (uint64_t)d->batch * d->cache.heads > 0x7FFFFFFFu)
     return Fail(HB_EINVAL, "attention of %u requests, %u new tokens, %u keys", d->batch, max_new,
                 d->max_kv);
-  if (int rc = Enter(ctx)) return rc;
-  hb::AttnArgs a{};
+  hb::AttnArgs& a = *to;
   a.q = d->q;
   a.out = d->out;
   a.q_token = d->q_token;
@@ -1580,6 +1581,15 @@ int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
   a.window = d->window;
   a.scale = d->scale;
   a.cap = d->softcap;
+  return HB_OK;
+}
+
+int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
+  hb::AttnArgs a{};
+  bool empty = false;
+  if (int rc = AttentionArgs(d, &a, &empty)) return rc;
+  if (empty) return ctx ? HB_OK : Enter(ctx);
+  if (int rc = Enter(ctx)) return rc;
   return Launched(ctx, hb::LaunchAttention(a, ctx->ws, ctx->stream), "attention launch", sync);
 }
 
@@ -1598,6 +1608,17 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* d) { return KvRows(ctx,
 int hb_kv_attention(hb_ctx* ctx, const hb_kv_attention_desc* d) { return KvAttention(ctx, d, true); }
 int hb_kv_attention_async(hb_ctx* ctx, const hb_kv_attention_desc* d) {
   return KvAttention(ctx, d, false);
+}
+int hb_kv_attention_way(const hb_kv_attention_desc* d, hb_kv_way* way) {
+  if (!way) return Fail(HB_EINVAL, "null way");
+  *way = hb_kv_way{};
+  hb::AttnArgs a{};
+  bool empty = false;
+  if (int rc = AttentionArgs(d, &a, &empty)) return rc;
+  if (empty) return HB_OK;
+  const hb::AttnWay how = hb::WayOfAttention(a);
+  *way = hb_kv_way{how.way, how.tiles_of_16, how.splits, 0, how.workspace};
+  return HB_OK;
 }
 
 }  // extern "C"

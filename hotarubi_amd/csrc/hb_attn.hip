@@ -497,57 +497,37 @@ Division Divide(const AttnArgs& a) {
 constexpr uint64_t kLeastShared = 64;  // records a CU
 
 template <uint32_t parts, uint32_t D, uint32_t R>
-hipError_t LaunchOf(AttnArgs& a, const Division& how, Workspace& ws, hipStream_t stream) {
+hipError_t LaunchOf(AttnArgs& a, const AttnWay& how, Workspace& ws, hipStream_t stream) {
   const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
-  const uint64_t tiles = (rows + R * 16 - 1) / (R * 16), pairs = (uint64_t)a.batch * a.heads;
-  a.splits = 1;
-  if (how.way == Division::kByRows) {
-    a.tiles = (uint32_t)((tiles + kWaves - 1) / kWaves);
-    const uint64_t grid = pairs * a.tiles;
-    if (grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
-    AttnKernel<parts, D, R, kRows><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
-    return hipGetLastError();
-  }
-  a.tiles = (uint32_t)tiles;
-  uint64_t records = ((uint64_t)a.max_kv + 31) / 32;
-  if (a.window > 0 && a.prefix == nullptr)
-    records = std::min<uint64_t>(records, ((uint64_t)a.window + 16 * R + 62) / 32);
-  records = std::max<uint64_t>(records, 1);
-  const uint64_t units = pairs * tiles, cus = (uint64_t)DeviceCus();
-  const uint64_t stored = std::min<uint64_t>(R * 16, rows);
-  // Requests of different lengths, with enough records that the sums over the
-  // requests (about 5 us a workgroup) are less than what uneven workgroups
-  // leave idle: 64 requests of 1,000 to 8,191 keys 84 us in splits, 72 in shares.
-  // (Every record that the tables have room for is counted in 32 bits, whatever
-  // kv_lens says.)
-  if (tiles == 1 && a.batch > 1 && a.batch <= kMaxShared && units * records >= kLeastShared * cus &&
-      units * std::max<uint64_t>((uint64_t)a.columns * a.groups, 1) < 0x7FFFFFFFu) {
-    a.splits = (uint32_t)(2 * cus);
-    const hipError_t err =
-        GrowWorkspace(ws, (units + a.splits) * stored * kPartial<D> * 4, stream);
-    if (err != hipSuccess) return err;
-    a.ws = ws.ptr + kSplitCounters;
-    AttnKernel<parts, D, R, kShares><<<a.splits, kThreads, 0, stream>>>(a);
-    JoinKernel<parts, D, R, kShares><<<(uint32_t)(units * stored), kThreads, 0, stream>>>(a);
-    return hipGetLastError();
-  }
-  a.split_records = (uint32_t)((records + how.splits - 1) / how.splits);
-  a.splits = (uint32_t)((records + a.split_records - 1) / a.split_records);
-  const uint64_t grid = units * a.splits;
+  const uint64_t pairs = (uint64_t)a.batch * a.heads, stored = std::min<uint64_t>(R * 16, rows);
+  const uint64_t grid = how.way == HB_KV_WAY_SHARES ? how.splits : pairs * how.tiles * how.splits;
   if (grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  if (a.splits > 1) {
-    const hipError_t err = GrowWorkspace(ws, grid * stored * kPartial<D> * 4, stream);
+  a.tiles = how.tiles;
+  a.splits = how.splits;
+  a.split_records = how.split_records;
+  if (how.workspace > 0) {
+    const hipError_t err = GrowWorkspace(ws, how.workspace, stream);
     if (err != hipSuccess) return err;
     a.ws = ws.ptr + kSplitCounters;
   }
-  AttnKernel<parts, D, R, kSplits><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
-  if (a.splits > 1)
-    JoinKernel<parts, D, R, kSplits><<<(uint32_t)(units * stored), kThreads, 0, stream>>>(a);
+  const uint32_t join = (uint32_t)(pairs * how.tiles * stored);
+  switch (how.way) {
+    case HB_KV_WAY_ROWS:
+      AttnKernel<parts, D, R, kRows><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
+      break;
+    case HB_KV_WAY_SHARES:
+      AttnKernel<parts, D, R, kShares><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
+      JoinKernel<parts, D, R, kShares><<<join, kThreads, 0, stream>>>(a);
+      break;
+    default:
+      AttnKernel<parts, D, R, kSplits><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
+      if (how.splits > 1) JoinKernel<parts, D, R, kSplits><<<join, kThreads, 0, stream>>>(a);
+  }
   return hipGetLastError();
 }
 
 template <uint32_t parts>
-hipError_t LaunchDim(AttnArgs& a, const Division& how, Workspace& ws, hipStream_t stream) {
+hipError_t LaunchDim(AttnArgs& a, const AttnWay& how, Workspace& ws, hipStream_t stream) {
   const bool two = how.tiles_of_16 == 2;
   switch (a.dim) {
     case 64:
@@ -561,6 +541,53 @@ hipError_t LaunchDim(AttnArgs& a, const Division& how, Workspace& ws, hipStream_
 }
 
 }  // namespace
+
+AttnWay WayOfAttention(const AttnArgs& a) {
+  const Division best = Divide(a);
+  AttnWay how{};
+  how.splits = 1;
+  const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
+  const uint64_t pairs = (uint64_t)a.batch * a.heads, cus = (uint64_t)DeviceCus();
+  if (best.way == Division::kByPrompt) {
+    how.way = HB_KV_WAY_PROMPT;
+    how.tiles_of_16 = PromptTiles(a.dim);
+    how.tiles = (uint32_t)((rows + PromptRows(a.dim) - 1) / PromptRows(a.dim));
+    how.workspace = PromptBytes(a);
+    return how;
+  }
+  how.tiles_of_16 = best.tiles_of_16;
+  const uint32_t of = 16 * how.tiles_of_16;
+  const uint64_t tiles = (rows + of - 1) / of;
+  if (best.way == Division::kByRows) {
+    how.way = HB_KV_WAY_ROWS;
+    how.tiles = (uint32_t)((tiles + kWaves - 1) / kWaves);
+    return how;
+  }
+  how.tiles = (uint32_t)tiles;
+  uint64_t records = ((uint64_t)a.max_kv + 31) / 32;
+  if (a.window > 0 && a.prefix == nullptr)
+    records = std::min<uint64_t>(records, ((uint64_t)a.window + of + 62) / 32);
+  records = std::max<uint64_t>(records, 1);
+  const uint64_t units = pairs * tiles;
+  const uint64_t part = std::min<uint64_t>(of, rows) * (a.dim + 4) * 4;  // bytes: kPartial
+  // Requests of different lengths, with enough records that the sums over the
+  // requests (about 5 us a workgroup) are less than what uneven workgroups
+  // leave idle: 64 requests of 1,000 to 8,191 keys 84 us in splits, 72 in shares.
+  // (Every record that the tables have room for is counted in 32 bits, whatever
+  // kv_lens says.)
+  if (tiles == 1 && a.batch > 1 && a.batch <= kMaxShared && units * records >= kLeastShared * cus &&
+      units * std::max<uint64_t>((uint64_t)a.columns * a.groups, 1) < 0x7FFFFFFFu) {
+    how.way = HB_KV_WAY_SHARES;
+    how.splits = (uint32_t)(2 * cus);
+    how.workspace = (units + how.splits) * part;
+    return how;
+  }
+  how.way = HB_KV_WAY_SPLITS;
+  how.split_records = (uint32_t)((records + best.splits - 1) / best.splits);
+  how.splits = (uint32_t)((records + how.split_records - 1) / how.split_records);
+  if (how.splits > 1) how.workspace = units * how.splits * part;
+  return how;
+}
 
 hipError_t LaunchAttention(const AttnArgs& in, Workspace& ws, hipStream_t stream) {
   AttnArgs a = in;
@@ -576,8 +603,8 @@ hipError_t LaunchAttention(const AttnArgs& in, Workspace& ws, hipStream_t stream
     a.cap = a.sign = 0.f;
     a.scale = 1.f;
   }
-  const Division how = Divide(a);
-  if (how.way == Division::kByPrompt) return LaunchPrompt(a, ws, stream);
+  const AttnWay how = WayOfAttention(a);
+  if (how.way == HB_KV_WAY_PROMPT) return LaunchPrompt(a, ws, stream);
   switch (a.type) {
     case HB_TYPE_BF16: return LaunchDim<1>(a, how, ws, stream);
     case HB_TYPE_F16: return LaunchDim<2>(a, how, ws, stream);

@@ -464,9 +464,18 @@ struct AttnArgs {
   uint32_t opened;
   uint8_t* opened_at;
 };
+// How a call is divided: HB_KV_WAY_*, 16-row tiles of a wave, tiles of a request
+// and K/V head, splits of a tile's records (workgroups of the shares), records
+// of a split, bytes of workspace.
+struct AttnWay {
+  uint32_t way, tiles_of_16, tiles, splits, split_records;
+  uint64_t workspace;
+};
+AttnWay WayOfAttention(const AttnArgs& a);
 hipError_t LaunchAttention(const AttnArgs& a, Workspace& ws, hipStream_t stream);
-// Many rows of 16-bit types (hb_prompt.hip); the rows of a workgroup, and the
-// workspace of a launch.
+// Many rows of 16-bit types (hb_prompt.hip): 16-row tiles of a wave, rows of a
+// workgroup, and the workspace of a launch.
+uint32_t PromptTiles(uint32_t dim);
 uint32_t PromptRows(uint32_t dim);
 uint64_t PromptBytes(const AttnArgs& a);
 hipError_t LaunchPrompt(const AttnArgs& a, Workspace& ws, hipStream_t stream);

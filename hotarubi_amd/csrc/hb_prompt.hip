@@ -425,6 +425,9 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
 
 }  // namespace
 
+uint32_t PromptTiles(uint32_t dim) {
+  return dim == 64 ? Shape<64>::kTiles : dim == 128 ? Shape<128>::kTiles : Shape<256>::kTiles;
+}
 uint32_t PromptRows(uint32_t dim) {
   return dim == 64 ? Shape<64>::kRows : dim == 128 ? Shape<128>::kRows : Shape<256>::kRows;
 }

@@ -689,7 +689,8 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * in a fixed order: results do not change from call to call.  Prompts keep
  * the records they look at in the workspace as operands while the call runs,
  * 128 dim bytes a record and 1 GiB at most.  A larger call than before grows
- * the workspace, so a first call belongs before a capture. */
+ * the workspace (hb_kv_attention_way tells its size), so a first call belongs
+ * before a capture. */
 typedef struct hb_kv_attention_desc {
   hb_kv_cache cache;
   const void* q;
@@ -705,6 +706,25 @@ typedef struct hb_kv_attention_desc {
 } hb_kv_attention_desc;
 int hb_kv_attention(hb_ctx* ctx, const hb_kv_attention_desc* desc);
 int hb_kv_attention_async(hb_ctx* ctx, const hb_kv_attention_desc* desc);
+
+/* How a call of hb_kv_attention divides its work on the current device, and
+ * what workspace it takes, without running it: the descriptor is checked as
+ * there, no memory that it names is read. */
+enum {
+  HB_KV_WAY_NONE = 0,   /* no rows */
+  HB_KV_WAY_ROWS = 1,   /* every wave rows of its own, over all their keys */
+  HB_KV_WAY_SPLITS = 2, /* a workgroup a tile of rows and a split of its keys */
+  HB_KV_WAY_SHARES = 3, /* workgroups of equal shares of all requests' keys */
+  HB_KV_WAY_PROMPT = 4  /* keys opened into the workspace once for all rows */
+};
+typedef struct hb_kv_way {
+  uint32_t way;
+  uint32_t tiles;  /* of 16 rows, of a wave */
+  uint32_t splits; /* of a tile's keys; with shares the workgroups */
+  uint32_t zero;
+  uint64_t workspace; /* bytes */
+} hb_kv_way;
+int hb_kv_attention_way(const hb_kv_attention_desc* desc, hb_kv_way* way);
 
 /* --------------------------------------------------------- formats -- */
 

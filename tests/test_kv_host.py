@@ -294,3 +294,32 @@ def test_scales_and_caps_that_are_not_finite_are_refused():
     for bad in (float("inf"), -float("inf"), float("nan")):
         refused(lambda: attention(scale=bad), "scale")
         refused(lambda: attention(softcap=bad), "softcap")
+
+
+def test_the_way_of_a_call_is_told_without_running_it():
+    """hb_kv_attention_way: sizes alone choose, no address is read (these are
+    in host memory), and what a call refuses it refuses."""
+    def way(batch, new, keys, hq, hk, dim, dtype, **kw):
+        q = torch.empty((1, 1, dim), dtype=dtype).expand(batch * new, hq, dim)
+        a = dict(q=q, out=q, cache=cache(heads=hk, dim=dim), table=ints(batch, keys // 64 + 1),
+                 cu=ints(batch + 1), kv_lens=ints(batch), max_new=new, max_kv=keys, scale=1.0)
+        a.update(kw)
+        return hb.kv_attention_way(**a)
+
+    f32, bf16 = torch.float32, torch.bfloat16
+    assert way(3, 0, 100, 4, 2, 64, bf16) == ("none", 0, 0, 0)
+    assert way(1, 1, 40, 8, 1, 64, f32) == ("splits", 1, 1, 0)
+    kind, tiles, splits, workspace = way(1, 1, 100000, 8, 1, 128, bf16)
+    assert (kind, tiles) == ("splits", 1) and workspace == splits * 8 * 132 * 4
+    kind, tiles, splits, workspace = way(24, 6, 12000, 8, 2, 128, f32)
+    assert (kind, tiles) == ("shares", 2) and workspace == (48 + splits) * 24 * 132 * 4
+    assert way(24, 60, 130, 32, 8, 64, f32)[:2] == ("rows", 2)
+    kind, tiles, _, workspace = way(16, 300, 500, 16, 2, 256, bf16)
+    assert (kind, tiles) == ("prompt", 1) and workspace == 16 * 32 * (128 * 256 + 4)
+    assert way(16, 300, 500, 16, 2, 256, f32)[0] == "rows"
+    refused(lambda: way(1, 1, 40, 8, 1, 64, f32, scale=float("nan")), "scale")
+    refused(lambda: way(1, 1, 40, 8, 1, 64, f32, cu=ints(3)), "cu")
+    lib = hb.lib()
+    assert lib.hb_kv_attention_way(None, None) == hb.HB_EINVAL and hb.last_error() == "null way"
+    assert lib.hb_kv_attention_way(None, bytes(hb.KV_WAY.size)) == hb.HB_EINVAL
+    assert hb.last_error() == "null descriptor"
