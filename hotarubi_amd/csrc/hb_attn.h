@@ -304,6 +304,16 @@ struct Query {
   }
 };
 
+// A finished value in the tensors' type: multiplied in fp32, then rounded.  (Left
+// to the compiler, fp16 rows are multiplied and rounded by one instruction on
+// some of the ways out and by two on others, which differ in the last bit now
+// and then: rows would depend on their alignment.)
+template <class T>
+__device__ __forceinline__ T Rounded(float x) {
+  asm("" : "+v"(x));
+  return (T)x;
+}
+
 template <uint32_t parts>
 __device__ __forceinline__ void StoreFour(const AttnArgs& a, uint64_t at, bool vec, f32x4 y) {
   typedef typename TypeOf<parts>::type T;
@@ -311,7 +321,7 @@ __device__ __forceinline__ void StoreFour(const AttnArgs& a, uint64_t at, bool v
   T* to = static_cast<T*>(a.out) + at;
   V z;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) z[j] = (T)y[j];
+  for (int j = 0; j < 4; ++j) z[j] = Rounded<T>(y[j]);
   if (vec) {
     *reinterpret_cast<V*>(to) = z;
   } else {

@@ -403,7 +403,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
         V y;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j)
-          y[j] = (typename TypeOf<parts>::type)(w.o[t][c + j][i] * inv);
+          y[j] = Rounded<typename TypeOf<parts>::type>(w.o[t][c + j][i] * inv);
         const uint32_t col = (4 * g + i) * (D / 16) + c;
         *reinterpret_cast<V*>(rows_lds + t * (32 * D) + PieceAt<D>(n, col / 8) + col % 8 * 2) = y;
       }

@@ -158,6 +158,12 @@ def compare(gpu, s, scale=None, window=0, cap=0.0):
     assert worst <= 1, f"{worst} of the tolerance"
 
 
+def attend(s, out, **kw):
+    hb.kv_attention(q=s["q"], out=out, cache=s["cache"], table=s["table"], cu=s["cu"],
+                    kv_lens=s["kv_lens"], max_new=s["max_new"], max_kv=s["max_kv"], scale=0.1,
+                    prefix=s["prefix"], **kw)
+
+
 # few rows; waves with rows of their own; prompts: (requests, K/V heads), a query head each
 ROWS = {"one": ([(300, 1, 0), (270, 1, 10)], 2), "rows": ([(300, 90, 0), (270, 70, 10)], 16),
         "prompt": ([(300, 200, 0), (270, 200, 10)] * 4, 40)}
@@ -266,13 +272,27 @@ def test_caps_of_any_size(gpu, dtype, dim, rows):
     compare(gpu, s, cap=1e5, scale=-1.0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_rows_do_not_depend_on_their_alignment(gpu, dtype, dim):
+    """The same bits in and out of rows aligned to 16 bytes, to 8 and to their
+    elements alone, in calls of few rows and of many."""
+    say("alignment", dtype, dim)
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    for requests, hq, hk in ([[(300, 3, 0), (90, 1, 0)], 8, 2], [[(500, 300, 0)] * 16, 16, 2]):
+        s = build(gen, requests, 64, hk, dim, dtype, hq)
+        tokens, outs = s["q"].shape[0], []
+        for pad in (0, 4, 1):
+            q, out = (torch.full((tokens, hq, dim + pad), 7.0, dtype=dtype, device=DEV)
+                      for _ in range(2))
+            q[..., pad:] = s["q"]
+            attend(dict(s, q=q[..., pad:]), out[..., pad:], ctx=gpu)
+            assert bool((out[..., :pad] == 7).all())
+            outs.append(out[..., pad:])
+        assert same(outs[0], outs[1]) and same(outs[0], outs[2])
+
+
 # --------------------------------------------------------------- streams --
-
-def attend(s, out, **kw):
-    hb.kv_attention(q=s["q"], out=out, cache=s["cache"], table=s["table"], cu=s["cu"],
-                    kv_lens=s["kv_lens"], max_new=s["max_new"], max_kv=s["max_kv"], scale=0.1,
-                    prefix=s["prefix"], **kw)
-
 
 def test_calls_without_a_context_run_on_torchs_current_stream(gpu):
     """After torch work that is still under way on the current stream, and
