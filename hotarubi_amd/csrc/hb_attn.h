@@ -99,11 +99,10 @@ __device__ __forceinline__ void ReadValues(const uint8_t* slot, Record<D>& r) {
 __device__ __forceinline__ float ScaleOf(uint32_t bytes, uint32_t i) {
   return __uint_as_float(((bytes >> (8 * i)) & 255u) << 23);
 }
-// The same of K.  Scales of 253 and 254, whose products pass the types' range,
-// count as 255: NaN.
-__device__ __forceinline__ float KeyScale(uint32_t bytes, uint32_t i) {
-  const uint32_t e = (bytes >> (8 * i)) & 255u;
-  return __uint_as_float(e >= 253u ? 255u << 23 : e << 23);
+// Scales of 253 and 254, whose products pass the types' range, count as 255,
+// NaN: nonzero where one of the 4 bytes is such a one.
+__device__ __forceinline__ uint32_t Nans(uint32_t x) {
+  return ((x & 0x7F7F7F7Fu) + 0x03030303u) & x & 0x80808080u;
 }
 
 // Two codes, byte `sel` of a word, as bf16 values (exact: E2M1 on E8M0 up to 252).
@@ -117,7 +116,7 @@ template <uint32_t D>
 __device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, uint32_t s) {
   const uint32_t word = tile * (D / 32) + s;
   const uint32_t w = r.k[word / 4][word % 4];
-  const float scale = KeyScale(r.ks[D == 256 ? s / 4 : 0], tile);
+  const float scale = ScaleOf(r.ks[D == 256 ? s / 4 : 0], tile);
   u32x4 x;
   x[0] = Two<0>(w, scale);
   x[1] = Two<1>(w, scale);
@@ -226,12 +225,21 @@ __device__ __forceinline__ void ToParts(const float* x, bf16x8* out) {
   }
 }
 
+// Largest of three (a NaN loses); of two where fmaxf would make sure of quiet
+// NaNs first.
+__device__ __forceinline__ float Max3(float a, float b, float c) {
+  float y;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+  return y;
+}
+__device__ __forceinline__ float Max2(float a, float b) { return Max3(a, b, b); }
+
 // Over the four lanes that share a row (n, 16 + n, 32 + n, 48 + n).
 __device__ __forceinline__ float RowMax(float x) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  x = Max2(__uint_as_float(a[0]), __uint_as_float(a[1]));
   auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return Max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float RowSum(float x) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -335,7 +343,7 @@ template <uint32_t D, uint32_t R>
 struct State {
   f32x4 o[R][D / 16];
   float m[R], l[R];
-  float slack;  // kSlack, less kRoom once large values were met
+  bool large;  // values were met that want kRoom
   Sight see[R];
   int32_t see_all, see_from, see_pre;  // every row sees keys see_from .. see_all, and < see_pre
 };
@@ -364,7 +372,7 @@ __device__ __forceinline__ void Begin(const AttnArgs& a, const RowSet& set, Stat
 #pragma unroll
     for (uint32_t c = 0; c < D / 16; ++c) w.o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  w.slack = kSlack;
+  w.large = false;
   w.see_all = min(span.total - span.count + (int32_t)(set.row0 / set.group), span.total - 1);
   w.see_from = SightOf(span, set.last / set.group, true, a.window).lo;
   w.see_pre = span.prefix;
@@ -443,21 +451,22 @@ __device__ __forceinline__ float Tanh(float x) {
   return y < 0.2f ? small : x != x ? x : large;
 }
 
-// Scores to powers of two: they are s c with the c returned.  Capped ones
-// (softcap tanh(s scale / softcap)) are done here; the 16-bit types take the
+// Scores to powers of two: they are s c with PowerOf's c, capped ones (softcap
+// tanh(s scale / softcap)) once Cap has been over them.  The 16-bit types take the
 // plain 1 - 2 / (1 + e^2x), off by 2^-22 of the cap, while that is at most
 // kPlainCap and the scores so off by 2^-16.
 constexpr float kPlainCap = 64.f;
 template <bool fine, uint32_t R>
-__device__ __forceinline__ float Capped(const AttnArgs& a, f32x4 (&s)[R][2]) {
-  if (!(a.cap > 0.f)) return a.scale * kLog2e;
+__device__ __forceinline__ void Cap(const AttnArgs& a, f32x4 (&s)[R][2]) {
   const float in = a.scale / a.cap, out = a.cap * kLog2e;
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j)
       s[t][j / 4][j % 4] = out * Tanh<fine>(in * s[t][j / 4][j % 4]);
-  return 1.f;
+}
+__device__ __forceinline__ float PowerOf(const AttnArgs& a) {
+  return a.cap > 0.f ? 1.f : a.scale * kLog2e;
 }
 
 // The record's key of a lane's score j.
@@ -480,26 +489,18 @@ __device__ __forceinline__ void Hide(const State<D, R>& w, int32_t key0, f32x4 (
     }
 }
 
-// Largest of three (a NaN loses).
-__device__ __forceinline__ float Max3(float a, float b, float c) {
-  float y;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
-  return y;
-}
-
 // The running maximum of tile t moves where a score passes it by kSlack, and
-// what it had so far shrinks.  With `slack` kSlack - kRoom it moves to kRoom
-// above the largest score.
+// what it had so far shrinks.  With `large` it stays kRoom above the scores.
 template <uint32_t D, uint32_t R>
 __device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
-                                      float slack) {
+                                      bool large) {
   const f32x4 x = s[0], y = s[1];
   const float top =
-      c * Max3(Max3(x[0], x[1], x[2]), Max3(x[3], y[0], y[1]), fmaxf(y[2], y[3]));
-  if (__builtin_amdgcn_ballot_w64(top > w.m[t] + slack) == 0) return;
+      c * Max3(Max3(x[0], x[1], x[2]), Max3(x[3], y[0], y[1]), Max2(y[2], y[3]));
+  if (__builtin_amdgcn_ballot_w64(top > w.m[t] + (large ? kSlack - kRoom : kSlack)) == 0) return;
   float m = RowMax(top);
-  if (slack != kSlack) m += kSlack - slack;
-  m = fmaxf(w.m[t], m);
+  if (large) m += kRoom;
+  m = Max2(w.m[t], m);
   // rows that have seen nothing yet stay at -inf, with o and l zero
   const float shrink = m == w.m[t] ? 1.f : __builtin_amdgcn_exp2f(w.m[t] - m);
   w.m[t] = m;
@@ -540,15 +541,19 @@ __device__ __forceinline__ f16x8 HalfWeights(const float* p) {
 template <uint32_t parts, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<D>& r,
                                      int32_t key0, f32x4 (&s)[R][2], Rows<parts, D, R>& w) {
-  const float c =
-      parts == 3 || a.cap > kPlainCap ? Capped<true, R>(a, s) : Capped<false, R>(a, s);
-  // Unusual scale bytes of V: a token whose V has a scale of NaN, or one whose
+  const float c = PowerOf(a);
+  if (a.cap > 0.f) {
+    if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s);
+    else Cap<false, R>(a, s);
+  }
+  // Unusual scale bytes: a token whose K or V has a scale of NaN, or one whose
   // products pass the types' range (253, 254), gives NaN scores to the rows
-  // that see it and nothing to others (0 x NaN would reach every row of the
+  // that see it and nothing to others (V's 0 x NaN would reach every row of the
   // tile); past the request's end any byte may lie.
   constexpr bool half = parts < 3;
   bool wide = false;
-  if (__builtin_amdgcn_ballot_w64((OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1])) != 0) != 0) {
+  const uint32_t keys = Nans(r.ks[0] | (D == 256 ? r.ks[D == 256] : 0u) << 16);
+  if (__builtin_amdgcn_ballot_w64((OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1]) | keys) != 0) != 0) {
     uint32_t nan = 0;
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
@@ -559,25 +564,36 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
     }
 #pragma unroll
     for (uint32_t d = 1; d < 16; d *= 2) nan |= __shfl_xor(nan, d);
+    // K's bytes lie with lane n for tokens n and 16 + n
+    uint32_t tokens[2];
+#pragma unroll
+    for (uint32_t tile = 0; tile < 2; ++tile) {
+      uint64_t lanes = __builtin_amdgcn_ballot_w64((keys & (tile ? 0x80008000u : 0x00800080u)) != 0);
+      lanes |= lanes >> 32;
+      tokens[tile] = (uint32_t)(lanes | lanes >> 16) & 0xFFFFu;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      nan |= (tokens[j / 4] >> (threadIdx.x % 64 / 16 * 4 + j % 4) & 1u) << j;
 #pragma unroll
     for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j)
         if (nan >> j & 1) s[t][j / 4][j % 4] = __builtin_nanf("");
     if (__builtin_amdgcn_ballot_w64((Large(r.vs[0]) | Large(r.vs[1])) != 0) != 0)
-      w.slack = kSlack - kRoom;
+      w.large = true;
     wide = half && __builtin_amdgcn_ballot_w64(
                        (OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1])) != 0) != 0;
   }
   // weights below 2^-48 are none in f16
-  if (half && w.slack != kSlack) wide = true;
+  if (half && w.large) wide = true;
   Hide<D, R>(w, key0, s);
   typename Value<half>::type pt[R][half ? 1 : parts];
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
     float p[8];
-    Raise<D, R>(w, t, s[t], c, w.slack);
+    Raise<D, R>(w, t, s[t], c, w.large);
     Weights<D, R>(w, t, s[t], c, p);
     if constexpr (half) {
       if (wide) {  // V in bf16, on two bf16 parts of a weight

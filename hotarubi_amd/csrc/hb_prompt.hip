@@ -109,7 +109,9 @@ __global__ __launch_bounds__(256) void OpenKernel(const AttnArgs a) {
 #pragma unroll
     for (uint32_t e = 0; e < D / 32; ++e) {
       const uint32_t word = tile * (D / 32) + e, w = r.k[word / 4][word % 4];
-      const float scale = KeyScale(r.ks[D == 256 ? e / 4 : 0], tile);
+      // (253 and 254 as 255: NaN)
+      const uint32_t byte = r.ks[D == 256 ? e / 4 : 0] >> (8 * tile) & 255u;
+      const float scale = __uint_as_float((byte >= 253u ? 255u : byte) << 23);
       u32x4 x;
       x[0] = TwoAs<0, parts == 2>(w, scale);
       x[1] = TwoAs<1, parts == 2>(w, scale);
@@ -366,13 +368,14 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
 #pragma unroll
           for (uint32_t t = 0; t < R; ++t) s[t][k] = Product(x, q[t][e], s[t][k]);
         }
-      const float c = Capped<fine, R>(a, s);
+      const float c = PowerOf(a);
+      if (a.cap > 0.f) Cap<fine, R>(a, s);
       Hide<D, R>(w, key0, s);
       f16x8 pt[R];
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t) {
         float p[8];
-        Raise<D, R>(w, t, s[t], c, kSlack);  // (V is within f16 here)
+        Raise<D, R>(w, t, s[t], c, false);  // (V is within f16 here)
         Weights<D, R>(w, t, s[t], c, p);
         pt[t] = HalfWeights(p);
       }
