@@ -233,6 +233,19 @@ __device__ __forceinline__ float Max3(float a, float b, float c) {
   return y;
 }
 __device__ __forceinline__ float Max2(float a, float b) { return Max3(a, b, b); }
+// Of a lane's scores.  The matrix cores' results may be read some cycles after
+// their last product only; the compiler keeps its own instructions from them so
+// long, but not an asm's, so an addition that reads both results goes first.
+__device__ __forceinline__ float MaxOf8(const f32x4 (&s)[2]) {
+  const float first = s[0][0] + s[1][0];
+  float a, b, c;
+  asm("v_max3_f32 %0, %1, %2, %3"
+      : "=v"(a) : "v"(s[0][0]), "v"(s[0][1]), "v"(s[0][2]), "v"(first));
+  asm("v_max3_f32 %0, %1, %2, %3"
+      : "=v"(b) : "v"(s[0][3]), "v"(s[1][0]), "v"(s[1][1]), "v"(first));
+  asm("v_max_f32 %0, %1, %2" : "=v"(c) : "v"(s[1][2]), "v"(s[1][3]), "v"(first));
+  return Max3(a, b, c);
+}
 
 // Over the four lanes that share a row (n, 16 + n, 32 + n, 48 + n).
 __device__ __forceinline__ float RowMax(float x) {
@@ -494,9 +507,7 @@ __device__ __forceinline__ void Hide(const State<D, R>& w, int32_t key0, f32x4 (
 template <uint32_t D, uint32_t R>
 __device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
                                       bool large) {
-  const f32x4 x = s[0], y = s[1];
-  const float top =
-      c * Max3(Max3(x[0], x[1], x[2]), Max3(x[3], y[0], y[1]), Max2(y[2], y[3]));
+  const float top = c * MaxOf8(s);
   if (__builtin_amdgcn_ballot_w64(top > w.m[t] + (large ? kSlack - kRoom : kSlack)) == 0) return;
   float m = RowMax(top);
   if (large) m += kRoom;
