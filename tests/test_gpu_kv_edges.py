@@ -82,6 +82,37 @@ def test_lengths_past_31_bits_are_refused(gpu):
         assert positions[new[0] + 2:] == [-1] * (4 - new[0])
 
 
+# ------------------------------------------------------------ cache rows --
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_read_gives_any_stored_byte(gpu, dtype, dim):
+    """Every element under every scale: its value rounded to the tensors' type,
+    infinite where that does not hold it, NaN under 255."""
+    say("read, any byte", dtype, dim)
+    cache = torch.zeros(hb.kv_cache_shape(8, 1, 32, dim), dtype=torch.uint8, device=DEV)
+    at = record_map(dim)
+    col = torch.arange(dim, device=DEV)
+    code = col % 16
+    grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device=DEV)
+    grid = torch.cat([grid, -grid])[code]
+    want = torch.empty((256, 1, dim), dtype=torch.float64, device=DEV)
+    for byte in range(256):
+        record = cache[byte // 32, 0, 0]
+        for codes, scales in ((at[0], at[2]), (at[1], at[3])):
+            record[scales[byte % 32]] = byte
+            pair = (code[::2] | code[1::2] << 4).to(torch.uint8)
+            record[codes[byte % 32, ::2]] = pair
+        want[byte, 0] = grid * (math.nan if byte == 255 else 2.0**(byte - 127))
+    k, v = (torch.full((256, 1, dim), 3.0, dtype=dtype, device=DEV) for _ in range(2))
+    hb.kv_read(k=k, v=v, slots=torch.arange(256, dtype=torch.int32, device=DEV), cache=cache,
+               ctx=gpu)
+    for got in (k, v):
+        assert same(got.isnan(), want.isnan())
+        assert same(got.nan_to_num(9, math.inf, -math.inf),
+                    want.to(dtype).nan_to_num(9, math.inf, -math.inf))
+
+
 # ------------------------------------------------------------- attention --
 
 def reference(s, scale, window, cap):

@@ -142,9 +142,30 @@ def test_prompts_with_masks_caps_and_bounds_too_small(gpu, dtype, dim):
         t = dict(s, max_kv=most)
         assert_way("prompt", t)
         check(gpu, t)
+    t = dict(s, max_new=250)  # the first requests' rows from 250 on stay as they are
+    assert_way("prompt", t)
+    check(gpu, t)
     t = dict(s, prefix=None)
     assert_way("prompt", t, window=100)
     compare(gpu, t, window=100)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompts_beside_single_tokens(gpu, dtype, dim):
+    """A step of prompts and decodes: requests of a token or two on the way
+    that the prompts' rows choose."""
+    say("mixed", dtype, dim)
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    requests = [(900, 1, 0), (700, 400, 0), (1, 1, 0), (0, 0, 0), (1500, 2, 40), (300, 300, 0),
+                (40, 1, 0), (650, 330, 90)] * 2
+    s = build(gen, requests, 64, 2, dim, dtype, 16)
+    want = "rows" if dtype is F32 else "prompt"
+    got = hb.kv_attention_way(q=s["q"], out=s["q"], cache=s["cache"], table=s["table"], cu=s["cu"],
+                              kv_lens=s["kv_lens"], max_new=400, max_kv=1500, scale=0.1,
+                              prefix=s["prefix"])
+    assert got[0] == want, got
+    check(gpu, s)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
