@@ -125,8 +125,8 @@ __device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, 
   return __builtin_bit_cast(bf16x8, x);
 }
 
-// P V in f16 for the 16-bit types: P's error is then below the output's
-// rounding (2^-12 of each weight against bf16's 2^-9), and V is exact in f16
+// P V in f16 for the 16-bit types: a weight is off by at most 2^-11 of itself,
+// less than bf16's output (2^-8) and as much as fp16's, and V is exact in f16
 // wherever its scale bytes lie in [104, 140] (0.5 x 2^-23 .. 6 x 2^13).  Other
 // records take V in bf16 and each weight as two bf16 parts (2^-16 of it).  fp32
 // takes three bf16 parts of P.
@@ -523,8 +523,8 @@ __device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&
 __device__ __forceinline__ float Reference(float m) {
   return kLift - (m == -__builtin_inff() ? 0.f : m);
 }
-// The record's weights and their sum.  They carry 2^kLift: at most 2^15, and
-// as small as 2^-31 of the maximum before f16 goes subnormal.
+// The record's weights and their sum.  They carry 2^kLift: at most 2^15, and in
+// f16 normal down to 2^-21 of the reference, off by 2^-32 of it below that.
 template <uint32_t D, uint32_t R>
 __device__ __forceinline__ void Weights(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
                                         float* p) {

@@ -15,9 +15,9 @@
 // record and head.  Few rows are bound by that: 8 query heads on each of 8 over
 // 262,147 keys, D 128, 285 MB, take 51 us and 5 for the join (5.6 TB/s before
 // it; the card copies at 4.9, reads and writes together), and 64 requests of
-// 1,000 to 8,191 keys, 321 MB, 70 us and 6.  Rows of 32 bits want three products
+// 1,000 to 8,191 keys, 321 MB, 71 us and 6.  Rows of 32 bits want three products
 // where others want one: 32 requests of 50 rows behind 150 keys, 15 heads on 5,
-// D 64, take 14.0 us in fp32 and 11.7 in bf16.
+// D 64, take 13.6 us a call in fp32 and 11.1 in bf16.
 #include <algorithm>
 #include <cmath>
 

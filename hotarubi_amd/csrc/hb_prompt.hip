@@ -9,9 +9,11 @@
 // it: at D 128 a wave's record is 256 cycles of products, about 260 of the
 // softmax's 33 vector instructions and 8 exponentials, and 16 KB read from LDS
 // (at D 64 the softmax is twice the products).  Three prompts of up to 4,096
-// tokens, 32 heads on 8, D 128, bf16, 346 GFLOP, take 375 us, 13 of them for
-// opening (924 TFLOP/s; a large library product reaches 1,231), and 400 with
-// the calls back to back; with the conversion in each workgroup they took 454.
+// tokens, 32 heads on 8, D 128, bf16, 346 GFLOP, take 13 us for opening and
+// 796,000 cycles: 353 us at the 2.27 GHz that an unbroken row of calls settles
+// at (366 us a call, 945 TFLOP/s; a large library product reaches 1,231), 398 at
+// 2.0 GHz between pauses, up to 486 at 1.64 GHz where such a row begins.  With
+// the conversion in each workgroup a call took 454 where it took 366 opened.
 // At D 256 one workgroup fills a CU's LDS, so a wave waits on its own chain, 1.3
 // us a record: eight chunks of 100 to 256 tokens, fp16, a window of 1,024 and
 // capped scores, take 63 us, 13 of them for opening and 7 for the cap.

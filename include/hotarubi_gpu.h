@@ -586,8 +586,9 @@ typedef enum hb_type { HB_TYPE_F32 = 0, HB_TYPE_BF16 = 1, HB_TYPE_F16 = 2 } hb_t
  *   slots, positions  int32 [size]: of each new token; past the last -1
  *   status     int32 [2]: pages taken, requests refused.  *free_count is left
  *              as it is: the caller takes status[0] from it.
- * Negative lengths count as 0.  Outputs share no memory with inputs, the
- * table apart.  The sum of the new tokens is below 2^31; a slot of 2^31 or
+ * Tokens of a refused request keep their rows and positions; attention takes
+ * their rows for its last cached ones.  Negative lengths count as 0.  Outputs
+ * share no memory with inputs, the table apart.  The sum of the new tokens is below 2^31; a slot of 2^31 or
  * more is -1. */
 typedef struct hb_kv_plan_desc {
   const int32_t* lens;
@@ -671,19 +672,21 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * (j < kv_lens[b]) if
  *   j <= p and (window == 0 or p - j < window), or j < prefix[b];
  * query head h reads K/V head h / (q_heads / heads).  Scores are
- * scale * q.k, softcap * tanh(scale * q.k / softcap) where softcap > 0 (both
- * finite);
+ * scale * q.k, softcap * tanh(scale * q.k / softcap) where softcap > 0 (scale
+ * and softcap are finite);
  *   out = sum_j softmax(scores)_j v_j, 0 for a row that sees no key.
  * q and out are [tokens][q_heads][dim] of `type`, strides in elements.  Scores,
  * maxima and sums are in 32 bits, and q and the cache's values enter the
- * products exactly, subnormal ones too (fp32 q to 2^-133).  The softmax's weights enter theirs in f16 for bf16 and
- * fp16 tensors (each off by 2^-12 of its value at most, their sum is of the
- * unrounded ones) and as three bf16 parts for fp32 ones (2^-24).
+ * products exactly, subnormal ones too (fp32 q to 2^-133).  The softmax's
+ * weights enter theirs in f16 for bf16 and fp16 tensors (each off by 2^-11 of
+ * itself or 2^-32 of the row's largest, whichever is more; on values that f16
+ * does not hold by 2^-16 of itself), and as three bf16 parts for fp32 ones
+ * (2^-24); what they are divided by is the sum of the unrounded ones.
  * Rows outside every request are not written.  max_new and max_kv bound the
- * requests' new tokens and keys; they choose the split of the work (a max_kv
- * that is too small costs time, no keys), and rows of a request past max_new
- * are not computed.  A block table entry that names
- * no page of the cache hides its keys.  A stored NaN (a scale of 253 or more)
+ * requests' new tokens and keys; they choose the split of the work.  Rows of a
+ * request past max_new are not computed.  A max_kv that is too small costs
+ * time, no keys: prompts of requests that pass it take about three times as
+ * long.  A block table entry that names no page of the cache hides its keys.  A stored NaN (a scale of 253 or more)
  * makes the rows that see its token NaN, no others.
  * Long caches are split over workgroups that meet in the context's workspace,
  * in a fixed order: results do not change from call to call.  Prompts keep
