@@ -4,6 +4,7 @@ implementations."""
 from __future__ import annotations
 
 import functools
+import gc
 import math
 import threading
 
@@ -17,6 +18,16 @@ from test_gpu_kv import record_map as make_record_map
 
 pytestmark = pytest.mark.gpu
 record_map = functools.lru_cache(make_record_map)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_given_back():
+    """Nothing stays in torch's allocator: tests of batched layers elsewhere
+    want tensors made one after another to lie at equal distances."""
+    yield
+    record_map.cache_clear()
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 def same(a, b):

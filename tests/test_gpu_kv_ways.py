@@ -11,7 +11,7 @@ import torch
 
 import hotarubi_amd as hb
 from test_gpu_kv import DEV, HALF, TINY, build, check, ints, make_cache, say
-from test_gpu_kv_edges import compare, reference, set_scale
+from test_gpu_kv_edges import compare, memory_given_back, reference, set_scale  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
