@@ -501,7 +501,8 @@ hipError_t LaunchOf(AttnArgs& a, const AttnWay& how, Workspace& ws, hipStream_t 
   const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
   const uint64_t pairs = (uint64_t)a.batch * a.heads, stored = std::min<uint64_t>(R * 16, rows);
   const uint64_t grid = how.way == HB_KV_WAY_SHARES ? how.splits : pairs * how.tiles * how.splits;
-  if (grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  const uint64_t join = how.workspace > 0 ? pairs * how.tiles * stored : 0;
+  if (grid > 0x7FFFFFFFu || join > 0x7FFFFFFFu) return hipErrorInvalidValue;
   a.tiles = how.tiles;
   a.splits = how.splits;
   a.split_records = how.split_records;
@@ -510,18 +511,17 @@ hipError_t LaunchOf(AttnArgs& a, const AttnWay& how, Workspace& ws, hipStream_t 
     if (err != hipSuccess) return err;
     a.ws = ws.ptr + kSplitCounters;
   }
-  const uint32_t join = (uint32_t)(pairs * how.tiles * stored);
   switch (how.way) {
     case HB_KV_WAY_ROWS:
       AttnKernel<parts, D, R, kRows><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
       break;
     case HB_KV_WAY_SHARES:
       AttnKernel<parts, D, R, kShares><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
-      JoinKernel<parts, D, R, kShares><<<join, kThreads, 0, stream>>>(a);
+      JoinKernel<parts, D, R, kShares><<<(uint32_t)join, kThreads, 0, stream>>>(a);
       break;
     default:
       AttnKernel<parts, D, R, kSplits><<<(uint32_t)grid, kThreads, 0, stream>>>(a);
-      if (how.splits > 1) JoinKernel<parts, D, R, kSplits><<<join, kThreads, 0, stream>>>(a);
+      if (join > 0) JoinKernel<parts, D, R, kSplits><<<(uint32_t)join, kThreads, 0, stream>>>(a);
   }
   return hipGetLastError();
 }

@@ -127,10 +127,10 @@ def test_read_gives_any_stored_byte(gpu, dtype, dim):
 # ------------------------------------------------------------- attention --
 
 def reference(s, scale, window, cap):
-    """fp64 rows and their tolerance, as test_gpu_kv's, but with what weights
-    too small for f16 lose (2^-32 of the largest weight each) by the columns'
-    own values, scale bytes of 253 and more as NaN, and caps above 64 off by
-    the score's own roundings instead of the cap's."""
+    """fp64 rows, their tolerance and which are computed, as test_gpu_kv's, but
+    with what weights too small for f16 lose (2^-32 of the largest weight each)
+    by the columns' own values, scale bytes of 253 and more as NaN, and caps
+    above 64 off by the score's own roundings instead of the cap's."""
     q, cache, table = s["q"], s["cache"], s["table"]
     tokens, hq, d = q.shape
     group, half = hq // cache.shape[1], q.dtype is not torch.float32
@@ -144,52 +144,62 @@ def reference(s, scale, window, cap):
         return torch.where(e >= 253, math.nan, x).reshape(-1, d)
 
     out = torch.zeros((tokens, hq, d), dtype=torch.float64, device=DEV)
-    tol = torch.zeros_like(out)
+    tol, there = torch.zeros_like(out), torch.zeros(tokens, dtype=torch.bool, device=DEV)
     cu, lens = s["cu"].tolist(), s["kv_lens"].tolist()
     for b, total in enumerate(lens):
-        n = cu[b + 1] - cu[b]
+        new = cu[b + 1] - cu[b]
+        n = min(new, s["max_new"])
+        mine = slice(cu[b], cu[b] + n)
+        there[mine] = True
         if n == 0 or total == 0:
             continue
-        mine = slice(cu[b], cu[b + 1])
         key = torch.arange(total, device=DEV)
-        pos = total - n + torch.arange(n, device=DEV)[:, None]
+        pos = total - new + torch.arange(n, device=DEV)[:, None]
         see = (key <= pos) & (pos - key < window if window else key >= 0)
         if s["prefix"] is not None:
             see = see | (key < s["prefix"][b])
         pages = table[b, :-(-total // (32 * cache.shape[2]))].long()
+        ok = (pages >= 0) & (pages < cache.shape[0])
+        see = see & ok.repeat_interleave(32 * cache.shape[2])[:total]
+        pages = torch.where(ok, pages, 0)
         for h in range(cache.shape[1]):
             rec = cache[pages, h].reshape(-1, 34 * d)
             k, v = rows(rec, at[0], at[2])[:total], rows(rec, at[1], at[3])[:total]
             dead = k.isnan().any(-1) | v.isnan().any(-1)
             k, v = torch.nan_to_num(k), torch.nan_to_num(v)
-            for g in range(h * group, (h + 1) * group):
-                x = q[mine, g].double()
-                y = x @ k.T * scale
-                ds = (d + 8) * 2.0**-24 * (x.abs() @ k.abs().T * abs(scale))
-                if cap:
-                    y = cap * torch.tanh(y / cap)
-                    ds = ds + (cap * 2.0**-21 if cap <= 64 else 2.0**-21 * y.abs())
-                y = torch.where(dead, math.nan, y).masked_fill(~see, -math.inf)
-                top = torch.nan_to_num(y, nan=-math.inf).amax(-1, keepdim=True)
-                p = torch.exp(y - torch.where(top.isinf(), 0, top))
-                p = p / torch.where(see.any(-1, keepdim=True), p.sum(-1, keepdim=True), 1)
-                out[mine, g] = p @ v
-                ds = torch.where(see, ds, 0).amax(-1, keepdim=True)
-                tol[mine, g] = p @ v.abs() * (2 * ds + (2.0**-11 if half else 0) +
-                                              total * 2.0**-23 + 2.0**-21)
-                tol[mine, g] += 2.0**-32 * (see.double() @ v.abs())
-    return out, tol
+            heads = slice(h * group, (h + 1) * group)
+            x = q[mine, heads].double().reshape(n * group, d)
+            sees = see.repeat_interleave(group, 0)
+            y = x @ k.T * scale
+            ds = (d + 8) * 2.0**-24 * (x.abs() @ k.abs().T * abs(scale))
+            if cap:
+                y = cap * torch.tanh(y / cap)
+                ds = ds + (cap * 2.0**-21 if cap <= 64 else 2.0**-21 * y.abs())
+            y = torch.where(dead, math.nan, y).masked_fill(~sees, -math.inf)
+            top = torch.nan_to_num(y, nan=-math.inf).amax(-1, keepdim=True)
+            p = torch.exp(y - torch.where(top.isinf(), 0, top))
+            p = p / torch.where(sees.any(-1, keepdim=True), p.sum(-1, keepdim=True), 1)
+            out[mine, heads] = (p @ v).view(n, group, d)
+            ds = torch.where(sees, ds, 0).amax(-1, keepdim=True)
+            off = p @ v.abs() * (2 * ds + (2.0**-11 if half else 0) + total * 2.0**-23 + 2.0**-21)
+            tol[mine, heads] = (off + 2.0**-32 * (sees.double() @ v.abs())).view(n, group, d)
+    return out, tol, there
 
 
-def compare(gpu, s, scale=None, window=0, cap=0.0):
+def compare(gpu, s, scale=None, window=0, cap=0.0, out=None):
+    """The call's rows against the reference, twice: the same bits."""
     q, d = s["q"], s["q"].shape[-1]
     scale = d ** -0.5 if scale is None else scale
-    out = torch.full_like(q, 7.0)
-    hb.kv_attention(q=q, out=out, cache=s["cache"], table=s["table"], cu=s["cu"],
-                    kv_lens=s["kv_lens"], max_new=s["max_new"], max_kv=s["max_kv"], scale=scale,
-                    prefix=s["prefix"], window=window, softcap=cap, ctx=gpu)
-    want, tol = reference(s, scale, window, cap)
-    got = out.double()
+    want, tol, mine = reference(s, scale, window, cap)
+    first, out = torch.full_like(q, 7.0), torch.empty_like(q) if out is None else out
+    out.fill_(7.0)
+    for to in (first, out):
+        hb.kv_attention(q=q, out=to, cache=s["cache"], table=s["table"], cu=s["cu"],
+                        kv_lens=s["kv_lens"], max_new=s["max_new"], max_kv=s["max_kv"],
+                        scale=scale, prefix=s["prefix"], window=window, softcap=cap, ctx=gpu)
+    assert same(first.nan_to_num(9, math.inf, -math.inf), out.nan_to_num(9, math.inf, -math.inf))
+    assert bool((out[~mine] == 7).all())
+    got, want, tol = out[mine].double(), want[mine], tol[mine]
     assert same(got.isnan(), want.isnan())
     tol = tol + HALF[q.dtype] * want.abs() + TINY[q.dtype]
     most = torch.finfo(q.dtype).max  # what rounds past it is an infinity
@@ -206,7 +216,8 @@ def attend(s, out, **kw):
                     prefix=s["prefix"], **kw)
 
 
-# few rows; waves with rows of their own; prompts: (requests, K/V heads), a query head each
+# a row of a request, 70 to 90, 200 (requests, K/V heads; a query head each): which way
+# of dividing the work these take differs by type and head size
 ROWS = {"one": ([(300, 1, 0), (270, 1, 10)], 2), "rows": ([(300, 90, 0), (270, 70, 10)], 16),
         "prompt": ([(300, 200, 0), (270, 200, 10)] * 4, 40)}
 
