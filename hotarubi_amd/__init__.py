@@ -16,6 +16,7 @@ include/hotarubi_gpu.h (libhotarubi_gpu.so, built by hotarubi_amd.build):
   kv_plan, norm_rope, kv_append, kv_read, kv_attention
                              a serving step's attention over a paged MXFP4
                              cache (torch tensors; no counterpart)
+  kv_attention_way           how kv_attention would divide a call's work
 
 Errors raise HbError; a command the reference rejects with Fail raises
 HbBadCommand carrying the reference's message.  The library is loaded from
