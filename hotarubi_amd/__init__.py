@@ -17,6 +17,12 @@ include/hotarubi_gpu.h (libhotarubi_gpu.so, built by hotarubi_amd.build):
                              a serving step's attention over a paged MXFP4
                              cache (torch tensors; no counterpart)
   kv_attention_way           how kv_attention would divide a call's work
+  kv8_append, kv8_read, kv8_attention, kv8_attention_way
+                             the same over a paged cache of 8 bits
+  kv_fork, kv_copy, kv_free, kv_compact
+                             pages that requests share, give back and move
+  token_logprobs             log probabilities, entropy and the most likely
+                             tokens of a step's logits
 
 Errors raise HbError; a command the reference rejects with Fail raises
 HbBadCommand carrying the reference's message.  The library is loaded from
@@ -69,6 +75,11 @@ EXPORTS = (
     "hb_kv_plan", "hb_kv_plan_async", "hb_norm_rope", "hb_norm_rope_async", "hb_kv_append",
     "hb_kv_append_async", "hb_kv_read", "hb_kv_read_async", "hb_kv_attention",
     "hb_kv_attention_async", "hb_kv_attention_way",
+    "hb_kv8_append", "hb_kv8_append_async", "hb_kv8_read", "hb_kv8_read_async",
+    "hb_kv8_attention", "hb_kv8_attention_async", "hb_kv8_attention_way",
+    "hb_kv_fork", "hb_kv_fork_async", "hb_kv_copy", "hb_kv_copy_async", "hb_kv_free",
+    "hb_kv_free_async", "hb_kv_compact", "hb_kv_compact_async", "hb_token_logprobs",
+    "hb_token_logprobs_async",
 )
 
 
@@ -248,6 +259,23 @@ def lib():
             "hb_kv_attention": (i, [vp, vp]),
             "hb_kv_attention_async": (i, [vp, vp]),
             "hb_kv_attention_way": (i, [vp, vp]),
+            "hb_kv8_attention_way": (i, [vp, vp]),
+            "hb_kv8_append": (i, [vp, vp]),
+            "hb_kv8_append_async": (i, [vp, vp]),
+            "hb_kv8_read": (i, [vp, vp]),
+            "hb_kv8_read_async": (i, [vp, vp]),
+            "hb_kv8_attention": (i, [vp, vp]),
+            "hb_kv8_attention_async": (i, [vp, vp]),
+            "hb_kv_fork": (i, [vp, vp]),
+            "hb_kv_fork_async": (i, [vp, vp]),
+            "hb_kv_copy": (i, [vp, vp]),
+            "hb_kv_copy_async": (i, [vp, vp]),
+            "hb_kv_free": (i, [vp, vp]),
+            "hb_kv_free_async": (i, [vp, vp]),
+            "hb_kv_compact": (i, [vp, vp]),
+            "hb_kv_compact_async": (i, [vp, vp]),
+            "hb_token_logprobs": (i, [vp, vp]),
+            "hb_token_logprobs_async": (i, [vp, vp]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -727,6 +755,12 @@ KV_PLAN_DESC = struct.Struct("@10P6I")
 NORM_ROPE_DESC = struct.Struct("@4P8Q3PQPf8I3I")
 KV_ROWS_DESC = struct.Struct("@P4I2P4QP2I")
 KV_ATTENTION_DESC = struct.Struct("@P4I2P4Q4P9I2f")
+KV8_ATTENTION_DESC = struct.Struct("@P4I2P4Q4P10I2f")
+KV_FORK_DESC = struct.Struct("@9P6I")
+KV_COPY_DESC = struct.Struct("@2P2Q3I")
+KV_FREE_DESC = struct.Struct("@7P7I")
+KV_COMPACT_DESC = struct.Struct("@7P8I")
+LOGPROBS_DESC = struct.Struct("@PQ5P4If")
 _types = None  # (torch.dtype -> hb_type, int32, uint8, float64, float32)
 
 
@@ -795,14 +829,14 @@ def _heads(t, dtype, name: str, shape, device: int):
     return t.data_ptr(), stride[0], stride[1]
 
 
-def _table(t, i32, device: int):
+def _table(t, i32, device: int, name: str = "table"):
     """(address, rows, entries of a row, row stride) of a block table."""
     stride = t.stride()
     if t.dtype is not i32 or len(stride) != 2 or \
             (stride[1] != 1 and t.shape[1] > 1 and t.numel() > 0):
-        raise _invalid(f"table must be int32 rows, not {tuple(t.shape)} of {t.dtype}")
+        raise _invalid(f"{name} must be int32 rows, not {tuple(t.shape)} of {t.dtype}")
     if t.get_device() != device:
-        _place(t, "table", device)
+        _place(t, name, device)
     batch, columns = t.shape
     return t.data_ptr(), batch, columns, stride[0]
 
@@ -816,6 +850,25 @@ def _cache(t, u8, device: int):
     if t.get_device() != device:
         _place(t, "cache", device)
     return t.data_ptr(), size[0], size[1], 32 * size[2], size[3] // 34
+
+
+def _cache8(t, u8, device: int):
+    """The same of a cache of 8 bits."""
+    size = t.shape
+    if t.dtype is not u8 or len(size) != 4 or size[3] % 64 != 16 or not t.is_contiguous():
+        raise _invalid("the cache must be contiguous uint8 [pages][heads][page / 32][64 dim + 16], "
+                       f"not {tuple(size)} of {t.dtype}")
+    if t.get_device() != device:
+        _place(t, "cache", device)
+    return t.data_ptr(), size[0], size[1], 32 * size[2], size[3] // 64
+
+
+def _pairs(t, i32, device: int) -> int:
+    """Address of [count][2] page numbers."""
+    if t.dtype is not i32 or t.dim() != 2 or t.shape[1] != 2 or not t.is_contiguous():
+        raise _invalid(f"pairs must be contiguous int32 [n][2], not {tuple(t.shape)} of {t.dtype}")
+    _place(t, "pairs", device)
+    return t.data_ptr()
 
 
 def _kind(kinds, t, name: str) -> int:
@@ -902,10 +955,10 @@ def norm_rope(q, positions, inv_freq, q_out, k=None, k_out=None, gamma_q=None, g
     _check((lib().hb_norm_rope if sync else lib().hb_norm_rope_async)(ctx.handle, d))
 
 
-def _kv_rows(fn, k, v, slots, cache, ctx) -> None:
+def _kv_rows(fn, k, v, slots, cache, ctx, layout=_cache) -> None:
     kinds, i32, u8, _, _ = _types or _torch_types()
     dev, dtype = ctx.device, k.dtype
-    c = _cache(cache, u8, dev)
+    c = layout(cache, u8, dev)
     kind = _kind(kinds, k, "k")
     ka, kt, kh = _heads(k, dtype, "k", None, dev)
     tokens, heads, dim = k.shape
@@ -935,10 +988,11 @@ def kv_read(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -
 
 
 def _attention_desc(dev: int, q, out, cache, table, cu, kv_lens, max_new, max_kv, scale, prefix,
-                    window, softcap) -> bytes:
+                    window, softcap, sinks=()) -> bytes:
     kinds, i32, u8, _, _ = _types or _torch_types()
     dtype = q.dtype
-    c = _cache(cache, u8, dev)
+    layout, c = (KV8_ATTENTION_DESC, _cache8(cache, u8, dev)) if sinks else \
+        (KV_ATTENTION_DESC, _cache(cache, u8, dev))
     kind = _kind(kinds, q, "q")
     qa, qt, qh = _heads(q, dtype, "q", None, dev)
     tokens, heads, dim = q.shape
@@ -946,11 +1000,11 @@ def _attention_desc(dev: int, q, out, cache, table, cu, kv_lens, max_new, max_kv
         raise _invalid(f"q has heads of {dim} elements, the cache of {c[4]}")
     oa, ot, oh = _heads(out, dtype, "out", q.shape, dev)
     at, batch, columns, stride = _table(table, i32, dev)
-    return _desc(KV_ATTENTION_DESC, *c, qa, oa, qt, qh, ot, oh, at,
+    return _desc(layout, *c, qa, oa, qt, qh, ot, oh, at,
                  _vector(cu, i32, "cu", batch + 1, dev),
                  _vector(kv_lens, i32, "kv_lens", batch, dev),
                  0 if prefix is None else _vector(prefix, i32, "prefix", batch, dev), kind, tokens,
-                 heads, batch, columns, stride, max_new, max_kv, window, scale, softcap)
+                 heads, batch, columns, stride, max_new, max_kv, window, *sinks, scale, softcap)
 
 
 def kv_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
@@ -983,3 +1037,166 @@ def kv_attention_way(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: in
                         prefix, window, softcap), way))
     kind, tiles, splits, _, workspace = KV_WAY.unpack(way.raw)
     return KV_WAYS[kind], tiles, splits, workspace
+
+
+def kv8_cache_shape(pages: int, heads: int, page_size: int, dim: int) -> tuple[int, int, int, int]:
+    """Shape of a paged cache of 8 bits (uint8); it starts as zeros."""
+    return pages, heads, page_size // 32, 64 * dim + 16
+
+
+def kv8_append(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv8_append: rows k, v [tokens][heads][dim] into the cache (uint8
+    [pages][heads][page / 32][64 dim + 16]) at int32 slots, the tokens of a
+    block of 32 in their order."""
+    _kv_rows(lib().hb_kv8_append if sync else lib().hb_kv8_append_async, k, v, slots, cache,
+             ctx or _torch_context(k, "k"), _cache8)
+
+
+def kv8_read(k, v, slots, cache, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv8_read: the stored values of slots into k, v [tokens][heads][dim]."""
+    _kv_rows(lib().hb_kv8_read if sync else lib().hb_kv8_read_async, k, v, slots, cache,
+             ctx or _torch_context(k, "k"), _cache8)
+
+
+def kv8_attention(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
+                  prefix=None, window: int = 0, sinks: int = 0, softcap: float = 0.0,
+                  ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv8_attention: kv_attention over a cache of 8 bits.  sinks: with a
+    window, the first tokens that stay visible to the rows behind them."""
+    ctx = ctx or _torch_context(q, "q")
+    d = _attention_desc(ctx.device, q, out, cache, table, cu, kv_lens, max_new, max_kv, scale,
+                        prefix, window, softcap, (sinks,))
+    _check((lib().hb_kv8_attention if sync else lib().hb_kv8_attention_async)(ctx.handle, d))
+
+
+def kv8_attention_way(q, out, cache, table, cu, kv_lens, max_new: int, max_kv: int, scale: float,
+                      prefix=None, window: int = 0, sinks: int = 0, softcap: float = 0.0):
+    """hb_kv8_attention_way: kv_attention_way for kv8_attention."""
+    way = C.create_string_buffer(KV_WAY.size)
+    _check(lib().hb_kv8_attention_way(
+        _attention_desc(q.get_device(), q, out, cache, table, cu, kv_lens, max_new, max_kv, scale,
+                        prefix, window, softcap, (sinks,)), way))
+    kind, tiles, splits, _, workspace = KV_WAY.unpack(way.raw)
+    return KV_WAYS[kind], tiles, splits, workspace
+
+
+def kv_fork(table, lens, source, target, free_pages, free_count, page_size: int, lens_out, pairs,
+            status, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_fork: request target[i] goes on from request source[i]'s tokens.
+    table int32 [batch][columns] gets the targets' entries; lens int32 [batch];
+    source, target int32 [forks]; free_pages int32 (a stack of free_count [1]
+    pages); lens_out [batch], pairs [forks][2] (for kv_copy) and status [2]
+    (pages taken, forks refused) are written."""
+    ctx = ctx or _torch_context(table, "table")
+    i32, dev = (_types or _torch_types())[1], ctx.device
+    at, batch, columns, stride = _table(table, i32, dev)
+    source_at = _vector(source, i32, "source", -1, dev)
+    forks = source.shape[0]
+    pairs_at = _pairs(pairs, i32, dev)
+    if pairs.shape[0] != forks:
+        raise _invalid(f"{pairs.shape[0]} pairs for {forks} forks")
+    free_at = _vector(free_pages, i32, "free_pages", -1, dev)
+    d = _desc(KV_FORK_DESC, at, _vector(lens, i32, "lens", batch, dev), source_at,
+              _vector(target, i32, "target", forks, dev), free_at,
+              _vector(free_count, i32, "free_count", 1, dev),
+              _vector(lens_out, i32, "lens_out", batch, dev), pairs_at,
+              _vector(status, i32, "status", 2, dev), batch, columns, stride, page_size, forks,
+              free_pages.shape[0])
+    _check((lib().hb_kv_fork if sync else lib().hb_kv_fork_async)(ctx.handle, d))
+
+
+def kv_copy(cache, pairs, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_copy: page pairs[i][0] over page pairs[i][1] (int32 [n][2]) of a
+    cache, of 4 or 8 bits: uint8 [pages][heads][page / 32][record], or with
+    [layers] in front of that."""
+    ctx = ctx or _torch_context(cache, "cache")
+    _, i32, u8, _, _ = _types or _torch_types()
+    size = cache.shape
+    if cache.dtype is not u8 or len(size) not in (4, 5) or not cache.is_contiguous():
+        raise _invalid("the cache must be contiguous uint8 [layers][pages][heads][page / 32]"
+                       f"[record], not {tuple(size)} of {cache.dtype}")
+    _place(cache, "cache", ctx.device)
+    page = size[-3] * size[-2] * size[-1]
+    d = _desc(KV_COPY_DESC, cache.data_ptr(), _pairs(pairs, i32, ctx.device), page,
+              page * size[-4], size[-4], size[0] if len(size) == 5 else 1, pairs.shape[0])
+    _check((lib().hb_kv_copy if sync else lib().hb_kv_copy_async)(ctx.handle, d))
+
+
+def kv_free(table, lens, rows, pages: int, free_pages, free_count, page_size: int, lens_out,
+            status, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_free: requests `rows` (int32) end: their pages that no other
+    request names go on the stack free_pages above its free_count [1] pages.
+    pages: of the cache; lens_out [batch] (0 for them) and status [2] (pages
+    put back, pages without room) are written."""
+    ctx = ctx or _torch_context(table, "table")
+    i32, dev = (_types or _torch_types())[1], ctx.device
+    at, batch, columns, stride = _table(table, i32, dev)
+    d = _desc(KV_FREE_DESC, at, _vector(lens, i32, "lens", batch, dev),
+              _vector(rows, i32, "rows", -1, dev), _vector(free_pages, i32, "free_pages", -1, dev),
+              _vector(free_count, i32, "free_count", 1, dev),
+              _vector(lens_out, i32, "lens_out", batch, dev),
+              _vector(status, i32, "status", 2, dev), batch, columns, stride, page_size,
+              rows.shape[0], pages, free_pages.shape[0])
+    _check((lib().hb_kv_free if sync else lib().hb_kv_free_async)(ctx.handle, d))
+
+
+def kv_compact(table, lens, pages: int, page_size: int, table_out, free_pages, free_count, pairs,
+               status, ctx: Context | None = None, sync: bool = True) -> None:
+    """hb_kv_compact: renumbers a cache of `pages` pages so that those in use
+    are the first.  table_out [batch][columns] (may be table), free_pages (at
+    least `pages`), free_count [1], pairs [at least pages / 2][2] (for kv_copy)
+    and status [2] (pages in use, pages that move) are written."""
+    ctx = ctx or _torch_context(table, "table")
+    i32, dev = (_types or _torch_types())[1], ctx.device
+    at, batch, columns, stride = _table(table, i32, dev)
+    out_at, out_batch, out_columns, out_stride = _table(table_out, i32, dev, "table_out")
+    if (out_batch, out_columns) != (batch, columns):
+        raise _invalid(f"table_out is {tuple(table_out.shape)}, table {tuple(table.shape)}")
+    d = _desc(KV_COMPACT_DESC, at, _vector(lens, i32, "lens", batch, dev), out_at,
+              _vector(free_pages, i32, "free_pages", -1, dev),
+              _vector(free_count, i32, "free_count", 1, dev), _pairs(pairs, i32, dev),
+              _vector(status, i32, "status", 2, dev), batch, columns, stride, out_stride,
+              page_size, pages, free_pages.shape[0], pairs.shape[0])
+    _check((lib().hb_kv_compact if sync else lib().hb_kv_compact_async)(ctx.handle, d))
+
+
+def _row_list(t, dtype, name: str, rows: int, top: int, device: int) -> int:
+    """Address of contiguous [rows][top]."""
+    if t.dtype is not dtype or tuple(t.shape) != (rows, top) or not t.is_contiguous():
+        raise _invalid(f"{name} must be contiguous {dtype} [{rows}][{top}], not "
+                       f"{tuple(t.shape)} of {t.dtype}")
+    _place(t, name, device)
+    return t.data_ptr()
+
+
+def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=None,
+                   top_logprobs=None, scale: float = 1.0, ctx: Context | None = None,
+                   sync: bool = True) -> None:
+    """hb_token_logprobs: of each row of scale * logits [rows][vocab], the log
+    probability of tokens[row] (int32; below 0: none) into logprobs, the
+    entropy, and the most likely tokens' columns and log probabilities into
+    top_ids (int32) and top_logprobs [rows][top].  Results are fp32; what is
+    None is left out."""
+    ctx = ctx or _torch_context(logits, "logits")
+    kinds, i32, _, _, f32 = _types or _torch_types()
+    kind, dev = _kind(kinds, logits, "logits"), ctx.device
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise _invalid(f"logits must be rows of neighbouring elements, not {tuple(logits.shape)} "
+                       f"with strides {logits.stride()}")
+    _place(logits, "logits", dev)
+    rows, vocab = logits.shape
+    if (tokens is None) != (logprobs is None) or (top_ids is None) != (top_logprobs is None):
+        raise _invalid("tokens and logprobs, top_ids and top_logprobs go together")
+    top = ids_at = top_at = 0
+    if top_ids is not None:
+        if top_ids.dim() != 2 or top_ids.shape[1] < 1:
+            raise _invalid(f"top_ids is {tuple(top_ids.shape)}, not [rows][top]")
+        top = top_ids.shape[1]
+        ids_at = _row_list(top_ids, i32, "top_ids", rows, top, dev)
+        top_at = _row_list(top_logprobs, f32, "top_logprobs", rows, top, dev)
+    d = _desc(LOGPROBS_DESC, logits.data_ptr(), logits.stride(0),
+              0 if tokens is None else _vector(tokens, i32, "tokens", rows, dev),
+              0 if logprobs is None else _vector(logprobs, f32, "logprobs", rows, dev),
+              0 if entropy is None else _vector(entropy, f32, "entropy", rows, dev), ids_at,
+              top_at, kind, rows, vocab, top, scale)
+    _check((lib().hb_token_logprobs if sync else lib().hb_token_logprobs_async)(ctx.handle, d))

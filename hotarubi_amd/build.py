@@ -21,7 +21,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhotarubi_gpu.so")
 SOURCES = ["hb_api.hip", "hb_gemm.hip", "hb_fast.hip", "hb_fast4.hip", "hb_skinny.hip", "hb_vec.hip",
            "hb_dma.hip", "hb_wave.hip", "hb_panel.hip", "hb_stream.hip", "hb_w8.hip", "hb_prep.hip",
-           "hb_kv.hip", "hb_attn.hip", "hb_prompt.hip"]
+           "hb_kv.hip", "hb_attn.hip", "hb_prompt.hip", "hb_kv8.hip", "hb_attn8.hip", "hb_pages.hip",
+           "hb_logprobs.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 DEVICE_FLAGS = [
@@ -38,9 +39,10 @@ DEVICE_FLAGS = [
 # hardware, so its first operand loads need no argument round trip.
 # hb_kv.hip: cache rows keep FP32 subnormals, which MXFP4's smallest scales
 # reach, and its tensors are ordinary floats rather than the NPU's; so do the
-# attention kernels that read them.
+# attention kernels that read them, the 8-bit cache's, and logits.
 SOURCE_FLAGS = {"hb_skinny.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=11"],
-                **dict.fromkeys(["hb_kv.hip", "hb_attn.hip", "hb_prompt.hip"],
+                **dict.fromkeys(["hb_kv.hip", "hb_attn.hip", "hb_prompt.hip", "hb_kv8.hip",
+                                 "hb_attn8.hip", "hb_logprobs.hip"],
                                 ["-fno-gpu-flush-denormals-to-zero"])}
 
 

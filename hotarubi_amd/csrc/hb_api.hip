@@ -12,6 +12,7 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <type_traits>
 #include <vector>
 #include <new>
 #include <string>
@@ -1493,7 +1494,7 @@ int NormRope(hb_ctx* ctx, const hb_norm_rope_desc* d, bool sync) {
   return Launched(ctx, hb::LaunchRope(a, ctx->stream), "norm and rotation launch", sync);
 }
 
-int KvRows(hb_ctx* ctx, const hb_kv_rows_desc* d, bool read, bool sync) {
+int KvRows(hb_ctx* ctx, const hb_kv_rows_desc* d, bool read, bool sync, bool eight = false) {
   if (!d) return Fail(HB_EINVAL, "null descriptor");
   if (int rc = CheckType(d->type)) return rc;
   if (int rc = CheckCache(d->cache)) return rc;
@@ -1525,11 +1526,16 @@ int KvRows(hb_ctx* ctx, const hb_kv_rows_desc* d, bool read, bool sync) {
   a.heads = d->cache.heads;
   a.groups = d->cache.page_size / 32;
   a.dim = d->cache.dim;
-  return Launched(ctx, hb::LaunchKvRows(a, read, ctx->stream), "cache row launch", sync);
+  const hipError_t err = eight ? hb::LaunchKv8Rows(a, read, ctx->stream)
+                               : hb::LaunchKvRows(a, read, ctx->stream);
+  return Launched(ctx, err, "cache row launch", sync);
 }
 
 // The checks, and the launch's arguments; *empty where there are no rows.
-int AttentionArgs(const hb_kv_attention_desc* d, hb::AttnArgs* to, bool* empty) {
+uint32_t SinksOf(const hb_kv_attention_desc&) { return 0; }
+uint32_t SinksOf(const hb_kv8_attention_desc& d) { return d.window > 0 ? d.sinks : 0; }
+template <class Desc>
+int AttentionArgs(const Desc* d, hb::AttnArgs* to, bool* empty) {
   if (!d) return Fail(HB_EINVAL, "null descriptor");
   if (int rc = CheckType(d->type)) return rc;
   if (int rc = CheckCache(d->cache)) return rc;
@@ -1579,18 +1585,183 @@ int AttentionArgs(const hb_kv_attention_desc* d, hb::AttnArgs* to, bool* empty) 
   a.max_new = max_new;
   a.max_kv = (uint32_t)std::min<uint64_t>(d->max_kv, (uint64_t)d->columns * d->cache.page_size);
   a.window = d->window;
+  a.sinks = SinksOf(*d);
   a.scale = d->scale;
   a.cap = d->softcap;
   return HB_OK;
 }
 
-int KvAttention(hb_ctx* ctx, const hb_kv_attention_desc* d, bool sync) {
+template <class Desc>
+int KvAttention(hb_ctx* ctx, const Desc* d, bool sync) {
   hb::AttnArgs a{};
   bool empty = false;
   if (int rc = AttentionArgs(d, &a, &empty)) return rc;
   if (empty) return ctx ? HB_OK : Enter(ctx);
   if (int rc = Enter(ctx)) return rc;
-  return Launched(ctx, hb::LaunchAttention(a, ctx->ws, ctx->stream), "attention launch", sync);
+  constexpr bool eight = std::is_same<Desc, hb_kv8_attention_desc>::value;
+  const hipError_t err = eight ? hb::LaunchAttention8(a, ctx->ws, ctx->stream)
+                               : hb::LaunchAttention(a, ctx->ws, ctx->stream);
+  return Launched(ctx, err, "attention launch", sync);
+}
+
+template <class Desc>
+int AttentionWay(const Desc* d, hb_kv_way* way) {
+  if (!way) return Fail(HB_EINVAL, "null way");
+  *way = hb_kv_way{};
+  hb::AttnArgs a{};
+  bool empty = false;
+  if (int rc = AttentionArgs(d, &a, &empty)) return rc;
+  if (empty) return HB_OK;
+  constexpr bool eight = std::is_same<Desc, hb_kv8_attention_desc>::value;
+  const hb::AttnWay how = eight ? hb::WayOfAttention8(a) : hb::WayOfAttention(a);
+  *way = hb_kv_way{how.way, how.tiles_of_16, how.splits, 0, how.workspace};
+  return HB_OK;
+}
+
+// A block table's rows, whose entries are counted in 31 bits.
+int CheckTable(const int32_t* table, uint32_t batch, uint32_t columns, uint32_t stride,
+               uint32_t page_size) {
+  if (page_size < 32 || page_size % 32 != 0)
+    return Fail(HB_EINVAL, "page size %u is not a multiple of 32", page_size);
+  if ((uint64_t)batch * columns > 0x7FFFFFFFu)
+    return Fail(HB_EINVAL, "table of %u rows of %u entries", batch, columns);
+  if (!table && (uint64_t)batch * columns > 0) return Fail(HB_EINVAL, "null table");
+  if (Misaligned(table, 4)) return Fail(HB_EINVAL, "tables must be 4-byte aligned");
+  if (batch > 1 && columns > stride)
+    return Fail(HB_EINVAL, "table rows of %u entries are %u apart", columns, stride);
+  return HB_OK;
+}
+
+// `count` 32-bit numbers each; lists of none may have no address.
+struct IntList {
+  const void* at;
+  uint64_t count;
+};
+template <int n>
+int CheckInts(const IntList (&lists)[n]) {
+  for (const IntList& x : lists) {
+    if (!x.at && x.count > 0) return Fail(HB_EINVAL, "null page argument");
+    if (Misaligned(x.at, 4)) return Fail(HB_EINVAL, "page lists must be 4-byte aligned");
+    if (x.count > 0xFFFFFFFEu) return Fail(HB_EINVAL, "page list of %llu", (unsigned long long)x.count);
+  }
+  return HB_OK;
+}
+
+int KvFork(hb_ctx* ctx, const hb_kv_fork_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (int rc = CheckTable(d->table, d->batch, d->columns, d->table_stride, d->page_size)) return rc;
+  if (d->batch > hb::kMostForkRows)
+    return Fail(HB_EUNSUPPORTED, "forks in a table of %u rows (up to %u)", d->batch,
+                hb::kMostForkRows);
+  if (d->forks > d->batch)
+    return Fail(HB_EINVAL, "%u forks in a table of %u rows", d->forks, d->batch);
+  if (d->free_size > 0x7FFFFFFFu) return Fail(HB_EINVAL, "%u free pages", d->free_size);
+  if (int rc = CheckInts({{d->lens, d->batch}, {d->source, d->forks}, {d->target, d->forks},
+                          {d->free_pages, d->free_size}, {d->free_count, 1},
+                          {d->lens_out, d->batch}, {d->pairs, 2ull * d->forks}, {d->status, 2}}))
+    return rc;
+  if (d->batch > 0 && d->lens == d->lens_out)
+    return Fail(HB_EINVAL, "lens_out must not be an input");
+  if (int rc = Enter(ctx)) return rc;
+  hb::ForkArgs a{d->table,    d->lens,   d->source,  d->target,       d->free_pages,
+                 d->free_count, d->lens_out, d->pairs, d->status,     d->batch,
+                 d->columns,  d->table_stride, d->page_size, d->forks, d->free_size};
+  return Launched(ctx, hb::LaunchFork(a, ctx->stream), "fork launch", sync);
+}
+
+int KvCopy(hb_ctx* ctx, const hb_kv_copy_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (!d->base) return Fail(HB_EINVAL, "null cache");
+  if (Misaligned(d->base, 16) || d->page_bytes % 16 != 0 || d->layer_bytes % 16 != 0)
+    return Fail(HB_EINVAL, "the cache, its pages and its layers must be 16-byte aligned");
+  if ((unsigned __int128)d->page_bytes * d->pages > (d->layers > 1 ? d->layer_bytes : ~0ull >> 1))
+    return Fail(HB_EINVAL, "%u pages of %llu bytes in layers of %llu", d->pages,
+                (unsigned long long)d->page_bytes, (unsigned long long)d->layer_bytes);
+  if (int rc = CheckInts({{d->pairs, 2ull * d->count}})) return rc;
+  if (d->count == 0 || d->layers == 0 || d->pages == 0 || d->page_bytes == 0)
+    return ctx ? HB_OK : Enter(ctx);
+  if (int rc = Enter(ctx)) return rc;
+  hb::CopyArgs a{static_cast<uint8_t*>(d->base), d->pairs, d->page_bytes, d->layer_bytes, d->pages,
+                 d->layers, d->count, 0, 0};
+  return Launched(ctx, hb::LaunchCopy(a, ctx->stream), "page copy launch", sync);
+}
+
+int CheckPages(uint32_t pages) {
+  if (pages > hb::kMostPages)
+    return Fail(HB_EUNSUPPORTED, "cache of %u pages (up to %u)", pages, hb::kMostPages);
+  return HB_OK;
+}
+
+int KvFree(hb_ctx* ctx, const hb_kv_free_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (int rc = CheckTable(d->table, d->batch, d->columns, d->table_stride, d->page_size)) return rc;
+  if (int rc = CheckPages(d->pages)) return rc;
+  if (d->batch > hb::kMostForkRows)
+    return Fail(HB_EUNSUPPORTED, "ends in a table of %u rows (up to %u)", d->batch,
+                hb::kMostForkRows);
+  if (d->free_size > 0x7FFFFFFFu || d->count > 0x7FFFFFFFu)
+    return Fail(HB_EINVAL, "%u rows, %u free pages", d->count, d->free_size);
+  if (int rc = CheckInts({{d->lens, d->batch}, {d->rows, d->count}, {d->free_pages, d->free_size},
+                          {d->free_count, 1}, {d->lens_out, d->batch}, {d->status, 2}}))
+    return rc;
+  if (d->batch > 0 && d->lens == d->lens_out)
+    return Fail(HB_EINVAL, "lens_out must not be an input");
+  if (int rc = Enter(ctx)) return rc;
+  hb::FreeArgs a{d->table,  d->lens,    d->rows,         d->free_pages, d->free_count,
+                 d->lens_out, d->status, d->batch,       d->columns,    d->table_stride,
+                 d->page_size, d->count, d->pages,       d->free_size};
+  return Launched(ctx, hb::LaunchFree(a, ctx->stream), "page free launch", sync);
+}
+
+int KvCompact(hb_ctx* ctx, const hb_kv_compact_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (int rc = CheckTable(d->table, d->batch, d->columns, d->table_stride, d->page_size)) return rc;
+  if (int rc = CheckTable(d->table_out, d->batch, d->columns, d->table_out_stride, d->page_size))
+    return rc;
+  if (int rc = CheckPages(d->pages)) return rc;
+  if (d->batch > 1 && d->table == d->table_out && d->table_stride != d->table_out_stride)
+    return Fail(HB_EINVAL, "one table with rows %u and %u apart", d->table_stride,
+                d->table_out_stride);
+  if (d->free_size < d->pages || d->pair_count < d->pages / 2)
+    return Fail(HB_EINVAL, "room for %u free pages and %u pairs of %u pages", d->free_size,
+                d->pair_count, d->pages);
+  if (int rc = CheckInts({{d->lens, d->batch}, {d->free_pages, d->pages}, {d->free_count, 1},
+                          {d->pairs, 2ull * d->pair_count}, {d->status, 2}}))
+    return rc;
+  if (int rc = Enter(ctx)) return rc;
+  hb::CompactArgs a{d->table,  d->lens,   d->table_out, d->free_pages, d->free_count,
+                    d->pairs,  d->status, d->batch,     d->columns,    d->table_stride,
+                    d->table_out_stride, d->page_size, d->pages, d->free_size, d->pair_count,
+                    nullptr};
+  return Launched(ctx, hb::LaunchCompact(a, ctx->ws, ctx->stream), "compaction launch", sync);
+}
+
+int TokenLogprobs(hb_ctx* ctx, const hb_logprobs_desc* d, bool sync) {
+  if (!d) return Fail(HB_EINVAL, "null descriptor");
+  if (int rc = CheckType(d->type)) return rc;
+  if (!(d->scale >= 0x1p-100f && d->scale <= 0x1p100f))
+    return Fail(HB_EINVAL, "scale %g (2^-100 to 2^100)", (double)d->scale);
+  if ((d->tokens == nullptr) != (d->logprobs == nullptr) ||
+      (d->top_ids == nullptr) != (d->top_logprobs == nullptr) ||
+      (d->rows > 0 && (d->top_ids == nullptr) != (d->top == 0)))
+    return Fail(HB_EINVAL, "log probability arguments that go together are null together");
+  if (d->vocab < 1 || d->vocab > 0x7FFFFFFFu || d->top > d->vocab)
+    return Fail(HB_EINVAL, "%u of %u tokens", d->top, d->vocab);
+  if (d->top > 64) return Fail(HB_EUNSUPPORTED, "%u most likely tokens (up to 64)", d->top);
+  if (d->rows == 0) return ctx ? HB_OK : Enter(ctx);
+  if (!d->logprobs && !d->entropy && d->top == 0)
+    return Fail(HB_EINVAL, "no log probabilities asked for");
+  if (!d->logits) return Fail(HB_EINVAL, "null logits");
+  if (d->rows > 0x7FFFFFFFu) return Fail(HB_EINVAL, "%u rows", d->rows);
+  const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;
+  if (Misaligned(d->logits, size) || Misaligned(d->tokens, 4) || Misaligned(d->logprobs, 4) ||
+      Misaligned(d->entropy, 4) || Misaligned(d->top_ids, 4) || Misaligned(d->top_logprobs, 4))
+    return Fail(HB_EINVAL, "log probability buffers must be aligned to their elements");
+  if (int rc = Enter(ctx)) return rc;
+  hb::LogprobsArgs a{d->logits, d->stride,       d->tokens, d->logprobs, d->entropy,
+                     d->top_ids, d->top_logprobs, d->type,   d->rows,     d->vocab,
+                     d->top,    d->scale};
+  return Launched(ctx, hb::LaunchLogprobs(a, ctx->ws, ctx->stream), "log probability launch", sync);
 }
 
 }  // namespace
@@ -1610,15 +1781,40 @@ int hb_kv_attention_async(hb_ctx* ctx, const hb_kv_attention_desc* d) {
   return KvAttention(ctx, d, false);
 }
 int hb_kv_attention_way(const hb_kv_attention_desc* d, hb_kv_way* way) {
-  if (!way) return Fail(HB_EINVAL, "null way");
-  *way = hb_kv_way{};
-  hb::AttnArgs a{};
-  bool empty = false;
-  if (int rc = AttentionArgs(d, &a, &empty)) return rc;
-  if (empty) return HB_OK;
-  const hb::AttnWay how = hb::WayOfAttention(a);
-  *way = hb_kv_way{how.way, how.tiles_of_16, how.splits, 0, how.workspace};
-  return HB_OK;
+  return AttentionWay(d, way);
+}
+int hb_kv8_append(hb_ctx* ctx, const hb_kv_rows_desc* d) { return KvRows(ctx, d, false, true, true); }
+int hb_kv8_append_async(hb_ctx* ctx, const hb_kv_rows_desc* d) {
+  return KvRows(ctx, d, false, false, true);
+}
+int hb_kv8_read(hb_ctx* ctx, const hb_kv_rows_desc* d) { return KvRows(ctx, d, true, true, true); }
+int hb_kv8_read_async(hb_ctx* ctx, const hb_kv_rows_desc* d) {
+  return KvRows(ctx, d, true, false, true);
+}
+int hb_kv8_attention(hb_ctx* ctx, const hb_kv8_attention_desc* d) {
+  return KvAttention(ctx, d, true);
+}
+int hb_kv8_attention_async(hb_ctx* ctx, const hb_kv8_attention_desc* d) {
+  return KvAttention(ctx, d, false);
+}
+int hb_kv8_attention_way(const hb_kv8_attention_desc* d, hb_kv_way* way) {
+  return AttentionWay(d, way);
+}
+int hb_kv_fork(hb_ctx* ctx, const hb_kv_fork_desc* d) { return KvFork(ctx, d, true); }
+int hb_kv_fork_async(hb_ctx* ctx, const hb_kv_fork_desc* d) { return KvFork(ctx, d, false); }
+int hb_kv_copy(hb_ctx* ctx, const hb_kv_copy_desc* d) { return KvCopy(ctx, d, true); }
+int hb_kv_copy_async(hb_ctx* ctx, const hb_kv_copy_desc* d) { return KvCopy(ctx, d, false); }
+int hb_kv_free(hb_ctx* ctx, const hb_kv_free_desc* d) { return KvFree(ctx, d, true); }
+int hb_kv_free_async(hb_ctx* ctx, const hb_kv_free_desc* d) { return KvFree(ctx, d, false); }
+int hb_kv_compact(hb_ctx* ctx, const hb_kv_compact_desc* d) { return KvCompact(ctx, d, true); }
+int hb_kv_compact_async(hb_ctx* ctx, const hb_kv_compact_desc* d) {
+  return KvCompact(ctx, d, false);
+}
+int hb_token_logprobs(hb_ctx* ctx, const hb_logprobs_desc* d) {
+  return TokenLogprobs(ctx, d, true);
+}
+int hb_token_logprobs_async(hb_ctx* ctx, const hb_logprobs_desc* d) {
+  return TokenLogprobs(ctx, d, false);
 }
 
 }  // extern "C"

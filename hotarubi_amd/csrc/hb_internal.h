@@ -453,7 +453,7 @@ struct AttnArgs {
   const uint8_t* cache;
   const int32_t *table, *cu, *kv_lens, *prefix;   // prefix may be null
   uint32_t type, tokens, batch, q_heads, heads, dim, pages, groups, columns, table_stride;
-  uint32_t max_new, max_kv, window;
+  uint32_t max_new, max_kv, window, sinks;        // sinks: 0 without a window
   float scale, cap;                               // cap 0: scores as they are
   // set by the launcher: tiles of rows of one (request, K/V head), splits of
   // a tile's records, records of a split, and the partial results
@@ -473,11 +473,67 @@ struct AttnWay {
 };
 AttnWay WayOfAttention(const AttnArgs& a);
 hipError_t LaunchAttention(const AttnArgs& a, Workspace& ws, hipStream_t stream);
+// The same over the 8-bit cache (hb_attn8.hip).
+AttnWay WayOfAttention8(const AttnArgs& a);
+hipError_t LaunchAttention8(const AttnArgs& a, Workspace& ws, hipStream_t stream);
 // Many rows of 16-bit types (hb_prompt.hip): 16-row tiles of a wave, rows of a
 // workgroup, and the workspace of a launch.
 uint32_t PromptTiles(uint32_t dim);
 uint32_t PromptRows(uint32_t dim);
 uint64_t PromptBytes(const AttnArgs& a);
 hipError_t LaunchPrompt(const AttnArgs& a, Workspace& ws, hipStream_t stream);
+
+// Pages (hb_pages.hip).
+constexpr uint32_t kMostForkRows = 65536;  // rows of a table whose requests fork or end
+constexpr uint32_t kMostPages = 524288;    // a bit each, twice, in a workgroup's LDS
+struct ForkArgs {
+  int32_t* table;
+  const int32_t *lens, *source, *target, *free_pages, *free_count;
+  int32_t *lens_out, *pairs, *status;
+  uint32_t batch, columns, table_stride, page, forks, free_size;
+};
+hipError_t LaunchFork(const ForkArgs& a, hipStream_t stream);
+struct CopyArgs {
+  uint8_t* base;
+  const int32_t* pairs;
+  uint64_t page_bytes, layer_bytes;
+  uint32_t pages, layers, count;
+  uint32_t stripes;  // set by the launcher, with the pieces of a page
+  uint64_t pieces;
+};
+// at least one pair, layer and byte
+hipError_t LaunchCopy(const CopyArgs& a, hipStream_t stream);
+struct FreeArgs {
+  const int32_t *table, *lens, *rows;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t *lens_out, *status;
+  uint32_t batch, columns, table_stride, page, count, pages, free_size;
+};
+hipError_t LaunchFree(const FreeArgs& a, hipStream_t stream);
+struct CompactArgs {
+  const int32_t *table, *lens;
+  int32_t *table_out, *free_pages, *free_count, *pairs, *status;
+  uint32_t batch, columns, table_stride, table_out_stride, page, pages, free_size,
+      pair_count;
+  uint32_t* place;  // set by the launcher
+};
+hipError_t LaunchCompact(const CompactArgs& a, Workspace& ws, hipStream_t stream);
+
+// Cache rows of 8 bits (hb_kv8.hip); tokens * heads < 2^31.
+hipError_t LaunchKv8Rows(const KvRowsArgs& a, bool read, hipStream_t stream);
+
+// Log probabilities (hb_logprobs.hip).
+struct LogprobsArgs {
+  const void* logits;
+  uint64_t stride;
+  const int32_t* tokens;   // null: no log probabilities of given tokens
+  float *logprobs, *entropy;
+  int32_t* top_ids;
+  float* top_logprobs;
+  uint32_t type, rows, vocab, top;
+  float scale;
+};
+hipError_t LaunchLogprobs(const LogprobsArgs& a, Workspace& ws, hipStream_t stream);
 
 }  // namespace hb

@@ -47,6 +47,32 @@ HB_KV_FN uint32_t KvVScale(uint32_t dim, uint32_t t, uint32_t col) {
   return 33 * dim + col / 32 * 32 + t % 16 / 4 * 8 + t % 4 + t / 16 * 4;
 }
 
+// The 8-bit cache's records, 64 dim + 16 bytes: E4M3 codes of K and V in the
+// order of the same lanes, and a scale byte for all of K and one for all of V.
+//   K codes   [chunk][g][n][16 B]: as above, dim/4 bytes a token
+//   V codes   [chunk][g][c][16 B]: lane (g, c) holds columns
+//             [c dim/16, (c + 1) dim/16), of each the 8 tokens above: V^T's
+//             operand without a permute
+// Scale bytes are E8M0, 10 to 246, so that every value is normal in fp32 and
+// bf16; 0 where no value but zeros was stored.
+HB_KV_FN uint32_t Kv8RecordBytes(uint32_t dim) { return 64 * dim + 16; }
+HB_KV_FN uint32_t Kv8KCode(uint32_t dim, uint32_t t, uint32_t col) {
+  const uint32_t quarter = dim / 4, at = t / 16 * quarter + col % quarter;
+  return at / 16 * 1024 + col / quarter * 256 + t % 16 * 16 + at % 16;
+}
+HB_KV_FN uint32_t Kv8VCode(uint32_t dim, uint32_t t, uint32_t col) {
+  const uint32_t part = dim / 16, at = col % part * 8 + t % 4 + t / 16 * 4;
+  return 32 * dim + at / 16 * 1024 + t % 16 / 4 * 256 + col / part * 16 + at % 16;
+}
+HB_KV_FN uint32_t Kv8Scale(uint32_t dim, uint32_t v) { return 64 * dim + v; }
+// The scale byte of values whose largest has these fp32 bits: the least
+// exponent within [-117, 119] that has it at 448 or below.
+HB_KV_FN uint32_t Kv8ScaleOf(uint32_t top_bits) {
+  if (top_bits == 0) return 0;
+  const uint32_t field = (top_bits + 0x1FFFFFu) >> 23;  // one up past 1.75 x 2^n
+  return field < 18 ? 10u : field > 254 ? 246u : field - 8;
+}
+
 // Record (its index over the whole cache) of head 0 at a slot, and the token
 // in it; false for a slot that the cache does not have.
 HB_KV_FN bool KvSlot(int32_t slot, uint32_t pages, uint32_t heads, uint32_t groups,
@@ -95,6 +121,14 @@ HB_KV_FN KvSpan KvRequest(int32_t cu0, int32_t cu1, int32_t kv_len, int32_t pref
   if (s.rows > tokens - s.first) s.rows = tokens - s.first;
   if (s.rows > max_new) s.rows = max_new;
   return s;
+}
+
+// Leading keys that a row at position `pos` sees whatever its window: the
+// prefix, and of the first `sinks` those up to its own.
+HB_KV_FN int32_t KvLead(int32_t prefix, uint32_t sinks, int32_t pos, int32_t total) {
+  int64_t lead = (int64_t)pos + 1 < (int64_t)sinks ? (int64_t)pos + 1 : (int64_t)sinks;
+  if (lead > total) lead = total;
+  return lead > prefix ? (int32_t)lead : prefix;
 }
 
 // The records that rows at positions [pos0, pos1] look at, in order:

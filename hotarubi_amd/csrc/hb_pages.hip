@@ -1,0 +1,370 @@
+// Pages of a paged cache that requests share, give back and move: forks, the
+// pages of requests that end, renumbering to the front, and the copies that
+// these ask for.  A page is in use while a row of the block table names it, so
+// there are no counts to keep: marks in LDS, a bit per page, find the pages
+// that nothing names.
+#include <algorithm>
+
+#include "hb_internal.h"
+
+namespace hb {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t PagesOf(int32_t tokens, uint32_t page) {
+  const uint32_t n = tokens < 0 ? 0u : (uint32_t)tokens;
+  return n / page + (n % page != 0 ? 1u : 0u);
+}
+
+// Inclusive sum over the workgroup's threads; *total the sum of all.  `part`
+// holds a value per wave.
+template <uint32_t threads>
+__device__ __forceinline__ uint32_t BlockSum(uint32_t x, uint32_t* part, uint32_t* total) {
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  for (uint32_t d = 1; d < 64; d *= 2) {
+    const uint32_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();  // the values of an earlier call have been read
+  if (lane == 63) part[wave] = x;
+  __syncthreads();
+  uint32_t sum = 0;
+  for (uint32_t w = 0; w < threads / 64; ++w) {
+    if (w < wave) x += part[w];
+    sum += part[w];
+  }
+  *total = sum;
+  return x;
+}
+
+// ------------------------------------------------------------------- fork --
+
+constexpr uint32_t kForkThreads = 256, kForkWaves = kForkThreads / 64;
+constexpr uint32_t kRowWindow = 8192;  // rows of the table looked at together
+
+// Every workgroup finds for itself which forks are in order (targets that are
+// a source, or another's target before them, are not) and sums the pages that
+// they want, as the step plan's do; then its waves take forks of their own and
+// copy their rows' entries.  Sources are not written, so no workgroup reads
+// what another writes.
+__global__ __launch_bounds__(kForkThreads) void ForkKernel(const ForkArgs a) {
+  __shared__ uint32_t first[kRowWindow], is_source[kRowWindow / 32];
+  __shared__ uint32_t bad[kMostForkRows / 32], again[kMostForkRows / 32];
+  __shared__ uint32_t place[kForkThreads], part[kForkWaves];
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  constexpr uint32_t kNone = 0xFFFFFFFFu;
+  for (uint32_t i = tid; i < (a.forks + 31) / 32; i += kForkThreads) bad[i] = again[i] = 0;
+  for (uint32_t base = 0; base < a.batch; base += kRowWindow) {
+    const uint32_t rows = min(kRowWindow, a.batch - base);
+    __syncthreads();  // the window before has been read
+    for (uint32_t i = tid; i < rows; i += kForkThreads) first[i] = kNone;
+    for (uint32_t i = tid; i < kRowWindow / 32; i += kForkThreads) is_source[i] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < a.forks; i += kForkThreads) {
+      const uint32_t s = (uint32_t)a.source[i] - base, t = (uint32_t)a.target[i] - base;
+      if (s < rows) atomicOr(&is_source[s / 32], 1u << (s % 32));
+      if (t < rows) atomicMin(&first[t], i);
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < a.forks; i += kForkThreads) {
+      const uint32_t t = (uint32_t)a.target[i] - base;
+      if (t >= rows) continue;
+      if (first[t] != i) atomicOr(&again[i / 32], 1u << (i % 32));
+      if (first[t] != i || (is_source[t / 32] >> (t % 32) & 1u))
+        atomicOr(&bad[i / 32], 1u << (i % 32));
+    }
+    // rows that are no target keep their lengths; the others' first fork says
+    for (uint32_t i = blockIdx.x * kForkThreads + tid; i < rows; i += gridDim.x * kForkThreads)
+      if (first[i] == kNone) a.lens_out[base + i] = a.lens[base + i];
+  }
+  __syncthreads();
+  const uint32_t free_count = (uint32_t)max(0, min(*a.free_count, (int32_t)a.free_size));
+  uint32_t wanted = 0, taken = 0, refused = 0;
+  constexpr uint32_t kRefused = 0xFFFFFFFFu, kNoPage = 0xFFFFFFFEu;
+  for (uint32_t base = 0; base < a.forks; base += kForkThreads) {
+    const uint32_t i = base + tid;
+    bool fits = false, need = false;
+    if (i < a.forks) {
+      const uint32_t s = (uint32_t)a.source[i], t = (uint32_t)a.target[i];
+      if (s < a.batch && t < a.batch && !(bad[i / 32] >> (i % 32) & 1u)) {
+        const int32_t n = a.lens[s];
+        fits = PagesOf(n, a.page) <= a.columns;
+        need = fits && n > 0 && (uint32_t)n % a.page != 0;
+      }
+    }
+    uint32_t total, good, spare;
+    const uint32_t stop = wanted + BlockSum<kForkThreads>(need, part, &total);
+    const bool ok = fits && (!need || stop <= free_count);
+    place[tid] = !ok ? kRefused : need ? free_count - stop : kNoPage;
+    BlockSum<kForkThreads>(ok && need, part, &good);
+    BlockSum<kForkThreads>(i < a.forks && !ok, part, &spare);
+    wanted += total;
+    taken += good;
+    refused += spare;
+    // (the sums' barriers stand between place's writes and its reads)
+    const uint32_t chunk = min(kForkThreads, a.forks - base);
+    for (uint32_t j = blockIdx.x * kForkWaves + wave; j < chunk; j += gridDim.x * kForkWaves) {
+      const uint32_t f = base + j, at = place[j];
+      const uint32_t s = (uint32_t)a.source[f], t = (uint32_t)a.target[f];
+      int32_t from = -1, to = -1;
+      if (at != kRefused) {
+        const int32_t n = a.lens[s];
+        const uint32_t whole = n > 0 ? (uint32_t)n / a.page : 0u;
+        const int32_t* const x = a.table + (uint64_t)s * a.table_stride;
+        int32_t* const y = a.table + (uint64_t)t * a.table_stride;
+        for (uint32_t c = lane; c < whole; c += 64) y[c] = x[c];
+        if (at != kNoPage) {
+          from = x[whole];
+          to = a.free_pages[at];
+          if (lane == 0) y[whole] = to;
+        }
+      }
+      if (lane == 0) {
+        a.pairs[2 * (uint64_t)f] = from;
+        a.pairs[2 * (uint64_t)f + 1] = to;
+        if (t < a.batch && !(again[f / 32] >> (f % 32) & 1u))
+          a.lens_out[t] = at != kRefused ? max(0, a.lens[s]) : a.lens[t];
+      }
+    }
+    __syncthreads();  // place has been read
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    a.status[0] = (int32_t)taken;
+    a.status[1] = (int32_t)refused;
+  }
+}
+
+// ------------------------------------------------------------------- copy --
+
+constexpr uint32_t kCopyThreads = 256, kCopyPiece = kCopyThreads * 16 * 2;
+
+// A workgroup takes a piece of a page in one layer, for pairs `stripes` apart:
+// it looks at 64 of them at a time, since lists of moves are mostly empty.
+__global__ __launch_bounds__(kCopyThreads) void CopyKernel(const CopyArgs a) {
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t stripe = blockIdx.x % a.stripes, slot = blockIdx.x / a.stripes;
+  const uint64_t piece = slot % a.pieces;
+  uint8_t* const base = a.base + slot / a.pieces * a.layer_bytes + piece * kCopyPiece;
+  const uint64_t left = a.page_bytes - piece * kCopyPiece;
+  const uint32_t at = threadIdx.x * 16;
+  const bool one = at < left, two = at + kCopyPiece / 2 < left;
+  for (uint64_t i = stripe; i < a.count; i += 64ull * a.stripes) {
+    const uint64_t mine = i + (uint64_t)lane * a.stripes;
+    uint32_t from = 0xFFFFFFFFu, to = 0xFFFFFFFFu;
+    if (mine < a.count) {
+      from = (uint32_t)a.pairs[2 * mine];
+      to = (uint32_t)a.pairs[2 * mine + 1];
+    }
+    uint64_t todo = __builtin_amdgcn_ballot_w64(from < a.pages && to < a.pages && from != to);
+    while (todo != 0) {
+      const int j = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const uint8_t* const x =
+          base + (uint32_t)__builtin_amdgcn_readlane((int)from, j) * a.page_bytes + at;
+      uint8_t* const y = base + (uint32_t)__builtin_amdgcn_readlane((int)to, j) * a.page_bytes + at;
+      u32x4 u, v;
+      if (one) u = *reinterpret_cast<const u32x4*>(x);
+      if (two) v = *reinterpret_cast<const u32x4*>(x + kCopyPiece / 2);
+      if (one) *reinterpret_cast<u32x4*>(y) = u;
+      if (two) *reinterpret_cast<u32x4*>(y + kCopyPiece / 2) = v;
+    }
+  }
+}
+
+// --------------------------------------------------------- free, compact --
+
+constexpr uint32_t kMarkThreads = 1024, kMarkWords = kMostPages / 32;
+
+// mark(page, row) for every entry of a row's pages.  All of the table is read,
+// so that a load waits for no length.
+template <class Mark>
+__device__ __forceinline__ void EachEntry(const int32_t* table, const int32_t* lens,
+                                          uint32_t batch, uint32_t columns, uint32_t stride,
+                                          uint32_t page, uint32_t pages, Mark&& mark) {
+  const uint32_t all = batch * columns;  // below 2^31
+  constexpr uint32_t kEach = 4;
+  for (uint32_t base = threadIdx.x; base < all; base += kEach * kMarkThreads) {
+    uint32_t entry[kEach], row[kEach], col[kEach];
+    int32_t len[kEach];
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+      const uint32_t i = base + j * kMarkThreads;
+      entry[j] = 0xFFFFFFFFu;
+      row[j] = col[j] = 0;
+      len[j] = 0;
+      if (i >= all) continue;
+      row[j] = i / columns;
+      col[j] = i % columns;
+      entry[j] = (uint32_t)table[(uint64_t)row[j] * stride + col[j]];
+      len[j] = lens[row[j]];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j)
+      if (entry[j] < pages && col[j] < PagesOf(len[j], page)) mark(entry[j], row[j]);
+  }
+}
+
+// One workgroup: the marks are a bit per page in its LDS, and a second launch
+// or a wait between workgroups would take longer than the table's entries.
+__global__ __launch_bounds__(kMarkThreads) void FreeKernel(const FreeArgs a) {
+  __shared__ uint32_t kept[kMarkWords], gone[kMarkWords], ends[kMostForkRows / 32];
+  __shared__ uint32_t part[kMarkThreads / 64];
+  const uint32_t tid = threadIdx.x, words = (a.pages + 31) / 32;
+  for (uint32_t i = tid; i < words; i += kMarkThreads) kept[i] = gone[i] = 0;
+  for (uint32_t i = tid; i < (a.batch + 31) / 32; i += kMarkThreads) ends[i] = 0;
+  __syncthreads();
+  for (uint32_t i = tid; i < a.count; i += kMarkThreads) {
+    const uint32_t r = (uint32_t)a.rows[i];
+    if (r < a.batch) atomicOr(&ends[r / 32], 1u << (r % 32));
+  }
+  const uint32_t free_count = (uint32_t)max(0, min(*a.free_count, (int32_t)a.free_size));
+  for (uint32_t i = tid; i < free_count; i += kMarkThreads) {
+    const uint32_t p = (uint32_t)a.free_pages[i];
+    if (p < a.pages) atomicOr(&kept[p / 32], 1u << (p % 32));
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < a.batch; i += kMarkThreads)
+    a.lens_out[i] = ends[i / 32] >> (i % 32) & 1u ? 0 : a.lens[i];
+  EachEntry(a.table, a.lens, a.batch, a.columns, a.table_stride, a.page, a.pages,
+            [&](uint32_t p, uint32_t row) {
+              uint32_t* const in = ends[row / 32] >> (row % 32) & 1u ? gone : kept;
+              atomicOr(&in[p / 32], 1u << (p % 32));
+            });
+  __syncthreads();
+  // the highest page first: thread 0 takes the last words
+  const uint32_t each = (words + kMarkThreads - 1) / kMarkThreads;
+  uint32_t sum = 0, total;
+  for (uint32_t j = 0; j < each; ++j) {
+    const uint32_t w = tid * each + j;
+    if (w < words) sum += (uint32_t)__builtin_popcount(gone[words - 1 - w] & ~kept[words - 1 - w]);
+  }
+  uint32_t at = BlockSum<kMarkThreads>(sum, part, &total) - sum;
+  const uint32_t room = a.free_size - free_count;
+  for (uint32_t j = 0; j < each; ++j) {
+    const uint32_t w = tid * each + j;
+    if (w >= words) break;
+    uint32_t bits = gone[words - 1 - w] & ~kept[words - 1 - w];
+    while (bits != 0) {
+      const uint32_t b = 31 - (uint32_t)__builtin_clz(bits);
+      bits &= ~(1u << b);
+      if (at < room) a.free_pages[free_count + at] = (int32_t)((words - 1 - w) * 32 + b);
+      ++at;
+    }
+  }
+  if (tid == 0) {
+    a.status[0] = (int32_t)min(total, room);
+    a.status[1] = (int32_t)(total - min(total, room));
+  }
+}
+
+// The pages in use, their ranks, and the pairs; `place` says for a page that
+// moves which pair is its.
+__global__ __launch_bounds__(kMarkThreads) void CompactKernel(const CompactArgs a) {
+  __shared__ uint32_t used[kMarkWords], part[kMarkThreads / 64];
+  __shared__ uint32_t before_u;
+  const uint32_t tid = threadIdx.x, words = (a.pages + 31) / 32;
+  for (uint32_t i = tid; i < words; i += kMarkThreads) used[i] = 0;
+  __syncthreads();
+  EachEntry(a.table, a.lens, a.batch, a.columns, a.table_stride, a.page, a.pages,
+            [&](uint32_t p, uint32_t) { atomicOr(&used[p / 32], 1u << (p % 32)); });
+  __syncthreads();
+  const uint32_t each = (words + kMarkThreads - 1) / kMarkThreads;
+  uint32_t sum = 0, count;
+  for (uint32_t j = 0; j < each; ++j) {
+    const uint32_t w = tid * each + j;
+    if (w < words) sum += (uint32_t)__builtin_popcount(used[w]);
+  }
+  const uint32_t start = BlockSum<kMarkThreads>(sum, part, &count) - sum;
+  // pages in use before `count`: the rank at which the moves begin
+  if (tid == 0) before_u = count;  // (all of them where count is the last page)
+  __syncthreads();
+  uint32_t rank = start;
+  for (uint32_t j = 0; j < each; ++j) {
+    const uint32_t w = tid * each + j;
+    if (w >= words) break;
+    if (w == count / 32)
+      before_u = rank + (uint32_t)__builtin_popcount(used[w] & ((1u << (count % 32)) - 1u));
+    rank += (uint32_t)__builtin_popcount(used[w]);
+  }
+  __syncthreads();
+  const uint32_t stay = before_u;
+  rank = start;
+  for (uint32_t j = 0; j < each; ++j) {
+    const uint32_t w = tid * each + j;
+    if (w >= words) break;
+    uint32_t hole = w * 32 - rank;  // unused pages before the word
+    for (uint32_t bits = ~used[w]; bits != 0; bits &= bits - 1, ++hole) {
+      const uint32_t p = w * 32 + (uint32_t)__builtin_ctz(bits);
+      if (p >= count) break;
+      a.pairs[2 * (uint64_t)hole + 1] = (int32_t)p;
+    }
+    for (uint32_t bits = used[w]; bits != 0; bits &= bits - 1, ++rank) {
+      const uint32_t p = w * 32 + (uint32_t)__builtin_ctz(bits);
+      if (p < count) continue;
+      a.pairs[2 * (uint64_t)(rank - stay)] = (int32_t)p;
+      a.place[p] = rank - stay;
+    }
+  }
+  if (tid == 0) {
+    a.status[0] = (int32_t)count;
+    a.status[1] = (int32_t)(count - stay);
+    *a.free_count = (int32_t)(a.pages - count);
+  }
+}
+
+// The tables' new numbers, and what is left of the lists.
+__global__ __launch_bounds__(256) void RenumberKernel(const CompactArgs a) {
+  const uint32_t count = (uint32_t)a.status[0], moved = (uint32_t)a.status[1];
+  const uint32_t first = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
+  for (uint32_t i = first; i < a.batch * a.columns; i += step) {  // below 2^31
+    const uint32_t row = i / a.columns, col = i % a.columns;
+    const uint32_t p = (uint32_t)a.table[(uint64_t)row * a.table_stride + col];
+    int32_t to = -1;
+    if (p < a.pages && col < PagesOf(a.lens[row], a.page))
+      to = p < count ? (int32_t)p : a.pairs[2 * (uint64_t)a.place[p] + 1];
+    a.table_out[(uint64_t)row * a.table_out_stride + col] = to;
+  }
+  for (uint64_t i = first; i < a.free_size; i += step)
+    a.free_pages[i] = i < a.pages - count ? (int32_t)(a.pages - 1 - (uint32_t)i) : -1;
+  for (uint64_t i = 2ull * moved + first; i < 2ull * a.pair_count; i += step) a.pairs[i] = -1;
+}
+
+}  // namespace
+
+hipError_t LaunchFork(const ForkArgs& a, hipStream_t stream) {
+  const uint32_t grid = std::min(kForkThreads / kForkWaves,
+                                 std::max(1u, (a.forks + kForkWaves - 1) / kForkWaves));
+  ForkKernel<<<grid, kForkThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t LaunchCopy(const CopyArgs& in, hipStream_t stream) {
+  CopyArgs a = in;
+  a.pieces = (a.page_bytes + kCopyPiece - 1) / kCopyPiece;
+  const uint64_t slots = a.pieces * a.layers;
+  if (slots > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  // about 8 workgroups a CU, as far as the pairs go
+  const uint64_t want = 8 * (uint64_t)DeviceCus();
+  a.stripes = (uint32_t)std::min<uint64_t>(a.count, std::max<uint64_t>(1, want / slots));
+  CopyKernel<<<(uint32_t)(slots * a.stripes), kCopyThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t LaunchFree(const FreeArgs& a, hipStream_t stream) {
+  FreeKernel<<<1, kMarkThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t LaunchCompact(const CompactArgs& in, Workspace& ws, hipStream_t stream) {
+  CompactArgs a = in;
+  const hipError_t err = GrowWorkspace(ws, (size_t)a.pages * 4, stream);
+  if (err != hipSuccess) return err;
+  a.place = reinterpret_cast<uint32_t*>(ws.ptr + kSplitCounters);
+  CompactKernel<<<1, kMarkThreads, 0, stream>>>(a);
+  const uint64_t most = std::max<uint64_t>((uint64_t)a.batch * a.columns, a.free_size);
+  RenumberKernel<<<(uint32_t)std::min<uint64_t>(1024, (most + 255) / 256), 256, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace hb

@@ -729,6 +729,187 @@ typedef struct hb_kv_way {
 } hb_kv_way;
 int hb_kv_attention_way(const hb_kv_attention_desc* desc, hb_kv_way* way);
 
+/* ------------------------------------------- the cache in 8 bits -- */
+
+/* A cache of 8-bit records beside the MXFP4 one: uint8
+ * [pages][heads][page_size / 32][64 dim + 16], a record per 32 tokens (a
+ * block) of one head, on the same pages, slots and block tables.  A record
+ * holds the K codes (32 dim bytes), the V codes (32 dim), the scale byte of
+ * K, that of V and 14 bytes that nothing reads.  With g = 0..3, n, c = 0..15
+ * and `chunk` counting 16-byte pieces:
+ *   K codes  [chunk dim/32][g][n][16 B]: (g, n) holds, in chunk order, columns
+ *            [g dim/4, (g + 1) dim/4) of token n and then of token 16 + n
+ *   V codes  [chunk dim/32][g][c][16 B]: (g, c) holds columns
+ *            [c dim/16, (c + 1) dim/16), of each tokens 4g..4g+3, 16+4g..16+4g+3
+ * A value is its E4M3 code (OCP, no infinities; 0x7F and 0xFF are NaN) times
+ * 2^(scale byte - 127).  Scale bytes are 0 (no value but zeros) or 10 to 246.
+ *
+ * hb_kv8_append writes K and V rows [tokens][heads][dim] of `type` at int32
+ * slots[token]; the tokens of a block come in their order, in one call or in
+ * several.  Rows next to one another whose slots are too, within a block, are
+ * a run.  A run that begins at a block's first token begins the block anew;
+ * otherwise the block's earlier tokens stay.  The scale is the least 2^e, e
+ * within [-117, 119], that has the run's largest value at 448 or below, and
+ * not below that of earlier tokens, whose codes are rounded again where it
+ * grows; values are rounded to nearest even (past 448 x 2^119: to that).  A
+ * token's head with an infinity or NaN in K or V is stored as NaN keys and
+ * zero values and moves no scale.  A slot below 0 or past the cache's pages
+ * is not written and ends a run.  A call brings each block at most one run.
+ * hb_kv8_read gives the stored values of slots, zeros where there is none.
+ * The descriptors are hb_kv_append's. */
+int hb_kv8_append(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+int hb_kv8_append_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+int hb_kv8_read(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+int hb_kv8_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
+
+/* Attention over the 8-bit cache: hb_kv_attention's rows, masks and sums.
+ * With a window the first `sinks` tokens stay visible to the rows behind
+ * them: row at p sees key j (j < kv_lens[b]) if
+ *   j <= p and (window == 0 or p - j < window or j < sinks), or j < prefix[b].
+ * q and the cache's values enter the products exactly.  The softmax's weights
+ * enter theirs in f16 for bf16 and fp16 tensors (each off by 2^-11 of itself
+ * or 2^-32 of the row's largest, whichever is more; beside V scales that f16
+ * does not hold, bytes outside 0 and 112 to 134, by 2^-16 of itself), and as
+ * three bf16 parts for fp32 ones (2^-24).  A NaN key makes the rows that see
+ * its token NaN, no others; V holds no NaN below kv_lens. */
+typedef struct hb_kv8_attention_desc {
+  hb_kv_cache cache;
+  const void* q;
+  void* out;
+  uint64_t q_token, q_head, out_token, out_head;
+  const int32_t* table;
+  const int32_t* cu;
+  const int32_t* kv_lens;
+  const int32_t* prefix; /* null: none */
+  uint32_t type, tokens, q_heads, batch, columns, table_stride;
+  uint32_t max_new, max_kv, window, sinks;
+  float scale, softcap; /* softcap 0: none */
+} hb_kv8_attention_desc;
+int hb_kv8_attention(hb_ctx* ctx, const hb_kv8_attention_desc* desc);
+int hb_kv8_attention_async(hb_ctx* ctx, const hb_kv8_attention_desc* desc);
+int hb_kv8_attention_way(const hb_kv8_attention_desc* desc, hb_kv_way* way);
+
+/* ------------------------------------------------- pages of a cache -- */
+
+/* Requests that share pages, end, and move, for caches of any record.  A page
+ * is in use while an entry of a request's first ceil(lens[b] / page_size)
+ * table entries names it: there are no counts of references.  Entries that
+ * name no page are passed over.  Lengths below 0 count as 0, and a row has
+ * `columns` entries whatever its length.  page_size is a multiple of 32.
+ *
+ * hb_kv_fork: request target[i] goes on from request source[i]'s tokens.  Its
+ * table row gets the source's entries of whole pages; a last page that is not
+ * full becomes a page of its own, from the top of the stack
+ * free_pages[0 .. *free_count) in the order of the forks, and pairs[i] says
+ * (source's page, new page) for hb_kv_copy, (-1, -1) where nothing is to be
+ * copied.  Entries past them stay.  lens_out is lens with the targets'
+ * new lengths.  A fork is refused (its row and length stay) if source or
+ * target is no row, the target is the source of a fork or the target of one
+ * before it, the source's pages pass the table's columns, or the pages wanted
+ * by it and the forks before it, whether they got them or not, the free ones.
+ * status int32 [2]: pages taken, forks refused.  *free_count is left as it is:
+ * the caller takes status[0] from it.  forks <= batch <= 65536. */
+typedef struct hb_kv_fork_desc {
+  int32_t* table;            /* [batch][columns], rows table_stride apart */
+  const int32_t* lens;       /* [batch] */
+  const int32_t* source;     /* [forks] */
+  const int32_t* target;     /* [forks] */
+  const int32_t* free_pages; /* [free_size] */
+  const int32_t* free_count; /* [1] */
+  int32_t* lens_out;         /* [batch], not lens */
+  int32_t* pairs;            /* [forks][2] */
+  int32_t* status;           /* [2] */
+  uint32_t batch, columns, table_stride, page_size, forks, free_size;
+} hb_kv_fork_desc;
+int hb_kv_fork(hb_ctx* ctx, const hb_kv_fork_desc* desc);
+int hb_kv_fork_async(hb_ctx* ctx, const hb_kv_fork_desc* desc);
+
+/* Copies page pairs[i][0] over page pairs[i][1] in each of `layers` caches
+ * layer_bytes apart, page_bytes a page (both and the base multiples of 16).  A
+ * pair that names no page, or one page twice, is passed over.  No page is
+ * written by two pairs or written by one and read by another. */
+typedef struct hb_kv_copy_desc {
+  void* base;
+  const int32_t* pairs; /* [count][2] */
+  uint64_t page_bytes, layer_bytes;
+  uint32_t pages, layers, count;
+} hb_kv_copy_desc;
+int hb_kv_copy(hb_ctx* ctx, const hb_kv_copy_desc* desc);
+int hb_kv_copy_async(hb_ctx* ctx, const hb_kv_copy_desc* desc);
+
+/* hb_kv_free: the requests rows[0 .. count) end (numbers that are no row are
+ * passed over).  Their pages that no other request names and that are not on
+ * the stack free_pages[0 .. *free_count) are put on it, the highest first, as
+ * far as free_size goes.  lens_out is lens, 0 for the rows that end.  status
+ * int32 [2]: pages put on the stack, pages that found no room.  *free_count
+ * and the table are left as they are: the caller adds status[0] to the count.
+ * pages <= 524288. */
+typedef struct hb_kv_free_desc {
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* rows;       /* [count] */
+  int32_t* free_pages;       /* [free_size] */
+  const int32_t* free_count; /* [1] */
+  int32_t* lens_out;         /* [batch], not lens */
+  int32_t* status;           /* [2] */
+  uint32_t batch, columns, table_stride, page_size, count, pages, free_size;
+} hb_kv_free_desc;
+int hb_kv_free(hb_ctx* ctx, const hb_kv_free_desc* desc);
+int hb_kv_free_async(hb_ctx* ctx, const hb_kv_free_desc* desc);
+
+/* hb_kv_compact: the U pages in use become the first U ones.  The i-th page in
+ * use from U on takes the place of the i-th unused one before U, and pairs[i]
+ * says (page, place) for hb_kv_copy, (-1, -1) past the last.  table_out gets
+ * the rows' entries with the new numbers, -1 past a row's pages and for
+ * entries that name no page; it may be the table.  free_pages becomes
+ * pages - 1, .., U (the lowest on top), -1 past them, and *free_count
+ * pages - U.  status int32 [2]: U, pages that move.  free_size >= pages, pair_count >= pages / 2,
+ * pages <= 524288. */
+typedef struct hb_kv_compact_desc {
+  const int32_t* table;
+  const int32_t* lens;
+  int32_t* table_out;  /* [batch][columns], rows table_out_stride apart */
+  int32_t* free_pages; /* [free_size] */
+  int32_t* free_count; /* [1] */
+  int32_t* pairs;      /* [pair_count][2] */
+  int32_t* status;     /* [2] */
+  uint32_t batch, columns, table_stride, table_out_stride, page_size, pages, free_size,
+      pair_count;
+} hb_kv_compact_desc;
+int hb_kv_compact(hb_ctx* ctx, const hb_kv_compact_desc* desc);
+int hb_kv_compact_async(hb_ctx* ctx, const hb_kv_compact_desc* desc);
+
+/* ------------------------------------------------ answers of a step -- */
+
+/* Of each row of logits (x = scale * logit, scale from 2^-100 to 2^100):
+ *   logprobs[r]      x[tokens[r]] - log sum_j e^x[j]; 0 where tokens[r] < 0,
+ *                    NaN where it is vocab or more
+ *   entropy[r]       -sum_j p[j] log p[j]
+ *   top_ids[r][i], top_logprobs[r][i]  the `top` largest logits' columns, the
+ *                    largest first and of equal ones the lowest column, and
+ *                    their log probabilities; a NaN ranks below -inf
+ * A logit of -inf has probability 0.  A row of nothing else has log
+ * probabilities -inf and entropy 0; a row with a NaN or +inf has NaN for all.
+ * Maxima and sums are in 32 bits.  tokens and logprobs are null together;
+ * entropy may be null; top_ids and top_logprobs are null together and top 0
+ * then.  logits is [rows][vocab] of `type`, rows `stride` elements apart; top
+ * <= 64 and <= vocab; the others are contiguous.
+ * Few long rows are split over workgroups that meet in the context's
+ * workspace, in a fixed order: results do not change from call to call. */
+typedef struct hb_logprobs_desc {
+  const void* logits;
+  uint64_t stride;
+  const int32_t* tokens;
+  float* logprobs;
+  float* entropy;
+  int32_t* top_ids;
+  float* top_logprobs;
+  uint32_t type, rows, vocab, top;
+  float scale;
+} hb_logprobs_desc;
+int hb_token_logprobs(hb_ctx* ctx, const hb_logprobs_desc* desc);
+int hb_token_logprobs_async(hb_ctx* ctx, const hb_logprobs_desc* desc);
+
 /* --------------------------------------------------------- formats -- */
 
 /* EncodeMxint8 + PackAbuf on device: x fp32 row-major [rows][cols] ->
