@@ -1,5 +1,6 @@
-// What the attention kernels share: records of the cache as the matrix cores'
-// operands, the softmax of a tile, rows and what they see.
+// What the attention kernels share: records of the caches as the matrix cores'
+// operands, the softmax of a tile, rows and what they see.  Fp4 and Fp8 name the
+// records, MXFP4 ones and those of 8 bits.
 #pragma once
 
 #include "hb_internal.h"
@@ -48,24 +49,77 @@ constexpr float kRoom = 64.f;
 
 // ---------------------------------------------------------------- records --
 
+struct Fp4 {
+  static constexpr bool kSinks = false;
+  // bf16 parts of q, by the tensors' type
+  static constexpr uint32_t Parts(uint32_t parts) { return parts; }
+  static constexpr uint32_t Bytes(uint32_t dim) { return KvRecordBytes(dim); }
+  static hipError_t Prompt(const AttnArgs& a, Workspace& ws, hipStream_t stream) {
+    return LaunchPrompt(a, ws, stream);
+  }
+};
+// E4M3 codes are exact in f16 whatever the scale, which is one for all keys of
+// the record and goes over their scores: fp16 queries take one product.
+struct Fp8 {
+  static constexpr bool kSinks = true;
+  static constexpr uint32_t Parts(uint32_t parts) { return parts == 2 ? 1 : parts; }
+  static constexpr uint32_t Bytes(uint32_t dim) { return Kv8RecordBytes(dim); }
+  static hipError_t Prompt(const AttnArgs& a, Workspace& ws, hipStream_t stream) {
+    return LaunchPrompt8(a, ws, stream);
+  }
+};
+// What q and K enter their products as.
+template <class F, uint32_t parts>
+struct QueryOperand {
+  typedef bf16x8 type;
+};
+template <>
+struct QueryOperand<Fp8, 2> {
+  typedef f16x8 type;
+};
+
+template <class F, uint32_t D>
+struct Record;
 template <uint32_t D>
-struct Record {
+struct Record<Fp4, D> {
   u32x4 k[D / 64], v[D / 64];
   uint32_t ks[D == 256 ? 2 : 1];  // scale bytes of tokens n, 16 + n of the lane's block(s)
   uint32_t vs[2];                 // scale bytes of the lane's 8 tokens
 };
 
+template <uint32_t D>
+struct Record<Fp8, D> {
+  u32x4 k[D / 32], v[D / 32];
+  uint32_t scales;  // K's byte and V's, the same in all lanes
+};
+
 // Records go from memory into LDS by direct loads, kDepth of them under way or
 // waiting per wave (a ring of its own, no barrier): what a CU needs in flight
 // to draw its share of HBM is 40 KB or more, which registers do not hold.
+template <class F, uint32_t D>
+struct Ring;
 template <uint32_t D>
-struct Ring {
+struct Ring<Fp4, D> {
   static constexpr uint32_t kSlot = D == 64 ? 2304 : 34 * D;  // whole loads
   static constexpr uint32_t kOps = D / 32 + (D == 256 ? 2 : 1);
   static constexpr uint32_t kDepth = D == 64 ? 7 : D == 128 ? 4 : 2;
 };
 template <uint32_t D>
+struct Ring<Fp8, D> {
+  static constexpr uint32_t kSlot = 64 * D + 256;
+  static constexpr uint32_t kOps = D / 16 + 1;
+  static constexpr uint32_t kDepth = D == 64 ? 4 : D == 128 ? 2 : 1;
+};
+template <class F, uint32_t D>
 __device__ __forceinline__ void FetchRecord(const uint8_t* base, uint32_t lds) {
+  if constexpr (__is_same(F, Fp8)) {
+    const uint32_t lane = threadIdx.x % 64;
+#pragma unroll
+    for (uint32_t c = 0; c < D / 16; ++c) ring::Dma16(base + c * 1024, lane * 16, lds + c * 1024);
+    // the record's last 16 bytes, over and over
+    ring::Dma4(base + 64 * D, lane % 4 * 4, lds + 64 * D);
+    return;
+  }
   const uint32_t lane = threadIdx.x % 64;
 #pragma unroll
   for (uint32_t c = 0; c < D / 32; ++c) ring::Dma16(base + c * 1024, lane * 16, lds + c * 1024);
@@ -75,7 +129,7 @@ __device__ __forceinline__ void FetchRecord(const uint8_t* base, uint32_t lds) {
   if (D == 256) ring::Dma4(base + 32 * D + 256, lane * 4, lds + 32 * D + 256);
 }
 template <uint32_t D>
-__device__ __forceinline__ void ReadKeys(const uint8_t* slot, Record<D>& r) {
+__device__ __forceinline__ void ReadKeys(const uint8_t* slot, Record<Fp4, D>& r) {
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
 #pragma unroll
   for (uint32_t c = 0; c < D / 64; ++c)
@@ -86,7 +140,7 @@ __device__ __forceinline__ void ReadKeys(const uint8_t* slot, Record<D>& r) {
     r.ks[D == 256] = *reinterpret_cast<const uint16_t*>(slot + 32 * D + block * 32 + 32 + n * 2);
 }
 template <uint32_t D>
-__device__ __forceinline__ void ReadValues(const uint8_t* slot, Record<D>& r) {
+__device__ __forceinline__ void ReadValues(const uint8_t* slot, Record<Fp4, D>& r) {
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
 #pragma unroll
   for (uint32_t c = 0; c < D / 64; ++c)
@@ -94,6 +148,22 @@ __device__ __forceinline__ void ReadValues(const uint8_t* slot, Record<D>& r) {
   const uint2 vs = *reinterpret_cast<const uint2*>(slot + 33 * D + n * D / 512 * 32 + g * 8);
   r.vs[0] = vs.x;
   r.vs[1] = vs.y;
+}
+
+template <uint32_t D>
+__device__ __forceinline__ void ReadKeys(const uint8_t* slot, Record<Fp8, D>& r) {
+  const uint32_t lane = threadIdx.x % 64;
+#pragma unroll
+  for (uint32_t c = 0; c < D / 32; ++c)
+    r.k[c] = *reinterpret_cast<const u32x4*>(slot + c * 1024 + lane * 16);
+  r.scales = *reinterpret_cast<const uint16_t*>(slot + 64 * D);
+}
+template <uint32_t D>
+__device__ __forceinline__ void ReadValues(const uint8_t* slot, Record<Fp8, D>& r) {
+  const uint32_t lane = threadIdx.x % 64;
+#pragma unroll
+  for (uint32_t c = 0; c < D / 32; ++c)
+    r.v[c] = *reinterpret_cast<const u32x4*>(slot + 32 * D + c * 1024 + lane * 16);
 }
 
 __device__ __forceinline__ float ScaleOf(uint32_t bytes, uint32_t i) {
@@ -112,8 +182,8 @@ __device__ __forceinline__ uint32_t Two(uint32_t word, float scale) {
                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, sel));
 }
 // Operand of K: tokens 16 tile + n, the lane's columns 8 s .. 8 s + 7.
-template <uint32_t D>
-__device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, uint32_t s) {
+template <uint32_t parts, uint32_t D>
+__device__ __forceinline__ bf16x8 KeyOperand(const Record<Fp4, D>& r, uint32_t tile, uint32_t s) {
   const uint32_t word = tile * (D / 32) + s;
   const uint32_t w = r.k[word / 4][word % 4];
   const float scale = ScaleOf(r.ks[D == 256 ? s / 4 : 0], tile);
@@ -123,6 +193,38 @@ __device__ __forceinline__ bf16x8 KeyOperand(const Record<D>& r, uint32_t tile, 
   x[2] = Two<2>(w, scale);
   x[3] = Two<3>(w, scale);
   return __builtin_bit_cast(bf16x8, x);
+}
+
+// Eight E4M3 codes, two words, as the operand's type (exact where the type's
+// range holds code x scale).
+template <bool half>
+__device__ __forceinline__ u32x4 EightOf(uint32_t lo, uint32_t hi, float scale) {
+  u32x4 x;
+  if constexpr (half) {
+    x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false));
+    x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true));
+    x[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false));
+    x[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true));
+  } else {
+    x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    x[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    x[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+  }
+  return x;
+}
+// 2^(byte - 127); byte 0 stands beside zeros (and NaN keys) only: 1.
+__device__ __forceinline__ float Scale8(uint32_t byte) {
+  return __uint_as_float((byte == 0 ? 127u : byte) << 23);
+}
+template <uint32_t parts, uint32_t D>
+__device__ __forceinline__ typename QueryOperand<Fp8, parts>::type KeyOperand(
+    const Record<Fp8, D>& r, uint32_t tile, uint32_t s) {
+  const uint32_t piece = tile * (D / 32) + s;  // of 8 bytes
+  return __builtin_bit_cast(
+      typename QueryOperand<Fp8, parts>::type,
+      EightOf<parts == 2>(r.k[piece / 2][piece % 2 * 2], r.k[piece / 2][piece % 2 * 2 + 1],
+                          parts == 2 ? 1.f : Scale8(r.scales & 255u)));
 }
 
 // P V in f16 for the 16-bit types: a weight is off by at most 2^-11 of itself,
@@ -144,6 +246,11 @@ struct Value<false> {
 __device__ __forceinline__ uint32_t OutsideHalf(uint32_t x) {
   const uint32_t low = x & 0x7F7F7F7Fu;
   return (((low + 0x73737373u) & x) | ~((low + 0x18181818u) | x)) & 0x80808080u;
+}
+// Whether f16 does not hold a record's values, for its scale byte: 2^-9 x 2^-15
+// .. 448 x 2^7, or zeros.
+__device__ __forceinline__ bool OutsideHalf8(uint32_t byte) {
+  return byte != 0 && byte - 112u > 22u;
 }
 // Nonzero where one of the 4 bytes is 206 or more: values of up to 2^81 do not
 // pass fp32 in sums of 2^31 weights of 2^15.
@@ -173,7 +280,7 @@ __device__ __forceinline__ uint32_t TwoOf(uint32_t word, float scale, uint32_t s
 // tiles 2 i and 2 i + 1) over the record's 32 tokens.  A byte holds two columns
 // of one token, so two conversions meet in two byte permutes.
 template <uint32_t D, bool half>
-__device__ __forceinline__ void ValueOperands(const Record<D>& r, uint32_t i,
+__device__ __forceinline__ void ValueOperands(const Record<Fp4, D>& r, uint32_t i,
                                               typename Value<half>::type* even,
                                               typename Value<half>::type* odd) {
   typedef typename Value<half>::type V;
@@ -191,6 +298,16 @@ __device__ __forceinline__ void ValueOperands(const Record<D>& r, uint32_t i,
   }
   *even = __builtin_bit_cast(V, lo);
   *odd = __builtin_bit_cast(V, hi);
+}
+// A column's 8 tokens are neighbours in a record of 8 bits.
+template <uint32_t D, bool half>
+__device__ __forceinline__ void ValueOperands(const Record<Fp8, D>& r, uint32_t i,
+                                              typename Value<half>::type* even,
+                                              typename Value<half>::type* odd) {
+  typedef typename Value<half>::type V;
+  const float scale = Scale8(r.scales >> 8);
+  *even = __builtin_bit_cast(V, EightOf<half>(r.v[i][0], r.v[i][1], scale));
+  *odd = __builtin_bit_cast(V, EightOf<half>(r.v[i][2], r.v[i][3], scale));
 }
 __device__ __forceinline__ f32x4 Product(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -267,14 +384,23 @@ __device__ __forceinline__ float RowSum(float x) {
 struct Sight {
   int32_t lo, hi, pre;
 };
+template <class F>
 __device__ __forceinline__ Sight SightOf(const KvSpan& s, uint32_t token, bool valid,
-                                         uint32_t window) {
+                                         uint32_t window, uint32_t sinks) {
   Sight v;
   const int32_t pos = s.total - s.count + (int32_t)token;
   v.hi = valid ? min(pos, s.total - 1) : -1;
   v.lo = window > 0 && (int64_t)pos + 1 > (int64_t)window ? pos + 1 - (int32_t)window : 0;
   v.pre = valid ? s.prefix : 0;
+  if (F::kSinks && valid) v.pre = KvLead(s.prefix, sinks, pos, s.total);
   return v;
+}
+// What every row from `token` on sees of the first keys; the rows up to `token`
+// see none of them past it but in their windows.
+template <class F>
+__device__ __forceinline__ int32_t LeadOf(const KvSpan& s, uint32_t token, uint32_t sinks) {
+  return F::kSinks ? KvLead(s.prefix, sinks, s.total - s.count + (int32_t)token, s.total)
+                   : s.prefix;
 }
 
 // Whether q's and out's rows allow loads and stores of four elements.
@@ -318,10 +444,17 @@ struct Query {
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) y[j] = a.sign * (float)x[2 * i + j / 4][j % 4];
   }
-  __device__ __forceinline__ void Parts(const AttnArgs& a, uint32_t i, bf16x8* out) const {
+  template <class F>
+  __device__ __forceinline__ void Parts(const AttnArgs& a, uint32_t i,
+                                        typename QueryOperand<F, parts>::type* out) const {
     float y[8];
     Eight(a, i, y);
-    ToParts<parts>(y, out);
+    if constexpr (F::Parts(parts) == parts) {
+      ToParts<parts>(y, out);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[0][j] = (_Float16)y[j];
+    }
   }
 };
 
@@ -360,9 +493,9 @@ struct State {
   Sight see[R];
   int32_t see_all, see_from, see_pre;  // every row sees keys see_from .. see_all, and < see_pre
 };
-template <uint32_t parts, uint32_t D, uint32_t R>
+template <class F, uint32_t parts, uint32_t D, uint32_t R>
 struct Rows : State<D, R> {
-  bf16x8 q[R][parts][D / 32];
+  typename QueryOperand<F, parts>::type q[R][F::Parts(parts)][D / 32];
 };
 
 // A wave's rows: row0 .. of the `rows` rows (token, query head of the group) of
@@ -373,13 +506,13 @@ struct RowSet {
 };
 
 // No keys seen yet.
-template <uint32_t D, uint32_t R>
+template <class F, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Begin(const AttnArgs& a, const RowSet& set, State<D, R>& w) {
   const KvSpan& span = set.span;
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
     const uint32_t row = set.row0 + t * 16 + threadIdx.x % 16;
-    w.see[t] = SightOf(span, row / set.group, row < set.rows, a.window);
+    w.see[t] = SightOf<F>(span, row / set.group, row < set.rows, a.window, a.sinks);
     w.m[t] = -__builtin_inff();
     w.l[t] = 0.f;
 #pragma unroll
@@ -387,8 +520,8 @@ __device__ __forceinline__ void Begin(const AttnArgs& a, const RowSet& set, Stat
   }
   w.large = false;
   w.see_all = min(span.total - span.count + (int32_t)(set.row0 / set.group), span.total - 1);
-  w.see_from = SightOf(span, set.last / set.group, true, a.window).lo;
-  w.see_pre = span.prefix;
+  w.see_from = SightOf<F>(span, set.last / set.group, true, a.window, 0).lo;
+  w.see_pre = LeadOf<F>(span, set.row0 / set.group, a.sinks);
 }
 
 // Where the lane's columns of tile t's row start in q; false past the rows.
@@ -426,8 +559,8 @@ __device__ __forceinline__ void Finish(const AttnArgs& a, const RowSet& set,
 }
 
 // One record: the products of its keys ...
-template <uint32_t parts, uint32_t D, uint32_t R>
-__device__ __forceinline__ void Scores(const Record<D>& r, const Rows<parts, D, R>& w,
+template <class F, uint32_t parts, uint32_t D, uint32_t R>
+__device__ __forceinline__ void Scores(const Record<F, D>& r, const Rows<F, parts, D, R>& w,
                                        f32x4 (&s)[R][2]) {
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -435,13 +568,20 @@ __device__ __forceinline__ void Scores(const Record<D>& r, const Rows<parts, D, 
   for (uint32_t i = 0; i < D / 32; ++i) {
 #pragma unroll
     for (uint32_t tile = 0; tile < 2; ++tile) {
-      const bf16x8 k = KeyOperand<D>(r, tile, i);
+      const auto k = KeyOperand<parts>(r, tile, i);
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
-        for (uint32_t p = parts; p-- > 0;)
+        for (uint32_t p = F::Parts(parts); p-- > 0;)
           s[t][tile] = Product(k, w.q[t][p][i], s[t][tile]);
     }
+  }
+  if constexpr (F::Parts(parts) != parts) {  // K's codes went in without their scale
+    const float scale = Scale8(r.scales & 255u);
+#pragma unroll
+    for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) s[t][j / 4][j % 4] *= scale;
   }
 }
 
@@ -485,6 +625,19 @@ __device__ __forceinline__ float PowerOf(const AttnArgs& a) {
 // The record's key of a lane's score j.
 __device__ __forceinline__ int32_t KeyOf(int32_t key0, uint32_t j) {
   return key0 + (int32_t)(j / 4 * 16 + threadIdx.x % 64 / 16 * 4 + j % 4);
+}
+
+// Zeros for the record's V past `total`.
+template <uint32_t D>
+__device__ __forceinline__ void DropPast(Record<Fp8, D>& r, int32_t key0, int32_t total) {
+  uint32_t keep[2] = {0, 0};
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j)
+    if (KeyOf(key0, j) < total) keep[j / 4] |= 255u << (8 * (j % 4));
+#pragma unroll
+  for (uint32_t c = 0; c < D / 32; ++c)
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) r.v[c][j] &= keep[j % 2];
 }
 
 // -inf for the keys a row does not see.
@@ -548,20 +701,15 @@ __device__ __forceinline__ f16x8 HalfWeights(const float* p) {
   return y;
 }
 
-// ... and the scores' running maximum and sum, and P V.
-template <uint32_t parts, uint32_t D, uint32_t R>
-__device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<D>& r,
-                                     int32_t key0, f32x4 (&s)[R][2], Rows<parts, D, R>& w) {
-  const float c = PowerOf(a);
-  if (a.cap > 0.f) {
-    if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s);
-    else Cap<false, R>(a, s);
-  }
+// Unusual records, before their scores are hidden from rows; true where V is not
+// within f16.
+template <bool half, uint32_t D, uint32_t R>
+__device__ __forceinline__ bool Unusual(const KvSpan& span, Record<Fp4, D>& r, int32_t key0,
+                                        f32x4 (&s)[R][2], State<D, R>& w) {
   // Unusual scale bytes: a token whose K or V has a scale of NaN, or one whose
   // products pass the types' range (253, 254), gives NaN scores to the rows
   // that see it and nothing to others (V's 0 x NaN would reach every row of the
   // tile); past the request's end any byte may lie.
-  constexpr bool half = parts < 3;
   bool wide = false;
   const uint32_t keys = Nans(r.ks[0] | (D == 256 ? r.ks[D == 256] : 0u) << 16);
   if (__builtin_amdgcn_ballot_w64((OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1]) | keys) != 0) != 0) {
@@ -596,6 +744,31 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
     wide = half && __builtin_amdgcn_ballot_w64(
                        (OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1])) != 0) != 0;
   }
+  return wide;
+}
+// Records of 8 bits: a NaN key's scores are NaN by themselves and V holds none,
+// but past the request's end, where any byte may lie.
+template <bool half, uint32_t D, uint32_t R>
+__device__ __forceinline__ bool Unusual(const KvSpan& span, Record<Fp8, D>& r, int32_t key0,
+                                        f32x4 (&)[R][2], State<D, R>& w) {
+  if (key0 + 32 > span.total) DropPast(r, key0, span.total);
+  const uint32_t scale = (uint32_t)__builtin_amdgcn_readfirstlane((int)(r.scales >> 8));
+  // values of up to 2^81 do not pass fp32 in sums of 2^31 weights of 2^15
+  if (scale >= 199u) w.large = true;
+  return half && OutsideHalf8(scale);
+}
+
+// ... and the scores' running maximum and sum, and P V.
+template <class F, uint32_t parts, uint32_t D, uint32_t R>
+__device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<F, D>& r,
+                                     int32_t key0, f32x4 (&s)[R][2], Rows<F, parts, D, R>& w) {
+  const float c = PowerOf(a);
+  if (a.cap > 0.f) {
+    if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s);
+    else Cap<false, R>(a, s);
+  }
+  constexpr bool half = parts < 3;
+  bool wide = Unusual<half>(span, r, key0, s, static_cast<State<D, R>&>(w));
   // weights below 2^-48 are none in f16
   if (half && w.large) wide = true;
   Hide<D, R>(w, key0, s);

@@ -482,6 +482,7 @@ uint32_t PromptTiles(uint32_t dim);
 uint32_t PromptRows(uint32_t dim);
 uint64_t PromptBytes(const AttnArgs& a);
 hipError_t LaunchPrompt(const AttnArgs& a, Workspace& ws, hipStream_t stream);
+hipError_t LaunchPrompt8(const AttnArgs& a, Workspace& ws, hipStream_t stream);
 
 // Pages (hb_pages.hip).
 constexpr uint32_t kMostForkRows = 65536;  // rows of a table whose requests fork or end

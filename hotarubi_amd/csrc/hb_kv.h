@@ -27,7 +27,7 @@
 namespace hb {
 
 // Bytes of one record.
-HB_KV_FN uint32_t KvRecordBytes(uint32_t dim) { return 34 * dim; }
+HB_KV_FN constexpr uint32_t KvRecordBytes(uint32_t dim) { return 34 * dim; }
 
 // Byte offsets within a record, for token t = 0..31 of the record: the byte
 // that holds column col (even) of K and V, and the scale bytes of its block.
@@ -55,7 +55,7 @@ HB_KV_FN uint32_t KvVScale(uint32_t dim, uint32_t t, uint32_t col) {
 //             operand without a permute
 // Scale bytes are E8M0, 10 to 246, so that every value is normal in fp32 and
 // bf16; 0 where no value but zeros was stored.
-HB_KV_FN uint32_t Kv8RecordBytes(uint32_t dim) { return 64 * dim + 16; }
+HB_KV_FN constexpr uint32_t Kv8RecordBytes(uint32_t dim) { return 64 * dim + 16; }
 HB_KV_FN uint32_t Kv8KCode(uint32_t dim, uint32_t t, uint32_t col) {
   const uint32_t quarter = dim / 4, at = t / 16 * quarter + col % quarter;
   return at / 16 * 1024 + col / quarter * 256 + t % 16 * 16 + at % 16;

@@ -60,12 +60,60 @@ __device__ __forceinline__ uint32_t OpenedAt(const KvWalk& walk, uint32_t r) {
   return r < walk.head ? r : walk.head + r - walk.from;
 }
 
-// A wave a record.  `odd` says where f16 does not hold a scale (K's count for
-// f16 queries): the rows that look at it take the general steps.  Tokens past
-// the request's end, where any byte may lie, are given a scale of 1.
+// Tokens past the request's end, where any byte may lie, made harmless; nonzero
+// where f16 does not hold a scale (K's count for f16 queries).
 template <uint32_t parts, uint32_t D>
+__device__ __forceinline__ uint32_t Readied(Record<Fp4, D>& r, int32_t key0, int32_t total) {
+  const uint32_t n = threadIdx.x % 16;
+  if (key0 + 32 > total) {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (KeyOf(key0, j) >= total)
+        r.vs[j / 4] = (r.vs[j / 4] & ~(255u << (8 * (j % 4)))) | 127u << (8 * (j % 4));
+#pragma unroll
+    for (uint32_t k = 0; k < (D == 256 ? 2 : 1); ++k) {
+      if (key0 + (int32_t)n >= total) r.ks[k] = (r.ks[k] & 0xFF00u) | 127u;
+      if (key0 + 16 + (int32_t)n >= total) r.ks[k] = (r.ks[k] & 0xFFu) | 127u << 8;
+    }
+  }
+  uint32_t outside = OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1]);
+  if constexpr (parts == 2)
+    outside |= OutsideHalf(r.ks[0] | (D == 256 ? r.ks[D == 256] : 0x7F7Fu) << 16);
+  return outside;
+}
+template <uint32_t parts, uint32_t D>
+__device__ __forceinline__ uint32_t Readied(Record<Fp8, D>& r, int32_t key0, int32_t total) {
+  if (key0 + 32 > total) DropPast(r, key0, total);
+  uint32_t outside = OutsideHalf8(r.scales >> 8);
+  if (parts == 2) outside |= OutsideHalf8(r.scales & 255u);
+  return outside;
+}
+// K's operand for token tile `tile` and step e, with its scale.
+template <uint32_t parts, uint32_t D>
+__device__ __forceinline__ u32x4 OpenedKeys(const Record<Fp4, D>& r, uint32_t tile, uint32_t e) {
+  const uint32_t word = tile * (D / 32) + e, w = r.k[word / 4][word % 4];
+  // (253 and 254 as 255: NaN)
+  const uint32_t byte = r.ks[D == 256 ? e / 4 : 0] >> (8 * tile) & 255u;
+  const float scale = __uint_as_float((byte >= 253u ? 255u : byte) << 23);
+  u32x4 x;
+  x[0] = TwoAs<0, parts == 2>(w, scale);
+  x[1] = TwoAs<1, parts == 2>(w, scale);
+  x[2] = TwoAs<2, parts == 2>(w, scale);
+  x[3] = TwoAs<3, parts == 2>(w, scale);
+  return x;
+}
+template <uint32_t parts, uint32_t D>
+__device__ __forceinline__ u32x4 OpenedKeys(const Record<Fp8, D>& r, uint32_t tile, uint32_t e) {
+  const uint32_t piece = tile * (D / 32) + e;
+  return EightOf<parts == 2>(r.k[piece / 2][piece % 2 * 2], r.k[piece / 2][piece % 2 * 2 + 1],
+                             Scale8(r.scales & 255u));
+}
+
+// A wave a record.  `odd` says where f16 does not hold a scale: the rows that
+// look at it take the general steps.
+template <class F, uint32_t parts, uint32_t D>
 __global__ __launch_bounds__(256) void OpenKernel(const AttnArgs a) {
-  const uint32_t lane = threadIdx.x % 64, n = lane % 16;
+  const uint32_t lane = threadIdx.x % 64;
   const uint32_t at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t pair = at / a.opened, i = at % a.opened, b = pair / a.heads;
   if (b >= a.batch) return;
@@ -75,7 +123,8 @@ __global__ __launch_bounds__(256) void OpenKernel(const AttnArgs a) {
   if (span.rows == 0) return;
   const int32_t pos0 = span.total - span.count;
   const KvWalk walk =
-      KvRecords(pos0, pos0 + (int32_t)span.rows - 1, span.total, span.prefix, a.window);
+      KvRecords(pos0, pos0 + (int32_t)span.rows - 1, span.total,
+                LeadOf<F>(span, span.rows - 1, a.sinks), a.window);
   if (i >= walk.count) return;
   uint32_t* const odd = reinterpret_cast<uint32_t*>(a.ws) + at;
   const uint32_t record = __builtin_amdgcn_readfirstlane(PageRecord(
@@ -84,25 +133,12 @@ __global__ __launch_bounds__(256) void OpenKernel(const AttnArgs a) {
     if (lane == 0) *odd = 0;
     return;
   }
-  const uint8_t* from = a.cache + (uint64_t)record * KvRecordBytes(D);
-  Record<D> r;
+  const uint8_t* from = a.cache + (uint64_t)record * F::Bytes(D);
+  Record<F, D> r;
   ReadKeys<D>(from, r);
   ReadValues<D>(from, r);
   const int32_t key0 = (int32_t)(32 * KvWalkRecord(walk, i));
-  if (key0 + 32 > span.total) {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
-      if (KeyOf(key0, j) >= span.total)
-        r.vs[j / 4] = (r.vs[j / 4] & ~(255u << (8 * (j % 4)))) | 127u << (8 * (j % 4));
-#pragma unroll
-    for (uint32_t k = 0; k < (D == 256 ? 2 : 1); ++k) {
-      if (key0 + (int32_t)n >= span.total) r.ks[k] = (r.ks[k] & 0xFF00u) | 127u;
-      if (key0 + 16 + (int32_t)n >= span.total) r.ks[k] = (r.ks[k] & 0xFFu) | 127u << 8;
-    }
-  }
-  uint32_t outside = OutsideHalf(r.vs[0]) | OutsideHalf(r.vs[1]);
-  if constexpr (parts == 2)
-    outside |= OutsideHalf(r.ks[0] | (D == 256 ? r.ks[D == 256] : 0x7F7Fu) << 16);
+  const uint32_t outside = Readied<parts>(r, key0, span.total);
   const uint64_t any = __builtin_amdgcn_ballot_w64(outside != 0);
   if (lane == 0) *odd = any != 0;
   u32x4* const to = reinterpret_cast<u32x4*>(a.opened_at + (uint64_t)at * kOpened<D>) + lane;
@@ -110,16 +146,7 @@ __global__ __launch_bounds__(256) void OpenKernel(const AttnArgs a) {
   for (uint32_t tile = 0; tile < 2; ++tile)
 #pragma unroll
     for (uint32_t e = 0; e < D / 32; ++e) {
-      const uint32_t word = tile * (D / 32) + e, w = r.k[word / 4][word % 4];
-      // (253 and 254 as 255: NaN)
-      const uint32_t byte = r.ks[D == 256 ? e / 4 : 0] >> (8 * tile) & 255u;
-      const float scale = __uint_as_float((byte >= 253u ? 255u : byte) << 23);
-      u32x4 x;
-      x[0] = TwoAs<0, parts == 2>(w, scale);
-      x[1] = TwoAs<1, parts == 2>(w, scale);
-      x[2] = TwoAs<2, parts == 2>(w, scale);
-      x[3] = TwoAs<3, parts == 2>(w, scale);
-      to[word * 64] = x;
+      to[(tile * (D / 32) + e) * 64] = OpenedKeys<parts>(r, tile, e);
     }
 #pragma unroll
   for (uint32_t e = 0; e < D / 32; ++e) {
@@ -165,7 +192,7 @@ __device__ __forceinline__ void WaveFence() {
 
 // (`fine`: caps above kPlainCap, in a kernel of their own: beside the plain one
 // in the loop, eight chunks with capped scores took 64.9 us for 63.8.)
-template <uint32_t parts, uint32_t D, bool fine>
+template <class F, uint32_t parts, uint32_t D, bool fine>
 __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void PromptKernel(
     const AttnArgs a) {
   constexpr uint32_t kWaves = Shape<D>::kWaves, R = Shape<D>::kTiles, kSteps = D / 32;
@@ -193,7 +220,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
   const int32_t base_pos = span.total - span.count;
   const KvWalk walk =
       KvRecords(base_pos + (int32_t)(first_row / group), base_pos + (int32_t)(last_row / group),
-                span.total, span.prefix, a.window);
+                span.total, LeadOf<F>(span, last_row / group, a.sinks), a.window);
 
   // a wave past the rows loads its share and computes nothing
   const uint32_t row0 = first_row + wave * R * 16;
@@ -201,7 +228,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
   const bool has_rows = row0 < rows;
   State<D, R> w;
   Q q[R][kSteps];
-  Begin<D, R>(a, set, w);
+  Begin<F, D, R>(a, set, w);
   uint8_t* const rows_lds = reinterpret_cast<uint8_t*>(stages) + wave * (R * 16 * D * 2);
   static_assert(kWaves * R * 16 * D * 2 <= sizeof stages, "the rows fit the stages");
   const bool whole = Whole(a.q, a.q_token, a.q_head);
@@ -228,14 +255,15 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
   }
   // the keys that any row of the wave sees
   const int32_t wave_hi = base_pos + (int32_t)(set.last / group);
-  const int32_t wave_lo = SightOf(span, row0 / group, true, a.window).lo;
+  const int32_t wave_lo = SightOf<F>(span, row0 / group, true, a.window, 0).lo;
+  const int32_t wave_lead = LeadOf<F>(span, set.last / group, a.sinks);
 
   const int32_t* const row = a.table + (uint64_t)b * a.table_stride;
   const uint32_t count = walk.count;
   // the request's opened records; those of pages that are not there, which
   // nothing was written for, are passed over below
   const KvWalk all = KvRecords(base_pos, base_pos + (int32_t)span.rows - 1, span.total,
-                               span.prefix, a.window);
+                               LeadOf<F>(span, span.rows - 1, a.sinks), a.window);
   const uint64_t first_opened = ((uint64_t)b * a.heads + head) * a.opened;
   bool slow = all.count > a.opened;
   for (uint32_t i = lane; i < count && !slow; i += 64) {
@@ -254,31 +282,31 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
       const uint32_t r0 = row0 + t * 16;
       if (r0 >= rows) return;
       const RowSet one{span, group, head, r0, rows, min(r0 + 16, rows) - 1};
-      Rows<parts, D, 1> v;
-      Begin<D, 1>(a, one, v);
+      Rows<F, parts, D, 1> v;
+      Begin<F, D, 1>(a, one, v);
       uint64_t from;
       const bool valid = QueryAt<parts, D>(a, one, 0, &from);
       Query<parts, D> again;
       again.Load(a, from, valid);
 #pragma unroll
       for (uint32_t i = 0; i < kSteps; ++i) {
-        bf16x8 x[parts];
-        again.Parts(a, i, x);
+        typename QueryOperand<F, parts>::type x[F::Parts(parts)];
+        again.template Parts<F>(a, i, x);
 #pragma unroll
-        for (uint32_t p = 0; p < parts; ++p) v.q[0][p][i] = x[p];
+        for (uint32_t p = 0; p < F::Parts(parts); ++p) v.q[0][p][i] = x[p];
       }
 #pragma unroll 1
       for (uint32_t i = 0; i < count; ++i) {
         const uint32_t record =
             __builtin_amdgcn_readfirstlane(PageRecord(a, walk, row, head, i, count));
         if (record == kNoRecord) continue;
-        const uint8_t* at_record = a.cache + (uint64_t)record * KvRecordBytes(D);
-        Record<D> r;
+        const uint8_t* at_record = a.cache + (uint64_t)record * F::Bytes(D);
+        Record<F, D> r;
         ReadKeys<D>(at_record, r);
         ReadValues<D>(at_record, r);
         f32x4 s[1][2];
-        Scores<parts, D, 1>(r, v, s);
-        Step<parts, D, 1>(a, span, r, key_of(i), s, v);
+        Scores<F, parts, D, 1>(r, v, s);
+        Step<F, parts, D, 1>(a, span, r, key_of(i), s, v);
       }
       v.l[0] = RowSum(v.l[0]);
       Finish<parts, D, 1>(a, one, v);
@@ -358,7 +386,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
     for (uint32_t u = 0; u < 2; ++u) {
       if (!has_rows || hidden(i + u)) continue;
       const int32_t key0 = key_of(i + u);
-      if (!((key0 <= wave_hi && key0 + 31 >= wave_lo) || key0 < span.prefix)) continue;
+      if (!((key0 <= wave_hi && key0 + 31 >= wave_lo) || key0 < wave_lead)) continue;
       f32x4 s[R][2];
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -442,7 +470,8 @@ uint32_t PromptRows(uint32_t dim) {
 static uint64_t OpenedRecords(const AttnArgs& a) {
   uint64_t records = ((uint64_t)a.max_kv + 31) / 32;
   if (a.window > 0 && a.prefix == nullptr)
-    records = std::min<uint64_t>(records, ((uint64_t)a.window + a.max_new + 62) / 32);
+    records = std::min<uint64_t>(records, ((uint64_t)a.window + a.max_new + 62) / 32 +
+                                              ((uint64_t)a.sinks + 31) / 32);
   return std::max<uint64_t>(records, 1);
 }
 uint64_t PromptBytes(const AttnArgs& a) {
@@ -450,7 +479,7 @@ uint64_t PromptBytes(const AttnArgs& a) {
   return records * 128 * a.dim + (records * 4 + 15) / 16 * 16;
 }
 
-template <uint32_t parts, uint32_t D>
+template <class F, uint32_t parts, uint32_t D>
 static hipError_t LaunchOf(AttnArgs& a, hipStream_t stream) {
   const uint64_t rows = (uint64_t)a.max_new * (a.q_heads / a.heads);
   const uint64_t tiles = (rows + Shape<D>::kRows - 1) / Shape<D>::kRows;
@@ -458,15 +487,16 @@ static hipError_t LaunchOf(AttnArgs& a, hipStream_t stream) {
   const uint64_t grid = tiles * pairs;
   if (grid > 0x7FFFFFFFu || records > 0x7FFFFFFFu) return hipErrorInvalidValue;
   a.tiles = (uint32_t)tiles;
-  OpenKernel<parts, D><<<(uint32_t)((records + 3) / 4), 256, 0, stream>>>(a);
+  OpenKernel<F, parts, D><<<(uint32_t)((records + 3) / 4), 256, 0, stream>>>(a);
   if (a.cap > kPlainCap)
-    PromptKernel<parts, D, true><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
+    PromptKernel<F, parts, D, true><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
   else
-    PromptKernel<parts, D, false><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
+    PromptKernel<F, parts, D, false><<<(uint32_t)grid, 64 * Shape<D>::kWaves, 0, stream>>>(a);
   return hipGetLastError();
 }
 
-hipError_t LaunchPrompt(const AttnArgs& in, Workspace& ws, hipStream_t stream) {
+template <class F>
+static hipError_t LaunchFormat(const AttnArgs& in, Workspace& ws, hipStream_t stream) {
   AttnArgs a = in;
   const hipError_t err = GrowWorkspace(ws, PromptBytes(a), stream);
   if (err != hipSuccess) return err;
@@ -476,10 +506,17 @@ hipError_t LaunchPrompt(const AttnArgs& in, Workspace& ws, hipStream_t stream) {
                 ((uint64_t)a.opened * a.batch * a.heads * 4 + 15) / 16 * 16;
   const bool half = a.type == HB_TYPE_F16;
   switch (a.dim) {
-    case 64: return half ? LaunchOf<2, 64>(a, stream) : LaunchOf<1, 64>(a, stream);
-    case 128: return half ? LaunchOf<2, 128>(a, stream) : LaunchOf<1, 128>(a, stream);
-    default: return half ? LaunchOf<2, 256>(a, stream) : LaunchOf<1, 256>(a, stream);
+    case 64: return half ? LaunchOf<F, 2, 64>(a, stream) : LaunchOf<F, 1, 64>(a, stream);
+    case 128: return half ? LaunchOf<F, 2, 128>(a, stream) : LaunchOf<F, 1, 128>(a, stream);
+    default: return half ? LaunchOf<F, 2, 256>(a, stream) : LaunchOf<F, 1, 256>(a, stream);
   }
+}
+
+hipError_t LaunchPrompt(const AttnArgs& a, Workspace& ws, hipStream_t stream) {
+  return LaunchFormat<Fp4>(a, ws, stream);
+}
+hipError_t LaunchPrompt8(const AttnArgs& a, Workspace& ws, hipStream_t stream) {
+  return LaunchFormat<Fp8>(a, ws, stream);
 }
 
 }  // namespace hb
