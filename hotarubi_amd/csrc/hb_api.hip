@@ -1760,7 +1760,7 @@ int TokenLogprobs(hb_ctx* ctx, const hb_logprobs_desc* d, bool sync) {
   if (int rc = Enter(ctx)) return rc;
   hb::LogprobsArgs a{d->logits, d->stride,       d->tokens, d->logprobs, d->entropy,
                      d->top_ids, d->top_logprobs, d->type,   d->rows,     d->vocab,
-                     d->top,    d->scale};
+                     d->top,    d->scale,      1,         nullptr};
   return Launched(ctx, hb::LaunchLogprobs(a, ctx->ws, ctx->stream), "log probability launch", sync);
 }
 

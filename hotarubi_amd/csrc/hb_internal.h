@@ -534,6 +534,9 @@ struct LogprobsArgs {
   float* top_logprobs;
   uint32_t type, rows, vocab, top;
   float scale;
+  // set by the launcher: workgroups of a row, and their results
+  uint32_t parts;
+  float* ws;
 };
 hipError_t LaunchLogprobs(const LogprobsArgs& a, Workspace& ws, hipStream_t stream);
 

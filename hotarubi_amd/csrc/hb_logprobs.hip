@@ -1,96 +1,491 @@
 // Log probabilities of given tokens, the entropy and the most likely tokens of
-// rows of logits.
+// rows of logits, one pass over them.
 //
-// With m = max x and s = sum e^(x - m) a token's log probability is
-// x - m - ln s and the entropy ln s - sum (x - m) e^(x - m) / s.
+// In powers of two, with c = scale log2 e, M the running maximum times c,
+// d = x c - M, l = sum 2^d and w = sum d 2^d, a token's log probability is
+// (x c - M - log2 l) ln 2 and the entropy (log2 l - w / l) ln 2.  Parts with
+// maxima M1, M2 meet at M = max as l = sum l_i f_i, w = sum (w_i + (M_i - M)
+// l_i) f_i, f_i = 2^(M_i - M).  M is rounded once and used as it is from then
+// on, so that rounding changes no probability.
+//
+// The most likely tokens: every lane keeps the maxima of its stretches of the
+// row in LDS.  `top` lanes reach the `top`-th largest of the lanes' maxima, so
+// that is a bound, and only stretches that reach it are read again, all at
+// once; their logits go into a list of sorted 64-bit keys, one a lane.
+#include <algorithm>
+
 #include "hb_internal.h"
 
 namespace hb {
 namespace {
 
-constexpr uint32_t kThreads = 256;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
+constexpr uint32_t kLoads = 2;  // 16-byte loads of a lane's batch
+constexpr uint32_t kStretches = 32;
+constexpr uint32_t kMostParts = 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// Larger logits, and of equal ones lower columns, have larger keys; a NaN the
-// least.
-__device__ __forceinline__ uint64_t KeyOf(float x, uint32_t column) {
+// Values of a 16-byte load, as fp32.
+template <class T>
+struct Packed;
+template <>
+struct Packed<float> {
+  static constexpr uint32_t kCount = 4, kLowest = 0xFF800000u;
+  static __device__ __forceinline__ float At(u32x4 x, uint32_t i) { return __uint_as_float(x[i]); }
+};
+template <>
+struct Packed<__bf16> {
+  static constexpr uint32_t kCount = 8, kLowest = 0xFF80FF80u;
+  static __device__ __forceinline__ float At(u32x4 x, uint32_t i) {
+    return __uint_as_float(i % 2 ? x[i / 2] & 0xFFFF0000u : x[i / 2] << 16);
+  }
+};
+template <>
+struct Packed<_Float16> {
+  static constexpr uint32_t kCount = 8, kLowest = 0xFC00FC00u;
+  static __device__ __forceinline__ float At(u32x4 x, uint32_t i) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(x[i / 2] >> (i % 2 * 16)));
+  }
+};
+
+// Larger logits have larger orders, a NaN 0; of equal logits lower columns have
+// larger keys.
+__device__ __forceinline__ uint32_t OrderOf(float x) {
   const uint32_t bits = __float_as_uint(x + 0.f);  // -0 as 0
-  const uint32_t order = x != x ? 0u : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-  return (uint64_t)order << 32 | (uint32_t)~column;
+  return x != x ? 0u : (int32_t)bits < 0 ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t KeyOf(float x, uint32_t column) {
+  return (uint64_t)OrderOf(x) << 32 | (uint32_t)~column;
+}
+__device__ __forceinline__ float LogitOf(uint64_t key) {
+  const uint32_t order = (uint32_t)(key >> 32);
+  return __uint_as_float((int32_t)order < 0 ? order ^ 0x80000000u : ~order);
+}
+
+// Largest of three (a NaN loses).
+__device__ __forceinline__ float Max3(float a, float b, float c) {
+  float y;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+  return y;
+}
+
+// (fmaxf would make sure of quiet NaNs first)
+__device__ __forceinline__ float AtLeast(float x, float least) {
+  float y;
+  asm("v_max_f32 %0, %1, %2" : "=v"(y) : "v"(x), "v"(least));
+  return y;
+}
+
+struct Sums {
+  float m, l, w;  // m: the maximum times c, -inf where nothing was seen
+};
+__device__ __forceinline__ float Reference(float m) { return m == -__builtin_inff() ? 0.f : m; }
+__device__ __forceinline__ Sums Joined(const Sums& a, const Sums& b) {
+  Sums y;
+  y.m = fmaxf(a.m, b.m);
+  const float ref = Reference(y.m);
+  // (nothing seen: l and w are 0; two +inf give NaN, as they should)
+  const float da = a.m == -__builtin_inff() ? 0.f : a.m - ref;
+  const float db = b.m == -__builtin_inff() ? 0.f : b.m - ref;
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  y.l = a.l * fa + b.l * fb;
+  y.w = (a.w + fmaxf(da, -1e4f) * a.l) * fa + (b.w + fmaxf(db, -1e4f) * b.l) * fb;
+  return y;
+}
+__device__ __forceinline__ Sums JoinedOverWave(Sums s) {
+#pragma unroll
+  for (uint32_t d = 1; d < 64; d *= 2)
+    s = Joined(s, Sums{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.w, d)});
+  return s;
+}
+
+__device__ __forceinline__ uint64_t ReadLane(uint64_t x, uint32_t lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, (int)lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), (int)lane);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// Keys in falling order, one a lane, and one that is none of them.
+__device__ __forceinline__ uint64_t Inserted(uint64_t list, uint64_t key) {
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t place = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(list > key));
+  // (from the lane before: wave_shr:1)
+  const uint32_t lo =
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)list, 0x138, 0xF, 0xF, false);
+  const uint32_t hi =
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(list >> 32), 0x138, 0xF, 0xF, false);
+  const uint64_t before = (uint64_t)hi << 32 | lo;
+  return lane < place ? list : lane == place ? key : before;
+}
+
+// The value of rank k (from 0) of a lane's each.
+__device__ __forceinline__ uint32_t OfRank(uint32_t x, uint32_t k) {
+  const uint32_t lane = threadIdx.x % 64;
+#pragma unroll
+  for (uint32_t size = 2; size <= 64; size *= 2)
+#pragma unroll
+    for (uint32_t d = size / 2; d > 0; d /= 2) {
+      const uint32_t y = (uint32_t)__shfl_xor((int)x, (int)d);
+      const bool falls = (lane & size) == 0, low = (lane & d) == 0;
+      x = falls == low ? max(x, y) : min(x, y);
+    }
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)k);
+}
+
+// Keys of `other` (k of them, falling) that are above `key`.
+__device__ __forceinline__ uint32_t Above(const uint64_t* other, uint32_t k, uint64_t key) {
+  uint32_t lo = 0, hi = k;
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (other[mid] > key) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+// `count` lists of k falling keys become one, in pairs: a key's place is its own
+// in its list and the number of keys above it in the other.  Lists of fewer keys
+// end in zeros.
+__device__ __forceinline__ const uint64_t* Merged(uint64_t* lists, uint64_t* other, uint32_t count,
+                                                  uint32_t k) {
+  while (count > 1) {
+    const uint32_t left = (count + 1) / 2;
+    for (uint32_t i = threadIdx.x; i < left * k; i += kThreads) other[i] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count * k; i += kThreads) {
+      const uint32_t list = i / k, pair = list ^ 1;
+      const uint64_t key = lists[i];
+      uint32_t place = i % k;
+      if (pair < count) place += Above(lists + pair * k, k, key);
+      if (place < k && key != 0) other[list / 2 * k + place] = key;
+    }
+    __syncthreads();
+    uint64_t* const t = lists;
+    lists = other;
+    other = t;
+    count = left;
+  }
+  return lists;
+}
+
+// A row's given token, -1 for none, and its logit: asked for before the row is
+// read, as two loads that wait for one another.
+template <class T>
+struct Given {
+  int32_t token = -1;
+  float logit = 0.f;
+  __device__ __forceinline__ Given(const LogprobsArgs& a, uint32_t row) {
+    if (a.tokens == nullptr) return;
+    token = a.tokens[row];
+    if (token >= 0 && (uint32_t)token < a.vocab)
+      logit = (float)static_cast<const T*>(a.logits)[row * a.stride + (uint32_t)token];
+  }
+};
+
+// What goes out for a row, from its sums and its keys, one a lane of a wave.
+template <class T>
+__device__ __forceinline__ void Finish(const LogprobsArgs& a, uint32_t row, const Given<T>& given,
+                                       Sums s, uint64_t key) {
+  const T* const x = static_cast<const T*>(a.logits) + row * a.stride;
+  const float c = a.scale * kLog2e, inf = __builtin_inff();
+  // +inf among them, or past what fp32 holds
+  if (s.m == inf) s.l = __builtin_nanf("");
+  const float ref = Reference(s.m), log = s.l == 0.f ? 0.f : __builtin_amdgcn_logf(s.l);
+  const auto logprob = [&](float logit) {
+    return s.l == 0.f ? -inf : (fmaf(logit, c, -ref) - log) * kLn2;
+  };
+  const uint32_t lane = threadIdx.x % 64;
+  if (lane == 0) {
+    if (a.tokens != nullptr)
+      a.logprobs[row] = given.token < 0                     ? 0.f
+                        : (uint32_t)given.token >= a.vocab ? __builtin_nanf("")
+                                                            : logprob(given.logit);
+    if (a.entropy != nullptr) a.entropy[row] = s.l == 0.f ? 0.f : (log - s.w / s.l) * kLn2;
+  }
+  if (a.top == 0) return;
+  const uint64_t at = (uint64_t)row * a.top;
+  if (lane < a.top && key != 0) {
+    a.top_ids[at + lane] = (int32_t)~(uint32_t)key;
+    a.top_logprobs[at + lane] = logprob(LogitOf(key));
+  }
+  // fewer numbers than were asked for: the first NaNs
+  uint32_t found = (uint32_t)__builtin_popcountll(
+      __builtin_amdgcn_ballot_w64(lane < a.top && key != 0));
+  for (uint64_t base = 0; found < a.top && base < a.vocab; base += 64) {
+    const bool odd = base + lane < a.vocab && (float)x[base + lane] != (float)x[base + lane];
+    const uint64_t all = __builtin_amdgcn_ballot_w64(odd);
+    const uint32_t place = found + (uint32_t)__builtin_popcountll(all & ((1ull << lane) - 1));
+    if (odd && place < a.top) {
+      a.top_ids[at + place] = (int32_t)(base + lane);
+      a.top_logprobs[at + place] = __builtin_nanf("");
+    }
+    found += (uint32_t)__builtin_popcountll(all);
+  }
+}
+
+// A part of a row in the workspace.
+__device__ __forceinline__ uint64_t* PartAt(const LogprobsArgs& a, uint64_t unit) {
+  return reinterpret_cast<uint64_t*>(a.ws) + unit * (a.top + 2);
+}
+
+// Ends what the wave's LDS accesses before may still do.
+__device__ __forceinline__ void WaveFence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// kW waves take a part of a row, batches of it in turn, the next one's loads
+// under way while a batch is summed up.
+template <class T, uint32_t kW>
+__global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs a) {
+  typedef Packed<T> P;
+  union Lds {
+    uint16_t maxima[kWaves][kStretches][64];  // orders' upper halves
+    uint64_t lists[2][kWaves * 64];
+  };
+  __shared__ Lds lds;
+  __shared__ uint16_t again[kWaves][128];  // stretches to be read again
+  __shared__ Sums sums[kWaves];
+  __shared__ uint32_t bound, odd;
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), mine = wave % kW;
+  const uint32_t unit = blockIdx.x * (kWaves / kW) + wave / kW;
+  if (kW == 1 && unit >= a.rows * a.parts) return;
+  const uint32_t row = unit / a.parts, part = unit % a.parts;
+  const T* const x = static_cast<const T*>(a.logits) + row * a.stride;
+  // 16-byte pieces from the one that the row begins in
+  const uint32_t skew = (uint32_t)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  const uint64_t last = skew + (uint64_t)a.vocab;
+  const uint32_t pieces = (uint32_t)((last + P::kCount - 1) / P::kCount);
+  const uint32_t each = (pieces + a.parts - 1) / a.parts;
+  const uint32_t begin = min(pieces, part * each), end = min(pieces, begin + each);
+  if (kW > 1) {
+    if (threadIdx.x == 0) bound = odd = 0;
+    __syncthreads();
+  }
+  auto piece_of = [&](uint32_t batch, uint32_t u, uint32_t of) {
+    return (uint64_t)begin + ((uint64_t)batch * kLoads + u) * 64 + of;
+  };
+  auto load = [&](uint64_t i) {
+    u32x4 y = {P::kLowest, P::kLowest, P::kLowest, P::kLowest};
+    if (i >= end) return y;
+    const uint64_t at = i * P::kCount;  // of its first value, from `skew` before the row
+    if (at >= skew && at + P::kCount <= last) return *reinterpret_cast<const u32x4*>(x + (at - skew));
+#pragma unroll
+    for (uint32_t j = 0; j < P::kCount; ++j) {  // the row's ends
+      if (at + j < skew || at + j >= last) continue;
+      const T one = x[at + j - skew];
+      if constexpr (sizeof(T) == 4) {
+        y[j] = __builtin_bit_cast(uint32_t, one);
+      } else {
+        const uint32_t bits = __builtin_bit_cast(uint16_t, one);
+        y[j / 2] = j % 2 ? (y[j / 2] & 0xFFFFu) | bits << 16 : (y[j / 2] & 0xFFFF0000u) | bits;
+      }
+    }
+    return y;
+  };
+  const float c = a.scale * kLog2e;
+  const uint32_t batches = (end - begin + kLoads * 64 - 1) / (kLoads * 64);
+  // batches of a stretch
+  const uint32_t run = (((batches + kW - 1) / kW) + kStretches - 1) / kStretches;
+  Sums s{-__builtin_inff(), 0.f, 0.f};
+  float m = -__builtin_inff(), high = m;
+  uint32_t stretch = 0, in = 0;
+  const Given<T> given(a, row);
+  u32x4 now[kLoads], next[kLoads];
+#pragma unroll
+  for (uint32_t u = 0; u < kLoads; ++u) now[u] = load(piece_of(mine, u, lane));
+#pragma unroll 1
+  for (uint32_t batch = mine; batch < batches; batch += kW) {
+    if (batch + kW < batches) {
+#pragma unroll
+      for (uint32_t u = 0; u < kLoads; ++u) next[u] = load(piece_of(batch + kW, u, lane));
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (uint32_t u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (uint32_t j = 0; j < P::kCount; j += 2)
+        top = Max3(top, P::At(now[u], j), P::At(now[u], j + 1));
+    if (top > m) {
+      const float to = top * c, less = s.m - to;
+      m = top;
+      if (s.m != -__builtin_inff()) {
+        const float f = __builtin_amdgcn_exp2f(less);
+        s.w = (s.w + fmaxf(less, -1e4f) * s.l) * f;
+        s.l *= f;
+      }
+      s.m = to;
+    }
+    const float ref = Reference(s.m);
+#pragma unroll
+    for (uint32_t u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (uint32_t j = 0; j < P::kCount; ++j) {
+        const float d = fmaf(P::At(now[u], j), c, -ref), p = __builtin_amdgcn_exp2f(d);
+        s.l += p;
+        s.w = fmaf(p, AtLeast(d, -1e4f), s.w);
+      }
+    if (a.top > 0) {
+      high = fmaxf(high, top);
+      if (++in == run || batch + kW >= batches) {
+        lds.maxima[wave][stretch][lane] = (uint16_t)(OrderOf(high) >> 16);
+        high = -__builtin_inff();
+        in = 0;
+        ++stretch;
+      }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kLoads; ++u) now[u] = next[u];
+  }
+  uint64_t list = 0;
+  if (a.top > 0) {
+    uint32_t least = OfRank(OrderOf(m), a.top - 1);
+    // a signalling NaN may have hidden what came before it from a maximum
+    bool all = __builtin_amdgcn_ballot_w64(s.l != s.l) != 0;
+    if (kW > 1) {
+      if (lane == 0) {
+        atomicMax(&bound, least);
+        if (all) atomicOr(&odd, 1u);
+      }
+      __syncthreads();
+      least = bound;
+      all = odd != 0;
+    } else {
+      WaveFence();
+    }
+    uint64_t last_key = 0;
+    uint32_t found = 0, next_stretch = 0;
+    const uint64_t below = (1ull << lane) - 1;
+    while (true) {
+      while (found < 64 && next_stretch < stretch) {
+        const bool flag = all || lds.maxima[wave][next_stretch][lane] >= least >> 16;
+        const uint64_t some = __builtin_amdgcn_ballot_w64(flag);
+        if (flag)
+          again[wave][found + (uint32_t)__builtin_popcountll(some & below)] =
+              (uint16_t)(next_stretch * 64 + lane);
+        found += (uint32_t)__builtin_popcountll(some);
+        ++next_stretch;
+      }
+      if (found == 0) break;
+      WaveFence();
+      const uint32_t take = min(found, 64u);
+      const uint32_t one = lane < take ? again[wave][lane] : 0;
+      const uint32_t rest = 64 + lane < found ? again[wave][64 + lane] : 0;
+      WaveFence();
+      if (64 + lane < found) again[wave][lane] = (uint16_t)rest;
+      found -= take;
+#pragma unroll 1
+      for (uint32_t g = 0; g < run; ++g) {
+        const uint32_t batch = mine + (one / 64 * run + g) * kW;
+#pragma unroll 1
+        for (uint32_t u = 0; u < kLoads; ++u) {
+          const uint64_t i = piece_of(batch, u, one % 64);
+          const bool there = lane < take && batch < batches && i < end;
+          const u32x4 y = load(there ? i : end);
+#pragma unroll
+          for (uint32_t j = 0; j < P::kCount; ++j) {
+            const uint64_t at = i * P::kCount + j - skew;
+            uint64_t key = there && at < a.vocab ? KeyOf(P::At(y, j), (uint32_t)at) : 0;
+            if ((uint32_t)(key >> 32) < max(least, 1u)) key = 0;
+            uint64_t more = __builtin_amdgcn_ballot_w64(key > last_key);
+            while (more != 0) {
+              list = Inserted(list, ReadLane(key, (uint32_t)__builtin_ctzll(more)));
+              last_key = ReadLane(list, a.top - 1);
+              more = __builtin_amdgcn_ballot_w64(key > last_key) & (more - 1) & more;
+            }
+          }
+        }
+      }
+    }
+  }
+  s = JoinedOverWave(s);
+  if (kW > 1) {
+    if (lane == 0) sums[wave] = s;
+    __syncthreads();  // the maxima have been read
+    if (lane < a.top) lds.lists[0][wave * a.top + lane] = list;
+    __syncthreads();
+    s = Joined(Joined(sums[0], sums[1]), Joined(sums[2], sums[3]));
+    const uint64_t* const keys = Merged(lds.lists[0], lds.lists[1], kWaves, a.top);
+    if (wave > 0) return;
+    list = lane < a.top ? keys[lane] : 0;
+  }
+  if (a.parts == 1) {
+    Finish<T>(a, row, given, s, list);
+    return;
+  }
+  uint64_t* const to = PartAt(a, unit);
+  if (lane < a.top) to[lane] = list;
+  if (lane == 0) {
+    to[a.top] = (uint64_t)__float_as_uint(s.l) << 32 | __float_as_uint(s.m);
+    to[a.top + 1] = __float_as_uint(s.w);
+  }
+}
+
+// A row's parts.
+template <class T>
+__global__ __launch_bounds__(kThreads) void JoinKernel(const LogprobsArgs a) {
+  __shared__ uint64_t lists[2][kMostParts * 64];
+  __shared__ Sums sums;
+  const uint32_t row = blockIdx.x, tid = threadIdx.x;
+  const uint64_t* const from = PartAt(a, (uint64_t)row * a.parts);
+  const Given<T> given(a, row);
+  for (uint32_t i = tid; i < a.parts * a.top; i += kThreads)
+    lists[0][i] = from[i / a.top * (a.top + 2) + i % a.top];
+  if (tid < 64) {
+    Sums s{-__builtin_inff(), 0.f, 0.f};
+    if (tid < a.parts) {
+      const uint64_t* const x = from + tid * (a.top + 2) + a.top;
+      s = Sums{__uint_as_float((uint32_t)x[0]), __uint_as_float((uint32_t)(x[0] >> 32)),
+               __uint_as_float((uint32_t)x[1])};
+    }
+    s = JoinedOverWave(s);
+    if (tid == 0) sums = s;
+  }
+  __syncthreads();
+  const uint64_t* const keys = Merged(lists[0], lists[1], a.parts, a.top);
+  if (tid < 64) Finish<T>(a, row, given, sums, tid < a.top ? keys[tid] : 0);
 }
 
 template <class T>
-__global__ __launch_bounds__(kThreads) void LogprobsKernel(const LogprobsArgs a) {
-  __shared__ float f[kThreads / 64];
-  __shared__ uint64_t keys[kThreads / 64];
-  const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-  const T* const x = static_cast<const T*>(a.logits) + row * a.stride;
-  const float c = a.scale * kLog2e;  // in powers of two from here on
-  auto sum = [&](float v) {
-    for (uint32_t d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    __syncthreads();
-    if (lane == 0) f[wave] = v;
-    __syncthreads();
-    return f[0] + f[1] + f[2] + f[3];
-  };
-  float m = -__builtin_inff();
-  for (uint32_t i = tid; i < a.vocab; i += kThreads) m = fmaxf(m, (float)x[i]);
-  for (uint32_t d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-  if (lane == 0) f[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
-  const float ref = m == -__builtin_inff() ? 0.f : m;
-  float l = 0.f, w = 0.f;
-  for (uint32_t i = tid; i < a.vocab; i += kThreads) {
-    const float d = ((float)x[i] - ref) * c, p = __builtin_amdgcn_exp2f(d);
-    l += p;
-    w += p * fmaxf(d, -1e4f);
+hipError_t LaunchType(LogprobsArgs& a, Workspace& ws, hipStream_t stream) {
+  // A row a wave where there are rows enough that its end is not what waits:
+  // 4,096 rows of 1,000 bf16 logits 9.4 us (20.3 with four waves a row), 2,000
+  // of 8,192 14.3 (18.7), 4,500 of 16,000 38 (47), 4,096 of 65,537 117 (126),
+  // but 1,024 of 32,000 35 (23), 2,048 of 65,537 75 (59), and 4,096 of 65,537 in
+  // fp32 208 (199).
+  const uint64_t cus = (uint64_t)DeviceCus();
+  const bool alone = a.rows >= 4 * cus && (a.vocab * sizeof(T) <= 16384 ||
+                                           (a.rows >= 16 * cus && sizeof(T) == 2));
+  // four workgroups a CU, of a batch a wave at least
+  const uint64_t per = kLoads * 64 * kWaves * Packed<T>::kCount;
+  const uint64_t want = (4 * cus + a.rows - 1) / a.rows;
+  a.parts = (uint32_t)std::min<uint64_t>({want, (a.vocab + per - 1) / per, kMostParts});
+  if (a.parts > 1) {
+    const hipError_t err =
+        GrowWorkspace(ws, (size_t)a.rows * a.parts * (a.top + 2) * sizeof(uint64_t), stream);
+    if (err != hipSuccess) return err;
+    a.ws = ws.ptr + kSplitCounters;
   }
-  l = sum(l);
-  w = sum(w);
-  const float log = l == 0.f ? 0.f : __builtin_amdgcn_logf(l);
-  auto logprob = [&](float logit) {
-    return l == 0.f ? -__builtin_inff() : ((logit - ref) * c - log) * kLn2;
-  };
-  if (tid == 0) {
-    if (a.tokens != nullptr) {
-      const int32_t t = a.tokens[row];
-      a.logprobs[row] = t < 0 ? 0.f
-                        : (uint32_t)t >= a.vocab ? __builtin_nanf("")
-                                                 : logprob((float)x[t]);
-    }
-    if (a.entropy != nullptr) a.entropy[row] = l == 0.f ? 0.f : (log - w / l) * kLn2;
-  }
-  uint64_t below = ~0ull;
-  for (uint32_t k = 0; k < a.top; ++k) {
-    uint64_t best = 0;
-    for (uint32_t i = tid; i < a.vocab; i += kThreads) {
-      const uint64_t key = KeyOf((float)x[i], i);
-      if (key < below) best = max(best, key);
-    }
-    for (uint32_t d = 1; d < 64; d *= 2) best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
-    __syncthreads();
-    if (lane == 0) keys[wave] = best;
-    __syncthreads();
-    best = max(max(keys[0], keys[1]), max(keys[2], keys[3]));
-    below = best;
-    if (tid == 0) {
-      const uint32_t column = ~(uint32_t)best;
-      a.top_ids[(uint64_t)row * a.top + k] = (int32_t)column;
-      a.top_logprobs[(uint64_t)row * a.top + k] = logprob((float)x[column]);
-    }
-  }
+  if (alone)
+    LogprobsKernel<T, 1><<<(a.rows * a.parts + kWaves - 1) / kWaves, kThreads, 0, stream>>>(a);
+  else
+    LogprobsKernel<T, kWaves><<<a.rows * a.parts, kThreads, 0, stream>>>(a);
+  if (a.parts > 1) JoinKernel<T><<<a.rows, kThreads, 0, stream>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t LaunchLogprobs(const LogprobsArgs& a, Workspace&, hipStream_t stream) {
+hipError_t LaunchLogprobs(const LogprobsArgs& in, Workspace& ws, hipStream_t stream) {
+  LogprobsArgs a = in;
   switch (a.type) {
-    case HB_TYPE_F32: LogprobsKernel<float><<<a.rows, kThreads, 0, stream>>>(a); break;
-    case HB_TYPE_BF16: LogprobsKernel<__bf16><<<a.rows, kThreads, 0, stream>>>(a); break;
-    default: LogprobsKernel<_Float16><<<a.rows, kThreads, 0, stream>>>(a);
+    case HB_TYPE_F32: return LaunchType<float>(a, ws, stream);
+    case HB_TYPE_BF16: return LaunchType<__bf16>(a, ws, stream);
+    default: return LaunchType<_Float16>(a, ws, stream);
   }
-  return hipGetLastError();
 }
 
 }  // namespace hb
