@@ -442,8 +442,17 @@ struct KvRowsArgs {
   const int32_t* slots;
   uint8_t* cache;
   uint32_t type, tokens, pages, heads, groups, dim;
-  uint32_t vec;                    // set by the launcher
+  uint32_t vec, window;            // set by the launchers
 };
+// Whether the rows allow loads and stores of four elements.
+inline bool KvRowsAligned(const KvRowsArgs& a, bool read) {
+  const uint32_t size = a.type == HB_TYPE_F32 ? 4 : 2;
+  const uint64_t strides = a.k_token | a.k_head | a.v_token | a.v_head;
+  const uintptr_t bases =
+      read ? reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)
+           : reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
+  return strides % 4 == 0 && bases % (4 * size) == 0;
+}
 // tokens * heads < 2^31
 hipError_t LaunchKvRows(const KvRowsArgs& a, bool read, hipStream_t stream);
 struct AttnArgs {

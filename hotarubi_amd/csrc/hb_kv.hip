@@ -645,12 +645,7 @@ hipError_t LaunchRope(const RopeArgs& in, hipStream_t stream) {
 
 hipError_t LaunchKvRows(const KvRowsArgs& in, bool read, hipStream_t stream) {
   KvRowsArgs a = in;
-  const uint32_t size = a.type == HB_TYPE_F32 ? 4 : 2;
-  const uint64_t strides = a.k_token | a.k_head | a.v_token | a.v_head;
-  const uintptr_t bases =
-      read ? reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)
-           : reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
-  a.vec = strides % 4 == 0 && bases % (4 * size) == 0;
+  a.vec = KvRowsAligned(a, read);
   const uint32_t tokens = kThreads / (a.dim / 8);  // of a workgroup
   const uint32_t grid = (a.tokens + tokens - 1) / tokens * a.heads;
   switch (a.type) {

@@ -9,10 +9,29 @@ namespace hb {
 namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kThreads = 256;
+template <class T>
+struct Four;
+template <>
+struct Four<float> {
+  typedef f32x4 type;
+};
+template <>
+struct Four<__bf16> {
+  typedef bf16x4 type;
+};
+template <>
+struct Four<_Float16> {
+  typedef f16x4 type;
+};
 
-// 2^(byte - 127) as a float, byte 0 to 246 (0 stands beside zeros only).
+constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
+
+// 2^(byte - 127), byte 0 to 246 (0 stands beside zeros only).
 __device__ __forceinline__ float ScaleOf(uint32_t byte) { return __uint_as_float(byte << 23); }
 // 2^(127 - byte), byte 10 to 246.
 __device__ __forceinline__ float Unscale(uint32_t byte) { return __uint_as_float((254 - byte) << 23); }
@@ -23,124 +42,260 @@ __device__ __forceinline__ uint32_t WaveMax(uint32_t x) {
   return x;
 }
 
-// The code of x times a power of two, nearest even; past 448 that.
-__device__ __forceinline__ uint8_t Code(float x) {
-  x = __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
-  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false);
+// Four values as codes, the first in the lowest byte: nearest even, past 448
+// that.
+__device__ __forceinline__ uint32_t Codes(float a, float b, float c, float d) {
+  a = __builtin_amdgcn_fmed3f(a, -448.f, 448.f);
+  b = __builtin_amdgcn_fmed3f(b, -448.f, 448.f);
+  c = __builtin_amdgcn_fmed3f(c, -448.f, 448.f);
+  d = __builtin_amdgcn_fmed3f(d, -448.f, 448.f);
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
 }
-__device__ __forceinline__ float Value(uint8_t code, float scale) {
-  return __builtin_amdgcn_cvt_f32_fp8((int)code, 0) * scale;
+// Four codes times f <= 1, which nothing passes 448 by and NaN stays in.
+__device__ __forceinline__ uint32_t Again(uint32_t codes, float f) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a[0] * f, a[1] * f, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[0] * f, b[1] * f, lo, true);
 }
 
-// A wave takes a run of rows (of neighbouring slots within a block) and a
-// head: the runs' first rows find them, waves of other rows end at once.
+template <class T>
+__device__ __forceinline__ void Load4(const T* x, bool vec, float* y) {
+  typedef typename Four<T>::type V;
+  if (vec) {
+    const V v = *reinterpret_cast<const V*>(x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (float)v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (float)x[j];
+  }
+}
+
+// A workgroup takes the runs that begin in `window` neighbouring rows, of one
+// head, one after another (a run: rows whose slots are neighbours within a
+// block): 4 columns of 2, 4 or 8 tokens a thread, all of a run in registers
+// between its maximum and its codes.  A run that is a whole block leaves through
+// LDS in the record's order, 16 bytes a store; of others a token's own bytes,
+// which lie all over the record.
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
-  constexpr uint32_t kCols = dim / 64;
-  const uint32_t lane = threadIdx.x % 64;
-  const uint64_t wave =
-      (uint64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t head = (uint32_t)(wave % g.heads);
-  const uint64_t row = wave / g.heads;
-  if (row >= g.tokens) return;
-  // slots of the row before, its own and 62 after it, a lane each
-  int32_t slot = -1;
-  if (row + lane >= 1 && row + lane - 1 < g.tokens) slot = g.slots[row + lane - 1];
-  const int32_t mine = __builtin_amdgcn_readlane(slot, 1);
+  constexpr uint32_t kRow = dim / 4, kGroups = kThreads / kRow, kRows = 32 / kGroups;
+  __shared__ __align__(16) uint8_t image[64 * dim];
+  __shared__ uint32_t tops[kWaves][2];
+  const uint32_t tid = threadIdx.x, lane = tid % 64;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const uint32_t head = blockIdx.x % g.heads;
+  const uint32_t row0 = blockIdx.x / g.heads * g.window;
+  const uint32_t group = tid / kRow, col = tid % kRow * 4;
+  // slots of the row before the window's and of 63 rows from there, a lane each
+  const uint64_t at = (uint64_t)row0 + lane;
+  const int32_t slot = at >= 1 && at - 1 < g.tokens ? g.slots[at - 1] : -1;
+  const int32_t before = __shfl_up(slot, 1);
+  const bool goes_on = lane > 0 && slot % 32 != 0 && slot > 0 && before == slot - 1;
   uint64_t record;
   uint32_t t0;
-  if (!KvSlot(mine, g.pages, g.heads, g.groups, &record, &t0)) return;
-  if (t0 > 0 && __builtin_amdgcn_readlane(slot, 0) == mine - 1) return;  // within a run
-  const bool follows = lane >= 1 && (int64_t)slot == (int64_t)mine + lane - 1 && t0 + lane <= 32;
-  const uint32_t count =
-      (uint32_t)__builtin_ctzll(~(__builtin_amdgcn_ballot_w64(follows) >> 1));
-  uint8_t* const to =
-      g.cache + (record + (uint64_t)head * g.groups) * Kv8RecordBytes(dim);
-  const uint32_t col0 = lane * kCols;
-  const T* const k = static_cast<const T*>(g.k) + row * g.k_token + head * g.k_head + col0;
-  const T* const v = static_cast<const T*>(g.v) + row * g.v_token + head * g.v_head + col0;
-  uint32_t bad = 0, k_top = 0, v_top = 0;
-  for (uint32_t t = 0; t < count; ++t) {
-    uint32_t kt = 0, vt = 0;
-    for (uint32_t c = 0; c < kCols; ++c) {
-      kt = max(kt, __float_as_uint((float)k[t * g.k_token + c]) & 0x7FFFFFFFu);
-      vt = max(vt, __float_as_uint((float)v[t * g.v_token + c]) & 0x7FFFFFFFu);
+  const bool there = KvSlot(slot, g.pages, g.heads, g.groups, &record, &t0);
+  const uint64_t on = __builtin_amdgcn_ballot_w64(goes_on);
+  uint64_t starts = __builtin_amdgcn_ballot_w64(there && !goes_on && lane > 0 && lane <= g.window);
+  for (; starts != 0; starts &= starts - 1) {
+    const uint32_t l = (uint32_t)__builtin_ctzll(starts);
+    const uint32_t row = row0 + l - 1;
+    const uint32_t count = 1 + (uint32_t)__builtin_ctzll(~(on >> (l + 1)));
+    (void)KvSlot(__builtin_amdgcn_readlane(slot, (int)l), g.pages, g.heads, g.groups, &record, &t0);
+    uint8_t* const to = g.cache + (record + (uint64_t)head * g.groups) * Kv8RecordBytes(dim);
+    const uint32_t had = t0 > 0 ? *reinterpret_cast<const uint16_t*>(to + Kv8Scale(dim, 0)) : 0;
+    float k[kRows][4], v[kRows][4];
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i) {
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) k[i][j] = v[i][j] = 0.f;
+      const uint32_t t = group * kRows + i;
+      if (t >= count) continue;
+      const uint64_t r = row + t;
+      Load4(static_cast<const T*>(g.k) + r * g.k_token + head * g.k_head + col, g.vec, k[i]);
+      Load4(static_cast<const T*>(g.v) + r * g.v_token + head * g.v_head + col, g.vec, v[i]);
     }
-    if (__builtin_amdgcn_ballot_w64(max(kt, vt) >= 0x7F800000u) != 0) {
-      bad |= 1u << t;
-      continue;
-    }
-    k_top = max(k_top, kt);
-    v_top = max(v_top, vt);
-  }
-  const uint32_t had_k = t0 > 0 ? to[Kv8Scale(dim, 0)] : 0, had_v = t0 > 0 ? to[Kv8Scale(dim, 1)] : 0;
-  const uint32_t ks = max(had_k, Kv8ScaleOf(WaveMax(k_top)));
-  const uint32_t vs = max(had_v, Kv8ScaleOf(WaveMax(v_top)));
-  if (ks > had_k && had_k > 0) {
-    const float f = ScaleOf(had_k) * Unscale(ks);
-    for (uint32_t t = 0; t < t0; ++t)
-      for (uint32_t c = 0; c < kCols; ++c) {
-        uint8_t* const at = to + Kv8KCode(dim, t, col0 + c);
-        if ((*at & 0x7F) != 0x7F) *at = Code(Value(*at, f));
+    uint32_t bad = 0, k_top = 0, v_top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i) {
+      uint32_t kt = 0, vt = 0;
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        kt = max(kt, __float_as_uint(k[i][j]) & 0x7FFFFFFFu);
+        vt = max(vt, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
       }
-  }
-  if (vs > had_v && had_v > 0) {
-    const float f = ScaleOf(had_v) * Unscale(vs);
-    for (uint32_t t = 0; t < t0; ++t)
-      for (uint32_t c = 0; c < kCols; ++c) {
-        uint8_t* const at = to + Kv8VCode(dim, t, col0 + c);
-        *at = Code(Value(*at, f));
+      // a row's threads are lanes of one wave
+      const uint64_t odd = __builtin_amdgcn_ballot_w64(max(kt, vt) >= 0x7F800000u);
+      const uint64_t mine = (~0ull >> (64 - kRow)) << (lane / kRow * kRow);
+      if ((odd & mine) != 0) {
+        bad |= 1u << i;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) k[i][j] = v[i][j] = 0.f;
+      } else {
+        k_top = max(k_top, kt);
+        v_top = max(v_top, vt);
       }
-  }
-  const float ku = ks > 0 ? Unscale(ks) : 0.f, vu = vs > 0 ? Unscale(vs) : 0.f;
-  for (uint32_t t = 0; t < count; ++t) {
-    const bool b = bad >> t & 1;
-    for (uint32_t c = 0; c < kCols; ++c) {
-      to[Kv8KCode(dim, t0 + t, col0 + c)] = b ? 0x7F : Code((float)k[t * g.k_token + c] * ku);
-      to[Kv8VCode(dim, t0 + t, col0 + c)] = b ? 0 : Code((float)v[t * g.v_token + c] * vu);
     }
-  }
-  if (lane == 0) {
-    to[Kv8Scale(dim, 0)] = (uint8_t)ks;
-    to[Kv8Scale(dim, 1)] = (uint8_t)vs;
+    k_top = WaveMax(k_top);
+    v_top = WaveMax(v_top);
+    if (lane == 0) {
+      tops[wave][0] = k_top;
+      tops[wave][1] = v_top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+      k_top = max(k_top, tops[w][0]);
+      v_top = max(v_top, tops[w][1]);
+    }
+    const uint32_t had_k = had & 255u, had_v = had >> 8;
+    const uint32_t ks = max(had_k, Kv8ScaleOf(k_top)), vs = max(had_v, Kv8ScaleOf(v_top));
+    const float ku = ks > 0 ? Unscale(ks) : 0.f, vu = vs > 0 ? Unscale(vs) : 0.f;
+    if (count == 32) {
+#pragma unroll
+      for (uint32_t i = 0; i < kRows; ++i) {
+        const uint32_t codes = Codes(k[i][0] * ku, k[i][1] * ku, k[i][2] * ku, k[i][3] * ku);
+        *reinterpret_cast<uint32_t*>(image + Kv8KCode(dim, group * kRows + i, col)) =
+            bad >> i & 1 ? 0x7F7F7F7Fu : codes;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        uint8_t* const y = image + Kv8VCode(dim, group * kRows, col + j);
+        if constexpr (kRows == 2) {
+          *reinterpret_cast<uint16_t*>(y) =
+              (uint16_t)Codes(v[0][j] * vu, v[1][j] * vu, 0.f, 0.f);
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < kRows; i += 4)  // 4 tokens on: the next lanes' piece
+            *reinterpret_cast<uint32_t*>(image + Kv8VCode(dim, group * kRows + i, col + j)) =
+                Codes(v[i][j] * vu, v[(i + 1) % kRows][j] * vu, v[(i + 2) % kRows][j] * vu,
+                      v[(i + 3) % kRows][j] * vu);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (uint32_t p = 0; p < 64 * dim; p += kThreads * 16)
+        *reinterpret_cast<u32x4*>(to + p + tid * 16) =
+            *reinterpret_cast<const u32x4*>(image + p + tid * 16);
+    } else {
+      // earlier tokens' codes where the scale grows, in 16-byte pieces
+      const bool k_grows = ks > had_k && had_k > 0, v_grows = vs > had_v && had_v > 0;
+      if (k_grows || v_grows) {
+        for (uint32_t p = tid; p < 4 * dim; p += kThreads) {
+          const bool is_k = p < 2 * dim;
+          if (!(is_k ? k_grows : v_grows)) continue;
+          const float f = is_k ? ScaleOf(had_k) * Unscale(ks) : ScaleOf(had_v) * Unscale(vs);
+          u32x4* const piece = reinterpret_cast<u32x4*>(to) + p;
+          u32x4 x = *piece;
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t y = Again(x[j], f);
+            if (is_k) {  // a piece is of one token
+              const uint32_t t = p / 64 / (dim / 64) * 16 + p % 16;
+              if (t < t0) x[j] = y;
+            } else {  // a word is of four
+              const uint32_t t = j % 2 * 16 + p % 64 / 16 * 4;
+              const uint32_t keep = t + 4 <= t0 ? ~0u : t >= t0 ? 0u : (1u << (8 * (t0 - t))) - 1;
+              x[j] = (y & keep) | (x[j] & ~keep);
+            }
+          }
+          *piece = x;
+        }
+        __syncthreads();  // before the new tokens' bytes
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < kRows; ++i) {
+        const uint32_t t = group * kRows + i;
+        if (t >= count) continue;
+        const uint32_t codes = Codes(k[i][0] * ku, k[i][1] * ku, k[i][2] * ku, k[i][3] * ku);
+        *reinterpret_cast<uint32_t*>(to + Kv8KCode(dim, t0 + t, col)) =
+            bad >> i & 1 ? 0x7F7F7F7Fu : codes;
+        const uint32_t values = Codes(v[i][0] * vu, v[i][1] * vu, v[i][2] * vu, v[i][3] * vu);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+          to[Kv8VCode(dim, t0 + t, col + j)] = (uint8_t)(values >> (8 * j));
+      }
+    }
+    if (tid == 0)
+      *reinterpret_cast<uint16_t*>(to + Kv8Scale(dim, 0)) = (uint16_t)(ks | vs << 8);
+    __syncthreads();  // image and tops have been read
   }
 }
 
-// The stored values of slots: a wave a token and head.
+template <class T>
+__device__ __forceinline__ void Store4(T* to, bool vec, uint32_t codes, float scale) {
+  typedef typename Four<T>::type V;
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  const float y[4] = {a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
+  if (vec) {
+    V v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (T)y[j];
+    *reinterpret_cast<V*>(to) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[j] = (T)y[j];
+  }
+}
+
+// The stored values of slots, 4 columns of kEach tokens a thread.
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void ReadKernel(const KvRowsArgs g) {
-  constexpr uint32_t kCols = dim / 64;
-  const uint32_t lane = threadIdx.x % 64;
-  const uint64_t wave =
-      (uint64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t head = (uint32_t)(wave % g.heads);
-  const uint64_t row = wave / g.heads;
-  if (row >= g.tokens) return;
-  T* const k = static_cast<T*>(g.k_out) + row * g.k_token + head * g.k_head + lane * kCols;
-  T* const v = static_cast<T*>(g.v_out) + row * g.v_token + head * g.v_head + lane * kCols;
-  uint64_t record;
-  uint32_t t;
-  const bool there = KvSlot(g.slots[row], g.pages, g.heads, g.groups, &record, &t);
-  const uint8_t* const from =
-      g.cache + (there ? record + (uint64_t)head * g.groups : 0) * Kv8RecordBytes(dim);
-  const float ks = ScaleOf(from[Kv8Scale(dim, 0)]), vs = ScaleOf(from[Kv8Scale(dim, 1)]);
-  for (uint32_t c = 0; c < kCols; ++c) {
-    k[c] = (T)(there ? Value(from[Kv8KCode(dim, t, lane * kCols + c)], ks) : 0.f);
-    v[c] = (T)(there ? Value(from[Kv8VCode(dim, t, lane * kCols + c)], vs) : 0.f);
+  constexpr uint32_t kRow = dim / 4, kGroups = kThreads / kRow, kEach = 4;
+  const uint32_t head = blockIdx.x % g.heads, col = threadIdx.x % kRow * 4;
+  const uint32_t row0 = blockIdx.x / g.heads * (kGroups * kEach) + threadIdx.x / kRow;
+  uint32_t k[kEach], v[kEach], scales[kEach];
+  uint64_t record[kEach];
+  uint32_t t[kEach];
+  bool there[kEach];
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint64_t row = (uint64_t)row0 + i * kGroups;
+    there[i] = KvSlot(row < g.tokens ? g.slots[row] : -1, g.pages, g.heads, g.groups, &record[i],
+                      &t[i]);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    k[i] = v[i] = scales[i] = 0;
+    if (!there[i]) continue;
+    const uint8_t* const from =
+        g.cache + (record[i] + (uint64_t)head * g.groups) * Kv8RecordBytes(dim);
+    k[i] = *reinterpret_cast<const uint32_t*>(from + Kv8KCode(dim, t[i], col));
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+      v[i] |= (uint32_t)from[Kv8VCode(dim, t[i], col + j)] << (8 * j);
+    scales[i] = *reinterpret_cast<const uint16_t*>(from + Kv8Scale(dim, 0));
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint64_t row = (uint64_t)row0 + i * kGroups;
+    if (row >= g.tokens) continue;
+    Store4(static_cast<T*>(g.k_out) + row * g.k_token + head * g.k_head + col, g.vec, k[i],
+           ScaleOf(scales[i] & 255u));
+    Store4(static_cast<T*>(g.v_out) + row * g.v_token + head * g.v_head + col, g.vec, v[i],
+           ScaleOf(scales[i] >> 8));
   }
 }
 
 template <class T, uint32_t dim>
-hipError_t LaunchOf(const KvRowsArgs& a, bool read, hipStream_t s) {
-  const uint64_t waves = (uint64_t)a.tokens * a.heads;
-  const uint32_t grid = (uint32_t)((waves + kThreads / 64 - 1) / (kThreads / 64));
-  if (read) ReadKernel<T, dim><<<grid, kThreads, 0, s>>>(a);
-  else AppendKernel<T, dim><<<grid, kThreads, 0, s>>>(a);
+hipError_t LaunchOf(KvRowsArgs& a, bool read, hipStream_t s) {
+  if (read) {
+    constexpr uint32_t kRows = kThreads / (dim / 4) * 4;
+    ReadKernel<T, dim><<<(a.tokens + kRows - 1) / kRows * a.heads, kThreads, 0, s>>>(a);
+  } else {
+    // eight workgroups a CU, of a block's rows at most
+    const uint64_t rows = (uint64_t)a.tokens * a.heads / (8 * (uint64_t)DeviceCus());
+    a.window = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(1, rows));
+    AppendKernel<T, dim><<<(a.tokens + a.window - 1) / a.window * a.heads, kThreads, 0, s>>>(a);
+  }
   return hipGetLastError();
 }
 
 template <class T>
-hipError_t LaunchType(const KvRowsArgs& a, bool read, hipStream_t s) {
+hipError_t LaunchType(KvRowsArgs& a, bool read, hipStream_t s) {
   switch (a.dim) {
     case 64: return LaunchOf<T, 64>(a, read, s);
     case 128: return LaunchOf<T, 128>(a, read, s);
@@ -151,7 +306,9 @@ hipError_t LaunchType(const KvRowsArgs& a, bool read, hipStream_t s) {
 
 }  // namespace
 
-hipError_t LaunchKv8Rows(const KvRowsArgs& a, bool read, hipStream_t stream) {
+hipError_t LaunchKv8Rows(const KvRowsArgs& in, bool read, hipStream_t stream) {
+  KvRowsArgs a = in;
+  a.vec = KvRowsAligned(a, read);
   switch (a.type) {
     case HB_TYPE_F32: return LaunchType<float>(a, read, stream);
     case HB_TYPE_BF16: return LaunchType<__bf16>(a, read, stream);
