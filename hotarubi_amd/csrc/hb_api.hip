@@ -1732,7 +1732,7 @@ int KvCompact(hb_ctx* ctx, const hb_kv_compact_desc* d, bool sync) {
   hb::CompactArgs a{d->table,  d->lens,   d->table_out, d->free_pages, d->free_count,
                     d->pairs,  d->status, d->batch,     d->columns,    d->table_stride,
                     d->table_out_stride, d->page_size, d->pages, d->free_size, d->pair_count,
-                    nullptr};
+                    nullptr, 0};
   return Launched(ctx, hb::LaunchCompact(a, ctx->ws, ctx->stream), "compaction launch", sync);
 }
 

@@ -527,6 +527,7 @@ struct CompactArgs {
   uint32_t batch, columns, table_stride, table_out_stride, page, pages, free_size,
       pair_count;
   uint32_t* place;  // set by the launcher
+  uint32_t whole;
 };
 hipError_t LaunchCompact(const CompactArgs& a, Workspace& ws, hipStream_t stream);
 

@@ -54,6 +54,14 @@ __global__ __launch_bounds__(kForkThreads) void ForkKernel(const ForkArgs a) {
   __shared__ uint32_t place[kForkThreads], part[kForkWaves];
   const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   constexpr uint32_t kNone = 0xFFFFFFFFu;
+  // a thread's first fork, which is most often its only one, is loaded once
+  const bool any = tid < a.forks;
+  const uint32_t source0 = any ? (uint32_t)a.source[tid] : kNone;
+  const uint32_t target0 = any ? (uint32_t)a.target[tid] : kNone;
+  const uint32_t free_count = (uint32_t)max(0, min(*a.free_count, (int32_t)a.free_size));
+  const int32_t len0 = source0 < a.batch ? a.lens[source0] : 0;
+  auto source = [&](uint32_t i) { return i == tid ? source0 : (uint32_t)a.source[i]; };
+  auto target = [&](uint32_t i) { return i == tid ? target0 : (uint32_t)a.target[i]; };
   for (uint32_t i = tid; i < (a.forks + 31) / 32; i += kForkThreads) bad[i] = again[i] = 0;
   for (uint32_t base = 0; base < a.batch; base += kRowWindow) {
     const uint32_t rows = min(kRowWindow, a.batch - base);
@@ -62,13 +70,13 @@ __global__ __launch_bounds__(kForkThreads) void ForkKernel(const ForkArgs a) {
     for (uint32_t i = tid; i < kRowWindow / 32; i += kForkThreads) is_source[i] = 0;
     __syncthreads();
     for (uint32_t i = tid; i < a.forks; i += kForkThreads) {
-      const uint32_t s = (uint32_t)a.source[i] - base, t = (uint32_t)a.target[i] - base;
+      const uint32_t s = source(i) - base, t = target(i) - base;
       if (s < rows) atomicOr(&is_source[s / 32], 1u << (s % 32));
       if (t < rows) atomicMin(&first[t], i);
     }
     __syncthreads();
     for (uint32_t i = tid; i < a.forks; i += kForkThreads) {
-      const uint32_t t = (uint32_t)a.target[i] - base;
+      const uint32_t t = target(i) - base;
       if (t >= rows) continue;
       if (first[t] != i) atomicOr(&again[i / 32], 1u << (i % 32));
       if (first[t] != i || (is_source[t / 32] >> (t % 32) & 1u))
@@ -79,16 +87,15 @@ __global__ __launch_bounds__(kForkThreads) void ForkKernel(const ForkArgs a) {
       if (first[i] == kNone) a.lens_out[base + i] = a.lens[base + i];
   }
   __syncthreads();
-  const uint32_t free_count = (uint32_t)max(0, min(*a.free_count, (int32_t)a.free_size));
   uint32_t wanted = 0, taken = 0, refused = 0;
   constexpr uint32_t kRefused = 0xFFFFFFFFu, kNoPage = 0xFFFFFFFEu;
   for (uint32_t base = 0; base < a.forks; base += kForkThreads) {
     const uint32_t i = base + tid;
     bool fits = false, need = false;
     if (i < a.forks) {
-      const uint32_t s = (uint32_t)a.source[i], t = (uint32_t)a.target[i];
+      const uint32_t s = source(i), t = target(i);
       if (s < a.batch && t < a.batch && !(bad[i / 32] >> (i % 32) & 1u)) {
-        const int32_t n = a.lens[s];
+        const int32_t n = i == tid ? len0 : a.lens[s];
         fits = PagesOf(n, a.page) <= a.columns;
         need = fits && n > 0 && (uint32_t)n % a.page != 0;
       }
@@ -176,32 +183,49 @@ __global__ __launch_bounds__(kCopyThreads) void CopyKernel(const CopyArgs a) {
 
 constexpr uint32_t kMarkThreads = 1024, kMarkWords = kMostPages / 32;
 
-// mark(page, row) for every entry of a row's pages.  All of the table is read,
-// so that a load waits for no length.
+// mark(page, row) for every entry of a row's pages.  A wave takes rows kWaves
+// apart, the lengths of 64 of them at once and then the entries of kEach of them,
+// as loads that wait for one another are what this takes: 512 rows of 8 to 55
+// pages 14.5 us with four entries a thread at a time, one length each.
 template <class Mark>
 __device__ __forceinline__ void EachEntry(const int32_t* table, const int32_t* lens,
                                           uint32_t batch, uint32_t columns, uint32_t stride,
                                           uint32_t page, uint32_t pages, Mark&& mark) {
-  const uint32_t all = batch * columns;  // below 2^31
-  constexpr uint32_t kEach = 4;
-  for (uint32_t base = threadIdx.x; base < all; base += kEach * kMarkThreads) {
-    uint32_t entry[kEach], row[kEach], col[kEach];
-    int32_t len[kEach];
+  constexpr uint32_t kWaves = kMarkThreads / 64, kEach = 16;
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  for (uint64_t base = wave; base < batch; base += 64 * kWaves) {
+    const uint64_t mine = base + (uint64_t)lane * kWaves;
+    const uint32_t of = mine < batch ? min(columns, PagesOf(lens[mine], page)) : 0u;
+    uint32_t rows = (uint32_t)min((uint64_t)64, (batch - base + kWaves - 1) / kWaves);
+    for (uint32_t r = 0; r < rows; r += kEach) {
+      uint32_t entry[kEach];
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-      const uint32_t i = base + j * kMarkThreads;
-      entry[j] = 0xFFFFFFFFu;
-      row[j] = col[j] = 0;
-      len[j] = 0;
-      if (i >= all) continue;
-      row[j] = i / columns;
-      col[j] = i % columns;
-      entry[j] = (uint32_t)table[(uint64_t)row[j] * stride + col[j]];
-      len[j] = lens[row[j]];
+      for (uint32_t j = 0; j < kEach; ++j) {
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)of, (int)((r + j) % 64));
+        entry[j] = 0xFFFFFFFFu;
+        if (r + j < rows && lane < n)
+          entry[j] = (uint32_t)table[(base + (uint64_t)(r + j) * kWaves) * stride + lane];
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < kEach; ++j)
+        if (entry[j] < pages) mark(entry[j], (uint32_t)(base + (r + j) * kWaves));
     }
+    for (uint32_t r = 0; r < rows; ++r) {  // what is past 64 pages of a row
+      const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)of, (int)r);
+      const uint64_t row = base + (uint64_t)r * kWaves;
+      for (uint32_t c = 64; c < n; c += 64 * kEach) {
+        uint32_t entry[kEach];
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j)
-      if (entry[j] < pages && col[j] < PagesOf(len[j], page)) mark(entry[j], row[j]);
+        for (uint32_t j = 0; j < kEach; ++j) {
+          const uint32_t at = c + j * 64 + lane;
+          entry[j] = at < n ? (uint32_t)table[row * stride + at] : 0xFFFFFFFFu;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j)
+          if (entry[j] < pages) mark(entry[j], (uint32_t)row);
+      }
+    }
   }
 }
 
@@ -258,8 +282,28 @@ __global__ __launch_bounds__(kMarkThreads) void FreeKernel(const FreeArgs a) {
   }
 }
 
+// The tables' new numbers, and what is left of the lists.
+__device__ __forceinline__ void Renumber(const CompactArgs& a, uint32_t count, uint32_t moved,
+                                         uint32_t first, uint32_t step) {
+  for (uint32_t i = first; i < a.batch * a.columns; i += step) {  // below 2^31
+    const uint32_t row = i / a.columns, col = i % a.columns;
+    const uint32_t p = (uint32_t)a.table[(uint64_t)row * a.table_stride + col];
+    int32_t to = -1;
+    if (p < a.pages && col < PagesOf(a.lens[row], a.page))
+      to = p < count ? (int32_t)p : a.pairs[2 * (uint64_t)a.place[p] + 1];
+    a.table_out[(uint64_t)row * a.table_out_stride + col] = to;
+  }
+  for (uint64_t i = first; i < a.free_size; i += step)
+    a.free_pages[i] = i < a.pages - count ? (int32_t)(a.pages - 1 - (uint32_t)i) : -1;
+  for (uint64_t i = 2ull * moved + first; i < 2ull * a.pair_count; i += step) a.pairs[i] = -1;
+}
+__global__ __launch_bounds__(256) void RenumberKernel(const CompactArgs a) {
+  Renumber(a, (uint32_t)a.status[0], (uint32_t)a.status[1], blockIdx.x * 256 + threadIdx.x,
+           gridDim.x * 256);
+}
+
 // The pages in use, their ranks, and the pairs; `place` says for a page that
-// moves which pair is its.
+// moves which pair is its.  `whole`: the tables and lists too.
 __global__ __launch_bounds__(kMarkThreads) void CompactKernel(const CompactArgs a) {
   __shared__ uint32_t used[kMarkWords], part[kMarkThreads / 64];
   __shared__ uint32_t before_u;
@@ -311,23 +355,10 @@ __global__ __launch_bounds__(kMarkThreads) void CompactKernel(const CompactArgs 
     a.status[1] = (int32_t)(count - stay);
     *a.free_count = (int32_t)(a.pages - count);
   }
-}
-
-// The tables' new numbers, and what is left of the lists.
-__global__ __launch_bounds__(256) void RenumberKernel(const CompactArgs a) {
-  const uint32_t count = (uint32_t)a.status[0], moved = (uint32_t)a.status[1];
-  const uint32_t first = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
-  for (uint32_t i = first; i < a.batch * a.columns; i += step) {  // below 2^31
-    const uint32_t row = i / a.columns, col = i % a.columns;
-    const uint32_t p = (uint32_t)a.table[(uint64_t)row * a.table_stride + col];
-    int32_t to = -1;
-    if (p < a.pages && col < PagesOf(a.lens[row], a.page))
-      to = p < count ? (int32_t)p : a.pairs[2 * (uint64_t)a.place[p] + 1];
-    a.table_out[(uint64_t)row * a.table_out_stride + col] = to;
-  }
-  for (uint64_t i = first; i < a.free_size; i += step)
-    a.free_pages[i] = i < a.pages - count ? (int32_t)(a.pages - 1 - (uint32_t)i) : -1;
-  for (uint64_t i = 2ull * moved + first; i < 2ull * a.pair_count; i += step) a.pairs[i] = -1;
+  if (a.whole == 0) return;
+  __threadfence_block();
+  __syncthreads();
+  Renumber(a, count, count - stay, tid, kMarkThreads);
 }
 
 }  // namespace
@@ -361,7 +392,11 @@ hipError_t LaunchCompact(const CompactArgs& in, Workspace& ws, hipStream_t strea
   const hipError_t err = GrowWorkspace(ws, (size_t)a.pages * 4, stream);
   if (err != hipSuccess) return err;
   a.place = reinterpret_cast<uint32_t*>(ws.ptr + kSplitCounters);
+  // Small lists in the same launch: 16,384 numbers are 16 a thread.
+  const uint64_t numbers = (uint64_t)a.batch * a.columns + a.free_size + 2ull * a.pair_count;
+  a.whole = numbers <= 16384;
   CompactKernel<<<1, kMarkThreads, 0, stream>>>(a);
+  if (a.whole) return hipGetLastError();
   const uint64_t most = std::max<uint64_t>((uint64_t)a.batch * a.columns, a.free_size);
   RenumberKernel<<<(uint32_t)std::min<uint64_t>(1024, (most + 255) / 256), 256, 0, stream>>>(a);
   return hipGetLastError();
