@@ -10,8 +10,9 @@
 //
 // The most likely tokens: every lane keeps the maxima of its stretches of the
 // row in LDS.  `top` lanes reach the `top`-th largest of the lanes' maxima, so
-// that is a bound, and only stretches that reach it are read again, all at
-// once; their logits go into a list of sorted 64-bit keys, one a lane.
+// that (its upper 16 bits) is a bound, and only stretches that reach it are read
+// again, all at once; their logits go into a list of sorted 64-bit keys, one a
+// lane, 64 of them at a time.
 #include <algorithm>
 
 #include "hb_internal.h"
@@ -23,7 +24,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 constexpr uint32_t kLoads = 2;  // 16-byte loads of a lane's batch
-constexpr uint32_t kStretches = 32;
+constexpr uint32_t kStretches = 24;
 constexpr uint32_t kMostParts = 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -107,42 +108,54 @@ __device__ __forceinline__ uint64_t ReadLane(uint64_t x, uint32_t lane) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// Keys in falling order, one a lane, and one that is none of them.
-__device__ __forceinline__ uint64_t Inserted(uint64_t list, uint64_t key) {
-  const uint32_t lane = threadIdx.x % 64;
-  const uint32_t place = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(list > key));
-  // (from the lane before: wave_shr:1)
-  const uint32_t lo =
-      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)list, 0x138, 0xF, 0xF, false);
-  const uint32_t hi =
-      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(list >> 32), 0x138, 0xF, 0xF, false);
-  const uint64_t before = (uint64_t)hi << 32 | lo;
-  return lane < place ? list : lane == place ? key : before;
+// Ends what the wave's LDS accesses before may still do.
+__device__ __forceinline__ void WaveFence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The value of rank k (from 0) of a lane's each.
-__device__ __forceinline__ uint32_t OfRank(uint32_t x, uint32_t k) {
+// The largest order of 16 upper bits that k lanes' each reach, found bit by bit.
+__device__ __forceinline__ uint32_t Reached(uint32_t order, uint32_t k) {
+  uint32_t least = 0;
+#pragma unroll
+  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit /= 2) {
+    const uint64_t there = __builtin_amdgcn_ballot_w64(order >= (least | bit));
+    if ((uint32_t)__builtin_popcountll(there) >= k) least |= bit;
+  }
+  return least;
+}
+
+// A sorted list and up to 64 keys that it does not have, one a lane, 0 for none
+// (`some` lanes have one), as a list of the largest 64: every key's place is the
+// number of keys above it.  Through `lds`, 64 keys of the wave's own.
+__device__ __forceinline__ uint64_t With(uint64_t list, uint32_t listed, uint64_t key,
+                                         uint64_t some, volatile uint64_t* lds) {
   const uint32_t lane = threadIdx.x % 64;
-#pragma unroll
-  for (uint32_t size = 2; size <= 64; size *= 2)
-#pragma unroll
-    for (uint32_t d = size / 2; d > 0; d /= 2) {
-      const uint32_t y = (uint32_t)__shfl_xor((int)x, (int)d);
-      const bool falls = (lane & size) == 0, low = (lane & d) == 0;
-      x = falls == low ? max(x, y) : min(x, y);
-    }
-  return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)k);
+  uint32_t key_place = 0, list_place = lane;
+  for (uint64_t left = some; left != 0; left &= left - 1) {
+    const uint64_t one = ReadLane(key, (uint32_t)__builtin_ctzll(left));
+    key_place += one > key;
+    list_place += one > list;
+  }
+  for (uint32_t i = 0; i < listed; ++i) key_place += ReadLane(list, i) > key;
+  lds[lane] = 0;
+  WaveFence();
+  if (list != 0 && list_place < 64) lds[list_place] = list;
+  if (key != 0 && key_place < 64) lds[key_place] = key;
+  WaveFence();
+  const uint64_t y = lds[lane];
+  WaveFence();
+  return y;
 }
 
 // Keys of `other` (k of them, falling) that are above `key`.
 __device__ __forceinline__ uint32_t Above(const uint64_t* other, uint32_t k, uint64_t key) {
-  uint32_t lo = 0, hi = k;
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (other[mid] > key) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
+  uint32_t n = 0;
+#pragma unroll
+  for (uint32_t step = 64; step > 0; step /= 2)
+    if (n + step <= k && other[n + step - 1] > key) n += step;
+  return n;
 }
 // `count` lists of k falling keys become one, in pairs: a key's place is its own
 // in its list and the number of keys above it in the other.  Lists of fewer keys
@@ -229,13 +242,6 @@ __device__ __forceinline__ uint64_t* PartAt(const LogprobsArgs& a, uint64_t unit
   return reinterpret_cast<uint64_t*>(a.ws) + unit * (a.top + 2);
 }
 
-// Ends what the wave's LDS accesses before may still do.
-__device__ __forceinline__ void WaveFence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // kW waves take a part of a row, batches of it in turn, the next one's loads
 // under way while a batch is summed up.
 template <class T, uint32_t kW>
@@ -247,6 +253,7 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
   };
   __shared__ Lds lds;
   __shared__ uint16_t again[kWaves][128];  // stretches to be read again
+  __shared__ uint64_t keys[kWaves][128];   // and keys that wait for the list
   __shared__ Sums sums[kWaves];
   __shared__ uint32_t bound, odd;
   const uint32_t lane = threadIdx.x % 64;
@@ -342,7 +349,7 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
   }
   uint64_t list = 0;
   if (a.top > 0) {
-    uint32_t least = OfRank(OrderOf(m), a.top - 1);
+    uint32_t least = Reached(OrderOf(m), a.top);
     // a signalling NaN may have hidden what came before it from a maximum
     bool all = __builtin_amdgcn_ballot_w64(s.l != s.l) != 0;
     if (kW > 1) {
@@ -357,6 +364,22 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
       WaveFence();
     }
     uint64_t last_key = 0;
+    uint32_t listed = 0, waiting = 0;
+    auto take_keys = [&]() {  // the keys that wait, up to 64
+      const uint32_t take = min(waiting, 64u);
+      WaveFence();
+      uint64_t key = lane < take ? keys[wave][lane] : 0;
+      const uint64_t rest = 64 + lane < waiting ? keys[wave][64 + lane] : 0;
+      WaveFence();
+      if (64 + lane < waiting) keys[wave][lane] = rest;
+      waiting -= take;
+      if (key <= last_key) key = 0;
+      const uint64_t some = __builtin_amdgcn_ballot_w64(key != 0);
+      if (some == 0) return;
+      list = With(list, listed, key, some, &keys[wave][64]);
+      listed = min(listed + (uint32_t)__builtin_popcountll(some), a.top);
+      last_key = ReadLane(list, a.top - 1);
+    };
     uint32_t found = 0, next_stretch = 0;
     const uint64_t below = (1ull << lane) - 1;
     while (true) {
@@ -390,16 +413,18 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
             const uint64_t at = i * P::kCount + j - skew;
             uint64_t key = there && at < a.vocab ? KeyOf(P::At(y, j), (uint32_t)at) : 0;
             if ((uint32_t)(key >> 32) < max(least, 1u)) key = 0;
-            uint64_t more = __builtin_amdgcn_ballot_w64(key > last_key);
-            while (more != 0) {
-              list = Inserted(list, ReadLane(key, (uint32_t)__builtin_ctzll(more)));
-              last_key = ReadLane(list, a.top - 1);
-              more = __builtin_amdgcn_ballot_w64(key > last_key) & (more - 1) & more;
-            }
+            if (key <= last_key) key = 0;
+            const uint64_t some = __builtin_amdgcn_ballot_w64(key != 0);
+            if (some == 0) continue;
+            if (key != 0)
+              keys[wave][waiting + (uint32_t)__builtin_popcountll(some & below)] = key;
+            waiting += (uint32_t)__builtin_popcountll(some);
+            if (waiting >= 64) take_keys();
           }
         }
       }
     }
+    if (waiting > 0) take_keys();
   }
   s = JoinedOverWave(s);
   if (kW > 1) {
@@ -408,9 +433,9 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
     if (lane < a.top) lds.lists[0][wave * a.top + lane] = list;
     __syncthreads();
     s = Joined(Joined(sums[0], sums[1]), Joined(sums[2], sums[3]));
-    const uint64_t* const keys = Merged(lds.lists[0], lds.lists[1], kWaves, a.top);
+    const uint64_t* const best = Merged(lds.lists[0], lds.lists[1], kWaves, a.top);
     if (wave > 0) return;
-    list = lane < a.top ? keys[lane] : 0;
+    list = lane < a.top ? best[lane] : 0;
   }
   if (a.parts == 1) {
     Finish<T>(a, row, given, s, list);
@@ -452,15 +477,16 @@ __global__ __launch_bounds__(kThreads) void JoinKernel(const LogprobsArgs a) {
 template <class T>
 hipError_t LaunchType(LogprobsArgs& a, Workspace& ws, hipStream_t stream) {
   // A row a wave where there are rows enough that its end is not what waits:
-  // 4,096 rows of 1,000 bf16 logits 9.4 us (20.3 with four waves a row), 2,000
-  // of 8,192 14.3 (18.7), 4,500 of 16,000 38 (47), 4,096 of 65,537 117 (126),
-  // but 1,024 of 32,000 35 (23), 2,048 of 65,537 75 (59), and 4,096 of 65,537 in
-  // fp32 208 (199).
+  // 4,096 rows of 1,000 bf16 logits 9 us (20 with four waves a row), 2,000 of
+  // 8,192 14 (19), 4,500 of 16,000 38 (47), 4,096 of 65,537 115 (126), but 1,024
+  // of 32,000 35 (23), 2,048 of 65,537 75 (59), and 4,096 of 65,537 in fp32 208
+  // (199).
   const uint64_t cus = (uint64_t)DeviceCus();
   const bool alone = a.rows >= 4 * cus && (a.vocab * sizeof(T) <= 16384 ||
                                            (a.rows >= 16 * cus && sizeof(T) == 2));
-  // four workgroups a CU, of a batch a wave at least
-  const uint64_t per = kLoads * 64 * kWaves * Packed<T>::kCount;
+  // four workgroups a CU, of two batches a wave at least (8 x 50,001 fp32, 20
+  // each: 14.3 us; 15.2 with one, 14.6 with four)
+  const uint64_t per = 2 * kLoads * 64 * kWaves * Packed<T>::kCount;
   const uint64_t want = (4 * cus + a.rows - 1) / a.rows;
   a.parts = (uint32_t)std::min<uint64_t>({want, (a.vocab + per - 1) / per, kMostParts});
   if (a.parts > 1) {
