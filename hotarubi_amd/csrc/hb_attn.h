@@ -50,7 +50,7 @@ constexpr float kRoom = 64.f;
 // ---------------------------------------------------------------- records --
 
 struct Fp4 {
-  static constexpr bool kSinks = false;
+  static constexpr bool kSinks = false, kAnyScore = false;
   // bf16 parts of q, by the tensors' type
   static constexpr uint32_t Parts(uint32_t parts) { return parts; }
   static constexpr uint32_t Bytes(uint32_t dim) { return KvRecordBytes(dim); }
@@ -58,10 +58,11 @@ struct Fp4 {
     return LaunchPrompt(a, ws, stream);
   }
 };
-// E4M3 codes are exact in f16 whatever the scale, which is one for all keys of
-// the record and goes over their scores: fp16 queries take one product.
+// E4M3 codes are exact in f16 too, and the scale, one for all keys of the record,
+// goes into what their scores are multiplied by: fp16 queries take one product.
+// Scores of any size that fp32 holds are taken (Weights).
 struct Fp8 {
-  static constexpr bool kSinks = true;
+  static constexpr bool kSinks = true, kAnyScore = true;
   static constexpr uint32_t Parts(uint32_t parts) { return parts == 2 ? 1 : parts; }
   static constexpr uint32_t Bytes(uint32_t dim) { return Kv8RecordBytes(dim); }
   static hipError_t Prompt(const AttnArgs& a, Workspace& ws, hipStream_t stream) {
@@ -224,7 +225,7 @@ __device__ __forceinline__ typename QueryOperand<Fp8, parts>::type KeyOperand(
   return __builtin_bit_cast(
       typename QueryOperand<Fp8, parts>::type,
       EightOf<parts == 2>(r.k[piece / 2][piece % 2 * 2], r.k[piece / 2][piece % 2 * 2 + 1],
-                          parts == 2 ? 1.f : Scale8(r.scales & 255u)));
+                          1.f));
 }
 
 // P V in f16 for the 16-bit types: a weight is off by at most 2^-11 of itself,
@@ -490,6 +491,7 @@ struct State {
   f32x4 o[R][D / 16];
   float m[R], l[R];
   bool large;  // values were met that want kRoom
+  bool far;    // a maximum has passed 2^20 (kept with any_score)
   Sight see[R];
   int32_t see_all, see_from, see_pre;  // every row sees keys see_from .. see_all, and < see_pre
 };
@@ -518,7 +520,7 @@ __device__ __forceinline__ void Begin(const AttnArgs& a, const RowSet& set, Stat
 #pragma unroll
     for (uint32_t c = 0; c < D / 16; ++c) w.o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  w.large = false;
+  w.large = w.far = false;
   w.see_all = min(span.total - span.count + (int32_t)(set.row0 / set.group), span.total - 1);
   w.see_from = SightOf<F>(span, set.last / set.group, true, a.window, 0).lo;
   w.see_pre = LeadOf<F>(span, set.row0 / set.group, a.sinks);
@@ -576,13 +578,6 @@ __device__ __forceinline__ void Scores(const Record<F, D>& r, const Rows<F, part
           s[t][tile] = Product(k, w.q[t][p][i], s[t][tile]);
     }
   }
-  if constexpr (F::Parts(parts) != parts) {  // K's codes went in without their scale
-    const float scale = Scale8(r.scales & 255u);
-#pragma unroll
-    for (uint32_t t = 0; t < R; ++t)
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) s[t][j / 4][j % 4] *= scale;
-  }
 }
 
 // tanh(x).  `fine`: to 2^-23 or so of 1, by the odd series to x^13 where 1 - 2 /
@@ -610,8 +605,8 @@ __device__ __forceinline__ float Tanh(float x) {
 // kPlainCap and the scores so off by 2^-16.
 constexpr float kPlainCap = 64.f;
 template <bool fine, uint32_t R>
-__device__ __forceinline__ void Cap(const AttnArgs& a, f32x4 (&s)[R][2]) {
-  const float in = a.scale / a.cap, out = a.cap * kLog2e;
+__device__ __forceinline__ void Cap(const AttnArgs& a, f32x4 (&s)[R][2], float in) {
+  const float out = a.cap * kLog2e;
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t)
 #pragma unroll
@@ -620,6 +615,15 @@ __device__ __forceinline__ void Cap(const AttnArgs& a, f32x4 (&s)[R][2]) {
 }
 __device__ __forceinline__ float PowerOf(const AttnArgs& a) {
   return a.cap > 0.f ? 1.f : a.scale * kLog2e;
+}
+// What a record's keys lack in their products.
+template <uint32_t D>
+__device__ __forceinline__ float KeyScale(const Record<Fp4, D>&) {
+  return 1.f;
+}
+template <uint32_t D>
+__device__ __forceinline__ float KeyScale(const Record<Fp8, D>& r) {
+  return Scale8(r.scales & 255u);
 }
 
 // The record's key of a lane's score j.
@@ -657,7 +661,7 @@ __device__ __forceinline__ void Hide(const State<D, R>& w, int32_t key0, f32x4 (
 
 // The running maximum of tile t moves where a score passes it by kSlack, and
 // what it had so far shrinks.  With `large` it stays kRoom above the scores.
-template <uint32_t D, uint32_t R>
+template <bool any_score, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
                                       bool large) {
   const float top = c * MaxOf8(s);
@@ -668,6 +672,8 @@ __device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&
   // rows that have seen nothing yet stay at -inf, with o and l zero
   const float shrink = m == w.m[t] ? 1.f : __builtin_amdgcn_exp2f(w.m[t] - m);
   w.m[t] = m;
+  if (any_score)
+    w.far |= __builtin_amdgcn_ballot_w64(fabsf(m) > 0x1p20f && fabsf(m) < __builtin_inff()) != 0;
   w.l[t] *= shrink;
 #pragma unroll
   for (uint32_t i = 0; i < D / 16; ++i) w.o[t][i] *= shrink;
@@ -678,15 +684,27 @@ __device__ __forceinline__ float Reference(float m) {
 }
 // The record's weights and their sum.  They carry 2^kLift: at most 2^15, and in
 // f16 normal down to 2^-21 of the reference, off by 2^-32 of it below that.
-template <uint32_t D, uint32_t R>
+// With `any_score` a row whose maximum passes 2^20 takes its scores as the maximum
+// took them, rounded, so that the largest is not 2^(half a step of the maximum)
+// of what it should be.
+template <bool any_score, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Weights(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
                                         float* p) {
   const float ref = Reference(w.m[t]);
   float sum = 0.f;
+  if (any_score && __builtin_expect(w.far, 0)) {
+    const float m = w.m[t] == -__builtin_inff() ? 0.f : w.m[t];
 #pragma unroll
-  for (uint32_t j = 0; j < 8; ++j) {
-    p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], c, ref));
-    sum += p[j];
+    for (uint32_t j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f((s[j / 4][j % 4] * c - m) + kLift);
+      sum += p[j];
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], c, ref));
+      sum += p[j];
+    }
   }
   w.l[t] += sum;
 }
@@ -762,10 +780,13 @@ __device__ __forceinline__ bool Unusual(const KvSpan& span, Record<Fp8, D>& r, i
 template <class F, uint32_t parts, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<F, D>& r,
                                      int32_t key0, f32x4 (&s)[R][2], Rows<F, parts, D, R>& w) {
-  const float c = PowerOf(a);
+  float c = PowerOf(a);
   if (a.cap > 0.f) {
-    if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s);
-    else Cap<false, R>(a, s);
+    const float in = a.scale / a.cap * KeyScale(r);
+    if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s, in);
+    else Cap<false, R>(a, s, in);
+  } else {
+    c *= KeyScale(r);
   }
   constexpr bool half = parts < 3;
   bool wide = Unusual<half>(span, r, key0, s, static_cast<State<D, R>&>(w));
@@ -777,8 +798,8 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
     float p[8];
-    Raise<D, R>(w, t, s[t], c, w.large);
-    Weights<D, R>(w, t, s[t], c, p);
+    Raise<F::kAnyScore>(static_cast<State<D, R>&>(w), t, s[t], c, w.large);
+    Weights<F::kAnyScore>(static_cast<State<D, R>&>(w), t, s[t], c, p);
     if constexpr (half) {
       if (wide) {  // V in bf16, on two bf16 parts of a weight
         bf16x8 part[2];

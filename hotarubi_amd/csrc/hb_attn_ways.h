@@ -238,7 +238,7 @@ __device__ __forceinline__ uint32_t Stored(const AttnArgs& a) {
 // card holds.  Two of them a CU (their rings fill its LDS), so 256 registers a
 // wave where those do.
 template <class F, uint32_t parts, uint32_t D, uint32_t R, Mode mode>
-__global__ __launch_bounds__(kThreads, D == 256 && parts > 1 ? 1 : 2) void AttnKernel(
+__global__ __launch_bounds__(kThreads, D == 256 && F::Parts(parts) > 1 ? 1 : 2) void AttnKernel(
     const AttnArgs a) {
   typedef attn::Ring<F, D> Ring;
   constexpr uint32_t kRing = kWaves * Ring::kDepth * Ring::kSlot;
@@ -413,13 +413,15 @@ Division ByPrompt(const Sizes& z, uint64_t tile, uint64_t opened) {
               (double)opened / 4e6};
 }
 
+template <class F>
 Division ByWaves(const Sizes& z, Division::Way way, uint32_t tiles_of_16) {
   // us a record of a wave by itself on its SIMD, by type, tiles and head size
   const double alone[3][2][3] = {{{0.72, 0.95, 1.25}, {0.95, 1.35, 0}},
                                  {{0.76, 1.05, 1.5}, {1.05, 1.5, 0}},
                                  {{0.8, 1.15, 1.85}, {1.15, 1.6, 0}}};
   // (one workgroup a CU where its waves take more than 256 registers)
-  const double slots = z.dim == 256 && z.parts > 1 ? (double)z.cus : 2.0 * (double)z.cus;
+  const double slots =
+      z.dim == 256 && F::Parts(z.parts) > 1 ? (double)z.cus : 2.0 * (double)z.cus;
   const uint32_t d = z.dim == 64 ? 0 : z.dim == 128 ? 1 : 2;
   const uint64_t tiles = (z.rows + 16 * tiles_of_16 - 1) / (16 * tiles_of_16);
   const uint64_t units =
@@ -467,14 +469,14 @@ Division Divide(const AttnArgs& a) {
   z.mean = mean;
   z.bytes = 2.0 * std::min<double>(a.tokens, (double)a.batch * a.max_new) * a.q_heads * a.dim *
             (z.parts == 3 ? 4 : 2);
-  Division best = ByWaves(z, Division::kBySplits, 1);
+  Division best = ByWaves<F>(z, Division::kBySplits, 1);
   const auto take = [&](const Division& d) {
     if (d.us < best.us) best = d;
   };
-  if (z.rows > 16 * (kWaves - 1)) take(ByWaves(z, Division::kByRows, 1));
+  if (z.rows > 16 * (kWaves - 1)) take(ByWaves<F>(z, Division::kByRows, 1));
   if (z.rows > 16 && z.dim < 256) {
-    take(ByWaves(z, Division::kBySplits, 2));
-    if (z.rows > 32 * (kWaves - 1)) take(ByWaves(z, Division::kByRows, 2));
+    take(ByWaves<F>(z, Division::kBySplits, 2));
+    if (z.rows > 32 * (kWaves - 1)) take(ByWaves<F>(z, Division::kByRows, 2));
   }
   if (z.parts < 3 && z.rows > 32 && PromptBytes(a) <= kMostOpened)
     take(ByPrompt(z, PromptRows(z.dim), PromptBytes(a)));

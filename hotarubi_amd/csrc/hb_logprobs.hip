@@ -1,12 +1,11 @@
 // Log probabilities of given tokens, the entropy and the most likely tokens of
 // rows of logits, one pass over them.
 //
-// In powers of two, with c = scale log2 e, M the running maximum times c,
-// d = x c - M, l = sum 2^d and w = sum d 2^d, a token's log probability is
-// (x c - M - log2 l) ln 2 and the entropy (log2 l - w / l) ln 2.  Parts with
-// maxima M1, M2 meet at M = max as l = sum l_i f_i, w = sum (w_i + (M_i - M)
-// l_i) f_i, f_i = 2^(M_i - M).  M is rounded once and used as it is from then
-// on, so that rounding changes no probability.
+// With c = scale log2 e, m the running maximum, t = x - m, l = sum 2^(c t) and
+// w = sum t 2^(c t), a token's log probability is (c t - log2 l) ln 2 and the
+// entropy (log2 l - c w / l) ln 2.  Parts with maxima m1, m2 meet at m = max as
+// l = sum l_i f_i, w = sum (w_i + (m_i - m) l_i) f_i, f_i = 2^(c (m_i - m)).  The
+// difference comes before the product, so that logits of any size have one.
 //
 // The most likely tokens: every lane keeps the maxima of its stretches of the
 // row in LDS.  `top` lanes reach the `top`-th largest of the lanes' maxima, so
@@ -79,26 +78,34 @@ __device__ __forceinline__ float AtLeast(float x, float least) {
   return y;
 }
 
+// What t may be down to in w, where its weight is 0.
+constexpr float kFar = -3e38f;
+
 struct Sums {
-  float m, l, w;  // m: the maximum times c, -inf where nothing was seen
+  float m, l, w;  // m: -inf where nothing was seen
 };
 __device__ __forceinline__ float Reference(float m) { return m == -__builtin_inff() ? 0.f : m; }
-__device__ __forceinline__ Sums Joined(const Sums& a, const Sums& b) {
+// w under a maximum that is `less` further up, f = 2^(c less); in this order no
+// product passes fp32.
+__device__ __forceinline__ float Moved(const Sums& a, float less, float f) {
+  return f == 0.f ? 0.f : a.w * f + fmaxf(less, kFar) * (a.l * f);
+}
+__device__ __forceinline__ Sums Joined(const Sums& a, const Sums& b, float c) {
   Sums y;
   y.m = fmaxf(a.m, b.m);
   const float ref = Reference(y.m);
   // (nothing seen: l and w are 0; two +inf give NaN, as they should)
   const float da = a.m == -__builtin_inff() ? 0.f : a.m - ref;
   const float db = b.m == -__builtin_inff() ? 0.f : b.m - ref;
-  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  const float fa = __builtin_amdgcn_exp2f(c * da), fb = __builtin_amdgcn_exp2f(c * db);
   y.l = a.l * fa + b.l * fb;
-  y.w = (a.w + fmaxf(da, -1e4f) * a.l) * fa + (b.w + fmaxf(db, -1e4f) * b.l) * fb;
+  y.w = Moved(a, da, fa) + Moved(b, db, fb);
   return y;
 }
-__device__ __forceinline__ Sums JoinedOverWave(Sums s) {
+__device__ __forceinline__ Sums JoinedOverWave(Sums s, float c) {
 #pragma unroll
   for (uint32_t d = 1; d < 64; d *= 2)
-    s = Joined(s, Sums{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.w, d)});
+    s = Joined(s, Sums{__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.w, d)}, c);
   return s;
 }
 
@@ -202,11 +209,9 @@ __device__ __forceinline__ void Finish(const LogprobsArgs& a, uint32_t row, cons
                                        Sums s, uint64_t key) {
   const T* const x = static_cast<const T*>(a.logits) + row * a.stride;
   const float c = a.scale * kLog2e, inf = __builtin_inff();
-  // +inf among them, or past what fp32 holds
-  if (s.m == inf) s.l = __builtin_nanf("");
   const float ref = Reference(s.m), log = s.l == 0.f ? 0.f : __builtin_amdgcn_logf(s.l);
   const auto logprob = [&](float logit) {
-    return s.l == 0.f ? -inf : (fmaf(logit, c, -ref) - log) * kLn2;
+    return s.l == 0.f ? -inf : ((logit - ref) * c - log) * kLn2;
   };
   const uint32_t lane = threadIdx.x % 64;
   if (lane == 0) {
@@ -214,7 +219,7 @@ __device__ __forceinline__ void Finish(const LogprobsArgs& a, uint32_t row, cons
       a.logprobs[row] = given.token < 0                     ? 0.f
                         : (uint32_t)given.token >= a.vocab ? __builtin_nanf("")
                                                             : logprob(given.logit);
-    if (a.entropy != nullptr) a.entropy[row] = s.l == 0.f ? 0.f : (log - s.w / s.l) * kLn2;
+    if (a.entropy != nullptr) a.entropy[row] = s.l == 0.f ? 0.f : (log - c * (s.w / s.l)) * kLn2;
   }
   if (a.top == 0) return;
   const uint64_t at = (uint64_t)row * a.top;
@@ -298,7 +303,7 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
   // batches of a stretch
   const uint32_t run = (((batches + kW - 1) / kW) + kStretches - 1) / kStretches;
   Sums s{-__builtin_inff(), 0.f, 0.f};
-  float m = -__builtin_inff(), high = m;
+  float high = -__builtin_inff();
   uint32_t stretch = 0, in = 0;
   const Given<T> given(a, row);
   u32x4 now[kLoads], next[kLoads];
@@ -316,24 +321,22 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
 #pragma unroll
       for (uint32_t j = 0; j < P::kCount; j += 2)
         top = Max3(top, P::At(now[u], j), P::At(now[u], j + 1));
-    if (top > m) {
-      const float to = top * c, less = s.m - to;
-      m = top;
+    if (top > s.m) {
       if (s.m != -__builtin_inff()) {
-        const float f = __builtin_amdgcn_exp2f(less);
-        s.w = (s.w + fmaxf(less, -1e4f) * s.l) * f;
+        const float less = s.m - top, f = __builtin_amdgcn_exp2f(c * less);
+        s.w = Moved(s, less, f);
         s.l *= f;
       }
-      s.m = to;
+      s.m = top;
     }
     const float ref = Reference(s.m);
 #pragma unroll
     for (uint32_t u = 0; u < kLoads; ++u)
 #pragma unroll
       for (uint32_t j = 0; j < P::kCount; ++j) {
-        const float d = fmaf(P::At(now[u], j), c, -ref), p = __builtin_amdgcn_exp2f(d);
+        const float t = P::At(now[u], j) - ref, p = __builtin_amdgcn_exp2f(c * t);
         s.l += p;
-        s.w = fmaf(p, AtLeast(d, -1e4f), s.w);
+        s.w = fmaf(p, AtLeast(t, kFar), s.w);
       }
     if (a.top > 0) {
       high = fmaxf(high, top);
@@ -349,7 +352,7 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
   }
   uint64_t list = 0;
   if (a.top > 0) {
-    uint32_t least = Reached(OrderOf(m), a.top);
+    uint32_t least = Reached(OrderOf(s.m), a.top);
     // a signalling NaN may have hidden what came before it from a maximum
     bool all = __builtin_amdgcn_ballot_w64(s.l != s.l) != 0;
     if (kW > 1) {
@@ -426,13 +429,13 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
     }
     if (waiting > 0) take_keys();
   }
-  s = JoinedOverWave(s);
+  s = JoinedOverWave(s, c);
   if (kW > 1) {
     if (lane == 0) sums[wave] = s;
     __syncthreads();  // the maxima have been read
     if (lane < a.top) lds.lists[0][wave * a.top + lane] = list;
     __syncthreads();
-    s = Joined(Joined(sums[0], sums[1]), Joined(sums[2], sums[3]));
+    s = Joined(Joined(sums[0], sums[1], c), Joined(sums[2], sums[3], c), c);
     const uint64_t* const best = Merged(lds.lists[0], lds.lists[1], kWaves, a.top);
     if (wave > 0) return;
     list = lane < a.top ? best[lane] : 0;
@@ -466,7 +469,7 @@ __global__ __launch_bounds__(kThreads) void JoinKernel(const LogprobsArgs a) {
       s = Sums{__uint_as_float((uint32_t)x[0]), __uint_as_float((uint32_t)(x[0] >> 32)),
                __uint_as_float((uint32_t)x[1])};
     }
-    s = JoinedOverWave(s);
+    s = JoinedOverWave(s, a.scale * kLog2e);
     if (tid == 0) sums = s;
   }
   __syncthreads();

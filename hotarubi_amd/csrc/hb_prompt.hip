@@ -85,8 +85,9 @@ template <uint32_t parts, uint32_t D>
 __device__ __forceinline__ uint32_t Readied(Record<Fp8, D>& r, int32_t key0, int32_t total) {
   if (key0 + 32 > total) DropPast(r, key0, total);
   uint32_t outside = OutsideHalf8(r.scales >> 8);
-  if (parts == 2) outside |= OutsideHalf8(r.scales & 255u);
-  return outside;
+  // K's: f16, or what products of bf16 do not pass fp32 with
+  const uint32_t k = r.scales & 255u;
+  return outside | (parts == 2 ? OutsideHalf8(k) : k != 0 && k - 64u > 126u);
 }
 // K's operand for token tile `tile` and step e, with its scale.
 template <uint32_t parts, uint32_t D>
@@ -399,14 +400,14 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
           for (uint32_t t = 0; t < R; ++t) s[t][k] = Product(x, q[t][e], s[t][k]);
         }
       const float c = PowerOf(a);
-      if (a.cap > 0.f) Cap<fine, R>(a, s);
+      if (a.cap > 0.f) Cap<fine, R>(a, s, a.scale / a.cap);
       Hide<D, R>(w, key0, s);
       f16x8 pt[R];
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t) {
         float p[8];
-        Raise<D, R>(w, t, s[t], c, false);  // (V is within f16 here)
-        Weights<D, R>(w, t, s[t], c, p);
+        Raise<F::kAnyScore>(w, t, s[t], c, false);  // (V is within f16 here)
+        Weights<F::kAnyScore>(w, t, s[t], c, p);
         pt[t] = HalfWeights(p);
       }
 #pragma unroll
