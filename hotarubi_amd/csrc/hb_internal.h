@@ -526,7 +526,9 @@ struct CompactArgs {
   int32_t *table_out, *free_pages, *free_count, *pairs, *status;
   uint32_t batch, columns, table_stride, table_out_stride, page, pages, free_size,
       pair_count;
-  uint32_t* place;  // set by the launcher
+  // set by the launcher: whether the lists are short, and where what was found
+  // lies if not
+  uint32_t* found;
   uint32_t whole;
 };
 hipError_t LaunchCompact(const CompactArgs& a, Workspace& ws, hipStream_t stream);

@@ -183,33 +183,47 @@ __global__ __launch_bounds__(kCopyThreads) void CopyKernel(const CopyArgs a) {
 
 constexpr uint32_t kMarkThreads = 1024, kMarkWords = kMostPages / 32;
 
-// mark(page, row) for every entry of a row's pages.  A wave takes rows kWaves
+// mark(page, kind) for every entry of a row's pages; which(row), a row a lane, is
+// the ballot of the rows' kinds.  A wave takes rows kMarkWaves
 // apart, the lengths of 64 of them at once and then the entries of kEach of them,
 // as loads that wait for one another are what this takes: 512 rows of 8 to 55
 // pages 14.5 us with four entries a thread at a time, one length each.
-template <class Mark>
+constexpr uint32_t kMarkWaves = kMarkThreads / 64;
+// The length of the lane's row among the wave's first 64, which a kernel asks for
+// before anything else.
+__device__ __forceinline__ int32_t FirstLength(const int32_t* lens, uint32_t batch) {
+  const uint32_t mine = threadIdx.x / 64 + threadIdx.x % 64 * kMarkWaves;
+  return mine < batch ? lens[mine] : 0;
+}
+template <class Which, class Mark>
 __device__ __forceinline__ void EachEntry(const int32_t* table, const int32_t* lens,
-                                          uint32_t batch, uint32_t columns, uint32_t stride,
-                                          uint32_t page, uint32_t pages, Mark&& mark) {
-  constexpr uint32_t kWaves = kMarkThreads / 64, kEach = 16;
+                                          int32_t first_length, uint32_t batch, uint32_t columns,
+                                          uint32_t stride, uint32_t page, uint32_t pages,
+                                          Which&& which, Mark&& mark) {
+  constexpr uint32_t kWaves = kMarkWaves, kEach = 16;
   const uint32_t lane = threadIdx.x % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   for (uint64_t base = wave; base < batch; base += 64 * kWaves) {
     const uint64_t mine = base + (uint64_t)lane * kWaves;
-    const uint32_t of = mine < batch ? min(columns, PagesOf(lens[mine], page)) : 0u;
-    uint32_t rows = (uint32_t)min((uint64_t)64, (batch - base + kWaves - 1) / kWaves);
+    const int32_t length = base == wave ? first_length : mine < batch ? lens[mine] : 0;
+    const uint32_t of = min(columns, PagesOf(length, page));
+    const uint32_t rows = (uint32_t)min((uint64_t)64, (batch - base + kWaves - 1) / kWaves);
+    const uint64_t marks = which(mine);
     for (uint32_t r = 0; r < rows; r += kEach) {
       uint32_t entry[kEach];
 #pragma unroll
       for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)of, (int)((r + j) % 64));
         entry[j] = 0xFFFFFFFFu;
-        if (r + j < rows && lane < n)
+        if (r + j >= rows) continue;  // (the same in all lanes)
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)of, (int)(r + j));
+        if (lane < n)
           entry[j] = (uint32_t)table[(base + (uint64_t)(r + j) * kWaves) * stride + lane];
       }
 #pragma unroll
-      for (uint32_t j = 0; j < kEach; ++j)
-        if (entry[j] < pages) mark(entry[j], (uint32_t)(base + (r + j) * kWaves));
+      for (uint32_t j = 0; j < kEach; ++j) {
+        if (r + j >= rows) continue;
+        if (entry[j] < pages) mark(entry[j], marks >> (r + j) & 1u);
+      }
     }
     for (uint32_t r = 0; r < rows; ++r) {  // what is past 64 pages of a row
       const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)of, (int)r);
@@ -223,7 +237,7 @@ __device__ __forceinline__ void EachEntry(const int32_t* table, const int32_t* l
         }
 #pragma unroll
         for (uint32_t j = 0; j < kEach; ++j)
-          if (entry[j] < pages) mark(entry[j], (uint32_t)row);
+          if (entry[j] < pages) mark(entry[j], marks >> r & 1u);
       }
     }
   }
@@ -235,25 +249,33 @@ __global__ __launch_bounds__(kMarkThreads) void FreeKernel(const FreeArgs a) {
   __shared__ uint32_t kept[kMarkWords], gone[kMarkWords], ends[kMostForkRows / 32];
   __shared__ uint32_t part[kMarkThreads / 64];
   const uint32_t tid = threadIdx.x, words = (a.pages + 31) / 32;
+  // what is most often all of the lists, before anything waits
+  const int32_t length = FirstLength(a.lens, a.batch);
+  const uint32_t end0 = tid < a.count ? (uint32_t)a.rows[tid] : ~0u;
+  const uint32_t free0 = tid < a.free_size ? (uint32_t)a.free_pages[tid] : ~0u;
+  const int32_t len0 = tid < a.batch ? a.lens[tid] : 0;
+  const uint32_t free_count = (uint32_t)max(0, min(*a.free_count, (int32_t)a.free_size));
   for (uint32_t i = tid; i < words; i += kMarkThreads) kept[i] = gone[i] = 0;
   for (uint32_t i = tid; i < (a.batch + 31) / 32; i += kMarkThreads) ends[i] = 0;
   __syncthreads();
   for (uint32_t i = tid; i < a.count; i += kMarkThreads) {
-    const uint32_t r = (uint32_t)a.rows[i];
+    const uint32_t r = i == tid ? end0 : (uint32_t)a.rows[i];
     if (r < a.batch) atomicOr(&ends[r / 32], 1u << (r % 32));
   }
-  const uint32_t free_count = (uint32_t)max(0, min(*a.free_count, (int32_t)a.free_size));
   for (uint32_t i = tid; i < free_count; i += kMarkThreads) {
-    const uint32_t p = (uint32_t)a.free_pages[i];
+    const uint32_t p = i == tid ? free0 : (uint32_t)a.free_pages[i];
     if (p < a.pages) atomicOr(&kept[p / 32], 1u << (p % 32));
   }
   __syncthreads();
   for (uint32_t i = tid; i < a.batch; i += kMarkThreads)
-    a.lens_out[i] = ends[i / 32] >> (i % 32) & 1u ? 0 : a.lens[i];
-  EachEntry(a.table, a.lens, a.batch, a.columns, a.table_stride, a.page, a.pages,
-            [&](uint32_t p, uint32_t row) {
-              uint32_t* const in = ends[row / 32] >> (row % 32) & 1u ? gone : kept;
-              atomicOr(&in[p / 32], 1u << (p % 32));
+    a.lens_out[i] = ends[i / 32] >> (i % 32) & 1u ? 0 : i == tid ? len0 : a.lens[i];
+  EachEntry(a.table, a.lens, length, a.batch, a.columns, a.table_stride, a.page, a.pages,
+            [&](uint64_t row) {
+              return __builtin_amdgcn_ballot_w64(
+                  row < a.batch && (ends[row / 32] >> (row % 32) & 1u) != 0);
+            },
+            [&](uint32_t p, bool ended) {
+              atomicOr((ended ? gone : kept) + p / 32, 1u << (p % 32));
             });
   __syncthreads();
   // the highest page first: thread 0 takes the last words
@@ -282,83 +304,112 @@ __global__ __launch_bounds__(kMarkThreads) void FreeKernel(const FreeArgs a) {
   }
 }
 
-// The tables' new numbers, and what is left of the lists.
-__device__ __forceinline__ void Renumber(const CompactArgs& a, uint32_t count, uint32_t moved,
-                                         uint32_t first, uint32_t step) {
+// The pages in use: a bit each, and the number of them before each word.
+struct Used {
+  uint32_t bits[kMarkWords], before[kMarkWords];
+  __device__ __forceinline__ bool Has(uint32_t p) const { return bits[p / 32] >> (p % 32) & 1u; }
+  __device__ __forceinline__ uint32_t Rank(uint32_t p) const {
+    return before[p / 32] + (uint32_t)__builtin_popcount(bits[p / 32] & ((1u << (p % 32)) - 1u));
+  }
+  // The unused page that `r` unused ones come before (there is one).
+  __device__ __forceinline__ uint32_t Hole(uint32_t r, uint32_t words) const {
+    uint32_t lo = 0, hi = words - 1;  // the last word that at most r come before
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi + 1) / 2;
+      if (mid * 32 - before[mid] <= r) lo = mid;
+      else hi = mid - 1;
+    }
+    uint32_t left = r - (lo * 32 - before[lo]), unused = ~bits[lo], at = 0;
+#pragma unroll
+    for (uint32_t half = 16; half > 0; half /= 2) {
+      const uint32_t n = (uint32_t)__builtin_popcount(unused & ((1u << half) - 1u));
+      if (left >= n) {
+        left -= n;
+        unused >>= half;
+        at += half;
+      }
+    }
+    return lo * 32 + at;
+  }
+};
+
+// Of `count` pages in use the `stay` below it keep their numbers; the others take
+// those of the holes below it, each by its rank: the table, the pairs and the
+// list of free pages, an entry a thread.
+__device__ __forceinline__ void Renumber(const CompactArgs& a, const Used& used, uint32_t count,
+                                         uint32_t stay, uint32_t first, uint32_t step) {
+  const uint32_t words = (a.pages + 31) / 32;
   for (uint32_t i = first; i < a.batch * a.columns; i += step) {  // below 2^31
     const uint32_t row = i / a.columns, col = i % a.columns;
     const uint32_t p = (uint32_t)a.table[(uint64_t)row * a.table_stride + col];
     int32_t to = -1;
     if (p < a.pages && col < PagesOf(a.lens[row], a.page))
-      to = p < count ? (int32_t)p : a.pairs[2 * (uint64_t)a.place[p] + 1];
+      to = (int32_t)(p < count ? p : used.Hole(used.Rank(p) - stay, words));
     a.table_out[(uint64_t)row * a.table_out_stride + col] = to;
   }
+  for (uint64_t p = count + first; p < a.pages; p += step) {
+    if (!used.Has((uint32_t)p)) continue;
+    const uint32_t i = used.Rank((uint32_t)p) - stay;
+    a.pairs[2 * (uint64_t)i] = (int32_t)p;
+    a.pairs[2 * (uint64_t)i + 1] = (int32_t)used.Hole(i, words);
+  }
+  for (uint64_t i = 2ull * (count - stay) + first; i < 2ull * a.pair_count; i += step)
+    a.pairs[i] = -1;
   for (uint64_t i = first; i < a.free_size; i += step)
     a.free_pages[i] = i < a.pages - count ? (int32_t)(a.pages - 1 - (uint32_t)i) : -1;
-  for (uint64_t i = 2ull * moved + first; i < 2ull * a.pair_count; i += step) a.pairs[i] = -1;
-}
-__global__ __launch_bounds__(256) void RenumberKernel(const CompactArgs a) {
-  Renumber(a, (uint32_t)a.status[0], (uint32_t)a.status[1], blockIdx.x * 256 + threadIdx.x,
-           gridDim.x * 256);
 }
 
-// The pages in use, their ranks, and the pairs; `place` says for a page that
-// moves which pair is its.  `whole`: the tables and lists too.
+// One workgroup finds the pages in use and, where the lists are short (`whole`),
+// renumbers them too; else it leaves what it found in the workspace for as many
+// workgroups as the lists want.
 __global__ __launch_bounds__(kMarkThreads) void CompactKernel(const CompactArgs a) {
-  __shared__ uint32_t used[kMarkWords], part[kMarkThreads / 64];
-  __shared__ uint32_t before_u;
+  __shared__ Used used;
+  __shared__ uint32_t part[kMarkThreads / 64];
   const uint32_t tid = threadIdx.x, words = (a.pages + 31) / 32;
-  for (uint32_t i = tid; i < words; i += kMarkThreads) used[i] = 0;
+  const int32_t length = FirstLength(a.lens, a.batch);
+  for (uint32_t i = tid; i < words; i += kMarkThreads) used.bits[i] = 0;
   __syncthreads();
-  EachEntry(a.table, a.lens, a.batch, a.columns, a.table_stride, a.page, a.pages,
-            [&](uint32_t p, uint32_t) { atomicOr(&used[p / 32], 1u << (p % 32)); });
+  EachEntry(a.table, a.lens, length, a.batch, a.columns, a.table_stride, a.page, a.pages,
+            [](uint64_t) { return (uint64_t)0; },
+            [&](uint32_t p, bool) { atomicOr(&used.bits[p / 32], 1u << (p % 32)); });
   __syncthreads();
   const uint32_t each = (words + kMarkThreads - 1) / kMarkThreads;
   uint32_t sum = 0, count;
   for (uint32_t j = 0; j < each; ++j) {
     const uint32_t w = tid * each + j;
-    if (w < words) sum += (uint32_t)__builtin_popcount(used[w]);
+    if (w < words) sum += (uint32_t)__builtin_popcount(used.bits[w]);
   }
-  const uint32_t start = BlockSum<kMarkThreads>(sum, part, &count) - sum;
-  // pages in use before `count`: the rank at which the moves begin
-  if (tid == 0) before_u = count;  // (all of them where count is the last page)
-  __syncthreads();
-  uint32_t rank = start;
+  uint32_t rank = BlockSum<kMarkThreads>(sum, part, &count) - sum;
   for (uint32_t j = 0; j < each; ++j) {
     const uint32_t w = tid * each + j;
     if (w >= words) break;
-    if (w == count / 32)
-      before_u = rank + (uint32_t)__builtin_popcount(used[w] & ((1u << (count % 32)) - 1u));
-    rank += (uint32_t)__builtin_popcount(used[w]);
+    used.before[w] = rank;
+    rank += (uint32_t)__builtin_popcount(used.bits[w]);
+    if (!a.whole) {
+      a.found[w] = used.bits[w];
+      a.found[words + w] = used.before[w];
+    }
   }
   __syncthreads();
-  const uint32_t stay = before_u;
-  rank = start;
-  for (uint32_t j = 0; j < each; ++j) {
-    const uint32_t w = tid * each + j;
-    if (w >= words) break;
-    uint32_t hole = w * 32 - rank;  // unused pages before the word
-    for (uint32_t bits = ~used[w]; bits != 0; bits &= bits - 1, ++hole) {
-      const uint32_t p = w * 32 + (uint32_t)__builtin_ctz(bits);
-      if (p >= count) break;
-      a.pairs[2 * (uint64_t)hole + 1] = (int32_t)p;
-    }
-    for (uint32_t bits = used[w]; bits != 0; bits &= bits - 1, ++rank) {
-      const uint32_t p = w * 32 + (uint32_t)__builtin_ctz(bits);
-      if (p < count) continue;
-      a.pairs[2 * (uint64_t)(rank - stay)] = (int32_t)p;
-      a.place[p] = rank - stay;
-    }
-  }
+  const uint32_t stay = count < a.pages ? used.Rank(count) : count;
   if (tid == 0) {
     a.status[0] = (int32_t)count;
     a.status[1] = (int32_t)(count - stay);
     *a.free_count = (int32_t)(a.pages - count);
   }
-  if (a.whole == 0) return;
-  __threadfence_block();
+  if (a.whole) Renumber(a, used, count, stay, tid, kMarkThreads);
+}
+__global__ __launch_bounds__(kMarkThreads) void RenumberKernel(const CompactArgs a) {
+  __shared__ Used used;
+  const uint32_t words = (a.pages + 31) / 32;
+  for (uint32_t w = threadIdx.x; w < words; w += kMarkThreads) {
+    used.bits[w] = a.found[w];
+    used.before[w] = a.found[words + w];
+  }
+  const uint32_t count = (uint32_t)a.status[0], stay = count - (uint32_t)a.status[1];
   __syncthreads();
-  Renumber(a, count, count - stay, tid, kMarkThreads);
+  Renumber(a, used, count, stay, blockIdx.x * kMarkThreads + threadIdx.x,
+           gridDim.x * kMarkThreads);
 }
 
 }  // namespace
@@ -389,16 +440,22 @@ hipError_t LaunchFree(const FreeArgs& a, hipStream_t stream) {
 
 hipError_t LaunchCompact(const CompactArgs& in, Workspace& ws, hipStream_t stream) {
   CompactArgs a = in;
-  const hipError_t err = GrowWorkspace(ws, (size_t)a.pages * 4, stream);
-  if (err != hipSuccess) return err;
-  a.place = reinterpret_cast<uint32_t*>(ws.ptr + kSplitCounters);
-  // Small lists in the same launch: 16,384 numbers are 16 a thread.
+  // Short lists in the same launch: 16,384 numbers are 16 a thread (two of eight
+  // requests end, 18.4 us a pass for 21.5).
   const uint64_t numbers = (uint64_t)a.batch * a.columns + a.free_size + 2ull * a.pair_count;
   a.whole = numbers <= 16384;
+  if (!a.whole) {
+    const size_t words = (a.pages + 31) / 32;
+    const hipError_t err = GrowWorkspace(ws, 2 * words * sizeof(uint32_t), stream);
+    if (err != hipSuccess) return err;
+    a.found = reinterpret_cast<uint32_t*>(ws.ptr + kSplitCounters);
+  }
   CompactKernel<<<1, kMarkThreads, 0, stream>>>(a);
-  if (a.whole) return hipGetLastError();
-  const uint64_t most = std::max<uint64_t>((uint64_t)a.batch * a.columns, a.free_size);
-  RenumberKernel<<<(uint32_t)std::min<uint64_t>(1024, (most + 255) / 256), 256, 0, stream>>>(a);
+  if (!a.whole) {
+    const uint64_t groups = (numbers + kMarkThreads - 1) / kMarkThreads;
+    RenumberKernel<<<(uint32_t)std::min<uint64_t>((uint64_t)DeviceCus(), groups), kMarkThreads, 0,
+                     stream>>>(a);
+  }
   return hipGetLastError();
 }
 
