@@ -435,7 +435,8 @@ Division ByWaves(const Sizes& z, Division::Way way, uint32_t tiles_of_16) {
   const double groups = (double)(units * splits);
   const double beside =
       std::min(slots / (double)z.cus - 1, std::max(0.0, groups / (double)z.cus - 1));
-  const double record = alone[z.parts - 1][tiles_of_16 - 1][d] *
+  const double format = way == Division::kBySplits ? F::kSplitRecord : 1.0;
+  const double record = format * alone[z.parts - 1][tiles_of_16 - 1][d] *
                         (1 + beside * (d == 2 ? 0.5 : 0.35));
   const double share = way == Division::kByRows ? 1 : 1.0 / (double)(kWaves * splits);
   return {way, tiles_of_16, splits,
