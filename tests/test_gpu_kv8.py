@@ -5,10 +5,11 @@ every way of dividing attention's work.
 Tolerances.  Rows: none, the stored values are whole codes times a power of
 two.  Attention, of a row with weights p and A = sum p |v|: the output's
 rounding; 2 ds A for scores off by ds (the products' sum over dim terms and the
-few operations after it, dim + 8 roundings of 2^-24); the weights' own rounding
-(2^-11 A in f16 for the 16-bit types, none for fp32) or 2^-32 of the largest
-value a key; 2^-24 A a term, twice, for the sums over the keys; 2^-21 A for
-exponentials and the division; caps 2^-21 of the cap on a score."""
+few operations after it, dim + 8 roundings of 2^-24, and of fp32 queries 2^-133
+an element, where bf16 ends); the weights' own rounding (2^-11 A in f16 for the
+16-bit types, none for fp32) or 2^-32 of the largest value a key; 2^-24 A a
+term, twice, for the sums over the keys; 2^-21 A for exponentials and the
+division; caps 2^-21 of the cap on a score."""
 from __future__ import annotations
 
 import math
@@ -282,6 +283,8 @@ def reference(s, scale, window, sinks, cap):
                 x = q[rows, g].double()
                 sc = x @ k.T.contiguous() * scale
                 ds = (d + 8) * 2.0**-24 * (x.abs() @ k.abs().T.contiguous() * abs(scale))
+                if not half:  # bf16 parts end at its last step, 2^-133: that much of an element
+                    ds = ds + 2.0**-133 * k.abs().sum(-1) * abs(scale)
                 if cap:
                     sc = cap * torch.tanh(sc / cap)
                     ds = ds + cap * 2.0**-21
