@@ -107,11 +107,16 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
     uint8_t* const to = g.cache + (record + (uint64_t)head * g.groups) * Kv8RecordBytes(dim);
     const uint32_t had = t0 > 0 ? *reinterpret_cast<const uint16_t*>(to + Kv8Scale(dim, 0)) : 0;
     float k[kRows][4], v[kRows][4];
+    // a whole block's thread has tokens that are neighbours, whose V codes are
+    // too; of a few tokens every group of threads has some
+    const auto token = [&](uint32_t i) {
+      return count == 32 ? group * kRows + i : i * kGroups + group;
+    };
 #pragma unroll
     for (uint32_t i = 0; i < kRows; ++i) {
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) k[i][j] = v[i][j] = 0.f;
-      const uint32_t t = group * kRows + i;
+      const uint32_t t = token(i);
       if (t >= count) continue;
       const uint64_t r = row + t;
       Load4(static_cast<const T*>(g.k) + r * g.k_token + head * g.k_head + col, g.vec, k[i]);
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
       }
 #pragma unroll
       for (uint32_t i = 0; i < kRows; ++i) {
-        const uint32_t t = group * kRows + i;
+        const uint32_t t = token(i);
         if (t >= count) continue;
         const uint32_t codes = Codes(k[i][0] * ku, k[i][1] * ku, k[i][2] * ku, k[i][3] * ku);
         *reinterpret_cast<uint32_t*>(to + Kv8KCode(dim, t0 + t, col)) =
