@@ -12,6 +12,13 @@
 // that (its upper 16 bits) is a bound, and only stretches that reach it are read
 // again, all at once; their logits go into a list of sorted 64-bit keys, one a
 // lane, 64 of them at a time.
+//
+// About 10 vector instructions a logit, four of an exponential's slots among them,
+// for 2 or 4 bytes: memory bounds long rows, 4,096 of 65,537 bf16 logits with the 5
+// likeliest 115 us = 4.7 TB/s (a reading of them once at what the card copies at
+// is 105; without the likeliest tokens 105), 2,048 of 65,537 in fp32 107 us = 5.0.
+// Of short calls the waves' chain does: 8 rows of 50,001 fp32 logits, 20 each,
+// 8.8 us and 4.6 for the join.
 #include <algorithm>
 
 #include "hb_internal.h"
