@@ -86,7 +86,7 @@ template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
   constexpr uint32_t kRow = dim / 4, kGroups = kThreads / kRow, kRows = 32 / kGroups;
   __shared__ __align__(16) uint8_t image[64 * dim];
-  __shared__ uint32_t tops[kWaves][2];
+  __shared__ uint32_t tops[kWaves][2], scales;
   const uint32_t tid = threadIdx.x, lane = tid % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const uint32_t head = blockIdx.x % g.heads;
@@ -108,7 +108,8 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
     const uint32_t count = 1 + (uint32_t)__builtin_ctzll(~(on >> (l + 1)));
     (void)KvSlot(__builtin_amdgcn_readlane(slot, (int)l), g.pages, g.heads, g.groups, &record, &t0);
     uint8_t* const to = g.cache + (record + (uint64_t)head * g.groups) * Kv8RecordBytes(dim);
-    const uint32_t had = t0 > 0 ? *reinterpret_cast<const uint16_t*>(to + Kv8Scale(dim, 0)) : 0;
+    uint32_t had = 0;  // one thread's, so that all see the same whatever others write
+    if (tid == 0 && t0 > 0) had = *reinterpret_cast<const uint16_t*>(to + Kv8Scale(dim, 0));
     float k[kRows][4], v[kRows][4];
     // a whole block's thread has tokens that are neighbours, whose V codes are
     // too; of a few tokens every group of threads has some
@@ -152,7 +153,9 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
       tops[wave][0] = k_top;
       tops[wave][1] = v_top;
     }
+    if (tid == 0) scales = had;
     __syncthreads();
+    had = scales;
 #pragma unroll
     for (uint32_t w = 0; w < kWaves; ++w) {
       k_top = max(k_top, tops[w][0]);
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
     }
     if (tid == 0)
       *reinterpret_cast<uint16_t*>(to + Kv8Scale(dim, 0)) = (uint16_t)(ks | vs << 8);
-    __syncthreads();  // image and tops have been read
+    __syncthreads();  // image, tops and scales have been read
   }
 }
 

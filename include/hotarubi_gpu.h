@@ -754,7 +754,8 @@ int hb_kv_attention_way(const hb_kv_attention_desc* desc, hb_kv_way* way);
  * grows; values are rounded to nearest even (past 448 x 2^119: to that).  A
  * token's head with an infinity or NaN in K or V is stored as NaN keys and
  * zero values and moves no scale.  A slot below 0 or past the cache's pages
- * is not written and ends a run.  A call brings each block at most one run.
+ * is not written and ends a run.  A call brings each block at most one run
+ * (what a block holds after two is not said; no other one is touched).
  * hb_kv8_read gives the stored values of slots, zeros where there is none.
  * The descriptors are hb_kv_append's. */
 int hb_kv8_append(hb_ctx* ctx, const hb_kv_rows_desc* desc);

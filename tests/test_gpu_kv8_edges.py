@@ -150,3 +150,19 @@ def test_calls_of_different_sizes_in_turn():
             assert int(count) == pages - 2000 and status.tolist() == [2000, len(moved)]
     finally:
         ctx.close()
+
+
+def test_two_runs_of_a_block_leave_others_alone(gpu):
+    """A call that brings a block several runs, its slots backwards or twice over:
+    what the block holds is not said, but the call ends and no other block's bytes
+    change."""
+    say("two runs of a block")
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    for slots in ([70, 69, 68, 67, 66], [64] * 40, [65, 66, 64, 65, 95, 94],
+                  list(range(95, 63, -1)) * 20):
+        cache = torch.full(hb.kv8_cache_shape(3, 4, 64, 128), 11, dtype=torch.uint8, device=DEV)
+        k, v = (torch.randn((len(slots), 4, 128), generator=gen, device=DEV) for _ in range(2))
+        hb.kv8_append(k=k, v=v, slots=ints(slots), cache=cache, ctx=gpu)
+        assert (cache[1, :, 0] != 11).any()
+        cache[1, :, 0] = 11
+        assert (cache == 11).all()
