@@ -186,11 +186,6 @@ __global__ __launch_bounds__(kCopyThreads) void CopyKernel(const CopyArgs a) {
 
 constexpr uint32_t kMarkThreads = 1024, kMarkWords = kMostPages / 32;
 
-// mark(page, kind) for every entry of a row's pages; which(row), a row a lane, is
-// the ballot of the rows' kinds.  A wave takes rows kMarkWaves
-// apart, the lengths of 64 of them at once and then the entries of kEach of them,
-// as loads that wait for one another are what this takes: 512 rows of 8 to 55
-// pages 14.5 us with four entries a thread at a time, one length each.
 constexpr uint32_t kMarkWaves = kMarkThreads / 64;
 // The length of the lane's row among the wave's first 64, which a kernel asks for
 // before anything else.
@@ -198,6 +193,11 @@ __device__ __forceinline__ int32_t FirstLength(const int32_t* lens, uint32_t bat
   const uint32_t mine = threadIdx.x / 64 + threadIdx.x % 64 * kMarkWaves;
   return mine < batch ? lens[mine] : 0;
 }
+// mark(page, kind) for every entry of a row's pages; which(row), a row a lane, is
+// the ballot of the rows' kinds.  A wave takes rows kMarkWaves apart, the lengths
+// of 64 of them at once and then the entries of kEach of them, as loads that wait
+// for one another are what this takes (512 rows of 8 to 55 pages: the compaction's
+// marks 7.8 us, 14.5 with four entries a thread at a time, a length each).
 template <class Which, class Mark>
 __device__ __forceinline__ void EachEntry(const int32_t* table, const int32_t* lens,
                                           int32_t first_length, uint32_t batch, uint32_t columns,

@@ -845,7 +845,7 @@ int hb_kv_copy_async(hb_ctx* ctx, const hb_kv_copy_desc* desc);
  * far as free_size goes.  lens_out is lens, 0 for the rows that end.  status
  * int32 [2]: pages put on the stack, pages that found no room.  *free_count
  * and the table are left as they are: the caller adds status[0] to the count.
- * pages <= 524288. */
+ * pages <= 524288, batch <= 65536. */
 typedef struct hb_kv_free_desc {
   const int32_t* table;
   const int32_t* lens;
