@@ -1499,7 +1499,8 @@ int KvRows(hb_ctx* ctx, const hb_kv_rows_desc* d, bool read, bool sync, bool eig
   if (int rc = CheckType(d->type)) return rc;
   if (int rc = CheckCache(d->cache)) return rc;
   if (d->tokens == 0) return ctx ? HB_OK : Enter(ctx);
-  if ((uint64_t)d->tokens * d->cache.heads > 0x7FFFFFFFu)
+  // (8 bits: 16 rows a workgroup of 256, 2^32 threads)
+  if ((uint64_t)d->tokens * d->cache.heads > (eight ? 0x0FFFFFFFu : 0x7FFFFFFFu))
     return Fail(HB_EINVAL, "%u tokens of %u heads in one call", d->tokens, d->cache.heads);
   if (!d->k || !d->v || !d->slots) return Fail(HB_EINVAL, "null cache row argument");
   const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;
@@ -1677,6 +1678,9 @@ int KvCopy(hb_ctx* ctx, const hb_kv_copy_desc* d, bool sync) {
   if ((unsigned __int128)d->page_bytes * d->pages > (d->layers > 1 ? d->layer_bytes : ~0ull >> 1))
     return Fail(HB_EINVAL, "%u pages of %llu bytes in layers of %llu", d->pages,
                 (unsigned long long)d->page_bytes, (unsigned long long)d->layer_bytes);
+  if ((unsigned __int128)(d->page_bytes / hb::kCopyPiece + 1) * d->layers > 0xFFFFFFu)
+    return Fail(HB_EINVAL, "pages of %llu bytes in %u layers in one call",
+                (unsigned long long)d->page_bytes, d->layers);
   if (int rc = CheckInts({{d->pairs, 2ull * d->count}})) return rc;
   if (d->count == 0 || d->layers == 0 || d->pages == 0 || d->page_bytes == 0)
     return ctx ? HB_OK : Enter(ctx);
@@ -1752,7 +1756,7 @@ int TokenLogprobs(hb_ctx* ctx, const hb_logprobs_desc* d, bool sync) {
   if (!d->logprobs && !d->entropy && d->top == 0)
     return Fail(HB_EINVAL, "no log probabilities asked for");
   if (!d->logits) return Fail(HB_EINVAL, "null logits");
-  if (d->rows > 0x7FFFFFFFu) return Fail(HB_EINVAL, "%u rows", d->rows);
+  if (d->rows > 0xFFFFFFu) return Fail(HB_EINVAL, "%u rows in one call", d->rows);
   const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;
   if (Misaligned(d->logits, size) || Misaligned(d->tokens, 4) || Misaligned(d->logprobs, 4) ||
       Misaligned(d->entropy, 4) || Misaligned(d->top_ids, 4) || Misaligned(d->top_logprobs, 4))

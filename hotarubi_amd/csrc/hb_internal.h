@@ -494,6 +494,7 @@ hipError_t LaunchPrompt(const AttnArgs& a, Workspace& ws, hipStream_t stream);
 hipError_t LaunchPrompt8(const AttnArgs& a, Workspace& ws, hipStream_t stream);
 
 // Pages (hb_pages.hip).
+constexpr uint32_t kCopyPiece = 8192;      // bytes of a page that a workgroup copies at a time
 constexpr uint32_t kMostForkRows = 65536;  // rows of a table whose requests fork or end
 constexpr uint32_t kMostPages = 524288;    // a bit each, twice, in a workgroup's LDS
 struct ForkArgs {

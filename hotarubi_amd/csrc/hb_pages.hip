@@ -147,7 +147,8 @@ __global__ __launch_bounds__(kForkThreads) void ForkKernel(const ForkArgs a) {
 
 // ------------------------------------------------------------------- copy --
 
-constexpr uint32_t kCopyThreads = 256, kCopyPiece = kCopyThreads * 16 * 2;
+constexpr uint32_t kCopyThreads = 256;
+static_assert(kCopyPiece == kCopyThreads * 16 * 2, "two loads a thread");
 
 // A workgroup takes a piece of a page in one layer, for pairs `stripes` apart:
 // it looks at 64 of them at a time, since lists of moves are mostly empty.
@@ -428,7 +429,6 @@ hipError_t LaunchCopy(const CopyArgs& in, hipStream_t stream) {
   CopyArgs a = in;
   a.pieces = (a.page_bytes + kCopyPiece - 1) / kCopyPiece;
   const uint64_t slots = a.pieces * a.layers;
-  if (slots > 0x7FFFFFFFu) return hipErrorInvalidValue;
   // about 8 workgroups a CU, as far as the pairs go
   const uint64_t want = 8 * (uint64_t)DeviceCus();
   a.stripes = (uint32_t)std::min<uint64_t>(a.count, std::max<uint64_t>(1, want / slots));

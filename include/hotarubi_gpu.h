@@ -757,7 +757,7 @@ int hb_kv_attention_way(const hb_kv_attention_desc* desc, hb_kv_way* way);
  * is not written and ends a run.  A call brings each block at most one run
  * (what a block holds after two is not said; no other one is touched).
  * hb_kv8_read gives the stored values of slots, zeros where there is none.
- * The descriptors are hb_kv_append's. */
+ * The descriptors are hb_kv_append's, tokens * heads below 2^28. */
 int hb_kv8_append(hb_ctx* ctx, const hb_kv_rows_desc* desc);
 int hb_kv8_append_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
 int hb_kv8_read(hb_ctx* ctx, const hb_kv_rows_desc* desc);
@@ -829,7 +829,8 @@ int hb_kv_fork_async(hb_ctx* ctx, const hb_kv_fork_desc* desc);
 /* Copies page pairs[i][0] over page pairs[i][1] in each of `layers` caches
  * layer_bytes apart, page_bytes a page (both and the base multiples of 16).  A
  * pair that names no page, or one page twice, is passed over.  No page is
- * written by two pairs or written by one and read by another. */
+ * written by two pairs or written by one and read by another.  A call's layers
+ * have fewer than 2^24 pieces of 8 KB of a page. */
 typedef struct hb_kv_copy_desc {
   void* base;
   const int32_t* pairs; /* [count][2] */
@@ -895,7 +896,7 @@ int hb_kv_compact_async(hb_ctx* ctx, const hb_kv_compact_desc* desc);
  * Maxima and sums are in 32 bits.  tokens and logprobs are null together;
  * entropy may be null; top_ids and top_logprobs are null together and top 0
  * then.  logits is [rows][vocab] of `type`, rows `stride` elements apart; top
- * <= 64 and <= vocab; the others are contiguous.
+ * <= 64 and <= vocab; rows below 2^24; the others are contiguous.
  * Few long rows are split over workgroups that meet in the context's
  * workspace, in a fixed order: results do not change from call to call. */
 typedef struct hb_logprobs_desc {

@@ -321,6 +321,34 @@ def test_c_entry_points_refuse_null_and_misaligned_descriptors():
     says(lib.hb_token_logprobs, logprobs_c(vocab=1 << 31), "tokens")
 
 
+def test_calls_of_more_threads_than_a_launch_has_are_refused():
+    """2^24 workgroups of 256 are 2^32 threads."""
+    lib, at = hb.lib(), 1 << 20
+
+    def says(fn, desc, text):
+        assert fn(None, desc) != hb.HB_OK and text in hb.last_error(), hb.last_error()
+
+    def rows_c(tokens, heads):
+        return hb.KV_ROWS_DESC.pack(at, 9, heads, 64, 256, at, at, heads * 256, 256, heads * 256,
+                                    256, at, hb.HB_TYPE_F16, tokens)
+    for fn in (lib.hb_kv8_append, lib.hb_kv8_read):
+        says(fn, rows_c((1 << 25) - 1, 8), "null context")
+        says(fn, rows_c(1 << 25, 8), "33554432 tokens of 8 heads in one call")
+    for fn in (lib.hb_kv_append, lib.hb_kv_read):
+        says(fn, rows_c(1 << 25, 8), "null context")
+
+    def logprobs_c(rows):
+        return hb.LOGPROBS_DESC.pack(at, 1, at, at, 0, 0, 0, hb.HB_TYPE_F16, rows, 1, 0, 1.0)
+    says(lib.hb_token_logprobs, logprobs_c((1 << 24) - 1), "null context")
+    says(lib.hb_token_logprobs, logprobs_c(1 << 24), "16777216 rows in one call")
+
+    def copy_c(page, layers):
+        return hb.KV_COPY_DESC.pack(at, at, page, 1 << 40, 9, layers, 3)
+    says(lib.hb_kv_copy, copy_c(8192 * 1023 + 16, 16383), "null context")
+    says(lib.hb_kv_copy, copy_c(8192 * 1023 + 16, 16384), "in 16384 layers in one call")
+    says(lib.hb_kv_copy, copy_c(1 << 36, (1 << 32) - 1), "layers in one call")
+
+
 def test_without_a_context_tensors_must_be_on_a_gpu():
     rows = torch.zeros(5, 2, 64)
     for call, name in [
