@@ -148,13 +148,15 @@ __device__ __forceinline__ void WaveFence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The largest order of 16 upper bits that k lanes' each reach, found bit by bit.
-__device__ __forceinline__ uint32_t Reached(uint32_t order, uint32_t k) {
+// The largest order of 16 upper bits that k of the lanes' reach (two a lane), found
+// bit by bit.
+__device__ __forceinline__ uint32_t Reached(uint32_t first, uint32_t second, uint32_t k) {
   uint32_t least = 0;
 #pragma unroll
   for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit /= 2) {
-    const uint64_t there = __builtin_amdgcn_ballot_w64(order >= (least | bit));
-    if ((uint32_t)__builtin_popcountll(there) >= k) least |= bit;
+    const uint64_t one = __builtin_amdgcn_ballot_w64(first >= (least | bit));
+    const uint64_t two = __builtin_amdgcn_ballot_w64(second >= (least | bit));
+    if ((uint32_t)(__builtin_popcountll(one) + __builtin_popcountll(two)) >= k) least |= bit;
   }
   return least;
 }
@@ -378,7 +380,14 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
   }
   uint64_t list = 0;
   if (a.top > 0) {
-    uint32_t least = Reached(OrderOf(s.m), a.top);
+    // the lane's two largest maxima (here, as registers in the loop above are dear)
+    uint32_t first = 0, second = 0;
+    for (uint32_t i = 0; i < stretch; ++i) {
+      const uint32_t one = lds.maxima[wave][i][lane];
+      second = max(second, min(first, one));
+      first = max(first, one);
+    }
+    uint32_t least = Reached(first << 16, second << 16, a.top);
     // a signalling NaN may have hidden what came before it from a maximum
     bool all = __builtin_amdgcn_ballot_w64(s.l != s.l) != 0;
     if (kW > 1) {
