@@ -8,10 +8,10 @@
 // difference comes before the product, so that logits of any size have one.
 //
 // The most likely tokens: every lane keeps the maxima of its stretches of the
-// row in LDS.  `top` logits reach the `top`-th largest of the lanes' two largest
-// maxima, so that (its upper 16 bits) is a bound, and only stretches that reach it
-// are read again, all at once; their logits go into a list of sorted 64-bit keys,
-// one a lane, 64 of them at a time.  (Two, as 64 likeliest tokens want all lanes of
+// row in LDS.  `top` logits reach the `top`-th largest of the lanes' largest or two
+// largest maxima, so that (its upper 16 bits) is a bound, and only stretches that
+// reach it are read again, all at once; their logits go into a list of sorted 64-bit
+// keys, one a lane, 64 of them at a time.  (64 likeliest tokens want all lanes of
 // one each: 200 rows of 100,001 in fp32 64 us, 40 with two.)
 //
 // About 10 vector instructions a logit, four of an exponential's slots among them,
@@ -32,6 +32,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 constexpr uint32_t kLoads = 2;  // 16-byte loads of a lane's batch
 constexpr uint32_t kStretches = 24;
+// Likeliest tokens up to which a lane's largest maximum makes the bound: 2,000 rows
+// of 50,001 bf16 logits with 20 each 51.5 us, 52.1 with two maxima a lane, but with
+// 32 54.3 and 54.0, with 64 108 and 70.
+constexpr uint32_t kOfOne = 24;
 constexpr uint32_t kMostParts = 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -149,14 +153,16 @@ __device__ __forceinline__ void WaveFence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The largest order of 16 upper bits that k of the lanes' reach (two a lane), found
-// bit by bit.
+// The largest order of 16 upper bits that k of the lanes' reach (two a lane, or
+// one), found bit by bit.
+template <bool two_each>
 __device__ __forceinline__ uint32_t Reached(uint32_t first, uint32_t second, uint32_t k) {
   uint32_t least = 0;
 #pragma unroll
   for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit /= 2) {
     const uint64_t one = __builtin_amdgcn_ballot_w64(first >= (least | bit));
-    const uint64_t two = __builtin_amdgcn_ballot_w64(second >= (least | bit));
+    const uint64_t two =
+        two_each ? __builtin_amdgcn_ballot_w64(second >= (least | bit)) : 0;
     if ((uint32_t)(__builtin_popcountll(one) + __builtin_popcountll(two)) >= k) least |= bit;
   }
   return least;
@@ -381,14 +387,19 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
   }
   uint64_t list = 0;
   if (a.top > 0) {
-    // the lane's two largest maxima (here, as registers in the loop above are dear)
-    uint32_t first = 0, second = 0;
-    for (uint32_t i = 0; i < stretch; ++i) {
-      const uint32_t one = lds.maxima[wave][i][lane];
-      second = max(second, min(first, one));
-      first = max(first, one);
+    uint32_t least;
+    if (a.top > kOfOne) {
+      // the lane's two largest maxima (here, as registers in the loop above are dear)
+      uint32_t first = 0, second = 0;
+      for (uint32_t i = 0; i < stretch; ++i) {
+        const uint32_t one = lds.maxima[wave][i][lane];
+        second = max(second, min(first, one));
+        first = max(first, one);
+      }
+      least = Reached<true>(first << 16, second << 16, a.top);
+    } else {
+      least = Reached<false>(OrderOf(s.m), 0, a.top);
     }
-    uint32_t least = Reached(first << 16, second << 16, a.top);
     // a signalling NaN may have hidden what came before it from a maximum
     bool all = __builtin_amdgcn_ballot_w64(s.l != s.l) != 0;
     if (kW > 1) {

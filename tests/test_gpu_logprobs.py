@@ -100,6 +100,22 @@ def test_sizes(gpu, dtype, rows, vocab, top):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,top", [
+    (1100, 1000, 40), (1040, 8000, 64), (4200, 9001, 33), (30, 1025, 25), (300, 3001, 64),
+    (2, 200001, 48)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_many_likeliest(gpu, dtype, rows, vocab, top, ties):
+    """Enough of them that most lanes of a wave have one or two; with ties, that
+    the lowest columns of many equal logits win."""
+    say("logprobs, many likeliest", dtype, rows, vocab, top, ties)
+    gen = torch.Generator(device=DEV).manual_seed(top)
+    x = (torch.randn((rows, vocab), generator=gen, device=DEV) * 2).to(dtype)
+    if ties:
+        x = x.round()
+    check(gpu, x, np.random.default_rng(top).integers(0, vocab, rows).tolist(), top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [6, 1100])
 @pytest.mark.parametrize("vocab", [40, 9001])
 def test_odd_rows(gpu, dtype, rows, vocab):
