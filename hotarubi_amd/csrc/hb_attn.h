@@ -60,8 +60,11 @@ struct Fp4 {
   }
 };
 // E4M3 codes are exact in f16 too, and the scale, one for all keys of the record,
-// goes into what their scores are multiplied by: fp16 queries take one product.
-// Scores of any size that fp32 holds are taken (Weights).
+// may go into what their scores are multiplied by: fp16 queries take one product
+// (2^33 at most).  bf16 and fp32 ones take keys with the part of their scale that
+// is below 1, so that a large query meets small keys and not their codes, and the
+// rest of it later, so that large keys' products do not pass fp32 before a small
+// `scale` has met them.  Scores of any size that fp32 holds are taken (Weights).
 struct Fp8 {
   static constexpr bool kSinks = true, kAnyScore = true;
   // what a record costs a split's wave beside an MXFP4 one: 2 x 1,500 new tokens
@@ -223,14 +226,17 @@ __device__ __forceinline__ u32x4 EightOf(uint32_t lo, uint32_t hi, float scale) 
 __device__ __forceinline__ float Scale8(uint32_t byte) {
   return __uint_as_float((byte == 0 ? 127u : byte) << 23);
 }
+// K's codes with the part of their scale that is below 1 in bf16 (exact: 2^-9 x
+// 2^-117 is normal), bare in f16; KeyScale is the rest.
 template <uint32_t parts, uint32_t D>
 __device__ __forceinline__ typename QueryOperand<Fp8, parts>::type KeyOperand(
     const Record<Fp8, D>& r, uint32_t tile, uint32_t s) {
   const uint32_t piece = tile * (D / 32) + s;  // of 8 bytes
+  const float scale = parts == 2 ? 1.f : Scale8(min(r.scales & 255u, 127u));
   return __builtin_bit_cast(
       typename QueryOperand<Fp8, parts>::type,
       EightOf<parts == 2>(r.k[piece / 2][piece % 2 * 2], r.k[piece / 2][piece % 2 * 2 + 1],
-                          1.f));
+                          scale));
 }
 
 // P V in f16 for the 16-bit types: a weight is off by at most 2^-11 of itself,
@@ -621,14 +627,15 @@ __device__ __forceinline__ void Cap(const AttnArgs& a, f32x4 (&s)[R][2], float i
 __device__ __forceinline__ float PowerOf(const AttnArgs& a) {
   return a.cap > 0.f ? 1.f : a.scale * kLog2e;
 }
-// What a record's keys lack in their products.
-template <uint32_t D>
+// What a record's keys lack in their products (KeyOperand).
+template <uint32_t parts, uint32_t D>
 __device__ __forceinline__ float KeyScale(const Record<Fp4, D>&) {
   return 1.f;
 }
-template <uint32_t D>
+template <uint32_t parts, uint32_t D>
 __device__ __forceinline__ float KeyScale(const Record<Fp8, D>& r) {
-  return Scale8(r.scales & 255u);
+  const uint32_t byte = r.scales & 255u;
+  return Scale8(parts == 2 ? byte : max(byte, 127u));
 }
 
 // The record's key of a lane's score j.
@@ -787,11 +794,11 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
                                      int32_t key0, f32x4 (&s)[R][2], Rows<F, parts, D, R>& w) {
   float c = PowerOf(a);
   if (a.cap > 0.f) {
-    const float in = a.scale / a.cap * KeyScale(r);
+    const float in = a.scale / a.cap * KeyScale<parts>(r);
     if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s, in);
     else Cap<false, R>(a, s, in);
   } else {
-    c *= KeyScale(r);
+    c *= KeyScale<parts>(r);
   }
   constexpr bool half = parts < 3;
   bool wide = Unusual<half>(span, r, key0, s, static_cast<State<D, R>&>(w));

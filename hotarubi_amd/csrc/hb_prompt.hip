@@ -85,9 +85,10 @@ template <uint32_t parts, uint32_t D>
 __device__ __forceinline__ uint32_t Readied(Record<Fp8, D>& r, int32_t key0, int32_t total) {
   if (key0 + 32 > total) DropPast(r, key0, total);
   uint32_t outside = OutsideHalf8(r.scales >> 8);
-  // K's: f16, or what products of bf16 do not pass fp32 with
+  // K's, which go into the operand whole: f16, or keys up to 2^72, that queries
+  // up to 2^48 do not pass fp32 with (the general steps take larger ones apart)
   const uint32_t k = r.scales & 255u;
-  return outside | (parts == 2 ? OutsideHalf8(k) : k != 0 && k - 64u > 126u);
+  return outside | (parts == 2 ? OutsideHalf8(k) : k > 190u);
 }
 // K's operand for token tile `tile` and step e, with its scale.
 template <uint32_t parts, uint32_t D>

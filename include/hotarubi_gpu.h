@@ -767,9 +767,10 @@ int hb_kv8_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * With a window the first `sinks` tokens stay visible to the rows behind
  * them: row at p sees key j (j < kv_lens[b]) if
  *   j <= p and (window == 0 or p - j < window or j < sinks), or j < prefix[b].
- * q and the cache's values enter the products exactly (fp32 q to 2^-133).  The
- * softmax's weights enter theirs in f16 for bf16 and fp16 tensors (each off by
- * 2^-11 of itself or 2^-32 of the row's largest, whichever is more; beside V
+ * q and the cache's values enter the products exactly (fp32 q to 2^-133), whose
+ * sums q.k, as there, are within fp32.  The softmax's weights enter theirs in
+ * f16 for bf16 and fp16 tensors (each off by 2^-11 of itself or 2^-32 of the
+ * row's largest, whichever is more; beside V
  * scales that f16 does not hold, bytes outside 0 and 112 to 134, by 2^-16 of
  * itself), and as three bf16 parts for fp32 ones (2^-24).  A NaN key makes the
  * rows that see its token NaN, no others; V holds no NaN below kv_lens.  The
