@@ -610,11 +610,13 @@ __device__ __forceinline__ float Tanh(float x) {
   return y < 0.2f ? small : x != x ? x : large;
 }
 
-// Scores to powers of two: they are s c with PowerOf's c, capped ones (softcap
+// Scores to powers of two: they are s c with Step's c, capped ones (softcap
 // tanh(s scale / softcap)) once Cap has been over them.  The 16-bit types take the
 // plain 1 - 2 / (1 + e^2x), off by 2^-22 of the cap, while that is at most
 // kPlainCap and the scores so off by 2^-16.
 constexpr float kPlainCap = 64.f;
+// A key's exponent that a factor without one of its own (AttnArgs) may meet.
+constexpr int32_t kNear = 126 - kMostFactor;
 template <bool fine, uint32_t R>
 __device__ __forceinline__ void Cap(const AttnArgs& a, f32x4 (&s)[R][2], float in) {
   const float out = a.cap * kLog2e;
@@ -624,18 +626,30 @@ __device__ __forceinline__ void Cap(const AttnArgs& a, f32x4 (&s)[R][2], float i
     for (uint32_t j = 0; j < 8; ++j)
       s[t][j / 4][j % 4] = out * Tanh<fine>(in * s[t][j / 4][j % 4]);
 }
-__device__ __forceinline__ float PowerOf(const AttnArgs& a) {
-  return a.cap > 0.f ? 1.f : a.scale * kLog2e;
-}
-// What a record's keys lack in their products (KeyOperand).
+// What a record's keys lack in their products (KeyOperand), as an exponent.
 template <uint32_t parts, uint32_t D>
-__device__ __forceinline__ float KeyScale(const Record<Fp4, D>&) {
-  return 1.f;
+__device__ __forceinline__ int32_t KeyExponent(const Record<Fp4, D>&) {
+  return 0;
 }
 template <uint32_t parts, uint32_t D>
-__device__ __forceinline__ float KeyScale(const Record<Fp8, D>& r) {
-  const uint32_t byte = r.scales & 255u;
-  return Scale8(parts == 2 ? byte : max(byte, 127u));
+__device__ __forceinline__ int32_t KeyExponent(const Record<Fp8, D>& r) {
+  const int32_t byte = __builtin_amdgcn_readfirstlane((int)(r.scales & 255u));
+  return byte == 0 ? 0 : parts == 2 ? byte - 127 : max(byte - 127, 0);
+}
+// What the products s are multiplied by where scale 2^exponent 2^key may be past
+// fp32 (an infinity there makes a NaN of a score of 0, a 0 that of a hidden key's
+// -inf): half of the exponent at once, and the rest.  Neither step then leaves fp32
+// where both together do not.
+template <uint32_t R>
+__device__ __forceinline__ float InTwoSteps(const AttnArgs& a, int32_t key, f32x4 (&s)[R][2]) {
+  const int32_t all = a.exponent + key + __builtin_amdgcn_frexp_expf(a.scale);
+  const int32_t e = min(max(all, -250), 250);  // (past it all products are 0 or past fp32)
+  const float half = __builtin_ldexpf(1.f, e / 2);
+#pragma unroll
+  for (uint32_t t = 0; t < R; ++t)
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) s[t][j / 4][j % 4] *= half;
+  return __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(a.scale), e - e / 2);
 }
 
 // The record's key of a lane's score j.
@@ -792,13 +806,19 @@ __device__ __forceinline__ bool Unusual(const KvSpan& span, Record<Fp8, D>& r, i
 template <class F, uint32_t parts, uint32_t D, uint32_t R>
 __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Record<F, D>& r,
                                      int32_t key0, f32x4 (&s)[R][2], Rows<F, parts, D, R>& w) {
-  float c = PowerOf(a);
-  if (a.cap > 0.f) {
-    const float in = a.scale / a.cap * KeyScale<parts>(r);
-    if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s, in);
-    else Cap<false, R>(a, s, in);
-  } else {
-    c *= KeyScale<parts>(r);
+  const int32_t key = KeyExponent<parts>(r);
+  float c = a.scale;
+  if (__is_same(F, Fp8)) c *= __uint_as_float((uint32_t)(key + 127) << 23);
+  // (one branch, on whole numbers, for what most calls have none of: with two, that
+  // the products' end and the softmax lay between, small calls took 1 us longer)
+  const bool far = a.exponent != 0 || key < -kNear || key > kNear;
+  if (__float_as_uint(a.cap) != 0 || __builtin_expect(far, 0)) {
+    if (far) c = InTwoSteps(a, key, s);
+    if (a.cap > 0.f) {
+      if (parts == 3 || a.cap > kPlainCap) Cap<true, R>(a, s, c);
+      else Cap<false, R>(a, s, c);
+      c = 1.f;
+    }
   }
   constexpr bool half = parts < 3;
   bool wide = Unusual<half>(span, r, key0, s, static_cast<State<D, R>&>(w));

@@ -594,6 +594,12 @@ hipError_t Launch(const AttnArgs& in, Workspace& ws, hipStream_t stream) {
     a.cap = a.sign = 0.f;
     a.scale = 1.f;
   }
+  const double factor =
+      a.cap > 0.f ? (double)a.scale / (double)a.cap : (double)a.scale * (double)kLog2e;
+  int exponent;
+  const double part = std::frexp(factor, &exponent);
+  a.exponent = std::abs(exponent) < kMostFactor ? 0 : exponent;
+  a.scale = (float)(a.exponent == 0 ? factor : part);
   const AttnWay how = WayOf<F>(a);
   if (how.way == HB_KV_WAY_PROMPT) return F::Prompt(a, ws, stream);
   switch (a.type) {

@@ -455,6 +455,7 @@ inline bool KvRowsAligned(const KvRowsArgs& a, bool read) {
 }
 // tokens * heads < 2^31
 hipError_t LaunchKvRows(const KvRowsArgs& a, bool read, hipStream_t stream);
+constexpr int32_t kMostFactor = 96;
 struct AttnArgs {
   const void* q;
   void* out;
@@ -471,6 +472,10 @@ struct AttnArgs {
   float* ws;
   // prompts: records of a request that are opened, and where
   uint32_t opened;
+  // What products are multiplied by is scale 2^exponent once the launcher has put
+  // the logarithm's base, or the cap, into it; 0 where it is within 2^kMostFactor
+  // either way.
+  int32_t exponent;
   uint8_t* opened_at;
 };
 // How a call is divided: HB_KV_WAY_*, 16-row tiles of a wave, tiles of a request

@@ -267,17 +267,18 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
   const KvWalk all = KvRecords(base_pos, base_pos + (int32_t)span.rows - 1, span.total,
                                LeadOf<F>(span, span.rows - 1, a.sinks), a.window);
   const uint64_t first_opened = ((uint64_t)b * a.heads + head) * a.opened;
-  bool slow = all.count > a.opened;
+  bool slow = all.count > a.opened || a.exponent != 0;
   for (uint32_t i = lane; i < count && !slow; i += 64) {
     const uint32_t r = OpenedAt(all, KvWalkRecord(walk, i));
     slow = reinterpret_cast<const uint32_t*>(a.ws)[first_opened + r] != 0;
   }
   slow = __builtin_amdgcn_ballot_w64(slow) != 0;
   auto key_of = [&](uint32_t i) { return (int32_t)(32 * KvWalkRecord(walk, i)); };
-  // Scale bytes that f16 does not hold, or more records than were opened: the
-  // rows a tile at a time on the general steps.  (Here, before the loop, so that
-  // nothing of this stays in registers through it; and told to be unlikely, so
-  // that its code lies behind: short prompts at D 64 36.9 us for 38.2.)
+  // Scale bytes that f16 does not hold, more records than were opened, or a factor
+  // that wants two steps: the rows a tile at a time on the general steps.  (Here,
+  // before the loop, so that nothing of this stays in registers through it; and
+  // told to be unlikely, so that its code lies behind: short prompts at D 64 36.9
+  // us for 38.2.)
   if (__builtin_expect(slow, 0)) {
 #pragma unroll 1
     for (uint32_t t = 0; t < R; ++t) {
@@ -400,8 +401,8 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
 #pragma unroll
           for (uint32_t t = 0; t < R; ++t) s[t][k] = Product(x, q[t][e], s[t][k]);
         }
-      const float c = PowerOf(a);
-      if (a.cap > 0.f) Cap<fine, R>(a, s, a.scale / a.cap);
+      const float c = a.cap > 0.f ? 1.f : a.scale;
+      if (a.cap > 0.f) Cap<fine, R>(a, s, a.scale);
       Hide<D, R>(w, key0, s);
       f16x8 pt[R];
 #pragma unroll
