@@ -2,8 +2,8 @@
 // rows of logits, one pass over them.
 //
 // With c = scale log2 e, m the running maximum, t = x - m, l = sum 2^(c t) and
-// w = sum t 2^(c t), a token's log probability is (c t - log2 l) ln 2 and the
-// entropy (log2 l - c w / l) ln 2.  Parts with maxima m1, m2 meet at m = max as
+// w = sum t 2^(c t), a token's log probability is scale t - ln l and the entropy
+// ln l - scale w / l.  Parts with maxima m1, m2 meet at m = max as
 // l = sum l_i f_i, w = sum (w_i + (m_i - m) l_i) f_i, f_i = 2^(c (m_i - m)).  The
 // difference comes before the product, so that logits of any size have one.
 //
@@ -243,10 +243,15 @@ template <class T>
 __device__ __forceinline__ void Finish(const LogprobsArgs& a, uint32_t row, const Given<T>& given,
                                        Sums s, uint64_t key) {
   const T* const x = static_cast<const T*>(a.logits) + row * a.stride;
-  const float c = a.scale * kLog2e, inf = __builtin_inff();
-  const float ref = Reference(s.m), log = s.l == 0.f ? 0.f : __builtin_amdgcn_logf(s.l);
+  const float inf = __builtin_inff(), ref = Reference(s.m);
+  const float log = s.l == 0.f ? 0.f : __builtin_amdgcn_logf(s.l) * kLn2;
   const auto logprob = [&](float logit) {
-    return s.l == 0.f ? -inf : ((logit - ref) * c - log) * kLn2;
+    if (s.l == 0.f) return -inf;
+    const float t = logit - ref;
+    // (by halves where the difference passes fp32 and the scale may bring it back;
+    // such a term is 0 in the sums)
+    return t == -inf ? fmaf(0.5f * logit - 0.5f * ref, 2.f * a.scale, -log)
+                     : fmaf(t, a.scale, -log);
   };
   const uint32_t lane = threadIdx.x % 64;
   if (lane == 0) {
@@ -254,7 +259,7 @@ __device__ __forceinline__ void Finish(const LogprobsArgs& a, uint32_t row, cons
       a.logprobs[row] = given.token < 0                     ? 0.f
                         : (uint32_t)given.token >= a.vocab ? __builtin_nanf("")
                                                             : logprob(given.logit);
-    if (a.entropy != nullptr) a.entropy[row] = s.l == 0.f ? 0.f : (log - c * (s.w / s.l)) * kLn2;
+    if (a.entropy != nullptr) a.entropy[row] = s.l == 0.f ? 0.f : fmaf(-a.scale, s.w / s.l, log);
   }
   if (a.top == 0) return;
   const uint64_t at = (uint64_t)row * a.top;
