@@ -1499,8 +1499,8 @@ int KvRows(hb_ctx* ctx, const hb_kv_rows_desc* d, bool read, bool sync, bool eig
   if (int rc = CheckType(d->type)) return rc;
   if (int rc = CheckCache(d->cache)) return rc;
   if (d->tokens == 0) return ctx ? HB_OK : Enter(ctx);
-  // (8 bits: 16 rows a workgroup of 256, 2^32 threads)
-  if ((uint64_t)d->tokens * d->cache.heads > (eight ? 0x0FFFFFFFu : 0x7FFFFFFFu))
+  if ((uint64_t)d->tokens * d->cache.heads > (eight ? 0x0FFFFFFFu : 0x7FFFFFFFu) ||
+      d->cache.heads > hb::kMostGroups)
     return Fail(HB_EINVAL, "%u tokens of %u heads in one call", d->tokens, d->cache.heads);
   if (!d->k || !d->v || !d->slots) return Fail(HB_EINVAL, "null cache row argument");
   const uint32_t size = d->type == HB_TYPE_F32 ? 4 : 2;

@@ -442,8 +442,22 @@ struct KvRowsArgs {
   const int32_t* slots;
   uint8_t* cache;
   uint32_t type, tokens, pages, heads, groups, dim;
-  uint32_t vec, window;            // set by the launchers
-};
+  uint32_t vec, window, first;     // set by the launchers; first: a launch's first
+};                                 // workgroup's place among those of a head
+// Workgroups of 256 threads that a launch has room for, 2^32 threads in all.
+constexpr uint32_t kMostGroups = 0xFFFFFF;
+// launch(grid) for the `groups` of each of the heads (fewer than 2^24), as many
+// together as a launch holds; nearly always in one.
+template <class Launch>
+hipError_t LaunchRowGroups(KvRowsArgs& a, uint32_t groups, Launch&& launch) {
+  const uint32_t most = kMostGroups / a.heads;
+  for (a.first = 0; a.first < groups; a.first += most) {
+    launch((groups - a.first < most ? groups - a.first : most) * a.heads);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
+}
 // Whether the rows allow loads and stores of four elements.
 inline bool KvRowsAligned(const KvRowsArgs& a, bool read) {
   const uint32_t size = a.type == HB_TYPE_F32 ? 4 : 2;
@@ -453,7 +467,7 @@ inline bool KvRowsAligned(const KvRowsArgs& a, bool read) {
            : reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
   return strides % 4 == 0 && bases % (4 * size) == 0;
 }
-// tokens * heads < 2^31
+// tokens * heads < 2^31, heads <= kMostGroups
 hipError_t LaunchKvRows(const KvRowsArgs& a, bool read, hipStream_t stream);
 constexpr int32_t kMostFactor = 96;
 struct AttnArgs {
@@ -539,7 +553,7 @@ struct CompactArgs {
 };
 hipError_t LaunchCompact(const CompactArgs& a, Workspace& ws, hipStream_t stream);
 
-// Cache rows of 8 bits (hb_kv8.hip); tokens * heads < 2^31.
+// Cache rows of 8 bits (hb_kv8.hip); tokens * heads < 2^31, heads <= kMostGroups.
 hipError_t LaunchKv8Rows(const KvRowsArgs& a, bool read, hipStream_t stream);
 
 // Log probabilities (hb_logprobs.hip).

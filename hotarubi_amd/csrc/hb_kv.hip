@@ -471,15 +471,15 @@ template <uint32_t dim>
 struct RowLanes {
   static constexpr uint32_t kLanes = dim / 8, kTokens = kThreads / kLanes;
   uint32_t token, head, col;
-  __device__ __forceinline__ explicit RowLanes(uint32_t heads) {
-    head = blockIdx.x % heads;
-    token = blockIdx.x / heads * kTokens + threadIdx.x / kLanes;
+  __device__ __forceinline__ explicit RowLanes(const KvRowsArgs& g) {
+    head = blockIdx.x % g.heads;
+    token = (blockIdx.x / g.heads + g.first) * kTokens + threadIdx.x / kLanes;
     col = threadIdx.x % kLanes * 8;
   }
 };
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
-  const RowLanes<dim> at(g.heads);
+  const RowLanes<dim> at(g);
   constexpr uint32_t kLanes = RowLanes<dim>::kLanes;
   float k[8] = {}, v[8] = {};
   int32_t slot = -1;
@@ -563,7 +563,7 @@ __device__ __forceinline__ void Store8(T* to, bool vec, const T* y) {
 // bounds it: the rows above back to fp32 in 11.9 us, 4.0 TB/s.
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void ReadKernel(const KvRowsArgs g) {
-  const RowLanes<dim> at(g.heads);
+  const RowLanes<dim> at(g);
   if (at.token >= g.tokens) return;
   uint64_t record;
   uint32_t t;
@@ -592,12 +592,13 @@ hipError_t LaunchRopeOf(const RopeArgs& a, bool vec, uint32_t grid, hipStream_t 
 }
 
 template <class T>
-hipError_t LaunchKvRowsOf(const KvRowsArgs& a, bool read, uint32_t grid, hipStream_t s) {
+hipError_t LaunchKvRowsOf(KvRowsArgs& a, bool read, uint32_t groups, hipStream_t s) {
 #define HB_ROWS_DIM(d)                                                   \
   case d:                                                                \
-    if (read) ReadKernel<T, d><<<grid, kThreads, 0, s>>>(a);             \
-    else AppendKernel<T, d><<<grid, kThreads, 0, s>>>(a);                \
-    break;
+    return LaunchRowGroups(a, groups, [&](uint32_t grid) {               \
+      if (read) ReadKernel<T, d><<<grid, kThreads, 0, s>>>(a);           \
+      else AppendKernel<T, d><<<grid, kThreads, 0, s>>>(a);              \
+    });
   switch (a.dim) {
     HB_ROWS_DIM(64)
     HB_ROWS_DIM(128)
@@ -647,11 +648,11 @@ hipError_t LaunchKvRows(const KvRowsArgs& in, bool read, hipStream_t stream) {
   KvRowsArgs a = in;
   a.vec = KvRowsAligned(a, read);
   const uint32_t tokens = kThreads / (a.dim / 8);  // of a workgroup
-  const uint32_t grid = (a.tokens + tokens - 1) / tokens * a.heads;
+  const uint32_t groups = (a.tokens + tokens - 1) / tokens;
   switch (a.type) {
-    case HB_TYPE_F32: return LaunchKvRowsOf<float>(a, read, grid, stream);
-    case HB_TYPE_BF16: return LaunchKvRowsOf<__bf16>(a, read, grid, stream);
-    default: return LaunchKvRowsOf<_Float16>(a, read, grid, stream);
+    case HB_TYPE_F32: return LaunchKvRowsOf<float>(a, read, groups, stream);
+    case HB_TYPE_BF16: return LaunchKvRowsOf<__bf16>(a, read, groups, stream);
+    default: return LaunchKvRowsOf<_Float16>(a, read, groups, stream);
   }
 }
 

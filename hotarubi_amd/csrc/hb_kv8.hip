@@ -90,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
   const uint32_t tid = threadIdx.x, lane = tid % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const uint32_t head = blockIdx.x % g.heads;
-  const uint32_t row0 = blockIdx.x / g.heads * g.window;
+  const uint32_t row0 = (blockIdx.x / g.heads + g.first) * g.window;
   const uint32_t group = tid / kRow, col = tid % kRow * 4;
   // slots of the row before the window's and of 63 rows from there, a lane each
   const uint64_t at = (uint64_t)row0 + lane;
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void ReadKernel(const KvRowsArgs g) {
   constexpr uint32_t kRow = dim / 4, kGroups = kThreads / kRow, kEach = 4;
   const uint32_t head = blockIdx.x % g.heads, col = threadIdx.x % kRow * 4;
   const uint64_t row0 =
-      (uint64_t)(blockIdx.x / g.heads) * (kGroups * kEach) + threadIdx.x / kRow * kEach;
+      (uint64_t)(blockIdx.x / g.heads + g.first) * (kGroups * kEach) + threadIdx.x / kRow * kEach;
   uint32_t k[kEach], v[kEach], scales[kEach], t[kEach];
   int32_t slot[kEach];
   const uint8_t* from[kEach];
@@ -321,14 +321,16 @@ template <class T, uint32_t dim>
 hipError_t LaunchOf(KvRowsArgs& a, bool read, hipStream_t s) {
   if (read) {
     constexpr uint32_t kRows = kThreads / (dim / 4) * 4;
-    ReadKernel<T, dim><<<(a.tokens + kRows - 1) / kRows * a.heads, kThreads, 0, s>>>(a);
-  } else {
-    // eight workgroups a CU, of a block's rows at most
-    const uint64_t rows = (uint64_t)a.tokens * a.heads / (8 * (uint64_t)DeviceCus());
-    a.window = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(1, rows));
-    AppendKernel<T, dim><<<(a.tokens + a.window - 1) / a.window * a.heads, kThreads, 0, s>>>(a);
+    return LaunchRowGroups(a, (a.tokens + kRows - 1) / kRows, [&](uint32_t grid) {
+      ReadKernel<T, dim><<<grid, kThreads, 0, s>>>(a);
+    });
   }
-  return hipGetLastError();
+  // eight workgroups a CU, of a block's rows at most
+  const uint64_t rows = (uint64_t)a.tokens * a.heads / (8 * (uint64_t)DeviceCus());
+  a.window = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(1, rows));
+  return LaunchRowGroups(a, (a.tokens + a.window - 1) / a.window, [&](uint32_t grid) {
+    AppendKernel<T, dim><<<grid, kThreads, 0, s>>>(a);
+  });
 }
 
 template <class T>

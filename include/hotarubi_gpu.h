@@ -653,7 +653,8 @@ typedef struct hb_kv_cache {
  * 6.  A token's head with an infinity or NaN in K or V is stored as NaN keys
  * (scale bytes 255) and zero values.  A slot below 0 or past the cache's
  * pages is not written, and reads as zeros.  Slots written by one call differ
- * from each other.  tokens * heads is below 2^31.  Strides in elements. */
+ * from each other.  tokens * heads is below 2^31, heads below
+ * 2^24.  Strides in elements. */
 typedef struct hb_kv_rows_desc {
   hb_kv_cache cache;
   void* k;  /* hb_kv_append reads k and v, hb_kv_read writes them */
@@ -757,7 +758,7 @@ int hb_kv_attention_way(const hb_kv_attention_desc* desc, hb_kv_way* way);
  * is not written and ends a run.  A call brings each block at most one run
  * (what a block holds after two is not said; no other one is touched).
  * hb_kv8_read gives the stored values of slots, zeros where there is none.
- * The descriptors are hb_kv_append's, tokens * heads below 2^28. */
+ * The descriptors are hb_kv_append's, tokens * heads below 2^28, heads below 2^24. */
 int hb_kv8_append(hb_ctx* ctx, const hb_kv_rows_desc* desc);
 int hb_kv8_append_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
 int hb_kv8_read(hb_ctx* ctx, const hb_kv_rows_desc* desc);
