@@ -492,7 +492,7 @@ hipError_t LaunchOf(AttnArgs& a, const AttnWay& how, Workspace& ws, hipStream_t 
   const uint64_t pairs = (uint64_t)a.batch * a.heads, stored = std::min<uint64_t>(R * 16, rows);
   const uint64_t grid = how.way == HB_KV_WAY_SHARES ? how.splits : pairs * how.tiles * how.splits;
   const uint64_t join = how.workspace > 0 ? pairs * how.tiles * stored : 0;
-  if (grid > 0x7FFFFFFFu || join > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (grid > kMostGroups || join > kMostGroups) return hipErrorInvalidConfiguration;
   a.tiles = how.tiles;
   a.splits = how.splits;
   a.split_records = how.split_records;

@@ -488,7 +488,8 @@ static hipError_t LaunchOf(AttnArgs& a, hipStream_t stream) {
   const uint64_t tiles = (rows + Shape<D>::kRows - 1) / Shape<D>::kRows;
   const uint64_t pairs = (uint64_t)a.batch * a.heads, records = pairs * a.opened;
   const uint64_t grid = tiles * pairs;
-  if (grid > 0x7FFFFFFFu || records > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (grid > kMostGroups / (Shape<D>::kWaves / 4) || records > kMostGroups)
+    return hipErrorInvalidConfiguration;
   a.tiles = (uint32_t)tiles;
   OpenKernel<F, parts, D><<<(uint32_t)((records + 3) / 4), 256, 0, stream>>>(a);
   if (a.cap > kPlainCap)
