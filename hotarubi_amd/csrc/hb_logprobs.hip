@@ -36,7 +36,9 @@ constexpr uint32_t kStretches = 24;
 // of 50,001 bf16 logits with 20 each 51.5 us, 52.1 with two maxima a lane, but with
 // 32 54.3 and 54.0, with 64 108 and 70.
 constexpr uint32_t kOfOne = 24;
-constexpr uint32_t kMostParts = 64;
+// Parts of a row and the keys that are joined of them: 9 x 161,526 fp32, 32 each, 17.4
+// us, 21.1 with 40 parts of 32 keys, 19.2 with 8.
+constexpr uint32_t kMostParts = 64, kJoined = 512;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // Values of a 16-byte load, as fp32.
@@ -511,7 +513,7 @@ __global__ __launch_bounds__(kThreads, 8) void LogprobsKernel(const LogprobsArgs
 // 13.7, 64 of 128,000 40 for 19.
 template <class T>
 __global__ __launch_bounds__(kThreads) void JoinKernel(const LogprobsArgs a) {
-  __shared__ uint64_t lists[2][kMostParts * 64];
+  __shared__ uint64_t lists[2][kJoined];
   __shared__ Sums sums;
   const uint32_t row = blockIdx.x, tid = threadIdx.x;
   const uint64_t* const from = PartAt(a, (uint64_t)row * a.parts);
@@ -547,9 +549,8 @@ hipError_t LaunchType(LogprobsArgs& a, Workspace& ws, hipStream_t stream) {
   // each: 14.3 us; 15.2 with one, 14.6 with four)
   const uint64_t per = 2 * kLoads * 64 * kWaves * Packed<T>::kCount;
   const uint64_t want = (4 * cus + a.rows - 1) / a.rows;
-  // and of about 512 keys to be joined: 9 x 161,526 fp32, 32 each, 17.4 us, 21.1
-  // with 40 parts of 32 keys, 19.2 with 8
-  const uint64_t few = std::max<uint64_t>(8, 512 / std::max(1u, a.top));
+  static_assert(kJoined / 64 >= 8, "parts of the most likeliest tokens");
+  const uint64_t few = kJoined / std::max(1u, a.top);
   a.parts = (uint32_t)std::min<uint64_t>({want, (a.vocab + per - 1) / per, kMostParts, few});
   if (a.parts > 1) {
     const hipError_t err =
