@@ -752,13 +752,18 @@ int hb_kv_attention_way(const hb_kv_attention_desc* desc, hb_kv_way* way);
  * a run.  A run that begins at a block's first token begins the block anew;
  * otherwise the block's earlier tokens stay.  The scale is the least 2^e, e
  * within [-117, 119], that has the run's largest value at 448 or below, and
- * not below that of earlier tokens, whose codes are rounded again where it
- * grows; values are rounded to nearest even (past 448 x 2^119: to that).  A
+ * not below the one that the block had, to which its earlier tokens' codes are
+ * rounded again where it grows; values are rounded to nearest even (past 448 x
+ * 2^119: to that).  So where a request's length is taken back within a block
+ * (drafts that were not accepted), the tokens that follow, and those that stay,
+ * keep the scale that the dropped ones brought, until the block begins anew.  A
  * token's head with an infinity or NaN in K or V is stored as NaN keys and
  * zero values and moves no scale.  A slot below 0 or past the cache's pages
  * is not written and ends a run.  A call brings each block at most one run
  * (what a block holds after two is not said; no other one is touched).
- * hb_kv8_read gives the stored values of slots, zeros where there is none.
+ * hb_kv8_read gives the stored values of slots, zeros where there is none; a
+ * stored value past 65504, to which fp16's largest may be rounded, is an
+ * infinity in fp16.
  * The descriptors are hb_kv_append's, tokens * heads below 2^28, heads below 2^24. */
 int hb_kv8_append(hb_ctx* ctx, const hb_kv_rows_desc* desc);
 int hb_kv8_append_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
