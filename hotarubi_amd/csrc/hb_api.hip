@@ -1729,7 +1729,7 @@ int KvCompact(hb_ctx* ctx, const hb_kv_compact_desc* d, bool sync) {
   if (d->free_size < d->pages || d->pair_count < d->pages / 2)
     return Fail(HB_EINVAL, "room for %u free pages and %u pairs of %u pages", d->free_size,
                 d->pair_count, d->pages);
-  if (int rc = CheckInts({{d->lens, d->batch}, {d->free_pages, d->pages}, {d->free_count, 1},
+  if (int rc = CheckInts({{d->lens, d->batch}, {d->free_pages, d->free_size}, {d->free_count, 1},
                           {d->pairs, 2ull * d->pair_count}, {d->status, 2}}))
     return rc;
   if (int rc = Enter(ctx)) return rc;
