@@ -5,19 +5,15 @@
 
 #include "hb_internal.h"
 #include "hb_kv.h"
+#include "hb_lanes.h"
 #include "hb_ring.h"
 
 namespace hb {
 namespace attn {
 
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 template <uint32_t parts>
@@ -25,17 +21,14 @@ struct TypeOf;  // the tensors' type by the bf16 parts that hold its values exac
 template <>
 struct TypeOf<1> {
   typedef __bf16 type;
-  typedef bf16x4 four;
 };
 template <>
 struct TypeOf<2> {
   typedef _Float16 type;
-  typedef f16x4 four;
 };
 template <>
 struct TypeOf<3> {
   typedef float type;
-  typedef f32x4 four;
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -354,13 +347,7 @@ __device__ __forceinline__ void ToParts(const float* x, bf16x8* out) {
   }
 }
 
-// Largest of three (a NaN loses); of two where fmaxf would make sure of quiet
-// NaNs first.
-__device__ __forceinline__ float Max3(float a, float b, float c) {
-  float y;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
-  return y;
-}
+// Largest of two, where fmaxf would make sure of quiet NaNs first.
 __device__ __forceinline__ float Max2(float a, float b) { return Max3(a, b, b); }
 // Of a lane's scores.  The matrix cores' results may be read some cycles after
 // their last product only; the compiler keeps its own instructions from them so
@@ -432,7 +419,7 @@ __device__ __forceinline__ bool OutAligned(const AttnArgs& a) {
 template <uint32_t parts, uint32_t D>
 struct Query {
   typedef typename TypeOf<parts>::type T;
-  typedef typename TypeOf<parts>::four V;
+  typedef typename Four<typename TypeOf<parts>::type>::type V;
   V x[D / 16];
   __device__ __forceinline__ void Load(const AttnArgs& a, uint64_t at, bool valid) {
     const T* from = static_cast<const T*>(a.q) + at;
@@ -483,7 +470,7 @@ __device__ __forceinline__ T Rounded(float x) {
 template <uint32_t parts>
 __device__ __forceinline__ void StoreFour(const AttnArgs& a, uint64_t at, bool vec, f32x4 y) {
   typedef typename TypeOf<parts>::type T;
-  typedef typename TypeOf<parts>::four V;
+  typedef typename Four<typename TypeOf<parts>::type>::type V;
   T* to = static_cast<T*>(a.out) + at;
   V z;
 #pragma unroll

@@ -4,30 +4,10 @@
 
 #include "hb_internal.h"
 #include "hb_kv.h"
+#include "hb_lanes.h"
 
 namespace hb {
 namespace {
-
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-
-template <class T>
-struct Four;
-template <>
-struct Four<float> {
-  typedef f32x4 type;
-};
-template <>
-struct Four<__bf16> {
-  typedef bf16x4 type;
-};
-template <>
-struct Four<_Float16> {
-  typedef f16x4 type;
-};
 
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 

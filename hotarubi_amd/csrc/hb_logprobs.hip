@@ -23,11 +23,10 @@
 #include <algorithm>
 
 #include "hb_internal.h"
+#include "hb_lanes.h"
 
 namespace hb {
 namespace {
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 constexpr uint32_t kLoads = 2;  // 16-byte loads of a lane's batch
@@ -76,13 +75,6 @@ __device__ __forceinline__ uint64_t KeyOf(float x, uint32_t column) {
 __device__ __forceinline__ float LogitOf(uint64_t key) {
   const uint32_t order = (uint32_t)(key >> 32);
   return __uint_as_float((int32_t)order < 0 ? order ^ 0x80000000u : ~order);
-}
-
-// Largest of three (a NaN loses).
-__device__ __forceinline__ float Max3(float a, float b, float c) {
-  float y;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
-  return y;
 }
 
 // (fmaxf would make sure of quiet NaNs first)
@@ -146,13 +138,6 @@ __device__ __forceinline__ uint64_t ReadLane(uint64_t x, uint32_t lane) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, (int)lane);
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), (int)lane);
   return (uint64_t)hi << 32 | lo;
-}
-
-// Ends what the wave's LDS accesses before may still do.
-__device__ __forceinline__ void WaveFence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // The largest order of 16 upper bits that k of the lanes' reach (two a lane, or

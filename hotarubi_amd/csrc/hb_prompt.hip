@@ -185,12 +185,6 @@ __device__ __forceinline__ uint64_t RowStart(const RowSet& set, uint32_t row, ui
 __device__ __forceinline__ bool Whole(const void* base, uint64_t token, uint64_t head) {
   return (token | head) % 8 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0;
 }
-// Ends what the wave's LDS accesses before may still do.
-__device__ __forceinline__ void WaveFence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 // (`fine`: caps above kPlainCap, in a kernel of their own: beside the plain one
 // in the loop, eight chunks with capped scores took 64.9 us for 63.8.)
@@ -428,7 +422,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
     return;
   }
   __syncthreads();  // the stages have been read
-  typedef typename TypeOf<parts>::four V;
+  typedef typename Four<typename TypeOf<parts>::type>::type V;
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
     const float inv = w.l[t] == 0.f ? 0.f : 1.f / w.l[t];
