@@ -43,7 +43,7 @@ constexpr float kRoom = 64.f;
 // ---------------------------------------------------------------- records --
 
 struct Fp4 {
-  static constexpr bool kSinks = false, kAnyScore = false;
+  static constexpr bool kSinks = false;
   static constexpr double kSplitRecord = 1;  // (Divide)
   // bf16 parts of q, by the tensors' type
   static constexpr uint32_t Parts(uint32_t parts) { return parts; }
@@ -57,9 +57,9 @@ struct Fp4 {
 // (2^33 at most).  bf16 and fp32 ones take keys with the part of their scale that
 // is below 1, so that a large query meets small keys and not their codes, and the
 // rest of it later, so that large keys' products do not pass fp32 before a small
-// `scale` has met them.  Scores of any size that fp32 holds are taken (Weights).
+// `scale` has met them.
 struct Fp8 {
-  static constexpr bool kSinks = true, kAnyScore = true;
+  static constexpr bool kSinks = true;
   // what a record costs a split's wave beside an MXFP4 one: 2 x 1,500 new tokens
   // behind 1,000, 15 heads on 5, D 64, bf16 51 us in splits, for 69 in the way
   // that the latter's figures choose
@@ -489,7 +489,7 @@ struct State {
   f32x4 o[R][D / 16];
   float m[R], l[R];
   bool large;  // values were met that want kRoom
-  bool far;    // a maximum has passed 2^20 (kept with any_score)
+  bool far;    // a maximum has passed 2^20
   Sight see[R];
   int32_t see_all, see_from, see_pre;  // every row sees keys see_from .. see_all, and < see_pre
 };
@@ -674,7 +674,7 @@ __device__ __forceinline__ void Hide(const State<D, R>& w, int32_t key0, f32x4 (
 
 // The running maximum of tile t moves where a score passes it by kSlack, and
 // what it had so far shrinks.  With `large` it stays kRoom above the scores.
-template <bool any_score, uint32_t D, uint32_t R>
+template <uint32_t D, uint32_t R>
 __device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
                                       bool large) {
   const float top = c * MaxOf8(s);
@@ -685,8 +685,7 @@ __device__ __forceinline__ void Raise(State<D, R>& w, uint32_t t, const f32x4 (&
   // rows that have seen nothing yet stay at -inf, with o and l zero
   const float shrink = m == w.m[t] ? 1.f : __builtin_amdgcn_exp2f(w.m[t] - m);
   w.m[t] = m;
-  if (any_score)
-    w.far |= __builtin_amdgcn_ballot_w64(fabsf(m) > 0x1p20f && fabsf(m) < __builtin_inff()) != 0;
+  w.far |= __builtin_amdgcn_ballot_w64(fabsf(m) > 0x1p20f && fabsf(m) < __builtin_inff()) != 0;
   w.l[t] *= shrink;
 #pragma unroll
   for (uint32_t i = 0; i < D / 16; ++i) w.o[t][i] *= shrink;
@@ -697,15 +696,15 @@ __device__ __forceinline__ float Reference(float m) {
 }
 // The record's weights and their sum.  They carry 2^kLift: at most 2^15, and in
 // f16 normal down to 2^-21 of the reference, off by 2^-32 of it below that.
-// With `any_score` a row whose maximum passes 2^20 takes its scores as the maximum
+// A row whose maximum passes 2^20 takes its scores as the maximum
 // took them, rounded, so that the largest is not 2^(half a step of the maximum)
 // of what it should be.
-template <bool any_score, uint32_t D, uint32_t R>
+template <uint32_t D, uint32_t R>
 __device__ __forceinline__ void Weights(State<D, R>& w, uint32_t t, const f32x4 (&s)[2], float c,
                                         float* p) {
   const float ref = Reference(w.m[t]);
   float sum = 0.f;
-  if (any_score && __builtin_expect(w.far, 0)) {
+  if (__builtin_expect(w.far, 0)) {
     const float m = w.m[t] == -__builtin_inff() ? 0.f : w.m[t];
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
@@ -817,8 +816,8 @@ __device__ __forceinline__ void Step(const AttnArgs& a, const KvSpan& span, Reco
 #pragma unroll
   for (uint32_t t = 0; t < R; ++t) {
     float p[8];
-    Raise<F::kAnyScore>(static_cast<State<D, R>&>(w), t, s[t], c, w.large);
-    Weights<F::kAnyScore>(static_cast<State<D, R>&>(w), t, s[t], c, p);
+    Raise(static_cast<State<D, R>&>(w), t, s[t], c, w.large);
+    Weights(static_cast<State<D, R>&>(w), t, s[t], c, p);
     if constexpr (half) {
       if (wide) {  // V in bf16, on two bf16 parts of a weight
         bf16x8 part[2];

@@ -402,8 +402,8 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, 2 * Shape<D>::kGroups) void 
 #pragma unroll
       for (uint32_t t = 0; t < R; ++t) {
         float p[8];
-        Raise<F::kAnyScore>(w, t, s[t], c, false);  // (V is within f16 here)
-        Weights<F::kAnyScore>(w, t, s[t], c, p);
+        Raise(w, t, s[t], c, false);  // (V is within f16 here)
+        Weights(w, t, s[t], c, p);
         pt[t] = HalfWeights(p);
       }
 #pragma unroll
