@@ -60,9 +60,12 @@ struct Fp4 {
 // `scale` has met them.
 struct Fp8 {
   static constexpr bool kSinks = true;
-  // what a record costs a split's wave beside an MXFP4 one: 2 x 1,500 new tokens
-  // behind 1,000, 15 heads on 5, D 64, bf16 51 us in splits, for 69 in the way
-  // that the latter's figures choose
+  // what a record costs a split's wave beside an MXFP4 one, whose figures the
+  // division's are: of 180 calls (1 to 32 requests of 3 to 1,500 new tokens, the
+  // types, D 64 to 256) it divides 22 otherwise than 1 does, 14 of them faster (2 x
+  // 1,500 new tokens behind 1,000, 15 heads on 5 of 64, bf16 54 us for 69; 3 x 1,500,
+  // 8 heads of 128, fp16 37 for 49), 5 alike, 3 slower (32 x 50 behind 150, 8 heads
+  // of 128, fp16 13.0 for 11.1, fp32 17.3 for 12.8)
   static constexpr double kSplitRecord = 0.65;
   static constexpr uint32_t Parts(uint32_t parts) { return parts == 2 ? 1 : parts; }
   static constexpr uint32_t Bytes(uint32_t dim) { return Kv8RecordBytes(dim); }

@@ -416,6 +416,7 @@ Division ByPrompt(const Sizes& z, uint64_t tile, uint64_t opened) {
 template <class F>
 Division ByWaves(const Sizes& z, Division::Way way, uint32_t tiles_of_16) {
   // us a record of a wave by itself on its SIMD, by type, tiles and head size
+  // (MXFP4 ones; for 8 bits kSplitRecord beside them)
   const double alone[3][2][3] = {{{0.72, 0.95, 1.25}, {0.95, 1.35, 0}},
                                  {{0.76, 1.05, 1.5}, {1.05, 1.5, 0}},
                                  {{0.8, 1.15, 1.85}, {1.15, 1.6, 0}}};

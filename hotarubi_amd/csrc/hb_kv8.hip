@@ -59,8 +59,8 @@ __device__ __forceinline__ void Load4(const T* x, bool vec, float* y) {
 // between its maximum and its codes.  A run that is a whole block leaves through
 // LDS in the record's order, 16 bytes a store; of others a token's own bytes,
 // which lie all over the record.  Memory bounds it: 16,001 tokens of 5 heads of 64
-// in fp32, 41 MB read and 10 written, 10.5 us = 4.9 TB/s (95 with a wave a run and
-// a byte a store); 64 single tokens of 8 heads of 128, bf16, 3.9 us, the chain from
+// in fp32, 41 MB read and 10 written, 12.3 us = 4.2 TB/s (95 with a wave a run and
+// a byte a store); 64 single tokens of 8 heads of 128, bf16, 4.8 us, the chain from
 // their slots over rows and scales to the stores.
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void AppendKernel(const KvRowsArgs g) {
@@ -235,7 +235,7 @@ __device__ __forceinline__ void Store4(T* to, bool vec, uint32_t codes, float sc
 // The stored values of slots, 4 columns of 4 neighbouring rows a thread.  Where
 // their slots are neighbours too, from a multiple of 4 on, a column's four V codes
 // are a word; else each is a load of its own.  The rows above back to fp32, 10 MB
-// read and 41 written, 9.0 us = 5.7 TB/s (12.1 with loads of their own).
+// read and 41 written, 10.6 us = 4.8 TB/s (12.1 with loads of their own).
 template <class T, uint32_t dim>
 __global__ __launch_bounds__(kThreads) void ReadKernel(const KvRowsArgs g) {
   constexpr uint32_t kRow = dim / 4, kGroups = kThreads / kRow, kEach = 4;

@@ -19,7 +19,7 @@
 // likeliest 115 us = 4.7 TB/s (a reading of them once at what the card copies at
 // is 105; without the likeliest tokens 105), 2,048 of 65,537 in fp32 107 us = 5.0.
 // Of short calls the waves' chain does: 8 rows of 50,001 fp32 logits, 20 each,
-// 8.8 us and 4.6 for the join.
+// 9.0 us and 5.4 for the join.
 #include <algorithm>
 
 #include "hb_internal.h"
@@ -526,7 +526,9 @@ hipError_t LaunchType(LogprobsArgs& a, Workspace& ws, hipStream_t stream) {
   // 4,096 rows of 1,000 bf16 logits 9 us (20 with four waves a row), 2,000 of
   // 8,192 14 (19), 4,500 of 16,000 38 (47), 4,096 of 65,537 115 (126), but 1,024
   // of 32,000 35 (23), 2,048 of 65,537 75 (59), and 4,096 of 65,537 in fp32 208
-  // (199).
+  // (199).  Between: 3,200 of 65,537 bf16 109 (101), 3,600 111 (114).  Over 82 such
+  // calls, 1,024 to 8,192 rows of 2,000 to 128,000, the choice is within 10% of the
+  // other, and mostly the better.
   const uint64_t cus = (uint64_t)DeviceCus();
   const bool alone = a.rows >= 4 * cus && (a.vocab * sizeof(T) <= 16384 ||
                                            (a.rows >= 16 * cus && sizeof(T) == 2));

@@ -84,6 +84,8 @@ __device__ __forceinline__ uint32_t Readied(Record<Fp4, D>& r, int32_t key0, int
 template <uint32_t parts, uint32_t D>
 __device__ __forceinline__ uint32_t Readied(Record<Fp8, D>& r, int32_t key0, int32_t total) {
   if (key0 + 32 > total) DropPast(r, key0, total);
+  // V's: a block whose largest value is below 0.0068 or past 57,344.  Three prompts of
+  // up to 4,096 tokens take 392 us, 528 with one such record, 1,097 with no other.
   uint32_t outside = OutsideHalf8(r.scales >> 8);
   // K's, which go into the operand whole: f16, or keys up to 2^72, that queries
   // up to 2^48 do not pass fp32 with (the general steps take larger ones apart)
