@@ -683,6 +683,8 @@ int hb_kv_read_async(hb_ctx* ctx, const hb_kv_rows_desc* desc);
  * itself or 2^-32 of the row's largest, whichever is more; on values that f16
  * does not hold by 2^-16 of itself), and as three bf16 parts for fp32 ones
  * (2^-24); what they are divided by is the sum of the unrounded ones.
+ * Values past 2^81 go with scores of up to 2^29, as the maximum keeps room for
+ * their sums.
  * Rows outside every request are not written.  A call of 2^24 workgroups or more
  * (as 65,536 requests of 256 K/V heads) is refused.  max_new and max_kv bound the
  * requests' new tokens and keys; they choose the split of the work.  Rows of a
